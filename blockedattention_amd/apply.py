@@ -9,7 +9,7 @@ wrong position (apply.py:41 against csrc/sparseBlockedAttention.cpp:127-128);
 here the call follows the extension's order, so ``blockSoftmax(x, rows, cols)``
 works as documented.
 """
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -88,6 +88,59 @@ def blockFusedAttention(
     """
     return blockAttention.sparseBlockedAttention(q, k, v, mat1Accum, mat2Accum, outAccum, MList, NList, KList,
                                                  float(scale))
+
+
+def pagedResize(
+    table: torch.Tensor, free: torch.Tensor, state: torch.Tensor,
+    lens: torch.Tensor, newLens: torch.Tensor, pageSize: int, tokens: int,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Request ``r`` goes from ``lens[r]`` to ``newLens[r]`` tokens: pages change hands, new tokens get places.
+
+    ``table`` (int32 ``[requests, width]``) holds every request's pages in the order of its tokens, ``free`` (int32) is a
+    stack whose first ``state[0]`` entries are the free pages; both are updated in place.  ``state`` is int64 ``[2]``:
+    that count and 0.  Lengths (int64) of 0 are requests that are not there.  Pages are taken in the order of requests,
+    first those that shrinking requests give back, then the free ones from the end of the stack.
+
+    Returns ``(slots, tokenAccum, lens, state)``: the places (``page * pageSize + row``, int64 ``[tokens]``) of the new
+    tokens, request after request, then -1; their exclusive prefix sums per request; the new lengths; the new state.
+    ``tokens`` is at least the number of new tokens.  Where there are too few pages, slots or entries in a row, or a
+    length is not valid, nothing changes hands, all slots are -1, the lengths come back as they were and ``state[1]`` is
+    a sum of 1 (too few pages), 2 (row too short), 4 (bad length), 8 (more new tokens than ``tokens``), 16 (bad
+    state).  A state with a verdict is refused again, so it may be looked at many steps later; nothing synchronises with
+    the host.
+    """
+    return tuple(blockAttention.pagedResize(table, free, state, lens, newLens, int(pageSize), int(tokens)))
+
+
+def pagedAppend(
+    k: torch.Tensor, v: torch.Tensor, kCache: torch.Tensor, vCache: torch.Tensor, slots: torch.Tensor,
+    kScale: Optional[torch.Tensor] = None, vScale: Optional[torch.Tensor] = None,
+) -> None:
+    """Writes the keys and values of new tokens to their places (``slots``, of ``pagedResize``) in a paged cache.
+
+    ``k`` and ``v`` are ``[heads, tokens * dim]`` (the layout of ``blockFusedAttention``) or ``[heads, tokens, dim]`` with any
+    strides of heads and tokens, the caches ``[pages, heads, page, dim]`` with any strides but the last.  The caches have
+    the dtype of ``k`` and ``v`` (fp16 or bf16), or are ``float8_e4m3fn``: then ``kScale`` and ``vScale`` (fp32
+    ``[heads]``) are what stored values are multiplied with; values are divided by it, limited to +-448 and rounded to
+    the nearest.  Places below 0 are skipped; no place may occur twice.
+    """
+    blockAttention.pagedAppend(k, v, kCache, vCache, slots, kScale, vScale)
+
+
+def pagedAttention(
+    q: torch.Tensor, kCache: torch.Tensor, vCache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+    scale: float = 1.0, window: int = 0,
+    kScale: Optional[torch.Tensor] = None, vScale: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``softmax(scale * q K^T) V`` of one query per request and head over the request's tokens in a paged cache.
+
+    ``q`` is ``[heads, requests * dim]`` or ``[heads, requests, dim]`` with any strides of heads and requests; its heads
+    are a multiple of the cache's, consecutive ones share a key head.  ``table`` and ``lens`` are those of
+    ``pagedResize``, the caches and scales those of ``pagedAppend``.  ``window`` > 0 looks at the last ``window`` tokens
+    only.  Requests of length 0 give zeros.  The result has the shape, dtype and order of dimensions of ``q``.  Forward
+    only; nothing synchronises with the host.
+    """
+    return blockAttention.pagedAttention(q, kCache, vCache, table, lens, float(scale), int(window), kScale, vScale)
 
 
 def set_schedule_cache(capacity: int) -> None:

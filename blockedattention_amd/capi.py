@@ -12,7 +12,7 @@ import torch
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "lib", "libblockedattn_hip.so")
 
-BA_F16, BA_BF16, BA_F32, BA_F64, BA_U8, BA_I8, BA_I16, BA_I32, BA_I64 = range(9)
+BA_F16, BA_BF16, BA_F32, BA_F64, BA_U8, BA_I8, BA_I16, BA_I32, BA_I64, BA_F8_E4M3 = range(10)
 META_FROM_LISTS, META_FROM_ACCUM, META_GIVEN = 0, 1, 2
 
 SYMBOLS = (
@@ -21,6 +21,7 @@ SYMBOLS = (
     "ba_varlen_gemm", "ba_blocked_softmax", "ba_blocked_softmax_backward", "ba_gemm_softmax",
     "ba_varlen_attention", "ba_attention_rows", "ba_varlen_attention_train", "ba_varlen_attention_backward",
     "ba_gemm_softmax_static", "ba_static_read", "ba_varlen_gemm_two",
+    "ba_paged_resize_workspace", "ba_paged_resize", "ba_paged_append", "ba_paged_attention_workspace", "ba_paged_attention",
 )
 MAILBOX_BYTES = 320
 STATIC_MAX_SEGMENTS = 4096   # BA_STATIC_MAX_SEGMENTS
@@ -42,6 +43,17 @@ class PlanInfo(ctypes.Structure):
 
     def as_dict(self):
         return {name: getattr(self, name) for name, _ in self._fields_}
+
+
+class PagedCache(ctypes.Structure):
+    """ba_paged_cache; ``paged_cache`` fills it from tensors."""
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("pages", ctypes.c_int64), ("heads", ctypes.c_int64), ("page", ctypes.c_int64), ("dim", ctypes.c_int64),
+        ("k_page_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64), ("k_token_stride", ctypes.c_int64),
+        ("v_page_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64), ("v_token_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int),
+    ]
 
 
 class BlockedAttentionError(RuntimeError):
@@ -108,6 +120,18 @@ def load():
     lib.ba_varlen_gemm_two.restype = i32
     lib.ba_varlen_gemm_two.argtypes = [i32, i64, vp, ctypes.POINTER(PlanInfo), vp, vp, vp, i64, i64, i64,
                                        vp, ctypes.POINTER(PlanInfo), vp, vp, vp, i64, i64, i64, vp]
+    cache = ctypes.POINTER(PagedCache)
+    lib.ba_paged_resize_workspace.restype = ctypes.c_size_t
+    lib.ba_paged_resize_workspace.argtypes = [i64]
+    lib.ba_paged_resize.restype = i32
+    lib.ba_paged_resize.argtypes = [vp, i64, i64, vp, i64, vp, vp, vp, i64, i64, vp, i64, vp, vp, vp, vp, ctypes.c_size_t, vp]
+    lib.ba_paged_append.restype = i32
+    lib.ba_paged_append.argtypes = [cache, i32, vp, i64, i64, vp, i64, i64, vp, i64, vp]
+    lib.ba_paged_attention_workspace.restype = ctypes.c_size_t
+    lib.ba_paged_attention_workspace.argtypes = [cache, i64, i64, i64]
+    lib.ba_paged_attention.restype = i32
+    lib.ba_paged_attention.argtypes = [cache, i32, vp, i64, i64, i64, i64, vp, i64, i64, vp, i64, f32, vp, i64, i64, vp,
+                                       ctypes.c_size_t, vp]
     _lib = lib
     return lib
 
@@ -315,3 +339,44 @@ def varlen_attention_backward(plan, Q, K, V, out, dO, lse, delta, dQ, dK, dV, H,
                                              _ptr(out), _ptr(dO), _ptr(lse), _ptr(delta), _ptr(dQ), _ptr(dK), _ptr(dV), H,
                                              Dm1, Dm2, Dout, float(scale), _stream())
     check(st, "ba_varlen_attention_backward")
+
+
+def paged_cache(kCache, vCache, kScale=None, vScale=None):
+    """ba_paged_cache of two arrays [pages, heads, page, dim] (fp16, bf16 or float8_e4m3fn) and, for the last, their scales."""
+    if kCache.shape != vCache.shape or kCache.dim() != 4 or kCache.dtype != vCache.dtype:
+        raise BlockedAttentionError("a paged cache is two arrays [pages, heads, page, dim] of one dtype")
+    for t in (kCache, vCache):
+        if t.stride(3) != 1 and t.size(3) > 1:
+            raise BlockedAttentionError("the last dimension of a paged cache must be contiguous")
+    dtype = BA_F8_E4M3 if kCache.dtype == torch.float8_e4m3fn else dtype_code(kCache.dtype)
+    return PagedCache(kCache.data_ptr(), vCache.data_ptr(), None if kScale is None else kScale.data_ptr(),
+                      None if vScale is None else vScale.data_ptr(), *kCache.shape, *kCache.stride()[:3], *vCache.stride()[:3], dtype)
+
+
+def paged_resize(table, free, state, lens, new_lens, page, slots, accum, lens_out, state_out):
+    """Pages and slots for requests that go from ``lens`` to ``new_lens`` tokens (see ba_paged_resize)."""
+    need = load().ba_paged_resize_workspace(lens.numel())
+    work = torch.empty(need, dtype=torch.uint8, device=table.device) if need else None
+    st = load().ba_paged_resize(_ptr(table), table.stride(0), table.size(1), _ptr(free), free.numel(), _ptr(state), _ptr(lens),
+                                _ptr(new_lens), lens.numel(), page, _ptr(slots), slots.numel(), _ptr(accum), _ptr(lens_out),
+                                _ptr(state_out), _ptr(work), need, _stream())
+    check(st, "ba_paged_resize")
+    return slots
+
+
+def paged_append(cache, k, v, slots):
+    """k, v [heads, tokens, dim] into the places ``slots`` of ``cache`` (see ba_paged_append)."""
+    st = load().ba_paged_append(ctypes.byref(cache), dtype_code(k.dtype), _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0),
+                                v.stride(1), _ptr(slots), slots.numel(), _stream())
+    check(st, "ba_paged_append")
+
+
+def paged_attention(cache, q, table, lens, out, scale=1.0, window=0):
+    """out [heads, requests, dim] <- attention of q over the requests' pages (see ba_paged_attention)."""
+    need = load().ba_paged_attention_workspace(ctypes.byref(cache), q.size(0), q.size(1), table.size(1))
+    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    st = load().ba_paged_attention(ctypes.byref(cache), dtype_code(q.dtype), _ptr(q), q.stride(0), q.stride(1), q.size(0), q.size(1),
+                                   _ptr(table), table.stride(0), table.size(1), _ptr(lens), window, float(scale), _ptr(out),
+                                   out.stride(0), out.stride(1), _ptr(work), need, _stream())
+    check(st, "ba_paged_attention")
+    return out

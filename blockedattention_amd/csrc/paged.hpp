@@ -1,0 +1,70 @@
+// What the kernels of the paged key-value cache share (paged_tables.hip, paged_append.hip, paged_attention.hip) and the
+// launchers that capi_paged.hip calls.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/blocked_attention.h"
+
+namespace ba {
+
+// Division of 0 <= n < 2^31 by a number given at run time: with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1,
+// n / d = (mulhi(n, m) + n) >> s (Granlund and Montgomery's round-up method; the sum stays below 2^32).
+struct PageDiv {
+    uint32_t d, mul, shift;
+    static PageDiv of(uint32_t d) {
+        uint32_t s = 0;
+        while ((uint64_t(1) << s) < d) ++s;
+        return {d, (uint32_t)(((((uint64_t)1 << s) - d) << 32) / d + 1), s};
+    }
+    __host__ __device__ __forceinline__ uint32_t div(uint32_t n) const {
+        return (uint32_t)((((uint64_t)n * mul) >> 32) + n) >> shift;
+    }
+};
+
+// One of the two arrays of a cache.
+struct PagedArray {
+    char *base;
+    const float *scale;                 // per head, 8-bit caches only
+    int64_t page_bytes, head_bytes;
+    int32_t token_bytes;
+};
+
+struct PagedTablesArgs {
+    int32_t *table, *free_pages;
+    const int64_t *state_in, *lens, *new_lens;
+    int64_t *slots, *accum, *lens_out, *state_out;
+    int64_t table_stride, pool;
+    int32_t requests, width, tokens;
+    PageDiv page;
+};
+
+struct PagedAppendArgs {
+    PagedArray to[2];
+    const char *from[2];
+    int64_t from_head_bytes[2], from_token_bytes[2];
+    const int64_t *slots;
+    int64_t tokens, places;             // places: pages * page
+    int32_t heads, dim;
+    PageDiv page;
+};
+
+struct PagedAttentionArgs {
+    PagedArray k, v;
+    const char *q;
+    char *out;
+    const int32_t *table;
+    const int64_t *lens;
+    int64_t q_head_bytes, q_row_bytes, out_head_bytes, out_row_bytes, table_stride;
+    int32_t requests, heads, group, dim, pages, width;
+    int32_t window;                     // tokens; 0: all
+    float scale;
+    PageDiv page;
+};
+
+int launch_paged_tables(const PagedTablesArgs &args, void *workspace, hipStream_t stream);
+int launch_paged_append(const PagedAppendArgs &args, int dtype, int cache_dtype, hipStream_t stream);
+size_t paged_attention_workspace(int64_t cache_heads, int64_t group, int64_t dim, int64_t requests, int64_t width, int64_t page);
+int launch_paged_attention(const PagedAttentionArgs &args, int dtype, int cache_dtype, void *workspace, hipStream_t stream);
+
+}  // namespace ba

@@ -9,6 +9,8 @@
 // Additions that keep the reference behaviour when left at their defaults:
 //   sparseBlockedSoftmaxScaled(src, rowList, colList, srcAccum?, scale)
 //   sparseBlockedGEMMSoftmax(mat1, mat2, ..., scale, out_fp32)   fused pair, forward only
+//   pagedResize, pagedAppend, pagedAttention                     paged key-value cache, forward only; no schedule, no
+//                                                                host synchronisation
 //
 // Every precondition the reference leaves to assert() is a TORCH_CHECK here.
 // The tensors are used as device memory only; all work happens in
@@ -637,6 +639,144 @@ Tensor sparseBlockedAttention_op(const Tensor &q, const Tensor &k, const Tensor 
     return attention_launch(q, k, v, s, scale, nullptr);
 }
 
+// ------------------------------------------------------------ paged key-value cache
+// Operands are read by their strides; only the last dimension has to be contiguous.
+void check_rows(const Tensor &t, const char *name, const Tensor &like) {
+    TORCH_CHECK(t.is_cuda(), name, " must be a GPU tensor");
+    TORCH_CHECK(t.device() == like.device(), name, " must be on the same device as the cache");
+    TORCH_CHECK(t.dim() >= 1 && (t.stride(-1) == 1 || t.size(-1) <= 1), name, ": the last dimension must be contiguous");
+}
+
+// [heads, rows * dim] or [heads, rows, dim], as head and row strides in elements.
+struct Rows {
+    int64_t heads, rows, head_stride, row_stride;
+};
+Rows rows_of(const Tensor &t, const char *name, int64_t dim) {
+    TORCH_CHECK(t.dim() == 2 || t.dim() == 3, name, " must be [heads, rows * dim] or [heads, rows, dim], got ", t.sizes());
+    if (t.dim() == 3) {
+        TORCH_CHECK(t.size(2) == dim, name, ": the cache holds rows of ", dim, " elements, got ", t.sizes());
+        return {t.size(0), t.size(1), t.stride(0), t.stride(1)};
+    }
+    TORCH_CHECK(t.size(1) % dim == 0, name, ": the cache holds rows of ", dim, " elements, got ", t.sizes());
+    return {t.size(0), t.size(1) / dim, t.stride(0), dim};
+}
+
+void check_no_grad(std::initializer_list<const Tensor *> tensors, const char *op) {
+    for (const Tensor *t : tensors)
+        TORCH_CHECK(!(at::GradMode::is_enabled() && t->requires_grad()), op, " has no backward pass: detach its operands or use torch.no_grad()");
+}
+
+// A kernel has written behind PyTorch's back: what watches version counters is told.
+void written(const Tensor &t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+ba_paged_cache cache_of(const Tensor &k, const Tensor &v, const OptTensor &k_scale, const OptTensor &v_scale) {
+    check_rows(k, "kCache", k); check_rows(v, "vCache", k);
+    TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes(), "kCache and vCache must both be [pages, heads, page, dim], got ", k.sizes(), " and ", v.sizes());
+    TORCH_CHECK(k.scalar_type() == v.scalar_type(), "kCache and vCache must have the same dtype");
+    ba_paged_cache c{};
+    const bool f8 = k.scalar_type() == at::kFloat8_e4m3fn;
+    TORCH_CHECK(f8 || k.scalar_type() == at::kHalf || k.scalar_type() == at::kBFloat16,
+                "a paged cache holds fp16, bf16 or float8_e4m3fn, got ", k.scalar_type());
+    TORCH_CHECK(k_scale.has_value() == f8 && v_scale.has_value() == f8,
+                f8 ? "a float8_e4m3fn cache needs kScale and vScale" : "kScale and vScale belong to a float8_e4m3fn cache");
+    TORCH_CHECK(k.size(1) >= 1 && k.size(2) >= 1 && k.size(3) >= 1 && k.size(3) <= 256,
+                "a paged cache has at least one head, one token a page and 1 to 256 dimensions, got ", k.sizes());
+    if (f8)
+        for (const OptTensor *s : {&k_scale, &v_scale}) {
+            check_data(**s, "kScale and vScale");
+            TORCH_CHECK((*s)->scalar_type() == at::kFloat && (*s)->dim() == 1 && (*s)->numel() == k.size(1) && (*s)->device() == k.device(),
+                        "kScale and vScale are fp32, one entry per head of the cache (", k.size(1), "), on its device");
+        }
+    c.k = k.data_ptr(); c.v = v.data_ptr();
+    c.k_scale = f8 ? k_scale->data_ptr<float>() : nullptr; c.v_scale = f8 ? v_scale->data_ptr<float>() : nullptr;
+    c.pages = k.size(0); c.heads = k.size(1); c.page = k.size(2); c.dim = k.size(3);
+    c.k_page_stride = k.stride(0); c.k_head_stride = k.stride(1); c.k_token_stride = k.stride(2);
+    c.v_page_stride = v.stride(0); c.v_head_stride = v.stride(1); c.v_token_stride = v.stride(2);
+    c.dtype = f8 ? BA_F8_E4M3 : k.scalar_type() == at::kHalf ? BA_F16 : BA_BF16;
+    return c;
+}
+
+void check_cache_operand(const Tensor &t, const char *name, const ba_paged_cache &c) {
+    TORCH_CHECK(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, name, " must be fp16 or bf16, got ", t.scalar_type());
+    TORCH_CHECK(c.dtype == BA_F8_E4M3 || c.dtype == (t.scalar_type() == at::kHalf ? BA_F16 : BA_BF16), name, " must have the cache's dtype");
+}
+
+void check_table(const Tensor &table, const Tensor &like) {
+    check_rows(table, "table", like);
+    TORCH_CHECK(table.scalar_type() == at::kInt && table.dim() == 2, "table must be int32 [requests, pages of a request]");
+}
+
+std::vector<Tensor> pagedResize_op(const Tensor &table, const Tensor &free_pages, const Tensor &state, const Tensor &lens,
+                                   const Tensor &new_lens, int64_t page, int64_t tokens) {
+    check_table(table, table);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(table.device());
+    const int64_t R = table.size(0);
+    TORCH_CHECK(page >= 1, "a page holds at least one token");
+    TORCH_CHECK(tokens >= 0, "tokens must not be negative");
+    check_data(free_pages, "free");
+    TORCH_CHECK(free_pages.scalar_type() == at::kInt && free_pages.dim() == 1 && free_pages.device() == table.device(),
+                "free must be 1-D int32 on the table's device");
+    check_meta(state, "state", table, 2); check_meta(lens, "lens", table, R); check_meta(new_lens, "newLens", table, R);
+    const auto opts = lens.options();
+    Tensor slots = at::empty({tokens}, opts), accum = at::empty({R + 1}, opts), lens_out = at::empty({R}, opts), state_out = at::empty({2}, opts);
+    const size_t bytes = ba_paged_resize_workspace(R);
+    Tensor work;
+    if (bytes) work = at::empty({(int64_t)bytes}, opts.dtype(at::kByte));
+    check_status(ba_paged_resize(table.data_ptr<int32_t>(), table.stride(0), table.size(1), free_pages.data_ptr<int32_t>(), free_pages.numel(),
+                                 state.data_ptr<int64_t>(), lens.data_ptr<int64_t>(), new_lens.data_ptr<int64_t>(), R, page,
+                                 slots.data_ptr<int64_t>(), tokens, accum.data_ptr<int64_t>(), lens_out.data_ptr<int64_t>(),
+                                 state_out.data_ptr<int64_t>(), bytes ? work.data_ptr() : nullptr, bytes, current_stream(table)),
+                 "ba_paged_resize");
+    written(table); written(free_pages);
+    return {slots, accum, lens_out, state_out};
+}
+
+void pagedAppend_op(const Tensor &k, const Tensor &v, const Tensor &k_cache, const Tensor &v_cache, const Tensor &slots,
+                    const OptTensor &k_scale, const OptTensor &v_scale) {
+    const ba_paged_cache c = cache_of(k_cache, v_cache, k_scale, v_scale);
+    check_rows(k, "k", k_cache); check_rows(v, "v", k_cache);
+    check_no_grad({&k, &v, &k_cache, &v_cache}, "pagedAppend");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
+    check_cache_operand(k, "k", c);
+    TORCH_CHECK(k.scalar_type() == v.scalar_type(), "k and v must have the same dtype");
+    const Rows kr = rows_of(k, "k", c.dim), vr = rows_of(v, "v", c.dim);
+    TORCH_CHECK(kr.heads == c.heads && vr.heads == c.heads, "k and v must have the cache's ", c.heads, " heads, got ", kr.heads, " and ", vr.heads);
+    TORCH_CHECK(kr.rows == vr.rows, "k and v disagree on the number of tokens");
+    check_meta(slots, "slots", k_cache, kr.rows);
+    check_status(ba_paged_append(&c, dtype_code(k, "pagedAppend"), k.data_ptr(), kr.head_stride, kr.row_stride, v.data_ptr(),
+                                 vr.head_stride, vr.row_stride, slots.data_ptr<int64_t>(), kr.rows, current_stream(k_cache)),
+                 "ba_paged_append");
+    written(k_cache); written(v_cache);
+}
+
+Tensor pagedAttention_op(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &table, const Tensor &lens,
+                         double scale, int64_t window, const OptTensor &k_scale, const OptTensor &v_scale) {
+    const ba_paged_cache c = cache_of(k_cache, v_cache, k_scale, v_scale);
+    check_rows(q, "q", k_cache);
+    check_table(table, k_cache);
+    check_no_grad({&q, &k_cache, &v_cache}, "pagedAttention");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
+    check_cache_operand(q, "q", c);
+    TORCH_CHECK(window >= 0, "window must not be negative (0: all tokens)");
+    const Rows qr = rows_of(q, "q", c.dim);
+    TORCH_CHECK(qr.heads >= 1 && qr.heads % c.heads == 0, "q must have a multiple of the cache's ", c.heads, " heads, got ", qr.heads);
+    TORCH_CHECK(table.size(0) == qr.rows, "q has ", qr.rows, " rows, table ", table.size(0));
+    check_meta(lens, "lens", k_cache, qr.rows);
+    Tensor out = at::empty_like(q);                          // q's order of dimensions
+    const Rows outr = rows_of(out, "out", c.dim);
+    const size_t bytes = ba_paged_attention_workspace(&c, qr.heads, qr.rows, table.size(1));
+    Tensor work;
+    if (bytes) work = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+    check_status(ba_paged_attention(&c, dtype_code(q, "pagedAttention"), q.data_ptr(), qr.head_stride, qr.row_stride, qr.heads, qr.rows,
+                                    table.data_ptr<int32_t>(), table.stride(0), table.size(1), lens.data_ptr<int64_t>(), window, (float)scale,
+                                    out.data_ptr(), outr.head_stride, outr.row_stride, bytes ? work.data_ptr() : nullptr, bytes,
+                                    current_stream(q)),
+                 "ba_paged_attention");
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -645,6 +785,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("sparseBlockedSoftmaxScaled", &sparseBlockedSoftmaxScaled_op, "sparseBlockedSoftmax with a fused scale");
     m.def("sparseBlockedGEMMSoftmax", &sparseBlockedGEMMSoftmax_op, "fused sparseBlockedGEMM + softmax forward");
     m.def("sparseBlockedAttention", &sparseBlockedAttention_op, "softmax(scale q k^T) v per segment, one pass");
+    m.def("pagedResize", &pagedResize_op, "page tables and slots from the requests' lengths before and after");
+    m.def("pagedAppend", &pagedAppend_op, "keys and values of new tokens into a paged cache, in place");
+    m.def("pagedAttention", &pagedAttention_op, "one query per request over a paged cache");
     m.def("set_schedule_cache", &set_schedule_cache, "number of schedules kept for repeated metadata (0 = off)");
     m.def("schedule_cache_stats", &schedule_cache_stats, "[hits, misses, entries, capacity]");
 }

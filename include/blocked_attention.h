@@ -46,7 +46,8 @@ typedef enum ba_status {
  * (csrc/cuda/spBlkSoftmax.cu:400), the fused pair and the attention BA_F16 / BA_BF16. */
 typedef enum ba_dtype {
     BA_F16 = 0, BA_BF16 = 1, BA_F32 = 2, BA_F64 = 3,
-    BA_U8 = 4, BA_I8 = 5, BA_I16 = 6, BA_I32 = 7, BA_I64 = 8
+    BA_U8 = 4, BA_I8 = 5, BA_I16 = 6, BA_I32 = 7, BA_I64 = 8,
+    BA_F8_E4M3 = 9 /* pages of a paged cache only: 4 exponent and 3 fraction bits, no infinities, +-448 */
 } ba_dtype;
 
 /* Which half of the metadata the caller supplies
@@ -324,6 +325,80 @@ int ba_varlen_gemm_two(int dtype, int64_t H, void *plan_a, const ba_plan_info *i
  * (so not for use under stream capture); after a single-launch call only nseg, Dm1, Dm2, Dout, bad_segments and
  * run_errors of the summary are meaningful.  No counterpart in the reference. */
 int ba_static_read(ba_plan_info *host_info, ba_stream_t stream);
+
+/*
+ * Paged key-value cache: what a program needs that answers a batch of requests token by token, next to the attention
+ * over whole segments above.  No counterpart in the reference, whose operands are whole segments back to back.
+ *
+ * The keys and values of all requests lie in `pages` pages of `page` tokens; a table row gives the pages of a request in
+ * the order of its tokens.  Token t of request r and key head h is the `dim` elements at
+ *     base + page_number * page_stride + h * head_stride + (t % page) * token_stride
+ * (strides in elements, any order of heads and tokens, the last dimension contiguous), page_number = table[r][t / page].
+ * dtype: BA_F16, BA_BF16, or BA_F8_E4M3 with `k_scale` and `v_scale` (fp32, one per head): what is stored times the
+ * head's scale is the value.  dim <= 256; the tokens of a page and head span less than 2^31 bytes.
+ * The structure itself is host memory, the pointers in it are device pointers.
+ */
+typedef struct ba_paged_cache {
+    void *k, *v;
+    const float *k_scale, *v_scale; /* BA_F8_E4M3 only, else NULL */
+    int64_t pages, heads, page, dim;
+    int64_t k_page_stride, k_head_stride, k_token_stride;
+    int64_t v_page_stride, v_head_stride, v_token_stride;
+    int dtype;
+} ba_paged_cache;
+
+/* Verdict of ba_paged_resize, state_out[1]: 0 or a sum of these (1 and 8 only where lengths and state are valid). */
+#define BA_PAGED_NO_PAGES 1   /* more pages needed than are free or given back */
+#define BA_PAGED_ROW_SHORT 2  /* a request needs more pages than a table row holds */
+#define BA_PAGED_BAD_LENGTH 4 /* a length is negative, or one before the call does not fit the row */
+#define BA_PAGED_NO_SLOTS 8   /* more new tokens than `tokens` */
+#define BA_PAGED_BAD_STATE 16 /* state_in's count is negative or, with the pages given back, beyond the stack */
+
+/*
+ * Request r goes from lens[r] to new_lens[r] tokens (int64, 0 = no request): pages change hands, new tokens get places.
+ * `table` is int32 [requests][width] at rows of table_stride entries, `free_pages` a stack of `pool` entries of which
+ * the first state_in[0] are free pages.  Pages that shrinking requests give back are numbered in the order of requests
+ * and columns, and so are pages that growing requests take: the i-th taken page is the i-th given back, beyond those the
+ * free stack from its top down.  What is given back and not taken goes on the stack, the last one first: growing and
+ * shrinking back leaves the stack as it was.
+ * slots[0 .. tokens) gets the places (page * page size + row) of the new tokens, request after request, then -1; accum
+ * (int64 [requests + 1]) their exclusive prefix sums, lens_out the new lengths, state_out (int64 [2]) the free count
+ * and the verdict.  Where the verdict is not 0, nothing has changed hands: table and stack are untouched, all slots are
+ * -1, accum is 0, lens_out = lens, state_out[0] = state_in[0]; a state with a verdict is refused again by the next call, so that a
+ * program may look at the verdict many steps later.  Inputs are not changed: the same call again writes the same.
+ * lens_out must not overlap the inputs.  `workspace`: ba_paged_resize_workspace bytes, 8-byte aligned (NULL where that
+ * is 0).  requests * width and width * page are below 2^31, and so is `tokens`.
+ */
+size_t ba_paged_resize_workspace(int64_t requests);
+int ba_paged_resize(int32_t *table, int64_t table_stride, int64_t width, int32_t *free_pages, int64_t pool,
+                    const int64_t *state_in, const int64_t *lens, const int64_t *new_lens, int64_t requests, int64_t page,
+                    int64_t *slots, int64_t tokens, int64_t *accum, int64_t *lens_out, int64_t *state_out,
+                    void *workspace, size_t workspace_bytes, ba_stream_t stream);
+
+/*
+ * Keys and values of new tokens into their places: token t of k and v ([heads][tokens][dim] by the strides given, in
+ * elements) goes to place slots[t]; places below 0 or past the last page are skipped.  No place may occur twice.
+ * dtype: BA_F16 or BA_BF16, the cache's own or, into a BA_F8_E4M3 cache, either: value / scale, limited to +-448, to
+ * the nearest, ties to even.
+ */
+int ba_paged_append(const ba_paged_cache *cache, int dtype, const void *k, int64_t k_head_stride, int64_t k_token_stride,
+                    const void *v, int64_t v_head_stride, int64_t v_token_stride, const int64_t *slots, int64_t tokens,
+                    ba_stream_t stream);
+
+/*
+ * out[h][r] = sum over t of softmax_t(scale * q[h][r] . K[r][h / group][t]) V[r][h / group][t]: one query per request and
+ * query head, over the request's lens[r] tokens or, with window > 0, the last `window` of them; group = heads / cache
+ * heads query heads share a key head.  Requests without tokens give zeros.  q and out are [heads][requests][dim] by the
+ * strides given (in elements); dtype: BA_F16 or BA_BF16, the cache's own or with a BA_F8_E4M3 cache either.  Sums, row
+ * maxima and the products' accumulators are fp32.  Tokens beyond the table's row do not exist; a page number outside the cache makes
+ * the rows of its request NaN instead of being read.  `workspace`: ba_paged_attention_workspace bytes, 256-byte aligned,
+ * used by this call alone.
+ */
+size_t ba_paged_attention_workspace(const ba_paged_cache *cache, int64_t heads, int64_t requests, int64_t width);
+int ba_paged_attention(const ba_paged_cache *cache, int dtype, const void *q, int64_t q_head_stride, int64_t q_row_stride,
+                       int64_t heads, int64_t requests, const int32_t *table, int64_t table_stride, int64_t width,
+                       const int64_t *lens, int64_t window, float scale, void *out, int64_t out_head_stride,
+                       int64_t out_row_stride, void *workspace, size_t workspace_bytes, ba_stream_t stream);
 
 #ifdef __cplusplus
 }
