@@ -92,7 +92,7 @@ __attribute__((visibility("default"))) int ba_paged_append(const ba_paged_cache 
 
 __attribute__((visibility("default"))) size_t ba_paged_attention_workspace(const ba_paged_cache *cache, int64_t heads,
                                                                            int64_t requests, int64_t width) {
-    if (check_cache(cache) != BA_OK || heads < 1 || heads % cache->heads || requests < 1 || width < 1) return 0;
+    if (check_cache(cache) != BA_OK || heads < 1 || heads % cache->heads || requests < 1 || width < 0) return 0;
     return paged_attention_workspace(cache->heads, heads / cache->heads, cache->dim, requests, width, cache->page);
 }
 
@@ -115,7 +115,7 @@ __attribute__((visibility("default"))) int ba_paged_attention(const ba_paged_cac
     if (requests > 1 && width > 0 && table_stride < width) return BA_ERR_INVALID_ARG;
     if (heads >= (1 << 20) || requests >= kTokenLimit / heads || width >= kTokenLimit / cache->page) return BA_ERR_UNSUPPORTED;
     const size_t need = ba_paged_attention_workspace(cache, heads, requests, width);
-    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))) return BA_ERR_WORKSPACE;
+    if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255)) return BA_ERR_WORKSPACE;
     PagedAttentionArgs a{};
     a.k = array_of(cache, false); a.v = array_of(cache, true);
     a.q = (const char *)q; a.out = (char *)out; a.table = table; a.lens = lens;

@@ -1,79 +1,509 @@
 // Attention of one new query per request over a paged key-value cache.
+//
+// out[h][r] = sum_t softmax_t(scale q[h][r] . K[t]) V[t] over the request's tokens t.  Every key and value is read once and
+// takes part in 4 x group operations a byte pair, so memory traffic is the floor; what the kernel is built for is bytes in
+// flight on every compute unit, whatever the lengths are.
+//
+// Split.  A unit is a request and up to 16 query heads that share a key head.  Its tokens are cut into tiles of 32, and
+// the tiles of all units, in order, are dealt out to the workgroups in equal shares (the lengths are on the GPU only, so
+// every workgroup adds them up itself).  A workgroup goes through its share unit by unit, its four wavefronts taking every
+// fourth tile each; at the end of a unit their results are joined in LDS.  A unit that lies in one share is done
+// then; for others each workgroup leaves its maximum, sum and fp32 accumulators, and a second small kernel joins them.
+//
+// One tile.  Scores: S[token][head] = K Q^T with 16 tokens as the rows of a 16 x 16 x 32 matrix instruction; a lane's
+// operand is 16 bytes of one key, loaded straight from the cache.  A lane then holds the scores of tokens 4g..4g+3 of both
+// halves of the tile for one head (g = lane / 16): packed to 16 bits these are, as they are, its operand of the second
+// product if the reduction runs over the tokens in the order (half, g, i) -- no lane exchanges a probability.  Values: O[d][head]
+// = V^T P.  A lane loads 2 or more adjacent dimensions of its eight tokens (16 lanes cover a row: whole lines) and turns
+// the small matrix in registers: the operand of dimension j is made of the j-th halves of its eight rows.  Nothing of the cache
+// passes through LDS.
+#include <algorithm>
+
 #include "ba_device.hpp"
+#include "ba_host.hpp"
 #include "paged.hpp"
 
 namespace ba {
 
-constexpr int kPagedThreads = 256;
-constexpr int kPagedWaves = kPagedThreads / 64;
+constexpr int kPagedWaves = 4;
+constexpr int kPagedThreads = 64 * kPagedWaves;
+constexpr int kPagedTile = 32;               // tokens
+constexpr int kPagedHeads = 16;              // query heads of a unit at most
+constexpr int kPagedShare = kPagedWaves;     // tiles of a workgroup at least
+constexpr int kPagedWhole = 8;               // units of up to so many tiles are not split between workgroups
 
-template <int DT, bool F8> __device__ __forceinline__ float cache_value(const char *p, int d) {
-    if (F8) return __builtin_amdgcn_cvt_f32_fp8((int)((const uint8_t *)p)[d], 0);
-    return Elem<DT>::to_float(((const uint16_t *)p)[d]);
-}
+// Probabilities are scaled by a power of two that keeps those of 2^-39 (and not 2^-24) of the largest apart from
+// zero in fp16; it is in the sums as well and drops out.
+template <int DT> constexpr float kLift = DT == 0 ? 14.f : 0.f;
 
-// One workgroup per request and query head, a wavefront takes every fourth token, a lane every 64th dimension.
-template <int DT, bool F8> __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(PagedAttentionArgs a) {
-    const int r = (int)blockIdx.x, hq = (int)blockIdx.y, h = hq / a.group;
-    const int lane = lane_id(), wave = (int)threadIdx.x / 64;
-    const int64_t room = (int64_t)a.width * a.page.d, length = a.lens[r];
-    const int len = (int)(length < 0 ? 0 : length < room ? length : room);
-    const int first = a.window && len > a.window ? len - a.window : 0;
-    const uint16_t *q = (const uint16_t *)(a.q + hq * a.q_head_bytes + r * a.q_row_bytes);
-    float qv[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-    const float k_scale = a.scale * kLog2e * (F8 ? a.k.scale[h] : 1.f);
+struct PagedPart {                           // what a workgroup leaves for a unit that others work on too
+    float m, l;
+};
+// Units of which a workgroup does the first tiles and not the last ones: who has to join what.
+struct PagedJoin {
+    int32_t request, unit, first, parts;     // parts 0: nothing to join; first: workgroup
+};
+
+struct PagedWork {
+    PagedJoin *joins;                        // one entry a unit, or a workgroup where there are fewer of those
+    PagedPart *parts;                        // [2 * groups][kPagedHeads]
+    float *sums;                             // [2 * groups][rows][dim]
+    int32_t groups, by_unit, tiles_a_head, rows;   // tiles_a_head: units of a key head; rows: query heads of the largest unit
+};
+
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+typedef uint32_t u32_any __attribute__((aligned(1)));
+typedef uint16_t u16_any __attribute__((aligned(1)));
+
+// N dwords from any address.  FULL: all of them; else the first `bytes` (any number, also none or negative), zeros behind.
+template <int N, bool FULL> __device__ __forceinline__ void load_piece(uint32_t (&x)[N], const char *p, int bytes) {
+    static_assert(N == 1 || N == 2 || N == 4);
+    if (!FULL) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) qv[i] = lane + 64 * i < a.dim ? Elem<DT>::to_float(q[lane + 64 * i]) : 0.f;
-    for (int t = first + wave; t < len; t += kPagedWaves) {
-        const uint32_t c = a.page.div((uint32_t)t), row = (uint32_t)t - c * a.page.d;
-        const int32_t page = a.table[r * a.table_stride + c];
-        if (page < 0 || page >= a.pages) { l = NAN; continue; }
-        const char *k = a.k.base + page * a.k.page_bytes + h * a.k.head_bytes + (int64_t)row * a.k.token_bytes;
-        const char *v = a.v.base + page * a.v.page_bytes + h * a.v.head_bytes + (int64_t)row * a.v.token_bytes;
-        float s = 0.f;
+        for (int i = 0; i < N; ++i) x[i] = 0;
+        if (bytes < 4 * N) {
+            if (bytes <= 0) return;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 64 * i < a.dim) s += qv[i] * cache_value<DT, F8>(k, lane + 64 * i);
-        s = wave_sum(s) * k_scale;
-        const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top;
-        const float shrink = exp2f(m - base), p = exp2f(s - base);
-        l = l * shrink + p;
-        m = top;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            o[i] *= shrink;
-            if (lane + 64 * i < a.dim) o[i] += p * cache_value<DT, F8>(v, lane + 64 * i);
+            for (int i = 0; i < N; ++i) {
+                const int left = bytes - 4 * i;
+                if (left >= 4) x[i] = *(const u32_any *)(p + 4 * i);
+                else if (left >= 2) x[i] = *(const u16_any *)(p + 4 * i) | (left == 3 ? (uint32_t)*(const uint8_t *)(p + 4 * i + 2) << 16 : 0u);
+                else if (left == 1) x[i] = *(const uint8_t *)(p + 4 * i);
+            }
+            return;
         }
     }
-    __shared__ float sm[kPagedWaves], sl[kPagedWaves], so[kPagedWaves][256];
-    if (lane == 0) { sm[wave] = m; sl[wave] = l; }
+    if (N == 4) {
+        const u32x4_any v = *(const u32x4_any *)p;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) so[wave][lane + 64 * i] = o[i];
-    __syncthreads();
-    const int d = (int)threadIdx.x;
-    if (d >= a.dim) return;
-    float top = -INFINITY, sum = 0.f, total = 0.f;
-    for (int w = 0; w < kPagedWaves; ++w) top = fmaxf(top, sm[w]);
-    const float base = top == -INFINITY ? 0.f : top;
-    for (int w = 0; w < kPagedWaves; ++w) {
-        const float f = exp2f(sm[w] - base);
-        sum += sl[w] * f;
-        total += so[w][d] * f;
+        for (int i = 0; i < N; ++i) x[i] = v[i];
+    } else if (N == 2) {
+        const u32x2_any v = *(const u32x2_any *)p;
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = v[i];
+    } else {
+        x[0] = *(const u32_any *)p;
     }
-    uint16_t *out = (uint16_t *)(a.out + hq * a.out_head_bytes + r * a.out_row_bytes);
-    out[d] = Elem<DT>::from_float(len > first ? total * (F8 ? a.v.scale[h] : 1.f) / sum : 0.f);
 }
 
-size_t paged_attention_workspace(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) { return 0; }
+// Two e4m3 values (HI: the upper two bytes) as two 16-bit numbers: exact in either type.
+template <int DT, bool HI> __device__ __forceinline__ uint32_t widen(uint32_t x) {
+    if (DT == 0) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)x, 1.f, HI));
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)x, 1.f, HI));
+}
 
-int launch_paged_attention(const PagedAttentionArgs &a, int dtype, int cache_dtype, void *, hipStream_t stream) {
-    const dim3 grid((unsigned)a.requests, (unsigned)(a.heads * a.group));
-    const bool f8 = cache_dtype == BA_F8_E4M3;
-    if (dtype == BA_F16 && !f8) paged_attention_kernel<0, false><<<grid, kPagedThreads, 0, stream>>>(a);
-    else if (dtype == BA_F16) paged_attention_kernel<0, true><<<grid, kPagedThreads, 0, stream>>>(a);
-    else if (!f8) paged_attention_kernel<1, false><<<grid, kPagedThreads, 0, stream>>>(a);
-    else paged_attention_kernel<1, true><<<grid, kPagedThreads, 0, stream>>>(a);
+struct Visible {
+    int first, len;                          // tokens first .. len - 1 are seen
+    __device__ __forceinline__ int start() const { return first & ~(kPagedTile - 1); }
+    // a request without tokens has one tile: its zeros are written by whoever gets it
+    __device__ __forceinline__ int tiles() const { return len > first ? (len - start() + kPagedTile - 1) / kPagedTile : 1; }
+};
+__device__ __forceinline__ Visible visible(const PagedAttentionArgs &a, int r) {
+    const int64_t room = (int64_t)a.width * a.page.d, length = a.lens[r];
+    const int len = (int)(length < 0 ? 0 : length < room ? length : room);
+    return {a.window && len > a.window ? len - a.window : 0, len};
+}
+
+// Position of the tile that the share of a workgroup begins with: request, unit of the request, tile of the unit.
+struct Place {
+    int request, unit, tile;
+    int64_t at;                              // number of the tile in the order of all
+};
+
+// DC: dimensions that the registers hold (64, 128, 256), FULL: dim == DC; P16: pages are whole halves of tiles.
+template <int DT, bool F8, int DC, bool FULL, bool P16>
+__global__ void __launch_bounds__(kPagedThreads, DC == 64 ? 4 : DC == 128 ? 3 : 2)
+paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
+    constexpr int EB = F8 ? 1 : 2;           // bytes of an element
+    constexpr int KK = DC / 32;              // matrix instructions of a half's scores
+    constexpr int KL = KK * EB / 2;          // 16-byte pieces of a key that a lane holds
+    constexpr int PW = DC / 16;              // dimensions of a value that a lane holds
+    constexpr int VN = PW * EB / 4 > 4 ? 4 : PW * EB / 4;      // dwords of one load of them
+    constexpr int VL = PW * EB / 4 / VN;     // loads
+    const int lane = lane_id(), l16 = lane & 15, g = lane >> 4, wave = uniform((int)threadIdx.x >> 6);
+    const int units = a.heads * w.tiles_a_head;
+
+    extern __shared__ float lds[];           // [waves][rows][dim + 4], then the scan's and the waves' m and l
+    __shared__ int64_t scan[kPagedWaves];
+    __shared__ Place places[2];
+    __shared__ float wave_m[kPagedWaves][kPagedHeads], wave_l[kPagedWaves][kPagedHeads];
+
+    // ---- the share.  Thread i adds up the tiles of requests [i c, (i + 1) c).
+    const int c = (a.requests + kPagedThreads - 1) / kPagedThreads, r0 = (int)threadIdx.x * c;
+    const int r1 = min(a.requests, r0 + c);
+    int64_t mine = 0;
+    for (int r = r0; r < r1; ++r) mine += visible(a, r).tiles();
+    int64_t upto = wave_inclusive_scan(mine);
+    if (lane == 63) scan[wave] = upto;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int i = 0; i < kPagedWaves; ++i) {
+        if (i < wave) upto += scan[i];
+        total += scan[i];
+    }
+    total *= units;
+    const int64_t groups = min((int64_t)w.groups, (total + kPagedShare - 1) / kPagedShare);
+    const int64_t group = blockIdx.x;
+    if (group >= groups) {
+        if (!w.by_unit && threadIdx.x == 0) w.joins[group].parts = 0;
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        int64_t at = (group + k) * total / groups;
+        if (at >= total) {
+            if (threadIdx.x == 0) places[k] = {a.requests, 0, 0, total};
+        } else if (at < upto * units && at >= (upto - mine) * units) {
+            int64_t before = (upto - mine) * units;
+            int r = r0, n = visible(a, r).tiles();
+            while (at >= before + (int64_t)n * units) {
+                before += (int64_t)n * units;
+                n = visible(a, ++r).tiles();
+            }
+            int unit = (int)((at - before) / n), tile = (int)((at - before) - (int64_t)unit * n);
+            if (n <= kPagedWhole && tile) {                    // short units go where most of them lies
+                at -= tile;
+                if (2 * tile > n) {
+                    at += n;
+                    if (++unit == units) { unit = 0; ++r; }
+                }
+                tile = 0;
+            }
+            places[k] = {r, unit, tile, at};
+        }
+    }
+    __syncthreads();
+    int request = uniform(places[0].request), unit = uniform(places[0].unit), tile = uniform(places[0].tile);
+    int64_t at = uniform64(places[0].at);
+    const int64_t end = uniform64(places[1].at);
+    PagedJoin join = {0, 0, 0, 0};
+
+    while (at < end) {
+        const Visible see = visible(a, request);
+        const int first = uniform(see.first), len = uniform(see.len), n = uniform(see.tiles()), start = uniform(see.start());
+        const int last = (int)min((int64_t)n, tile + (end - at));      // tiles of this unit in this share: [tile, last)
+        const int h = unit / w.tiles_a_head, q0 = h * a.group + (unit - h * w.tiles_a_head) * w.rows;
+        const int rows = min(w.rows, (h + 1) * a.group - q0);
+        const char *const kh = a.k.base + h * a.k.head_bytes, *const vh = a.v.base + h * a.v.head_bytes;
+        typedef const __attribute__((address_space(4))) int32_t *Row;
+        const Row row = (Row)(uintptr_t)(a.table + request * a.table_stride);
+
+        // queries: head l16 in the order of dimensions in which the keys arrive
+        u32x4 qf[KK];
+#pragma unroll
+        for (int i = 0; i < KK; ++i) {
+            const int d = F8 ? 64 * (i / 2) + 16 * g + 8 * (i % 2) : 32 * i + 8 * g;
+            uint32_t x[4] = {0, 0, 0, 0};
+            if (l16 < rows) load_piece<4, FULL>(x, a.q + (q0 + l16) * a.q_head_bytes + request * a.q_row_bytes + 2 * d, 2 * (a.dim - d));
+            qf[i] = u32x4{x[0], x[1], x[2], x[3]};
+        }
+        const float to_log2 = a.scale * kLog2e * (F8 ? a.k.scale[h] : 1.f);
+
+        f32x4 o[PW];
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int j = 0; j < PW; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+        for (int s = tile + wave; s < last && len > first; s += kPagedWaves) {
+            const int t0 = start + s * kPagedTile;
+            // ---- where the keys and values of the tile lie
+            const char *kp[2], *vp[8];
+            bool bad;
+            if (P16) {
+                // a half without a token that is seen borrows the other one's page
+                int ta = t0, tb = t0 + 16;
+                if (tb >= len) tb = ta;
+                if (ta + 16 <= first) ta = tb;
+                const uint32_t ca = a.page.div((uint32_t)ta), cb = a.page.div((uint32_t)tb);
+                const int32_t pa = uniform(row[ca]), pb = uniform(row[cb]);
+                bad = (uint32_t)pa >= (uint32_t)a.pages || (uint32_t)pb >= (uint32_t)a.pages;
+                const int32_t ra = ta - (int)(ca * a.page.d), rb = tb - (int)(cb * a.page.d);
+                const char *const ka = kh + pa * a.k.page_bytes + (int64_t)ra * a.k.token_bytes;
+                const char *const kb = kh + pb * a.k.page_bytes + (int64_t)rb * a.k.token_bytes;
+                const char *const va = vh + pa * a.v.page_bytes + (int64_t)ra * a.v.token_bytes;
+                const char *const vb = vh + pb * a.v.page_bytes + (int64_t)rb * a.v.token_bytes;
+                kp[0] = ka + (uint32_t)(l16 * a.k.token_bytes); kp[1] = kb + (uint32_t)(l16 * a.k.token_bytes);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    vp[i] = va + (uint32_t)((4 * g + i) * a.v.token_bytes);
+                    vp[4 + i] = vb + (uint32_t)((4 * g + i) * a.v.token_bytes);
+                }
+            } else {
+                // token by token; one that is not seen borrows a neighbour's place
+                const int t = min(max(t0 + (lane & 31), first), len - 1);
+                const uint32_t col = a.page.div((uint32_t)t);
+                const int32_t page = a.table[request * a.table_stride + col], line = t - (int)(col * a.page.d);
+                bad = __any((uint32_t)page >= (uint32_t)a.pages);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int from = 16 * i + l16;
+                    kp[i] = kh + __shfl(page, from) * a.k.page_bytes + (int64_t)__shfl(line, from) * a.k.token_bytes;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int from = 16 * (i / 4) + 4 * g + i % 4;
+                    vp[i] = vh + __shfl(page, from) * a.v.page_bytes + (int64_t)__shfl(line, from) * a.v.token_bytes;
+                }
+            }
+            if (bad) { l = NAN; continue; }
+            uint32_t kx[2][KL][4], vx[8][VL][VN];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int k = 0; k < KL; ++k) {
+                    const int b = 64 * k + 16 * g;
+                    load_piece<4, FULL>(kx[i][k], kp[i] + b, EB * a.dim - b);
+                }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int k = 0; k < VL; ++k) {
+                    const int b = EB * PW * l16 + 16 * k;
+                    load_piece<VN, FULL>(vx[i][k], vp[i] + b, EB * a.dim - b);
+                }
+
+            // ---- scores of tokens t0 + 16 i + 4 g + e
+            f32x4 sc[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                sc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < KL; ++k) {
+                    if (F8) {
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const uint32_t x = kx[i][k][2 * half], y = kx[i][k][2 * half + 1];
+                            sc[i] = Elem<DT>::mfma(u32x4{widen<DT, false>(x), widen<DT, true>(x), widen<DT, false>(y), widen<DT, true>(y)},
+                                                   qf[(2 * k + half) % KK], sc[i]);
+                        }
+                    } else {
+                        sc[i] = Elem<DT>::mfma(u32x4{kx[i][k][0], kx[i][k][1], kx[i][k][2], kx[i][k][3]}, qf[k % KK], sc[i]);
+                    }
+                }
+                sc[i] *= to_log2;
+            }
+            if (t0 < first || t0 + kPagedTile > len) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int t = t0 + 16 * (i / 4) + 4 * g + i % 4;
+                    const bool seen = t >= first && t < len;
+                    sc[i / 4][i % 4] = seen ? sc[i / 4][i % 4] : -INFINITY;
+#pragma unroll
+                    for (int k = 0; k < VL; ++k)
+#pragma unroll
+                        for (int x = 0; x < VN; ++x) vx[i][k][x] = seen ? vx[i][k][x] : 0u;    // (a probability of 0 times what lies there may be NaN)
+                }
+            }
+            float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                              fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+            top = fmaxf(m, quad_column_max(top));
+            const float base = (top == -INFINITY ? 0.f : top) - kLift<DT>;
+            if (__any(top != m)) {
+                const float shrink = __builtin_amdgcn_exp2f(m - kLift<DT> - base);
+                l *= shrink;
+#pragma unroll
+                for (int j = 0; j < PW; ++j) o[j] *= shrink;
+                m = top;
+            }
+            float p[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                p[i] = __builtin_amdgcn_exp2f(sc[i / 4][i % 4] - base);
+                l += p[i];
+            }
+            // Probabilities in two 16-bit terms: one alone would cost as much accuracy as the rounding of the result, and the
+            // matrix unit has time to spare.
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                hi[i] = Elem<DT>::pack2(p[2 * i], p[2 * i + 1]);
+                lo[i] = Elem<DT>::pack2(p[2 * i] - Elem<DT>::to_float((uint16_t)hi[i]), p[2 * i + 1] - Elem<DT>::to_float((uint16_t)(hi[i] >> 16)));
+            }
+            // ---- values
+#pragma unroll
+            for (int j = 0; j < PW; ++j) {
+                uint32_t f[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (F8) {
+                        // byte j of both rows next to each other, then widened together
+                        const uint32_t both = __builtin_amdgcn_perm(vx[2 * i + 1][j / 4 / VN][j / 4 % VN], vx[2 * i][j / 4 / VN][j / 4 % VN],
+                                                                    0x0c0c0400u + (uint32_t)(j % 4) * 0x0101u);
+                        f[i] = widen<DT, false>(both);
+                    } else {
+                        f[i] = __builtin_amdgcn_perm(vx[2 * i + 1][j / 2 / VN][j / 2 % VN], vx[2 * i][j / 2 / VN][j / 2 % VN],
+                                                     j % 2 ? 0x07060302u : 0x05040100u);
+                    }
+                }
+                const u32x4 v = {f[0], f[1], f[2], f[3]};
+                o[j] = Elem<DT>::mfma(v, u32x4{hi[0], hi[1], hi[2], hi[3]}, o[j]);
+                o[j] = Elem<DT>::mfma(v, u32x4{lo[0], lo[1], lo[2], lo[3]}, o[j]);
+            }
+        }
+
+        // ---- join the wavefronts: lane (g, l16) has dimensions PW (4 g + i) + j of head l16
+        const int pitch = a.dim + 4;
+        const int busy = min(last - tile, kPagedWaves);
+        l = quad_column_sum(l);
+        if (wave < busy) {
+            if (g == 0) { wave_m[wave][l16] = m; wave_l[wave][l16] = l; }
+            if (l16 < rows) {
+                float *const mineo = lds + (wave * w.rows + l16) * pitch;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < PW; ++j)
+                        if (FULL || PW * (4 * g + i) + j < a.dim) mineo[PW * (4 * g + i) + j] = o[j][i];
+            }
+        }
+        __syncthreads();
+        const bool begun = tile == 0, done = last == n, whole = begun && done;
+        const int slot = 2 * (int)group + (begun ? 1 : 0);
+        for (int x = (int)threadIdx.x; x < rows * a.dim; x += kPagedThreads) {
+            const int hd = x / a.dim, d = x - hd * a.dim;
+            float top = -INFINITY, sum = 0.f, acc = 0.f;
+            for (int i = 0; i < busy; ++i) top = fmaxf(top, wave_m[i][hd]);
+            const float base = top == -INFINITY ? 0.f : top;
+            for (int i = 0; i < busy; ++i) {
+                const float f = __builtin_amdgcn_exp2f(wave_m[i][hd] - base);
+                sum += f * wave_l[i][hd];
+                acc += f * lds[(i * w.rows + hd) * pitch + d];
+            }
+            if (whole) {
+                const float v = len > first ? acc * (F8 ? a.v.scale[h] : 1.f) / sum : 0.f;
+                ((uint16_t *)(a.out + (q0 + hd) * a.out_head_bytes + request * a.out_row_bytes))[d] = Elem<DT>::from_float(v);
+            } else {
+                w.sums[((int64_t)slot * w.rows + hd) * a.dim + d] = acc;
+                if (d == 0) w.parts[slot * kPagedHeads + hd] = {top, sum};
+            }
+        }
+        if (begun) {
+            // who has the unit's last tile
+            const int parts = done ? 0 : (int)(((at - tile + n) * groups + total - 1) / total - group);
+            join = {request, unit, (int)group, parts};
+            if (w.by_unit && threadIdx.x == 0) w.joins[(int64_t)request * units + unit] = join;
+        }
+        at += last - tile;
+        tile = 0;
+        if (++unit == units) { unit = 0; ++request; }
+        __syncthreads();
+    }
+    if (!w.by_unit && threadIdx.x == 0) w.joins[group] = join;
+}
+
+// One workgroup per unit that was split (entry of the list) and query head.
+template <int DT> __global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(PagedAttentionArgs a, PagedWork w) {
+    const PagedJoin join = w.joins[blockIdx.x];
+    const int h = join.unit / w.tiles_a_head, q = h * a.group + (join.unit - h * w.tiles_a_head) * w.rows + (int)blockIdx.y;
+    if (join.parts == 0 || q >= (h + 1) * a.group || (int)blockIdx.y >= w.rows) return;
+    extern __shared__ float lds[];           // factor of each part, then the partial sums of the rows of threads
+    __shared__ float wave_x[kPagedWaves];
+    const int lane = lane_id(), wave = (int)threadIdx.x >> 6;
+    auto slot = [&](int p) { return 2 * (int64_t)(join.first + p) + (p == 0 ? 1 : 0); };
+    float top = -INFINITY;
+    for (int p = (int)threadIdx.x; p < join.parts; p += kPagedThreads) top = fmaxf(top, w.parts[slot(p) * kPagedHeads + blockIdx.y].m);
+    top = wave_max(top);
+    if (lane == 0) wave_x[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPagedWaves; ++i) top = fmaxf(top, wave_x[i]);
+    __syncthreads();
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    for (int p = (int)threadIdx.x; p < join.parts; p += kPagedThreads) {
+        const PagedPart x = w.parts[slot(p) * kPagedHeads + blockIdx.y];
+        const float f = __builtin_amdgcn_exp2f(x.m - base);
+        lds[p] = f;
+        sum += f * x.l;
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) wave_x[wave] = sum;
+    __syncthreads();
+    sum = wave_x[0] + wave_x[1] + wave_x[2] + wave_x[3];
+    // threads [i * wide, (i + 1) * wide) add every `deep`-th part
+    const int wide = a.dim > 128 ? 256 : a.dim > 64 ? 128 : 64, deep = kPagedThreads / wide;
+    const int d = (int)threadIdx.x % wide, i = (int)threadIdx.x / wide;
+    float acc = 0.f;
+    if (d < a.dim)
+#pragma unroll 4
+        for (int p = i; p < join.parts; p += deep) acc += lds[p] * w.sums[(slot(p) * w.rows + blockIdx.y) * a.dim + d];
+    float *const rest = lds + join.parts;
+    rest[threadIdx.x] = acc;
+    __syncthreads();
+    if (i || d >= a.dim) return;
+    for (int k = 1; k < deep; ++k) acc += rest[k * wide + d];
+    const float v = acc * (a.v.scale ? a.v.scale[h] : 1.f) / sum;
+    ((uint16_t *)(a.out + q * a.out_head_bytes + join.request * a.out_row_bytes))[d] = Elem<DT>::from_float(v);
+}
+
+// ------------------------------------------------------------------ host
+static int dim_class(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+// Workgroups: as many as are resident, or fewer where the longest possible requests would not give each its least share.
+static PagedWork work_of(int64_t heads, int64_t group, int64_t dim, int64_t requests, int64_t width, int64_t page, void *workspace, size_t *bytes) {
+    PagedWork w{};
+    w.tiles_a_head = (int32_t)((group + kPagedHeads - 1) / kPagedHeads);
+    w.rows = (int32_t)((group + w.tiles_a_head - 1) / w.tiles_a_head);
+    const int64_t resident = (int64_t)device_cu_count() * (dim_class(dim) == 64 ? 4 : dim_class(dim) == 128 ? 3 : 2);
+    const int64_t units = requests * heads * w.tiles_a_head;
+    const double tiles = (double)units * ((double)width * page / kPagedTile + 1);
+    w.groups = (int32_t)std::max<int64_t>(1, (int64_t)std::min<double>((double)resident, tiles / kPagedShare + 1));
+    w.by_unit = units <= w.groups;
+    const size_t entries = (size_t)(w.by_unit ? units : w.groups);
+    const size_t joins = (entries * sizeof(PagedJoin) + 255) & ~size_t(255);
+    const size_t parts = (2 * (size_t)w.groups * kPagedHeads * sizeof(PagedPart) + 255) & ~size_t(255);
+    const size_t sums = 2 * (size_t)w.groups * w.rows * dim * sizeof(float);
+    if (bytes) *bytes = joins + parts + sums;
+    if (workspace) {
+        w.joins = (PagedJoin *)workspace;
+        w.parts = (PagedPart *)((char *)workspace + joins);
+        w.sums = (float *)((char *)workspace + joins + parts);
+    }
+    return w;
+}
+
+size_t paged_attention_workspace(int64_t heads, int64_t group, int64_t dim, int64_t requests, int64_t width, int64_t page) {
+    size_t bytes = 0;
+    work_of(heads, group, dim, requests, width, page, nullptr, &bytes);
+    return bytes;
+}
+
+template <int DT, bool F8, int DC, bool FULL, bool P16>
+static int launch_split(const PagedAttentionArgs &a, const PagedWork &w, size_t lds, hipStream_t stream) {
+    constexpr int kMostLds = kPagedWaves * kPagedHeads * (DC + 4) * (int)sizeof(float);
+    if constexpr (kMostLds > 65536) {
+        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&paged_attention_kernel<DT, F8, DC, FULL, P16>),
+                                                           hipFuncAttributeMaxDynamicSharedMemorySize, kMostLds);
+        if (attr != hipSuccess) return BA_ERR_LAUNCH;
+    }
+    paged_attention_kernel<DT, F8, DC, FULL, P16><<<w.groups, kPagedThreads, lds, stream>>>(a, w);
+    return BA_OK;
+}
+
+template <int DT, bool F8, int DC, bool FULL> static int launch_class(const PagedAttentionArgs &a, const PagedWork &w, hipStream_t stream) {
+    const size_t lds = (size_t)kPagedWaves * w.rows * (a.dim + 4) * sizeof(float);
+    const int st = a.page.d % 16 == 0 ? launch_split<DT, F8, DC, FULL, true>(a, w, lds, stream) : launch_split<DT, F8, DC, FULL, false>(a, w, lds, stream);
+    if (st != BA_OK) return st;
+    const dim3 grid((unsigned)(w.by_unit ? a.requests * a.heads * w.tiles_a_head : w.groups), (unsigned)w.rows);
+    paged_join_kernel<DT><<<grid, kPagedThreads, (w.groups + kPagedThreads) * sizeof(float), stream>>>(a, w);
     return hipGetLastError() == hipSuccess ? BA_OK : BA_ERR_LAUNCH;
+}
+
+template <int DT, bool F8> static int launch_dtype(const PagedAttentionArgs &a, const PagedWork &w, hipStream_t stream) {
+    switch (dim_class(a.dim)) {
+        case 64: return a.dim == 64 ? launch_class<DT, F8, 64, true>(a, w, stream) : launch_class<DT, F8, 64, false>(a, w, stream);
+        case 128: return a.dim == 128 ? launch_class<DT, F8, 128, true>(a, w, stream) : launch_class<DT, F8, 128, false>(a, w, stream);
+        default: return a.dim == 256 ? launch_class<DT, F8, 256, true>(a, w, stream) : launch_class<DT, F8, 256, false>(a, w, stream);
+    }
+}
+
+int launch_paged_attention(const PagedAttentionArgs &a, int dtype, int cache_dtype, void *workspace, hipStream_t stream) {
+    const PagedWork w = work_of(a.heads, a.group, a.dim, a.requests, a.width, a.page.d, workspace, nullptr);
+    const bool f8 = cache_dtype == BA_F8_E4M3;
+    if (dtype == BA_F16) return f8 ? launch_dtype<0, true>(a, w, stream) : launch_dtype<0, false>(a, w, stream);
+    return f8 ? launch_dtype<1, true>(a, w, stream) : launch_dtype<1, false>(a, w, stream);
 }
 
 }  // namespace ba
