@@ -41,8 +41,7 @@ using namespace ba;
 extern "C" {
 
 __attribute__((visibility("default"))) size_t ba_paged_resize_workspace(int64_t requests) {
-    (void)requests;
-    return 0;
+    return paged_tables_workspace(requests);
 }
 
 __attribute__((visibility("default"))) int ba_paged_resize(int32_t *table, int64_t table_stride, int64_t width,

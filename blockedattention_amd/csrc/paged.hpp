@@ -62,6 +62,43 @@ struct PagedAttentionArgs {
     PageDiv page;
 };
 
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+typedef uint32_t u32_any __attribute__((aligned(1)));
+typedef uint16_t u16_any __attribute__((aligned(1)));
+
+// N dwords from any address.  FULL: all of them; else the first `bytes` (any number, also none or negative), zeros behind.
+template <int N, bool FULL> __device__ __forceinline__ void load_piece(uint32_t (&x)[N], const char *p, int bytes) {
+    static_assert(N == 1 || N == 2 || N == 4);
+    if (!FULL) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = 0;
+        if (bytes < 4 * N) {
+            if (bytes <= 0) return;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int left = bytes - 4 * i;
+                if (left >= 4) x[i] = *(const u32_any *)(p + 4 * i);
+                else if (left >= 2) x[i] = *(const u16_any *)(p + 4 * i) | (left == 3 ? (uint32_t)*(const uint8_t *)(p + 4 * i + 2) << 16 : 0u);
+                else if (left == 1) x[i] = *(const uint8_t *)(p + 4 * i);
+            }
+            return;
+        }
+    }
+    if (N == 4) {
+        const u32x4_any v = *(const u32x4_any *)p;
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = v[i];
+    } else if (N == 2) {
+        const u32x2_any v = *(const u32x2_any *)p;
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = v[i];
+    } else {
+        x[0] = *(const u32_any *)p;
+    }
+}
+
+size_t paged_tables_workspace(int64_t requests);
 int launch_paged_tables(const PagedTablesArgs &args, void *workspace, hipStream_t stream);
 int launch_paged_append(const PagedAppendArgs &args, int dtype, int cache_dtype, hipStream_t stream);
 size_t paged_attention_workspace(int64_t cache_heads, int64_t group, int64_t dim, int64_t requests, int64_t width, int64_t page);

@@ -1,4 +1,7 @@
-// Keys and values of new tokens into the pages of a cache, in 16 bits or rounded to 8 (e4m3).
+// Keys and values of new tokens into the pages of a cache, in 16 bits or rounded to 8 (e4m3).  A copy: what it reads and
+// writes is its floor.  A thread takes pieces of eight elements (16 bytes of the source); within a workgroup the
+// pieces follow each other as they lie in the cache -- the tokens of a head or the heads of a token, whichever are closer --
+// so that adjacent lanes write whole lines.
 #include <algorithm>
 
 #include "ba_device.hpp"
@@ -7,34 +10,95 @@
 namespace ba {
 
 constexpr int kAppendThreads = 256;
+constexpr int kAppendPieces = 4;             // of a thread, their loads in flight together
+constexpr int kPieceElems = 8;
 
-// One element a thread, grid (elements of a token, tokens, keys or values).
-template <int DT, bool F8> __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedAppendArgs a) {
-    const int i = (int)(blockIdx.x * kAppendThreads + threadIdx.x), which = (int)blockIdx.z;
-    const int h = i / a.dim, d = i - h * a.dim;
-    if (h >= a.heads) return;
-    for (int64_t t = blockIdx.y; t < a.tokens; t += gridDim.y) {
-        const int64_t slot = a.slots[t];
-        if (slot < 0 || slot >= a.places) continue;
-        const uint32_t page = a.page.div((uint32_t)slot), row = (uint32_t)slot - page * a.page.d;
-        const PagedArray &to = a.to[which];
-        char *dst = to.base + page * to.page_bytes + h * to.head_bytes + (int64_t)row * to.token_bytes;
-        const uint16_t x = ((const uint16_t *)(a.from[which] + h * a.from_head_bytes[which] + t * a.from_token_bytes[which]))[d];
-        if (F8) {
-            float y = Elem<DT>::to_float(x) / to.scale[h];
-            y = y > 448.f ? 448.f : y < -448.f ? -448.f : y;      // (a NaN stays one)
-            ((uint8_t *)dst)[d] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false);
+struct AppendShape {
+    PageDiv per_token, per_row;              // pieces of a token in one workgroup's order, of a row
+    int32_t tokens, heads_inner;             // tokens of a workgroup; whether it takes all heads of them
+};
+
+template <int DT, bool F8, bool WHOLE> __device__ __forceinline__ void store_piece(char *dst, const uint32_t (&x)[4], float scale, int left) {
+    if (F8) {
+        uint32_t y[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float lo = Elem<DT>::to_float((uint16_t)x[i]) / scale, hi = Elem<DT>::to_float((uint16_t)(x[i] >> 16)) / scale;
+            lo = lo > 448.f ? 448.f : lo < -448.f ? -448.f : lo;      // (a NaN stays one)
+            hi = hi > 448.f ? 448.f : hi < -448.f ? -448.f : hi;
+            if (i % 2) y[i / 2] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, (int)y[i / 2], true);
+            else y[i / 2] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, (int)y[i / 2], false);
+        }
+        if (WHOLE || left >= kPieceElems) {
+            *(u32x2_any *)dst = u32x2_any{y[0], y[1]};
         } else {
-            ((uint16_t *)dst)[d] = x;
+#pragma unroll
+            for (int i = 0; i < kPieceElems - 1; ++i)
+                if (i < left) ((uint8_t *)dst)[i] = (uint8_t)(y[i / 4] >> (8 * (i % 4)));
+        }
+    } else if (WHOLE || left >= kPieceElems) {
+        *(u32x4_any *)dst = u32x4_any{x[0], x[1], x[2], x[3]};
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPieceElems - 1; ++i)
+            if (i < left) ((u16_any *)dst)[i] = (uint16_t)(x[i / 2] >> (16 * (i % 2)));
+    }
+}
+
+// Grid (tokens, heads or 1, keys and values).  WHOLE: rows are whole pieces.
+template <int DT, bool F8, bool WHOLE> __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedAppendArgs a, AppendShape s) {
+    const int which = (int)blockIdx.z;
+    const int64_t t0 = (int64_t)blockIdx.x * s.tokens;
+    const uint32_t most = (uint32_t)(min((int64_t)s.tokens, a.tokens - t0) * s.per_token.d);
+    for (uint32_t i0 = threadIdx.x; i0 < most; i0 += kAppendPieces * kAppendThreads) {
+        int64_t slot[kAppendPieces];
+        int head[kAppendPieces], at[kAppendPieces];
+        uint32_t x[kAppendPieces][4];
+#pragma unroll
+        for (int k = 0; k < kAppendPieces; ++k) {
+            const uint32_t i = i0 + k * kAppendThreads;
+            slot[k] = -1;
+            if (i < most) {
+                const uint32_t t = s.per_token.div(i), rest = i - t * s.per_token.d, row = s.per_row.div(rest);
+                head[k] = s.heads_inner ? (int)row : (int)blockIdx.y;
+                at[k] = (int)(rest - row * s.per_row.d) * kPieceElems;
+                slot[k] = a.slots[t0 + t];
+                const char *const src = a.from[which] + head[k] * a.from_head_bytes[which] + (t0 + t) * a.from_token_bytes[which] + 2 * at[k];
+                load_piece<4, WHOLE>(x[k], src, 2 * (a.dim - at[k]));
+            }
+        }
+        const PagedArray &to = a.to[which];
+#pragma unroll
+        for (int k = 0; k < kAppendPieces; ++k) {
+            if (slot[k] < 0 || slot[k] >= a.places) continue;
+            const uint32_t page = a.page.div((uint32_t)slot[k]), row = (uint32_t)slot[k] - page * a.page.d;
+            char *const dst = to.base + page * to.page_bytes + head[k] * to.head_bytes + (int64_t)row * to.token_bytes + (F8 ? 1 : 2) * at[k];
+            store_piece<DT, F8, WHOLE>(dst, x[k], F8 ? to.scale[head[k]] : 1.f, a.dim - at[k]);
         }
     }
 }
 
+template <int DT, bool F8> static void launch_append(const PagedAppendArgs &a, const AppendShape &s, dim3 grid, hipStream_t stream) {
+    if (a.dim % kPieceElems == 0) paged_append_kernel<DT, F8, true><<<grid, kAppendThreads, 0, stream>>>(a, s);
+    else paged_append_kernel<DT, F8, false><<<grid, kAppendThreads, 0, stream>>>(a, s);
+}
+
 int launch_paged_append(const PagedAppendArgs &a, int dtype, int cache_dtype, hipStream_t stream) {
-    const dim3 grid((unsigned)((a.heads * a.dim + kAppendThreads - 1) / kAppendThreads), (unsigned)std::min<int64_t>(a.tokens, 65535), 2);
-    if (cache_dtype != BA_F8_E4M3) paged_append_kernel<0, false><<<grid, kAppendThreads, 0, stream>>>(a);
-    else if (dtype == BA_F16) paged_append_kernel<0, true><<<grid, kAppendThreads, 0, stream>>>(a);
-    else paged_append_kernel<1, true><<<grid, kAppendThreads, 0, stream>>>(a);
+    const uint32_t row = (uint32_t)(a.dim + kPieceElems - 1) / kPieceElems;
+    AppendShape s;
+    s.heads_inner = a.to[0].head_bytes < a.to[0].token_bytes || a.heads > 65535;
+    s.per_row = PageDiv::of(row);
+    s.per_token = PageDiv::of(s.heads_inner ? row * a.heads : row);
+    // one round of pieces for every thread, or a token if that is more; fewer where the call is small and would otherwise
+    // leave compute units idle
+    int64_t tokens = std::max<int64_t>(1, kAppendPieces * kAppendThreads / s.per_token.d);
+    const int64_t planes = s.heads_inner ? 2 : 2 * a.heads;
+    while (tokens > 1 && a.tokens * planes < 256 * tokens) tokens /= 2;
+    s.tokens = (int32_t)tokens;
+    const dim3 grid((unsigned)((a.tokens + tokens - 1) / tokens), s.heads_inner ? 1u : (unsigned)a.heads, 2);
+    if (cache_dtype != BA_F8_E4M3) launch_append<0, false>(a, s, grid, stream);
+    else if (dtype == BA_F16) launch_append<0, true>(a, s, grid, stream);
+    else launch_append<1, true>(a, s, grid, stream);
     return hipGetLastError() == hipSuccess ? BA_OK : BA_ERR_LAUNCH;
 }
 

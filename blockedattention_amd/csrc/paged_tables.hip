@@ -1,67 +1,186 @@
 // Page tables and slot maps from the requests' lengths before and after a call.
+//
+// With o and n the pages of a request before and after, take = max(n - o, 0), drop = max(o - n, 0), grow = max(new - old, 0):
+// three prefix sums over the requests give every new token its request (the place of its number in the sums of grow) and
+// every new page its number i, and i tells where the page comes from without anyone having moved anything: the i-th
+// page given back (found in the sums of drop, read from the row of the request that gives it) or, past those, a place
+// of the free stack.  So every token works out its own slot, nothing waits for a write of another thread, and the
+// call writes the same when it is made again.  It is bound by latency: the lengths, one page and one table entry are
+// loads one behind the other.
+#include <algorithm>
+
 #include "ba_device.hpp"
 #include "paged.hpp"
 
 namespace ba {
 
+constexpr int kTableThreads = 512;
+constexpr int kTableWaves = kTableThreads / 64;
+constexpr int kTableRequests = 4096;         // with so many requests every workgroup keeps the three sums in LDS
+constexpr int kTableTokens = 2048;           // tokens of a workgroup
+
 __device__ __forceinline__ int pages_of(const PageDiv &page, int tokens) {
     return tokens > 0 ? (int)page.div((uint32_t)(tokens - 1)) + 1 : 0;
 }
 
-// One thread, one request after the other.
-__global__ void paged_tables_kernel(PagedTablesArgs a) {
-    if (threadIdx.x) return;
-    const int64_t count = a.state_in[0], limit = (int64_t)a.width * a.page.d;
-    int64_t verdict = a.state_in[1], take = 0, drop = 0, grow = 0;
-    for (int r = 0; r < a.requests; ++r) {
-        const int64_t o = a.lens[r], n = a.new_lens[r];
-        a.accum[r] = grow;
-        if (o < 0 || n < 0 || o > limit) { verdict |= BA_PAGED_BAD_LENGTH; continue; }
-        if (n > limit) { verdict |= BA_PAGED_ROW_SHORT; continue; }
-        const int po = pages_of(a.page, (int)o), pn = pages_of(a.page, (int)n);
-        take += max(pn - po, 0); drop += max(po - pn, 0); grow += n > o ? n - o : 0;
-    }
-    a.accum[a.requests] = grow;
-    if (count < 0 || count + drop > a.pool) verdict |= BA_PAGED_BAD_STATE;
-    if (!verdict) verdict = (take > count + drop ? BA_PAGED_NO_PAGES : 0) | (grow > a.tokens ? BA_PAGED_NO_SLOTS : 0);
-    a.state_out[0] = verdict ? count : count + drop - take;
-    a.state_out[1] = verdict;
-    int64_t slot = 0, taken = 0;
-    if (!verdict) {
-        // the pages given back lie on the stack first, the last one lowest
-        int64_t j = 0;
-        for (int r = 0; r < a.requests; ++r) {
-            const int po = pages_of(a.page, (int)a.lens[r]), pn = pages_of(a.page, (int)a.new_lens[r]);
-            for (int c = pn; c < po; ++c, ++j)
-                if (j >= take) a.free_pages[count + drop - 1 - j] = a.table[r * a.table_stride + c];
-        }
-        int r2 = -1, c2 = 0, e2 = 0;              // the next page given back
-        for (int r = 0; r < a.requests; ++r) {
-            const int o = (int)a.lens[r], n = (int)a.new_lens[r];
-            const int po = pages_of(a.page, o), pn = pages_of(a.page, n);
-            for (int c = po; c < pn; ++c, ++taken) {
-                int32_t page;
-                if (taken < drop) {
-                    while (c2 >= e2) { ++r2; e2 = pages_of(a.page, (int)a.lens[r2]); c2 = pages_of(a.page, (int)a.new_lens[r2]); }
-                    page = a.table[r2 * a.table_stride + c2++];
-                } else {
-                    page = a.free_pages[count - 1 - (taken - drop)];
-                }
-                a.table[r * a.table_stride + c] = page;
-            }
-            for (int t = o; t < n; ++t) {
-                const uint32_t c = a.page.div((uint32_t)t);
-                a.slots[slot++] = (int64_t)a.table[r * a.table_stride + c] * a.page.d + ((uint32_t)t - c * a.page.d);
-            }
-        }
-    }
-    for (; slot < a.tokens; ++slot) a.slots[slot] = -1;
-    for (int r = 0; r < a.requests; ++r) a.lens_out[r] = verdict ? a.lens[r] : a.new_lens[r];
-    for (int r = 0; verdict && r <= a.requests; ++r) a.accum[r] = 0;
+struct Change {
+    int64_t take, drop, grow;
+    int verdict;
+};
+__device__ __forceinline__ Change change_of(const PagedTablesArgs &a, int r) {
+    const int64_t o = a.lens[r], n = a.new_lens[r], limit = (int64_t)a.width * a.page.d;
+    if (o < 0 || n < 0 || o > limit || n > limit)
+        return {0, 0, 0, (o < 0 || n < 0 || o > limit ? BA_PAGED_BAD_LENGTH : 0) | (n > limit ? BA_PAGED_ROW_SHORT : 0)};
+    const int d = pages_of(a.page, (int)n) - pages_of(a.page, (int)o);
+    return {max(d, 0), max(-d, 0), n > o ? n - o : 0, 0};
 }
 
-int launch_paged_tables(const PagedTablesArgs &a, void *, hipStream_t stream) {
-    paged_tables_kernel<<<1, 64, 0, stream>>>(a);
+// What all requests together change, and the verdict on it.
+struct Totals {
+    int64_t count, take, drop, grow;
+    int verdict;
+};
+__device__ __forceinline__ void judge(const PagedTablesArgs &a, Totals &t) {
+    if (t.count < 0 || t.count + t.drop > a.pool) t.verdict |= BA_PAGED_BAD_STATE;
+    if (!t.verdict) t.verdict = (t.take > t.count + t.drop ? BA_PAGED_NO_PAGES : 0) | (t.grow > a.tokens ? BA_PAGED_NO_SLOTS : 0);
+}
+
+// Prefix sums of `v` over the workgroup: exclusive for each thread; `sum` gets the total.
+template <int WAVES> __device__ __forceinline__ Change scan_changes(const Change &v, Change &sum, Change *waves) {
+    const int lane = lane_id(), wave = (int)threadIdx.x >> 6;
+    Change upto = {wave_inclusive_scan(v.take), wave_inclusive_scan(v.drop), wave_inclusive_scan(v.grow), v.verdict};
+#pragma unroll
+    for (int bit = 1; bit <= BA_PAGED_BAD_STATE; bit *= 2) upto.verdict |= __any(v.verdict & bit) ? bit : 0;
+    if (lane == 63) waves[wave] = upto;
+    __syncthreads();
+    sum = {0, 0, 0, 0};
+    Change before = {upto.take - v.take, upto.drop - v.drop, upto.grow - v.grow, 0};
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) {
+        if (i < wave) { before.take += waves[i].take; before.drop += waves[i].drop; before.grow += waves[i].grow; }
+        sum.take += waves[i].take; sum.drop += waves[i].drop; sum.grow += waves[i].grow; sum.verdict |= waves[i].verdict;
+    }
+    __syncthreads();
+    return before;
+}
+
+// The request r with sums[r] <= i < sums[r + 1].
+template <typename T> __device__ __forceinline__ int owner(const T *sums, int requests, int64_t i) {
+    int lo = 0, len = requests;
+    while (len > 1) {
+        const int half = len >> 1;
+        if ((int64_t)sums[lo + half] <= i) { lo += half; len -= half; }
+        else len = half;
+    }
+    return lo;
+}
+
+// Slots, pages and stack entries, thread `me` of `all`.
+template <typename P, typename G>
+__device__ __forceinline__ void fill(const PagedTablesArgs &a, const Totals &t, const P *take, const P *drop, const G *grow, int64_t me, int64_t all) {
+    auto given = [&](int64_t j) {
+        const int r = owner(drop, a.requests, j);
+        return a.table[r * a.table_stride + pages_of(a.page, (int)a.new_lens[r]) + (j - (int64_t)drop[r])];
+    };
+    for (int64_t i = me; i < a.tokens; i += all) {
+        if (t.verdict || i >= t.grow) { a.slots[i] = -1; continue; }
+        const int r = owner(grow, a.requests, i);
+        const int old = (int)a.lens[r], at = old + (int)(i - (int64_t)grow[r]);
+        const int column = (int)a.page.div((uint32_t)at), line = at - column * (int)a.page.d, had = pages_of(a.page, old);
+        int32_t *const entry = a.table + r * a.table_stride + column;
+        int32_t page;
+        if (column < had) {
+            page = *entry;
+        } else {
+            const int64_t number = (int64_t)take[r] + column - had;
+            page = number < t.drop ? given(number) : a.free_pages[t.count - 1 - (number - t.drop)];
+            if (line == 0) *entry = page;            // (a page's first token is always new where the page is)
+        }
+        a.slots[i] = (int64_t)page * a.page.d + line;
+    }
+    if (!t.verdict)
+        for (int64_t j = t.take + me; j < t.drop; j += all) a.free_pages[t.count + t.drop - 1 - j] = given(j);
+    if (me == 0) {
+        a.state_out[0] = t.verdict ? t.count : t.count + t.drop - t.take;
+        a.state_out[1] = t.verdict;
+    }
+}
+
+// Every workgroup makes the three sums for itself, in LDS.
+__global__ void __launch_bounds__(kTableThreads) paged_tables_kernel(PagedTablesArgs a) {
+    __shared__ Change waves[kTableWaves];
+    extern __shared__ int32_t sums[];               // take, drop, grow: [requests] each
+    int32_t *const take = sums, *const drop = sums + a.requests, *const grow = drop + a.requests;
+    const int c = (a.requests + kTableThreads - 1) / kTableThreads;
+    const int r0 = min(a.requests, (int)threadIdx.x * c), r1 = min(a.requests, r0 + c);
+    Totals t = {a.state_in[0], 0, 0, 0, (int)a.state_in[1]};
+    Change mine = {0, 0, 0, 0}, all;
+    for (int r = r0; r < r1; ++r) {
+        const Change x = change_of(a, r);
+        mine = {mine.take + x.take, mine.drop + x.drop, mine.grow + x.grow, mine.verdict | x.verdict};
+    }
+    Change before = scan_changes<kTableWaves>(mine, all, waves);
+    t.take = all.take; t.drop = all.drop; t.grow = all.grow; t.verdict |= all.verdict;
+    judge(a, t);
+    for (int r = r0; r < r1; ++r) {
+        const Change x = change_of(a, r);
+        take[r] = (int32_t)before.take; drop[r] = (int32_t)before.drop; grow[r] = (int32_t)before.grow;
+        if (blockIdx.x == 0) {
+            a.accum[r] = t.verdict ? 0 : before.grow;
+            a.lens_out[r] = t.verdict ? a.lens[r] : a.new_lens[r];
+        }
+        before = {before.take + x.take, before.drop + x.drop, before.grow + x.grow, 0};
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.accum[a.requests] = t.verdict ? 0 : t.grow;
+    __syncthreads();
+    fill(a, t, take, drop, grow, (int64_t)blockIdx.x * kTableThreads + threadIdx.x, (int64_t)gridDim.x * kTableThreads);
+}
+
+// More requests: one workgroup makes the sums (grow: the accum result), a second launch reads them.
+struct TableSums {
+    Totals totals;
+    int64_t sums[];                                  // take, drop: [requests] each
+};
+__global__ void __launch_bounds__(1024) paged_table_sums_kernel(PagedTablesArgs a, TableSums *w) {
+    __shared__ Change waves[16];
+    Totals t = {a.state_in[0], 0, 0, 0, (int)a.state_in[1]};
+    for (int first = 0; first < a.requests; first += 1024) {
+        const int r = first + (int)threadIdx.x;
+        Change all;
+        const Change mine = r < a.requests ? change_of(a, r) : Change{0, 0, 0, 0}, before = scan_changes<16>(mine, all, waves);
+        if (r < a.requests) {
+            w->sums[r] = t.take + before.take;
+            w->sums[a.requests + r] = t.drop + before.drop;
+            a.accum[r] = t.grow + before.grow;
+        }
+        t.take += all.take; t.drop += all.drop; t.grow += all.grow; t.verdict |= all.verdict;
+    }
+    judge(a, t);
+    if (threadIdx.x == 0) {
+        w->totals = t;
+        a.accum[a.requests] = t.verdict ? 0 : t.grow;
+    }
+    for (int r = (int)threadIdx.x; r < a.requests; r += 1024) {
+        a.lens_out[r] = t.verdict ? a.lens[r] : a.new_lens[r];
+        if (t.verdict) a.accum[r] = 0;              // (this thread's own writes)
+    }
+}
+__global__ void __launch_bounds__(kTableThreads) paged_table_fill_kernel(PagedTablesArgs a, const TableSums *w) {
+    fill(a, w->totals, w->sums, w->sums + a.requests, a.accum, (int64_t)blockIdx.x * kTableThreads + threadIdx.x, (int64_t)gridDim.x * kTableThreads);
+}
+
+size_t paged_tables_workspace(int64_t requests) {
+    return requests > kTableRequests ? sizeof(TableSums) + 2 * (size_t)requests * sizeof(int64_t) : 0;
+}
+
+int launch_paged_tables(const PagedTablesArgs &a, void *workspace, hipStream_t stream) {
+    const unsigned groups = (unsigned)std::min<int64_t>(256, std::max<int64_t>(1, ((int64_t)a.tokens + kTableTokens - 1) / kTableTokens));
+    if (a.requests > kTableRequests) {
+        paged_table_sums_kernel<<<1, 1024, 0, stream>>>(a, (TableSums *)workspace);
+        paged_table_fill_kernel<<<groups, kTableThreads, 0, stream>>>(a, (const TableSums *)workspace);
+    } else {
+        paged_tables_kernel<<<groups, kTableThreads, 3 * a.requests * sizeof(int32_t), stream>>>(a);
+    }
     return hipGetLastError() == hipSuccess ? BA_OK : BA_ERR_LAUNCH;
 }
 
