@@ -67,34 +67,36 @@ typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint32_t u32_any __attribute__((aligned(1)));
 typedef uint16_t u16_any __attribute__((aligned(1)));
 
-// N dwords from any address.  FULL: all of them; else the first `bytes` (any number, also none or negative), zeros behind.
-template <int N, bool FULL> __device__ __forceinline__ void load_piece(uint32_t (&x)[N], const char *p, int bytes) {
+// N dwords from any address, past the caches (what streams through once is read at 7.0 TB/s that way, 6.2 otherwise).
+template <int N> __device__ __forceinline__ void load_stream(uint32_t (&x)[N], const char *p) {
     static_assert(N == 1 || N == 2 || N == 4);
-    if (!FULL) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = 0;
-        if (bytes < 4 * N) {
-            if (bytes <= 0) return;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int left = bytes - 4 * i;
-                if (left >= 4) x[i] = *(const u32_any *)(p + 4 * i);
-                else if (left >= 2) x[i] = *(const u16_any *)(p + 4 * i) | (left == 3 ? (uint32_t)*(const uint8_t *)(p + 4 * i + 2) << 16 : 0u);
-                else if (left == 1) x[i] = *(const uint8_t *)(p + 4 * i);
-            }
-            return;
-        }
-    }
     if (N == 4) {
-        const u32x4_any v = *(const u32x4_any *)p;
+        const u32x4_any v = __builtin_nontemporal_load((const u32x4_any *)p);
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = v[i];
     } else if (N == 2) {
-        const u32x2_any v = *(const u32x2_any *)p;
+        const u32x2_any v = __builtin_nontemporal_load((const u32x2_any *)p);
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = v[i];
     } else {
-        x[0] = *(const u32_any *)p;
+        x[0] = __builtin_nontemporal_load((const u32_any *)p);
+    }
+}
+// The first `bytes` of N dwords (any number, also none or negative), zeros behind.
+template <int N> __device__ __forceinline__ void load_part(uint32_t (&x)[N], const char *p, int bytes) {
+    if (bytes >= 4 * N) {
+        load_stream<N>(x, p);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = 0;
+    if (bytes <= 0) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int left = bytes - 4 * i;
+        if (left >= 4) x[i] = *(const u32_any *)(p + 4 * i);
+        else if (left >= 2) x[i] = *(const u16_any *)(p + 4 * i) | (left == 3 ? (uint32_t)*(const uint8_t *)(p + 4 * i + 2) << 16 : 0u);
+        else if (left == 1) x[i] = *(const uint8_t *)(p + 4 * i);
     }
 }
 

@@ -64,7 +64,8 @@ template <int DT, bool F8, bool WHOLE> __global__ void __launch_bounds__(kAppend
                 at[k] = (int)(rest - row * s.per_row.d) * kPieceElems;
                 slot[k] = a.slots[t0 + t];
                 const char *const src = a.from[which] + head[k] * a.from_head_bytes[which] + (t0 + t) * a.from_token_bytes[which] + 2 * at[k];
-                load_piece<4, WHOLE>(x[k], src, 2 * (a.dim - at[k]));
+                if (WHOLE) load_stream<4>(x[k], src);
+                else load_part<4>(x[k], src, 2 * (a.dim - at[k]));
             }
         }
         const PagedArray &to = a.to[which];

@@ -57,6 +57,11 @@ template <int DT, bool HI> __device__ __forceinline__ uint32_t widen(uint32_t x)
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)x, 1.f, HI));
 }
 
+// What is known of the head dimension: it fills the registers (64, 128, 256), it is whole pieces (16 bytes of a key), or neither.
+enum Shape { kFull, kPieces, kAny };
+// What is known of the pages: whole halves of tiles, whole groups of four tokens, nothing.
+enum Pages { kHalves, kFours, kTokens };
+
 struct Visible {
     int first, len;                          // tokens first .. len - 1 are seen
     __device__ __forceinline__ int start() const { return first & ~(kPagedTile - 1); }
@@ -75,8 +80,8 @@ struct Place {
     int64_t at;                              // number of the tile in the order of all
 };
 
-// DC: dimensions that the registers hold (64, 128, 256), FULL: dim == DC; P16: pages are whole halves of tiles.
-template <int DT, bool F8, int DC, bool FULL, bool P16>
+// DC: dimensions that the registers hold (64, 128, 256).
+template <int DT, bool F8, int DC, Shape SHAPE, Pages PAGES>
 __global__ void __launch_bounds__(kPagedThreads, DC == 64 ? 4 : DC == 128 ? 3 : 2)
 paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
     constexpr int EB = F8 ? 1 : 2;           // bytes of an element
@@ -88,7 +93,7 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
     const int lane = lane_id(), l16 = lane & 15, g = lane >> 4, wave = uniform((int)threadIdx.x >> 6);
     const int units = a.heads * w.tiles_a_head;
 
-    extern __shared__ float lds[];           // [waves][rows][dim + 4], then the scan's and the waves' m and l
+    extern __shared__ __attribute__((aligned(16))) float lds[];           // [waves][rows][dim + 4]
     __shared__ int64_t scan[kPagedWaves];
     __shared__ Place places[2];
     __shared__ float wave_m[kPagedWaves][kPagedHeads], wave_l[kPagedWaves][kPagedHeads];
@@ -160,7 +165,11 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
         for (int i = 0; i < KK; ++i) {
             const int d = F8 ? 64 * (i / 2) + 16 * g + 8 * (i % 2) : 32 * i + 8 * g;
             uint32_t x[4] = {0, 0, 0, 0};
-            if (l16 < rows) load_piece<4, FULL>(x, a.q + (q0 + l16) * a.q_head_bytes + request * a.q_row_bytes + 2 * d, 2 * (a.dim - d));
+            const char *const p = a.q + (q0 + l16) * a.q_head_bytes + request * a.q_row_bytes + 2 * d;
+            if (l16 < rows) {
+                if (SHAPE == kAny) load_part<4>(x, p, 2 * (a.dim - d));
+                else if (SHAPE == kFull || d < a.dim) load_stream<4>(x, p);
+            }
             qf[i] = u32x4{x[0], x[1], x[2], x[3]};
         }
         const float to_log2 = a.scale * kLog2e * (F8 ? a.k.scale[h] : 1.f);
@@ -170,63 +179,92 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
 #pragma unroll
         for (int j = 0; j < PW; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+        uint32_t kx[2][KL][4], vx[8][VL][VN];
+        // Pages of a tile's two halves (kHalves: for all lanes), else of the lane's token of the 32.  Tokens that are not seen may
+        // have no page (any more): a half, a group of four or a token without any that is seen borrows the place of one with.
+        int32_t page[2] = {0, 0}, line[2] = {0, 0};
+        auto look_up = [&](int t0) {
+            if (PAGES == kHalves) {
+                int ta = t0, tb = t0 + 16;
+                if (tb >= len) tb = ta;
+                if (ta + 16 <= first) ta = tb;
+                const uint32_t ca = a.page.div((uint32_t)ta), cb = a.page.div((uint32_t)tb);
+                page[0] = row[ca]; page[1] = row[cb];
+                line[0] = ta - (int)(ca * a.page.d); line[1] = tb - (int)(cb * a.page.d);
+            } else {
+                const int mine = t0 + (lane & 31), four = PAGES == kFours ? 3 : 0;
+                const int t = min(max(mine & ~four, first & ~four), (len - 1) & ~four) + (mine & four);
+                const uint32_t col = a.page.div((uint32_t)t);
+                page[0] = a.table[request * a.table_stride + col];
+                line[0] = t - (int)(col * a.page.d);
+            }
+        };
+        if (len > first && tile + wave < last) look_up(start + (tile + wave) * kPagedTile);
         for (int s = tile + wave; s < last && len > first; s += kPagedWaves) {
             const int t0 = start + s * kPagedTile;
             // ---- where the keys and values of the tile lie
             const char *kp[2], *vp[8];
             bool bad;
-            if (P16) {
-                // a half without a token that is seen borrows the other one's page
-                int ta = t0, tb = t0 + 16;
-                if (tb >= len) tb = ta;
-                if (ta + 16 <= first) ta = tb;
-                const uint32_t ca = a.page.div((uint32_t)ta), cb = a.page.div((uint32_t)tb);
-                const int32_t pa = uniform(row[ca]), pb = uniform(row[cb]);
-                bad = (uint32_t)pa >= (uint32_t)a.pages || (uint32_t)pb >= (uint32_t)a.pages;
-                const int32_t ra = ta - (int)(ca * a.page.d), rb = tb - (int)(cb * a.page.d);
-                const char *const ka = kh + pa * a.k.page_bytes + (int64_t)ra * a.k.token_bytes;
-                const char *const kb = kh + pb * a.k.page_bytes + (int64_t)rb * a.k.token_bytes;
-                const char *const va = vh + pa * a.v.page_bytes + (int64_t)ra * a.v.token_bytes;
-                const char *const vb = vh + pb * a.v.page_bytes + (int64_t)rb * a.v.token_bytes;
-                kp[0] = ka + (uint32_t)(l16 * a.k.token_bytes); kp[1] = kb + (uint32_t)(l16 * a.k.token_bytes);
+            if (PAGES == kHalves) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    vp[i] = va + (uint32_t)((4 * g + i) * a.v.token_bytes);
-                    vp[4 + i] = vb + (uint32_t)((4 * g + i) * a.v.token_bytes);
+                for (int i = 0; i < 2; ++i) {
+                    const int32_t pg = uniform(page[i]), ln = uniform(line[i]);
+                    kp[i] = kh + pg * a.k.page_bytes + (int64_t)ln * a.k.token_bytes + (uint32_t)(l16 * a.k.token_bytes);
+                    const char *const vb = vh + pg * a.v.page_bytes + (int64_t)ln * a.v.token_bytes;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) vp[4 * i + e] = vb + (uint32_t)((4 * g + e) * a.v.token_bytes);
                 }
+                bad = (uint32_t)page[0] >= (uint32_t)a.pages || (uint32_t)page[1] >= (uint32_t)a.pages;
             } else {
-                // token by token; one that is not seen borrows a neighbour's place
-                const int t = min(max(t0 + (lane & 31), first), len - 1);
-                const uint32_t col = a.page.div((uint32_t)t);
-                const int32_t page = a.table[request * a.table_stride + col], line = t - (int)(col * a.page.d);
-                bad = __any((uint32_t)page >= (uint32_t)a.pages);
+                bad = __any((uint32_t)page[0] >= (uint32_t)a.pages);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int from = 16 * i + l16;
-                    kp[i] = kh + __shfl(page, from) * a.k.page_bytes + (int64_t)__shfl(line, from) * a.k.token_bytes;
+                    kp[i] = kh + __shfl(page[0], from) * a.k.page_bytes + (int64_t)__shfl(line[0], from) * a.k.token_bytes;
                 }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
+                    // (kFours: tokens 4 g .. 4 g + 3 of a half lie in one page, one behind the other)
                     const int from = 16 * (i / 4) + 4 * g + i % 4;
-                    vp[i] = vh + __shfl(page, from) * a.v.page_bytes + (int64_t)__shfl(line, from) * a.v.token_bytes;
+                    if (PAGES == kTokens || i % 4 == 0)
+                        vp[i] = vh + __shfl(page[0], from) * a.v.page_bytes + (int64_t)__shfl(line[0], from) * a.v.token_bytes;
+                    else vp[i] = vp[i - i % 4] + (uint32_t)(i % 4 * a.v.token_bytes);
                 }
             }
+            if (s + kPagedWaves < last) look_up(t0 + kPagedWaves * kPagedTile);
             if (bad) { l = NAN; continue; }
-            uint32_t kx[2][KL][4], vx[8][VL][VN];
+            // Pieces that are not there (kPieces) are loaded from the row's front: those of a key count as zeros, those of a value
+            // make results that nobody stores.
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int k = 0; k < KL; ++k) {
+                const int b = 64 * k + 16 * g;
+                const bool there = SHAPE != kPieces || b < EB * a.dim;
 #pragma unroll
-                for (int k = 0; k < KL; ++k) {
-                    const int b = 64 * k + 16 * g;
-                    load_piece<4, FULL>(kx[i][k], kp[i] + b, EB * a.dim - b);
+                for (int i = 0; i < 2; ++i) {
+                    if (SHAPE == kAny) load_part<4>(kx[i][k], kp[i] + b, EB * a.dim - b);
+                    else load_stream<4>(kx[i][k], kp[i] + (there ? b : 0));
                 }
+            }
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int k = 0; k < VL; ++k) {
+                const int b = EB * PW * l16 + 16 * k;
+                const bool there = SHAPE != kPieces || b < EB * a.dim;
 #pragma unroll
-                for (int k = 0; k < VL; ++k) {
-                    const int b = EB * PW * l16 + 16 * k;
-                    load_piece<VN, FULL>(vx[i][k], vp[i] + b, EB * a.dim - b);
+                for (int i = 0; i < 8; ++i) {
+                    if (SHAPE == kAny) load_part<VN>(vx[i][k], vp[i] + b, EB * a.dim - b);
+                    else load_stream<VN>(vx[i][k], vp[i] + (there ? b : 0));
                 }
+            }
+            if (SHAPE == kPieces) {
+#pragma unroll
+                for (int k = 0; k < KL; ++k)
+                    if (64 * k + 64 > EB * a.dim) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) kx[i][k][x] = 64 * k + 16 * g < EB * a.dim ? kx[i][k][x] : 0u;
+                    }
+            }
 
             // ---- scores of tokens t0 + 16 i + 4 g + e
             f32x4 sc[2];
@@ -318,8 +356,16 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < PW; ++j)
-                        if (FULL || PW * (4 * g + i) + j < a.dim) mineo[PW * (4 * g + i) + j] = o[j][i];
+                    for (int j = 0; j < PW; j += 4) {
+                        const int d = PW * (4 * g + i) + j;
+                        if (SHAPE != kAny) {
+                            if (SHAPE == kFull || d < a.dim) *(f32x4 *)(mineo + d) = f32x4{o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]};
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (d + e < a.dim) mineo[d + e] = o[j + e][i];
+                        }
+                    }
             }
         }
         __syncthreads();
@@ -362,7 +408,7 @@ template <int DT> __global__ void __launch_bounds__(kPagedThreads) paged_join_ke
     const PagedJoin join = w.joins[blockIdx.x];
     const int h = join.unit / w.tiles_a_head, q = h * a.group + (join.unit - h * w.tiles_a_head) * w.rows + (int)blockIdx.y;
     if (join.parts == 0 || q >= (h + 1) * a.group || (int)blockIdx.y >= w.rows) return;
-    extern __shared__ float lds[];           // factor of each part, then the partial sums of the rows of threads
+    extern __shared__ __attribute__((aligned(16))) float lds[];           // factor of each part, then the partial sums of the rows of threads
     __shared__ float wave_x[kPagedWaves];
     const int lane = lane_id(), wave = (int)threadIdx.x >> 6;
     auto slot = [&](int p) { return 2 * (int64_t)(join.first + p) + (p == 0 ? 1 : 0); };
@@ -434,32 +480,34 @@ size_t paged_attention_workspace(int64_t heads, int64_t group, int64_t dim, int6
     return bytes;
 }
 
-template <int DT, bool F8, int DC, bool FULL, bool P16>
-static int launch_split(const PagedAttentionArgs &a, const PagedWork &w, size_t lds, hipStream_t stream) {
+template <int DT, bool F8, int DC, Shape SHAPE, Pages PAGES>
+static int launch_split(const PagedAttentionArgs &a, const PagedWork &w, hipStream_t stream) {
     constexpr int kMostLds = kPagedWaves * kPagedHeads * (DC + 4) * (int)sizeof(float);
     if constexpr (kMostLds > 65536) {
-        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&paged_attention_kernel<DT, F8, DC, FULL, P16>),
+        static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&paged_attention_kernel<DT, F8, DC, SHAPE, PAGES>),
                                                            hipFuncAttributeMaxDynamicSharedMemorySize, kMostLds);
         if (attr != hipSuccess) return BA_ERR_LAUNCH;
     }
-    paged_attention_kernel<DT, F8, DC, FULL, P16><<<w.groups, kPagedThreads, lds, stream>>>(a, w);
-    return BA_OK;
-}
-
-template <int DT, bool F8, int DC, bool FULL> static int launch_class(const PagedAttentionArgs &a, const PagedWork &w, hipStream_t stream) {
     const size_t lds = (size_t)kPagedWaves * w.rows * (a.dim + 4) * sizeof(float);
-    const int st = a.page.d % 16 == 0 ? launch_split<DT, F8, DC, FULL, true>(a, w, lds, stream) : launch_split<DT, F8, DC, FULL, false>(a, w, lds, stream);
-    if (st != BA_OK) return st;
+    paged_attention_kernel<DT, F8, DC, SHAPE, PAGES><<<w.groups, kPagedThreads, lds, stream>>>(a, w);
     const dim3 grid((unsigned)(w.by_unit ? a.requests * a.heads * w.tiles_a_head : w.groups), (unsigned)w.rows);
     paged_join_kernel<DT><<<grid, kPagedThreads, (w.groups + kPagedThreads) * sizeof(float), stream>>>(a, w);
     return hipGetLastError() == hipSuccess ? BA_OK : BA_ERR_LAUNCH;
 }
 
+// Pages of 16, 32, ... tokens and those of 4, 8, 12, 20, ... have builds of their own where rows are whole pieces; all else
+// runs through the build that takes every token and byte by itself.
+template <int DT, bool F8, int DC> static int launch_class(const PagedAttentionArgs &a, const PagedWork &w, hipStream_t stream) {
+    if (a.page.d % 4 || a.dim % (F8 ? 16 : 8)) return launch_split<DT, F8, DC, kAny, kTokens>(a, w, stream);
+    if (a.page.d % 16) return a.dim == DC ? launch_split<DT, F8, DC, kFull, kFours>(a, w, stream) : launch_split<DT, F8, DC, kPieces, kFours>(a, w, stream);
+    return a.dim == DC ? launch_split<DT, F8, DC, kFull, kHalves>(a, w, stream) : launch_split<DT, F8, DC, kPieces, kHalves>(a, w, stream);
+}
+
 template <int DT, bool F8> static int launch_dtype(const PagedAttentionArgs &a, const PagedWork &w, hipStream_t stream) {
     switch (dim_class(a.dim)) {
-        case 64: return a.dim == 64 ? launch_class<DT, F8, 64, true>(a, w, stream) : launch_class<DT, F8, 64, false>(a, w, stream);
-        case 128: return a.dim == 128 ? launch_class<DT, F8, 128, true>(a, w, stream) : launch_class<DT, F8, 128, false>(a, w, stream);
-        default: return a.dim == 256 ? launch_class<DT, F8, 256, true>(a, w, stream) : launch_class<DT, F8, 256, false>(a, w, stream);
+        case 64: return launch_class<DT, F8, 64>(a, w, stream);
+        case 128: return launch_class<DT, F8, 128>(a, w, stream);
+        default: return launch_class<DT, F8, 256>(a, w, stream);
     }
 }
 
