@@ -18,6 +18,7 @@
 // the small matrix in registers: the operand of dimension j is made of the j-th halves of its eight rows.  Nothing of the cache
 // passes through LDS.
 #include <algorithm>
+#include <type_traits>
 
 #include "ba_device.hpp"
 #include "ba_host.hpp"
@@ -47,14 +48,26 @@ struct PagedJoin {
 struct PagedWork {
     PagedJoin *joins;                        // one entry a unit, or a workgroup where there are fewer of those
     PagedPart *parts;                        // [2 * groups][kPagedHeads]
-    float *sums;                             // [2 * groups][rows][dim]
-    int32_t groups, by_unit, tiles_a_head, rows;   // tiles_a_head: units of a key head; rows: query heads of the largest unit
+    float *sums;                             // [2 * groups][rows][pitch]
+    int32_t groups, by_unit, tiles_a_head, rows, pitch;   // tiles_a_head: units of a key head; rows: query heads of the largest unit
 };
 
 // Two e4m3 values (HI: the upper two bytes) as two 16-bit numbers: exact in either type.
 template <int DT, bool HI> __device__ __forceinline__ uint32_t widen(uint32_t x) {
     if (DT == 0) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)x, 1.f, HI));
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)x, 1.f, HI));
+}
+
+// Dimensions d .. d + 3 of a result, as far as there are `dim`.
+template <int DT> __device__ __forceinline__ void store_result(char *row, int d, int dim, f32x4 x) {
+    u16_any *const p = (u16_any *)row + d;
+    if (d + 4 <= dim) {
+        *(u32x2_any *)p = u32x2_any{Elem<DT>::pack2(x[0], x[1]), Elem<DT>::pack2(x[2], x[3])};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (d + i < dim) p[i] = Elem<DT>::from_float(x[i]);
+    }
 }
 
 // What is known of the head dimension: it fills the registers (64, 128, 256), it is whole pieces (16 bytes of a key), or neither.
@@ -77,8 +90,15 @@ __device__ __forceinline__ Visible visible(const PagedAttentionArgs &a, int r) {
 // Position of the tile that the share of a workgroup begins with: request, unit of the request, tile of the unit.
 struct Place {
     int request, unit, tile;
+    Visible see;                             // of the request
     int64_t at;                              // number of the tile in the order of all
 };
+
+// x y / z, rounded down, z > 0: most often all of it fits 32 bits, where a division costs a fifth.
+__device__ __forceinline__ int64_t scaled(int64_t x, int64_t y, int64_t z) {
+    const int64_t p = x * y;
+    return ((uint64_t)p | (uint64_t)z) >> 32 ? p / z : (int64_t)((uint32_t)p / (uint32_t)z);
+}
 
 // DC: dimensions that the registers hold (64, 128, 256).
 template <int DT, bool F8, int DC, Shape SHAPE, Pages PAGES>
@@ -93,7 +113,7 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
     const int lane = lane_id(), l16 = lane & 15, g = lane >> 4, wave = uniform((int)threadIdx.x >> 6);
     const int units = a.heads * w.tiles_a_head;
 
-    extern __shared__ __attribute__((aligned(16))) float lds[];           // [waves][rows][dim + 4]
+    extern __shared__ __attribute__((aligned(16))) float lds[];           // [waves][rows][DC + 4]
     __shared__ int64_t scan[kPagedWaves];
     __shared__ Place places[2];
     __shared__ float wave_m[kPagedWaves][kPagedHeads], wave_l[kPagedWaves][kPagedHeads];
@@ -102,7 +122,12 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
     const int c = (a.requests + kPagedThreads - 1) / kPagedThreads, r0 = (int)threadIdx.x * c;
     const int r1 = min(a.requests, r0 + c);
     int64_t mine = 0;
-    for (int r = r0; r < r1; ++r) mine += visible(a, r).tiles();
+    Visible front = {0, 0};
+    for (int r = r0; r < r1; ++r) {
+        const Visible v = visible(a, r);
+        if (r == r0) front = v;
+        mine += v.tiles();
+    }
     int64_t upto = wave_inclusive_scan(mine);
     if (lane == 63) scan[wave] = upto;
     __syncthreads();
@@ -112,7 +137,7 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
         if (i < wave) upto += scan[i];
         total += scan[i];
     }
-    total *= units;
+    total = uniform64(total) * units;
     const int64_t groups = min((int64_t)w.groups, (total + kPagedShare - 1) / kPagedShare);
     const int64_t group = blockIdx.x;
     if (group >= groups) {
@@ -121,37 +146,42 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        int64_t at = (group + k) * total / groups;
+        int64_t at = scaled(group + k, total, groups);
         if (at >= total) {
-            if (threadIdx.x == 0) places[k] = {a.requests, 0, 0, total};
+            if (threadIdx.x == 0) places[k] = {a.requests, 0, 0, {0, 0}, total};
         } else if (at < upto * units && at >= (upto - mine) * units) {
             int64_t before = (upto - mine) * units;
-            int r = r0, n = visible(a, r).tiles();
+            Visible see = front;
+            int r = r0, n = see.tiles();
             while (at >= before + (int64_t)n * units) {
                 before += (int64_t)n * units;
-                n = visible(a, ++r).tiles();
+                see = visible(a, ++r);
+                n = see.tiles();
             }
-            int unit = (int)((at - before) / n), tile = (int)((at - before) - (int64_t)unit * n);
+            int unit = (int)scaled(at - before, 1, n), tile = (int)((at - before) - (int64_t)unit * n);
             if (n <= kPagedWhole && tile) {                    // short units go where most of them lies
                 at -= tile;
                 if (2 * tile > n) {
                     at += n;
-                    if (++unit == units) { unit = 0; ++r; }
+                    if (++unit == units) {
+                        unit = 0;
+                        if (++r < a.requests) see = visible(a, r);
+                    }
                 }
                 tile = 0;
             }
-            places[k] = {r, unit, tile, at};
+            places[k] = {r, unit, tile, see, at};
         }
     }
     __syncthreads();
     int request = uniform(places[0].request), unit = uniform(places[0].unit), tile = uniform(places[0].tile);
     int64_t at = uniform64(places[0].at);
     const int64_t end = uniform64(places[1].at);
+    Visible see = {uniform(places[0].see.first), uniform(places[0].see.len)};
     PagedJoin join = {0, 0, 0, 0};
 
     while (at < end) {
-        const Visible see = visible(a, request);
-        const int first = uniform(see.first), len = uniform(see.len), n = uniform(see.tiles()), start = uniform(see.start());
+        const int first = see.first, len = see.len, n = see.tiles(), start = see.start();
         const int last = (int)min((int64_t)n, tile + (end - at));      // tiles of this unit in this share: [tile, last)
         const int h = unit / w.tiles_a_head, q0 = h * a.group + (unit - h * w.tiles_a_head) * w.rows;
         const int rows = min(w.rows, (h + 1) * a.group - q0);
@@ -179,82 +209,81 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
 #pragma unroll
         for (int j = 0; j < PW; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-        uint32_t kx[2][KL][4], vx[8][VL][VN];
-        // Pages of a tile's two halves (kHalves: for all lanes), else of the lane's token of the 32.  Tokens that are not seen may
-        // have no page (any more): a half, a group of four or a token without any that is seen borrows the place of one with.
-        int32_t page[2] = {0, 0}, line[2] = {0, 0};
+        // Pages and lines of a tile.  Tokens that are not seen may have no page (any more): a half, a group of four or a token
+        // without any that is seen borrows the place of one with.  Page numbers outside the cache become page 0 and poison
+        // the result.
+        constexpr int NK = 2, NV = PAGES == kHalves ? 0 : PAGES == kFours ? 2 : 8;
+        int32_t page[NK + NV], line[NK + NV];
+        bool poison = a.pages == 0;
         auto look_up = [&](int t0) {
             if (PAGES == kHalves) {
-                int ta = t0, tb = t0 + 16;
-                if (tb >= len) tb = ta;
-                if (ta + 16 <= first) ta = tb;
-                const uint32_t ca = a.page.div((uint32_t)ta), cb = a.page.div((uint32_t)tb);
-                page[0] = row[ca]; page[1] = row[cb];
-                line[0] = ta - (int)(ca * a.page.d); line[1] = tb - (int)(cb * a.page.d);
+                int t[2] = {t0, t0 + 16};
+                if (t[1] >= len) t[1] = t[0];
+                if (t[0] + 16 <= first) t[0] = t[1];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t c = a.page.div((uint32_t)t[i]);
+                    page[i] = row[c];
+                    line[i] = t[i] - (int)(c * a.page.d);
+                }
             } else {
-                const int mine = t0 + (lane & 31), four = PAGES == kFours ? 3 : 0;
-                const int t = min(max(mine & ~four, first & ~four), (len - 1) & ~four) + (mine & four);
-                const uint32_t col = a.page.div((uint32_t)t);
-                page[0] = a.table[request * a.table_stride + col];
-                line[0] = t - (int)(col * a.page.d);
+                constexpr int four = PAGES == kFours ? 3 : 0;
+#pragma unroll
+                for (int i = 0; i < NK + NV; ++i) {
+                    const int mine = i < NK ? t0 + 16 * i + l16
+                                     : PAGES == kFours ? t0 + 16 * (i - NK) + 4 * g
+                                                       : t0 + 16 * ((i - NK) / 4) + 4 * g + (i - NK) % 4;
+                    const int t = min(max(mine & ~four, first & ~four), (len - 1) & ~four) + (mine & four);
+                    const uint32_t c = a.page.div((uint32_t)t);
+                    page[i] = a.table[request * a.table_stride + c];
+                    line[i] = t - (int)(c * a.page.d);
+                }
             }
         };
-        if (len > first && tile + wave < last) look_up(start + (tile + wave) * kPagedTile);
-        for (int s = tile + wave; s < last && len > first; s += kPagedWaves) {
-            const int t0 = start + s * kPagedTile;
-            // ---- where the keys and values of the tile lie
-            const char *kp[2], *vp[8];
-            bool bad;
-            if (PAGES == kHalves) {
+        auto checked = [&](int i) {
+            const int32_t p = PAGES == kHalves ? uniform(page[i]) : page[i];
+            const bool bad = (uint32_t)p >= (uint32_t)a.pages;
+            poison |= bad;
+            return bad ? 0 : p;
+        };
+        // Pieces that are not there (kPieces) are loaded from the row's front: those of a key count as zeros, those of a value
+        // make results that nobody stores.
+        uint32_t kx[2][KL][4], vx[8][VL][VN];
+        auto load_keys = [&] {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int32_t pg = uniform(page[i]), ln = uniform(line[i]);
-                    kp[i] = kh + pg * a.k.page_bytes + (int64_t)ln * a.k.token_bytes + (uint32_t)(l16 * a.k.token_bytes);
-                    const char *const vb = vh + pg * a.v.page_bytes + (int64_t)ln * a.v.token_bytes;
+            for (int i = 0; i < 2; ++i) {
+                const int32_t p = checked(i), ln = PAGES == kHalves ? uniform(line[i]) : line[i];
+                const char *const base = kh + p * a.k.page_bytes + (int64_t)ln * a.k.token_bytes;
+                const uint32_t mine = PAGES == kHalves ? (uint32_t)(l16 * a.k.token_bytes) : 0u;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) vp[4 * i + e] = vb + (uint32_t)((4 * g + e) * a.v.token_bytes);
-                }
-                bad = (uint32_t)page[0] >= (uint32_t)a.pages || (uint32_t)page[1] >= (uint32_t)a.pages;
-            } else {
-                bad = __any((uint32_t)page[0] >= (uint32_t)a.pages);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int from = 16 * i + l16;
-                    kp[i] = kh + __shfl(page[0], from) * a.k.page_bytes + (int64_t)__shfl(line[0], from) * a.k.token_bytes;
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    // (kFours: tokens 4 g .. 4 g + 3 of a half lie in one page, one behind the other)
-                    const int from = 16 * (i / 4) + 4 * g + i % 4;
-                    if (PAGES == kTokens || i % 4 == 0)
-                        vp[i] = vh + __shfl(page[0], from) * a.v.page_bytes + (int64_t)__shfl(line[0], from) * a.v.token_bytes;
-                    else vp[i] = vp[i - i % 4] + (uint32_t)(i % 4 * a.v.token_bytes);
+                for (int k = 0; k < KL; ++k) {
+                    const uint32_t b = 64 * k + 16 * g;
+                    if (SHAPE == kAny) load_part<4>(kx[i][k], base + (mine + b), EB * a.dim - (int)b);
+                    else if (SHAPE == kPieces) load_stream<4>(kx[i][k], base + (mine + ((int)b < EB * a.dim ? b : 0u)));
+                    else load_stream<4>(kx[i][k], base + (mine + 16u * g) + 64 * k);
                 }
             }
-            if (s + kPagedWaves < last) look_up(t0 + kPagedWaves * kPagedTile);
-            if (bad) { l = NAN; continue; }
-            // Pieces that are not there (kPieces) are loaded from the row's front: those of a key count as zeros, those of a value
-            // make results that nobody stores.
+        };
+        auto load_values = [&] {
 #pragma unroll
-            for (int k = 0; k < KL; ++k) {
-                const int b = 64 * k + 16 * g;
-                const bool there = SHAPE != kPieces || b < EB * a.dim;
+            for (int i = 0; i < 8; ++i) {
+                const int from = PAGES == kHalves ? i / 4 : PAGES == kFours ? NK + i / 4 : NK + i;
+                const int32_t p = checked(from), ln = PAGES == kHalves ? uniform(line[from]) : line[from];
+                const char *const base = vh + p * a.v.page_bytes + (int64_t)ln * a.v.token_bytes;
+                const uint32_t mine = PAGES == kHalves ? (uint32_t)((4 * g + i % 4) * a.v.token_bytes) : PAGES == kFours ? (uint32_t)(i % 4 * a.v.token_bytes) : 0u;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    if (SHAPE == kAny) load_part<4>(kx[i][k], kp[i] + b, EB * a.dim - b);
-                    else load_stream<4>(kx[i][k], kp[i] + (there ? b : 0));
+                for (int k = 0; k < VL; ++k) {
+                    const uint32_t b = EB * PW * l16 + 16 * k;
+                    if (SHAPE == kAny) load_part<VN>(vx[i][k], base + (mine + b), EB * a.dim - (int)b);
+                    else if (SHAPE == kPieces) load_stream<VN>(vx[i][k], base + (mine + ((int)b < EB * a.dim ? b : 0u)));
+                    else load_stream<VN>(vx[i][k], base + (mine + (uint32_t)(EB * PW * l16)) + 16 * k);
                 }
             }
-#pragma unroll
-            for (int k = 0; k < VL; ++k) {
-                const int b = EB * PW * l16 + 16 * k;
-                const bool there = SHAPE != kPieces || b < EB * a.dim;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (SHAPE == kAny) load_part<VN>(vx[i][k], vp[i] + b, EB * a.dim - b);
-                    else load_stream<VN>(vx[i][k], vp[i] + (there ? b : 0));
-                }
-            }
+        };
+        // The tile that begins with token t0; MORE: the wavefront's next one follows, whose keys are asked for as soon as the
+        // scores have used this one's, and its values likewise.
+        auto attend = [&](auto more, int t0) {
+            constexpr bool MORE = decltype(more)::value;
             if (SHAPE == kPieces) {
 #pragma unroll
                 for (int k = 0; k < KL; ++k)
@@ -265,7 +294,6 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
                             for (int x = 0; x < 4; ++x) kx[i][k][x] = 64 * k + 16 * g < EB * a.dim ? kx[i][k][x] : 0u;
                     }
             }
-
             // ---- scores of tokens t0 + 16 i + 4 g + e
             f32x4 sc[2];
 #pragma unroll
@@ -286,6 +314,7 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
                 }
                 sc[i] *= to_log2;
             }
+            if (MORE) load_keys();
             if (t0 < first || t0 + kPagedTile > len) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -343,10 +372,25 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
                 o[j] = Elem<DT>::mfma(v, u32x4{hi[0], hi[1], hi[2], hi[3]}, o[j]);
                 o[j] = Elem<DT>::mfma(v, u32x4{lo[0], lo[1], lo[2], lo[3]}, o[j]);
             }
+            if (MORE) load_values();
+        };
+        int s = tile + wave;
+        if (s < last && len > first && a.pages > 0) {
+            constexpr int kStep = kPagedWaves * kPagedTile;
+            int t0 = start + s * kPagedTile;
+            look_up(t0);
+            load_keys();
+            load_values();
+            for (; s + kPagedWaves < last; s += kPagedWaves, t0 += kStep) {
+                look_up(t0 + kStep);
+                attend(std::true_type{}, t0);
+            }
+            attend(std::false_type{}, t0);
         }
+        if (__any(poison)) l = NAN;
 
         // ---- join the wavefronts: lane (g, l16) has dimensions PW (4 g + i) + j of head l16
-        const int pitch = a.dim + 4;
+        constexpr int pitch = DC + 4;
         const int busy = min(last - tile, kPagedWaves);
         l = quad_column_sum(l);
         if (wave < busy) {
@@ -358,94 +402,114 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
 #pragma unroll
                     for (int j = 0; j < PW; j += 4) {
                         const int d = PW * (4 * g + i) + j;
-                        if (SHAPE != kAny) {
-                            if (SHAPE == kFull || d < a.dim) *(f32x4 *)(mineo + d) = f32x4{o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]};
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (d + e < a.dim) mineo[d + e] = o[j + e][i];
-                        }
+                        if (SHAPE == kFull || d < a.dim) *(f32x4 *)(mineo + d) = f32x4{o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]};
                     }
             }
         }
         __syncthreads();
         const bool begun = tile == 0, done = last == n, whole = begun && done;
         const int slot = 2 * (int)group + (begun ? 1 : 0);
-        for (int x = (int)threadIdx.x; x < rows * a.dim; x += kPagedThreads) {
-            const int hd = x / a.dim, d = x - hd * a.dim;
-            float top = -INFINITY, sum = 0.f, acc = 0.f;
+        for (int x = 4 * (int)threadIdx.x; x < rows * DC; x += 4 * kPagedThreads) {
+            const int hd = x / DC, d = x % DC;
+            if (d >= a.dim) continue;
+            float top = -INFINITY, sum = 0.f;
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
             for (int i = 0; i < busy; ++i) top = fmaxf(top, wave_m[i][hd]);
             const float base = top == -INFINITY ? 0.f : top;
             for (int i = 0; i < busy; ++i) {
                 const float f = __builtin_amdgcn_exp2f(wave_m[i][hd] - base);
                 sum += f * wave_l[i][hd];
-                acc += f * lds[(i * w.rows + hd) * pitch + d];
+                acc += f * *(const f32x4 *)(lds + (i * w.rows + hd) * pitch + d);
             }
             if (whole) {
-                const float v = len > first ? acc * (F8 ? a.v.scale[h] : 1.f) / sum : 0.f;
-                ((uint16_t *)(a.out + (q0 + hd) * a.out_head_bytes + request * a.out_row_bytes))[d] = Elem<DT>::from_float(v);
+                const float f = len > first ? (F8 ? a.v.scale[h] : 1.f) / sum : 0.f;
+                if (len <= first) acc = f32x4{0.f, 0.f, 0.f, 0.f};
+                store_result<DT>(a.out + (q0 + hd) * a.out_head_bytes + request * a.out_row_bytes, d, a.dim, acc * f);
             } else {
-                w.sums[((int64_t)slot * w.rows + hd) * a.dim + d] = acc;
+                *(f32x4 *)(w.sums + ((int64_t)slot * w.rows + hd) * w.pitch + d) = acc;
                 if (d == 0) w.parts[slot * kPagedHeads + hd] = {top, sum};
             }
         }
         if (begun) {
             // who has the unit's last tile
-            const int parts = done ? 0 : (int)(((at - tile + n) * groups + total - 1) / total - group);
+            const int parts = done ? 0 : (int)(scaled(at - tile + n, groups, total) + (scaled(at - tile + n, groups, total) * total < (at - tile + n) * groups) - group);
             join = {request, unit, (int)group, parts};
             if (w.by_unit && threadIdx.x == 0) w.joins[(int64_t)request * units + unit] = join;
         }
         at += last - tile;
         tile = 0;
-        if (++unit == units) { unit = 0; ++request; }
+        if (++unit == units) {
+            unit = 0;
+            if (++request < a.requests) {
+                const Visible v = visible(a, request);
+                see = {uniform(v.first), uniform(v.len)};
+            }
+        }
         __syncthreads();
     }
     if (!w.by_unit && threadIdx.x == 0) w.joins[group] = join;
 }
 
-// One workgroup per unit that was split (entry of the list) and query head.
-template <int DT> __global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(PagedAttentionArgs a, PagedWork w) {
+// Joins units that were split: grid (entries of the list, query heads / `heads`).  DC / 4 threads read a row of
+// partial sums; the rest of a workgroup's threads take other heads, or every so manieth part of the same ones.
+template <int DT, int DC> __global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(PagedAttentionArgs a, PagedWork w, int heads) {
+    constexpr int kLanes = DC / 4, kRows = kPagedThreads / kLanes, kAhead = 4;
     const PagedJoin join = w.joins[blockIdx.x];
-    const int h = join.unit / w.tiles_a_head, q = h * a.group + (join.unit - h * w.tiles_a_head) * w.rows + (int)blockIdx.y;
-    if (join.parts == 0 || q >= (h + 1) * a.group || (int)blockIdx.y >= w.rows) return;
-    extern __shared__ __attribute__((aligned(16))) float lds[];           // factor of each part, then the partial sums of the rows of threads
-    __shared__ float wave_x[kPagedWaves];
-    const int lane = lane_id(), wave = (int)threadIdx.x >> 6;
-    auto slot = [&](int p) { return 2 * (int64_t)(join.first + p) + (p == 0 ? 1 : 0); };
-    float top = -INFINITY;
-    for (int p = (int)threadIdx.x; p < join.parts; p += kPagedThreads) top = fmaxf(top, w.parts[slot(p) * kPagedHeads + blockIdx.y].m);
-    top = wave_max(top);
-    if (lane == 0) wave_x[wave] = top;
-    __syncthreads();
+    if (join.parts == 0) return;
+    __shared__ float rest_m[kRows], rest_l[kRows];
+    __shared__ f32x4 rest_acc[kRows][kLanes];
+    const int mine = (int)threadIdx.x / kLanes, d = 4 * ((int)threadIdx.x % kLanes), deep = kRows / heads;
+    const int hd = (int)blockIdx.y * heads + mine % heads, sub = mine / heads;
+    const int h = join.unit / w.tiles_a_head, q = h * a.group + (join.unit - h * w.tiles_a_head) * w.rows + hd;
+    const bool there = hd < w.rows && q < (h + 1) * a.group && d < a.dim;
+    float m = -INFINITY, l = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    if (there)
+        for (int p0 = sub; p0 < join.parts; p0 += kAhead * deep) {
+            PagedPart x[kAhead];
+            f32x4 y[kAhead];
 #pragma unroll
-    for (int i = 0; i < kPagedWaves; ++i) top = fmaxf(top, wave_x[i]);
-    __syncthreads();
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    for (int p = (int)threadIdx.x; p < join.parts; p += kPagedThreads) {
-        const PagedPart x = w.parts[slot(p) * kPagedHeads + blockIdx.y];
-        const float f = __builtin_amdgcn_exp2f(x.m - base);
-        lds[p] = f;
-        sum += f * x.l;
+            for (int i = 0; i < kAhead; ++i) {
+                const int p = p0 + i * deep;
+                x[i] = {-INFINITY, 0.f};
+                y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (p < join.parts) {
+                    const int64_t slot = 2 * (int64_t)(join.first + p) + (p == 0 ? 1 : 0);
+                    x[i] = w.parts[slot * kPagedHeads + hd];
+                    y[i] = *(const f32x4 *)(w.sums + (slot * w.rows + hd) * w.pitch + d);
+                }
+            }
+            float top = m;
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) top = fmaxf(top, x[i].m);
+            const float base = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f(m - base);
+            l *= old;
+            acc *= old;
+            m = top;
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const float f = __builtin_amdgcn_exp2f(x[i].m - base);
+                l += f * x[i].l;
+                acc += f * y[i];
+            }
+        }
+    if (deep > 1) {
+        rest_acc[mine][d / 4] = acc;
+        if (d == 0) { rest_m[mine] = m; rest_l[mine] = l; }
+        __syncthreads();
+        if (sub) return;
+        float top = m;
+        for (int i = 1; i < deep; ++i) top = fmaxf(top, rest_m[mine + i * heads]);
+        const float base = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f(m - base);
+        l *= old;
+        acc *= old;
+        for (int i = 1; i < deep; ++i) {
+            const float f = __builtin_amdgcn_exp2f(rest_m[mine + i * heads] - base);
+            l += f * rest_l[mine + i * heads];
+            acc += f * rest_acc[mine + i * heads][d / 4];
+        }
     }
-    sum = wave_sum(sum);
-    if (lane == 0) wave_x[wave] = sum;
-    __syncthreads();
-    sum = wave_x[0] + wave_x[1] + wave_x[2] + wave_x[3];
-    // threads [i * wide, (i + 1) * wide) add every `deep`-th part
-    const int wide = a.dim > 128 ? 256 : a.dim > 64 ? 128 : 64, deep = kPagedThreads / wide;
-    const int d = (int)threadIdx.x % wide, i = (int)threadIdx.x / wide;
-    float acc = 0.f;
-    if (d < a.dim)
-#pragma unroll 4
-        for (int p = i; p < join.parts; p += deep) acc += lds[p] * w.sums[(slot(p) * w.rows + blockIdx.y) * a.dim + d];
-    float *const rest = lds + join.parts;
-    rest[threadIdx.x] = acc;
-    __syncthreads();
-    if (i || d >= a.dim) return;
-    for (int k = 1; k < deep; ++k) acc += rest[k * wide + d];
-    const float v = acc * (a.v.scale ? a.v.scale[h] : 1.f) / sum;
-    ((uint16_t *)(a.out + q * a.out_head_bytes + join.request * a.out_row_bytes))[d] = Elem<DT>::from_float(v);
+    if (there) store_result<DT>(a.out + q * a.out_head_bytes + join.request * a.out_row_bytes, d, a.dim, acc * ((a.v.scale ? a.v.scale[h] : 1.f) / l));
 }
 
 // ------------------------------------------------------------------ host
@@ -464,7 +528,8 @@ static PagedWork work_of(int64_t heads, int64_t group, int64_t dim, int64_t requ
     const size_t entries = (size_t)(w.by_unit ? units : w.groups);
     const size_t joins = (entries * sizeof(PagedJoin) + 255) & ~size_t(255);
     const size_t parts = (2 * (size_t)w.groups * kPagedHeads * sizeof(PagedPart) + 255) & ~size_t(255);
-    const size_t sums = 2 * (size_t)w.groups * w.rows * dim * sizeof(float);
+    w.pitch = (int32_t)((dim + 3) & ~int64_t(3));
+    const size_t sums = 2 * (size_t)w.groups * w.rows * w.pitch * sizeof(float);
     if (bytes) *bytes = joins + parts + sums;
     if (workspace) {
         w.joins = (PagedJoin *)workspace;
@@ -488,10 +553,15 @@ static int launch_split(const PagedAttentionArgs &a, const PagedWork &w, hipStre
                                                            hipFuncAttributeMaxDynamicSharedMemorySize, kMostLds);
         if (attr != hipSuccess) return BA_ERR_LAUNCH;
     }
-    const size_t lds = (size_t)kPagedWaves * w.rows * (a.dim + 4) * sizeof(float);
+    const size_t lds = (size_t)kPagedWaves * w.rows * (DC + 4) * sizeof(float);
     paged_attention_kernel<DT, F8, DC, SHAPE, PAGES><<<w.groups, kPagedThreads, lds, stream>>>(a, w);
-    const dim3 grid((unsigned)(w.by_unit ? a.requests * a.heads * w.tiles_a_head : w.groups), (unsigned)w.rows);
-    paged_join_kernel<DT><<<grid, kPagedThreads, (w.groups + kPagedThreads) * sizeof(float), stream>>>(a, w);
+    // Few units have many parts each, and a workgroup joins one head of one; of many units most were not split, and a
+    // workgroup takes as many heads as it has threads for.
+    const int most = kPagedThreads / (DC / 4);
+    int heads = 1;
+    while (!w.by_unit && heads < most && heads < w.rows) heads *= 2;
+    const dim3 grid((unsigned)(w.by_unit ? a.requests * a.heads * w.tiles_a_head : w.groups), (unsigned)((w.rows + heads - 1) / heads));
+    paged_join_kernel<DT, DC><<<grid, kPagedThreads, 0, stream>>>(a, w, heads);
     return hipGetLastError() == hipSuccess ? BA_OK : BA_ERR_LAUNCH;
 }
 
