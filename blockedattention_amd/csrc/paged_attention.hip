@@ -10,13 +10,17 @@
 // fourth tile each; at the end of a unit their results are joined in LDS.  A unit that lies in one share is done
 // then; for others each workgroup leaves its maximum, sum and fp32 accumulators, and a second small kernel joins them.
 //
-// One tile.  Scores: S[token][head] = K Q^T with 16 tokens as the rows of a 16 x 16 x 32 matrix instruction; a lane's
-// operand is 16 bytes of one key, loaded straight from the cache.  A lane then holds the scores of tokens 4g..4g+3 of both
-// halves of the tile for one head (g = lane / 16): packed to 16 bits these are, as they are, its operand of the second
-// product if the reduction runs over the tokens in the order (half, g, i) -- no lane exchanges a probability.  Values: O[d][head]
-// = V^T P.  A lane loads 2 or more adjacent dimensions of its eight tokens (16 lanes cover a row: whole lines) and turns
-// the small matrix in registers: the operand of dimension j is made of the j-th halves of its eight rows.  Nothing of the cache
-// passes through LDS.
+// One tile.  Lanes that follow each other read bytes that follow each other, four lanes 64 of them and sixteen a row (of
+// 128 dimensions); nothing of the cache passes through LDS.  With lane = 16 g + 4 q + c:
+//   Scores, S[token][head] = K Q^T on the 16 x 16 x 32 matrix instruction.  It wants a lane to hold dimensions of token
+//   lane % 16, but loaded so every lane would be a memory access of its own and every line be asked for twice.  Instead
+//   load j gives the lane piece 4 g + c of token 4 q + j.  Multiplied with piece 4 g + c' of the queries, for c' = 0 .. 3,
+//   the rows 4 q + c of the result are right where c = c', and those lie in register c of the lanes that hold the rows of q:
+//   the score is the sum of register c' of product c'.  Four times the products, of which the matrix unit has plenty.
+//   A lane then holds the scores of tokens 4 g + j of both halves of the tile for head lane % 16: packed to 16 bits these
+//   are, as they are, its operand of the second product if that runs over the tokens in the order (half, g, j).
+//   Values, O[d][head] = V^T P.  A lane loads a piece of its eight tokens and turns the small matrix in registers: the
+//   operand of dimension j is made of the j-th halves of its eight rows.
 #include <algorithm>
 #include <type_traits>
 
@@ -36,6 +40,17 @@ constexpr int kPagedWhole = 8;               // units of up to so many tiles are
 // Probabilities are scaled by a power of two that keeps those of 2^-39 (and not 2^-24) of the largest apart from
 // zero in fp16; it is in the sums as well and drops out.
 template <int DT> constexpr float kLift = DT == 0 ? 14.f : 0.f;
+
+#ifndef BA_O64
+#define BA_O64 4
+#endif
+#ifndef BA_O128
+#define BA_O128 3
+#endif
+#ifndef BA_O256
+#define BA_O256 2
+#endif
+constexpr int resident_groups(int dim_class) { return dim_class == 64 ? BA_O64 : dim_class == 128 ? BA_O128 : BA_O256; }
 
 struct PagedPart {                           // what a workgroup leaves for a unit that others work on too
     float m, l;
@@ -75,6 +90,35 @@ enum Shape { kFull, kPieces, kAny };
 // What is known of the pages: whole halves of tiles, whole groups of four tokens, nothing.
 enum Pages { kHalves, kFours, kTokens };
 
+// The matrix product of part x of a load of a key (rows) with the same dimensions of the queries (columns).
+template <int DT, bool F8, int E, int N> __device__ __forceinline__ f32x4 product(const uint32_t (&k)[N], int x, u32x4 q, f32x4 c) {
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (F8) {
+#pragma unroll
+        for (int i = 0; i < (E < 8 ? 1 : 2); ++i) { w[2 * i] = widen<DT, false>(k[2 * x + i]); w[2 * i + 1] = widen<DT, true>(k[2 * x + i]); }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = k[i];
+    }
+    if constexpr (E < 8) {                   // four dimensions a lane
+        typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        const u32x2 ka = {w[0], w[1]}, qa = {q[0], q[1]};
+        if constexpr (DT == 0) return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, ka), __builtin_bit_cast(f16x4, qa), c, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, ka), __builtin_bit_cast(s16x4, qa), c, 0, 0, 0);
+    }
+    return Elem<DT>::mfma(u32x4{w[0], w[1], w[2], w[3]}, q, c);
+}
+
+// Whether keys are loaded in whole lines (see above).
+#ifndef BA_QUAD16
+#define BA_QUAD16 false
+#endif
+template <bool F8, int DC, Shape SHAPE> constexpr bool quad_keys = SHAPE != kAny && (F8 || BA_QUAD16);
+
+// Barrier that waits for this wavefront's LDS traffic only (the loads of the next unit stay in flight).
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 struct Visible {
     int first, len;                          // tokens first .. len - 1 are seen
     __device__ __forceinline__ int start() const { return first & ~(kPagedTile - 1); }
@@ -102,15 +146,18 @@ __device__ __forceinline__ int64_t scaled(int64_t x, int64_t y, int64_t z) {
 
 // DC: dimensions that the registers hold (64, 128, 256).
 template <int DT, bool F8, int DC, Shape SHAPE, Pages PAGES>
-__global__ void __launch_bounds__(kPagedThreads, DC == 64 ? 4 : DC == 128 ? 3 : 2)
+__global__ void __launch_bounds__(kPagedThreads, resident_groups(DC))
 paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
     constexpr int EB = F8 ? 1 : 2;           // bytes of an element
-    constexpr int KK = DC / 32;              // matrix instructions of a half's scores
-    constexpr int KL = KK * EB / 2;          // 16-byte pieces of a key that a lane holds
-    constexpr int PW = DC / 16;              // dimensions of a value that a lane holds
-    constexpr int VN = PW * EB / 4 > 4 ? 4 : PW * EB / 4;      // dwords of one load of them
-    constexpr int VL = PW * EB / 4 / VN;     // loads
-    const int lane = lane_id(), l16 = lane & 15, g = lane >> 4, wave = uniform((int)threadIdx.x >> 6);
+    constexpr int PW = DC / 16;              // dimensions of a row that a lane holds
+    constexpr int E = PW * EB < 16 ? PW : 16 / EB, N = E * EB / 4;      // those of one load, its dwords
+    constexpr int L = PW / E;                // loads; load k of lane x of a row: dimensions 16 E k + E x ..
+    constexpr bool QUAD = quad_keys<F8, DC, SHAPE>;
+    constexpr int PARTS = QUAD && E > 8 ? E / 8 : 1;           // matrix instructions that a load of a key feeds (for each c')
+    constexpr int KR = QUAD ? 8 : 2, KL = QUAD ? L : DC * EB / 64, KN = QUAD ? N : 4;      // a lane's tokens of a tile, loads of each, dwords
+    constexpr int QC = QUAD ? 4 : 1, QK = QUAD ? L * PARTS : DC / 32;                    // operands of the queries
+    constexpr int NPK = PAGES == kTokens && QUAD ? 8 : 2, NPV = PAGES == kHalves ? 0 : PAGES == kFours ? 2 : 8;
+    const int lane = lane_id(), l16 = lane & 15, g = lane >> 4, q4 = l16 >> 2, c4 = l16 & 3, wave = uniform((int)threadIdx.x >> 6);
     const int units = a.heads * w.tiles_a_head;
 
     extern __shared__ __attribute__((aligned(16))) float lds[];           // [waves][rows][DC + 4]
@@ -174,242 +221,298 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
         }
     }
     __syncthreads();
-    int request = uniform(places[0].request), unit = uniform(places[0].unit), tile = uniform(places[0].tile);
-    int64_t at = uniform64(places[0].at);
+    // What a workgroup does of a unit: tiles [tile, last) of n.
+    struct Unit {
+        int request, unit, tile, last, n, first, len, start, h, q0, rows;
+        int64_t at;                          // number of tile `tile` in the order of all
+    };
     const int64_t end = uniform64(places[1].at);
-    Visible see = {uniform(places[0].see.first), uniform(places[0].see.len)};
+    auto unit_of = [&](int request, int unit, int tile, int64_t at, Visible see) {
+        Unit u;
+        u.request = request; u.unit = unit; u.tile = tile; u.at = at;
+        u.first = see.first; u.len = see.len; u.n = see.tiles(); u.start = see.start();
+        u.last = (int)min((int64_t)u.n, tile + (end - at));
+        u.h = unit / w.tiles_a_head;
+        u.q0 = u.h * a.group + (unit - u.h * w.tiles_a_head) * w.rows;
+        u.rows = min(w.rows, (u.h + 1) * a.group - u.q0);
+        return u;
+    };
+    const Place place = places[0];
     PagedJoin join = {0, 0, 0, 0};
+    if (place.at >= end) {
+        if (!w.by_unit && threadIdx.x == 0) w.joins[group] = join;
+        return;
+    }
+    Unit cur = unit_of(uniform(place.request), uniform(place.unit), uniform(place.tile), uniform64(place.at),
+                       {uniform(place.see.first), uniform(place.see.len)});
 
-    while (at < end) {
-        const int first = see.first, len = see.len, n = see.tiles(), start = see.start();
-        const int last = (int)min((int64_t)n, tile + (end - at));      // tiles of this unit in this share: [tile, last)
-        const int h = unit / w.tiles_a_head, q0 = h * a.group + (unit - h * w.tiles_a_head) * w.rows;
-        const int rows = min(w.rows, (h + 1) * a.group - q0);
-        const char *const kh = a.k.base + h * a.k.head_bytes, *const vh = a.v.base + h * a.v.head_bytes;
-        typedef const __attribute__((address_space(4))) int32_t *Row;
-        const Row row = (Row)(uintptr_t)(a.table + request * a.table_stride);
-
-        // queries: head l16 in the order of dimensions in which the keys arrive
-        u32x4 qf[KK];
+    // queries: of head l16, in the order of dimensions in which the keys arrive
+    u32x4 qf[QC][QK];
+    auto load_queries = [&](const Unit &u) {
 #pragma unroll
-        for (int i = 0; i < KK; ++i) {
-            const int d = F8 ? 64 * (i / 2) + 16 * g + 8 * (i % 2) : 32 * i + 8 * g;
-            uint32_t x[4] = {0, 0, 0, 0};
-            const char *const p = a.q + (q0 + l16) * a.q_head_bytes + request * a.q_row_bytes + 2 * d;
-            if (l16 < rows) {
-                if (SHAPE == kAny) load_part<4>(x, p, 2 * (a.dim - d));
-                else if (SHAPE == kFull || d < a.dim) load_stream<4>(x, p);
-            }
-            qf[i] = u32x4{x[0], x[1], x[2], x[3]};
-        }
-        const float to_log2 = a.scale * kLog2e * (F8 ? a.k.scale[h] : 1.f);
-
-        f32x4 o[PW];
-        float m = -INFINITY, l = 0.f;
+        for (int c = 0; c < QC; ++c)
 #pragma unroll
-        for (int j = 0; j < PW; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-        // Pages and lines of a tile.  Tokens that are not seen may have no page (any more): a half, a group of four or a token
-        // without any that is seen borrows the place of one with.  Page numbers outside the cache become page 0 and poison
-        // the result.
-        constexpr int NK = 2, NV = PAGES == kHalves ? 0 : PAGES == kFours ? 2 : 8;
-        int32_t page[NK + NV], line[NK + NV];
-        bool poison = a.pages == 0;
-        auto look_up = [&](int t0) {
-            if (PAGES == kHalves) {
-                int t[2] = {t0, t0 + 16};
-                if (t[1] >= len) t[1] = t[0];
-                if (t[0] + 16 <= first) t[0] = t[1];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t c = a.page.div((uint32_t)t[i]);
-                    page[i] = row[c];
-                    line[i] = t[i] - (int)(c * a.page.d);
+            for (int k = 0; k < QK; ++k) {
+                constexpr int QN = QUAD && E < 8 ? 2 : 4;
+                const int d = QUAD ? 16 * E * (k / PARTS) + E * (4 * g + c) + 8 * (k % PARTS)
+                              : F8 ? 64 * (k / 2) + 16 * g + 8 * (k % 2) : 32 * k + 8 * g;
+                uint32_t x[QN] = {};
+                const char *const p = a.q + (u.q0 + l16) * a.q_head_bytes + u.request * a.q_row_bytes + 2 * d;
+                if (l16 < u.rows) {
+                    if (SHAPE == kAny) load_part<QN>(x, p, 2 * (a.dim - d));
+                    else if (SHAPE == kFull || d < a.dim) load_stream<QN>(x, p);
                 }
-            } else {
-                constexpr int four = PAGES == kFours ? 3 : 0;
-#pragma unroll
-                for (int i = 0; i < NK + NV; ++i) {
-                    const int mine = i < NK ? t0 + 16 * i + l16
-                                     : PAGES == kFours ? t0 + 16 * (i - NK) + 4 * g
-                                                       : t0 + 16 * ((i - NK) / 4) + 4 * g + (i - NK) % 4;
-                    const int t = min(max(mine & ~four, first & ~four), (len - 1) & ~four) + (mine & four);
-                    const uint32_t c = a.page.div((uint32_t)t);
-                    page[i] = a.table[request * a.table_stride + c];
-                    line[i] = t - (int)(c * a.page.d);
-                }
+                qf[c][k] = u32x4{x[0], x[1], x[QN - 2], x[QN - 1]};
             }
-        };
-        auto checked = [&](int i) {
-            const int32_t p = PAGES == kHalves ? uniform(page[i]) : page[i];
-            const bool bad = (uint32_t)p >= (uint32_t)a.pages;
-            poison |= bad;
-            return bad ? 0 : p;
-        };
-        // Pieces that are not there (kPieces) are loaded from the row's front: those of a key count as zeros, those of a value
-        // make results that nobody stores.
-        uint32_t kx[2][KL][4], vx[8][VL][VN];
-        auto load_keys = [&] {
+    };
+
+    // Pages and lines of a tile.  Tokens that are not seen may have no page (any more): a half, a group of four or a token
+    // without any that is seen borrows the place of one with.  Page numbers outside the cache become page 0 and poison
+    // the result.
+    int32_t page[NPK + NPV], line[NPK + NPV];
+    bool poison = false;
+    auto look_up = [&](const Unit &u, int t0) {
+        if (PAGES == kHalves) {
+            typedef const __attribute__((address_space(4))) int32_t *Row;      // the same for all lanes: scalar loads
+            const Row row = (Row)(uintptr_t)(a.table + u.request * a.table_stride);
+            int t[2] = {t0, t0 + 16};
+            if (t[1] >= u.len) t[1] = t[0];
+            if (t[0] + 16 <= u.first) t[0] = t[1];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int32_t p = checked(i), ln = PAGES == kHalves ? uniform(line[i]) : line[i];
-                const char *const base = kh + p * a.k.page_bytes + (int64_t)ln * a.k.token_bytes;
+                const uint32_t c = a.page.div((uint32_t)t[i]);
+                page[i] = row[c];
+                line[i] = t[i] - (int)(c * a.page.d);
+            }
+        } else {
+            constexpr int four = PAGES == kFours ? 3 : 0;
+#pragma unroll
+            for (int i = 0; i < NPK + NPV; ++i) {
+                const int k = i < NPK ? i : i - NPK, x = i < NPK ? q4 : g;
+                const int mine = i < NPK && !QUAD ? t0 + 16 * k + l16 : PAGES == kFours ? t0 + 16 * k + 4 * x : t0 + 16 * (k / 4) + 4 * x + k % 4;
+                const int t = min(max(mine & ~four, u.first & ~four), (u.len - 1) & ~four) + (mine & four);
+                const uint32_t c = a.page.div((uint32_t)t);
+                page[i] = a.table[u.request * a.table_stride + c];
+                line[i] = t - (int)(c * a.page.d);
+            }
+        }
+    };
+    // Where token line[i] of page[i] lies in an array, for a head.
+    auto place_of = [&](const PagedArray &array, int h, int i) {
+        int32_t p = page[i], ln = line[i];
+        if (PAGES == kHalves) { p = uniform(p); ln = uniform(ln); }
+        const bool bad = (uint32_t)p >= (uint32_t)a.pages;
+        poison |= bad;
+        return array.base + h * array.head_bytes + (bad ? 0 : p) * array.page_bytes + (int64_t)ln * array.token_bytes;
+    };
+    // Pieces that are not there (kPieces) are loaded from the row's front: those of a key count as zeros, those of a value
+    // make results that nobody stores.
+    uint32_t kx[KR][KL][KN], vx[8][L][N];
+    auto load_keys = [&](const Unit &u) {
+        if (QUAD) {
+#pragma unroll
+            for (int i = 0; i < KR; ++i) {
+                const char *const base = place_of(a.k, u.h, PAGES == kTokens ? i : i / 4);
+                const uint32_t mine = PAGES == kHalves ? (uint32_t)((4 * q4 + i % 4) * a.k.token_bytes) : PAGES == kFours ? (uint32_t)(i % 4 * a.k.token_bytes) : 0u;
+#pragma unroll
+                for (int k = 0; k < KL; ++k) {
+                    const uint32_t b = EB * E * (16 * k + 4 * g + c4);
+                    if (SHAPE == kPieces) load_stream<KN>(kx[i][k], base + (mine + ((int)b < EB * a.dim ? b : 0u)));
+                    else load_stream<KN>(kx[i][k], base + (mine + (uint32_t)(EB * E * (4 * g + c4))) + EB * E * 16 * k);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < KR; ++i) {
+                const char *const base = place_of(a.k, u.h, i);
                 const uint32_t mine = PAGES == kHalves ? (uint32_t)(l16 * a.k.token_bytes) : 0u;
 #pragma unroll
                 for (int k = 0; k < KL; ++k) {
                     const uint32_t b = 64 * k + 16 * g;
-                    if (SHAPE == kAny) load_part<4>(kx[i][k], base + (mine + b), EB * a.dim - (int)b);
-                    else if (SHAPE == kPieces) load_stream<4>(kx[i][k], base + (mine + ((int)b < EB * a.dim ? b : 0u)));
-                    else load_stream<4>(kx[i][k], base + (mine + 16u * g) + 64 * k);
+                    if (SHAPE == kAny) load_part<KN>(kx[i][k], base + (mine + b), EB * a.dim - (int)b);
+                    else if (SHAPE == kPieces) load_stream<KN>(kx[i][k], base + (mine + ((int)b < EB * a.dim ? b : 0u)));
+                    else load_stream<KN>(kx[i][k], base + (mine + 16u * g) + 64 * k);
                 }
             }
-        };
-        auto load_values = [&] {
+        }
+    };
+    auto load_values = [&](const Unit &u) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const char *const base = place_of(a.v, u.h, PAGES == kHalves ? i / 4 : PAGES == kFours ? NPK + i / 4 : NPK + i);
+            const uint32_t mine = PAGES == kHalves ? (uint32_t)((4 * g + i % 4) * a.v.token_bytes) : PAGES == kFours ? (uint32_t)(i % 4 * a.v.token_bytes) : 0u;
+#pragma unroll
+            for (int k = 0; k < L; ++k) {
+                const uint32_t b = EB * E * (16 * k + l16);
+                if (SHAPE == kAny) load_part<N>(vx[i][k], base + (mine + b), EB * a.dim - (int)b);
+                else if (SHAPE == kPieces) load_stream<N>(vx[i][k], base + (mine + ((int)b < EB * a.dim ? b : 0u)));
+                else load_stream<N>(vx[i][k], base + (mine + (uint32_t)(EB * E * l16)) + EB * E * 16 * k);
+            }
+        }
+    };
+    // The wavefront's first tile of a unit.
+    auto has_tile = [&](const Unit &u) { return u.tile + wave < u.last && u.len > u.first && a.pages > 0; };
+    auto load_first = [&](const Unit &u) {
+        load_queries(u);
+        if (has_tile(u)) {
+            look_up(u, u.start + (u.tile + wave) * kPagedTile);
+            load_keys(u);
+            load_values(u);
+        }
+    };
+
+    f32x4 o[PW];
+    float m, l;
+    // The tile that begins with token t0; MORE: the wavefront's next one of the unit follows, whose keys are asked for as soon
+    // as the scores have used this one's, and its values likewise.
+    auto attend = [&](const Unit &u, auto more, int t0, float to_log2) {
+        constexpr bool MORE = decltype(more)::value;
+        if (SHAPE == kPieces) {
+#pragma unroll
+            for (int k = 0; k < KL; ++k) {
+                const int b = QUAD ? EB * E * (16 * k + 4 * g + c4) : 64 * k + 16 * g;
+                if ((QUAD ? EB * E * 16 : 64) * (k + 1) > EB * a.dim) {
+#pragma unroll
+                    for (int i = 0; i < KR; ++i)
+#pragma unroll
+                        for (int x = 0; x < KN; ++x) kx[i][k][x] = b < EB * a.dim ? kx[i][k][x] : 0u;
+                }
+            }
+        }
+        // ---- scores of tokens t0 + 16 i + 4 g + j
+        f32x4 sc[2];
+        if (QUAD) {
+#pragma unroll
+            for (int i = 0; i < KR; ++i) {
+                f32x4 s4[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    s4[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < QK; ++k) s4[c] = product<DT, F8, E>(kx[i][k / PARTS], k % PARTS, qf[c % QC][k], s4[c]);
+                }
+                sc[i / 4][i % 4] = ((s4[0][0] + s4[1][1]) + (s4[2][2] + s4[3][3])) * to_log2;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < KR; ++i) {
+                f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < QK; ++k) s = product<DT, F8, F8 ? 16 : 8>(kx[i][F8 ? k / 2 : k], F8 ? k % 2 : 0, qf[0][k], s);
+                sc[i % 2] = s * to_log2;
+            }
+        }
+        if (MORE) load_keys(u);
+        if (t0 < u.first || t0 + kPagedTile > u.len) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int from = PAGES == kHalves ? i / 4 : PAGES == kFours ? NK + i / 4 : NK + i;
-                const int32_t p = checked(from), ln = PAGES == kHalves ? uniform(line[from]) : line[from];
-                const char *const base = vh + p * a.v.page_bytes + (int64_t)ln * a.v.token_bytes;
-                const uint32_t mine = PAGES == kHalves ? (uint32_t)((4 * g + i % 4) * a.v.token_bytes) : PAGES == kFours ? (uint32_t)(i % 4 * a.v.token_bytes) : 0u;
+                const int t = t0 + 16 * (i / 4) + 4 * g + i % 4;
+                const bool seen = t >= u.first && t < u.len;
+                sc[i / 4][i % 4] = seen ? sc[i / 4][i % 4] : -INFINITY;
 #pragma unroll
-                for (int k = 0; k < VL; ++k) {
-                    const uint32_t b = EB * PW * l16 + 16 * k;
-                    if (SHAPE == kAny) load_part<VN>(vx[i][k], base + (mine + b), EB * a.dim - (int)b);
-                    else if (SHAPE == kPieces) load_stream<VN>(vx[i][k], base + (mine + ((int)b < EB * a.dim ? b : 0u)));
-                    else load_stream<VN>(vx[i][k], base + (mine + (uint32_t)(EB * PW * l16)) + 16 * k);
-                }
+                for (int k = 0; k < L; ++k)
+#pragma unroll
+                    for (int x = 0; x < N; ++x) vx[i][k][x] = seen ? vx[i][k][x] : 0u;    // (a probability of 0 times what lies there may be NaN)
             }
-        };
-        // The tile that begins with token t0; MORE: the wavefront's next one follows, whose keys are asked for as soon as the
-        // scores have used this one's, and its values likewise.
-        auto attend = [&](auto more, int t0) {
-            constexpr bool MORE = decltype(more)::value;
-            if (SHAPE == kPieces) {
+        }
+        float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                          fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+        top = fmaxf(m, quad_column_max(top));
+        const float base = (top == -INFINITY ? 0.f : top) - kLift<DT>;
+        if (__any(top != m)) {
+            const float shrink = __builtin_amdgcn_exp2f(m - kLift<DT> - base);
+            l *= shrink;
 #pragma unroll
-                for (int k = 0; k < KL; ++k)
-                    if (64 * k + 64 > EB * a.dim) {
+            for (int j = 0; j < PW; ++j) o[j] *= shrink;
+            m = top;
+        }
+        float p[8];
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 8; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(sc[i / 4][i % 4] - base);
+            l += p[i];
+        }
+        // Probabilities in two 16-bit terms: one alone would cost as much accuracy as the rounding of the result, and the
+        // matrix unit has time to spare.
+        uint32_t hi[4], lo[4];
 #pragma unroll
-                            for (int x = 0; x < 4; ++x) kx[i][k][x] = 64 * k + 16 * g < EB * a.dim ? kx[i][k][x] : 0u;
-                    }
-            }
-            // ---- scores of tokens t0 + 16 i + 4 g + e
-            f32x4 sc[2];
+        for (int i = 0; i < 4; ++i) {
+            hi[i] = Elem<DT>::pack2(p[2 * i], p[2 * i + 1]);
+            lo[i] = Elem<DT>::pack2(p[2 * i] - Elem<DT>::to_float((uint16_t)hi[i]), p[2 * i + 1] - Elem<DT>::to_float((uint16_t)(hi[i] >> 16)));
+        }
+        // ---- values
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                sc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int k = 0; k < KL; ++k) {
-                    if (F8) {
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const uint32_t x = kx[i][k][2 * half], y = kx[i][k][2 * half + 1];
-                            sc[i] = Elem<DT>::mfma(u32x4{widen<DT, false>(x), widen<DT, true>(x), widen<DT, false>(y), widen<DT, true>(y)},
-                                                   qf[(2 * k + half) % KK], sc[i]);
-                        }
-                    } else {
-                        sc[i] = Elem<DT>::mfma(u32x4{kx[i][k][0], kx[i][k][1], kx[i][k][2], kx[i][k][3]}, qf[k % KK], sc[i]);
-                    }
-                }
-                sc[i] *= to_log2;
-            }
-            if (MORE) load_keys();
-            if (t0 < first || t0 + kPagedTile > len) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int t = t0 + 16 * (i / 4) + 4 * g + i % 4;
-                    const bool seen = t >= first && t < len;
-                    sc[i / 4][i % 4] = seen ? sc[i / 4][i % 4] : -INFINITY;
-#pragma unroll
-                    for (int k = 0; k < VL; ++k)
-#pragma unroll
-                        for (int x = 0; x < VN; ++x) vx[i][k][x] = seen ? vx[i][k][x] : 0u;    // (a probability of 0 times what lies there may be NaN)
-                }
-            }
-            float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
-                              fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
-            top = fmaxf(m, quad_column_max(top));
-            const float base = (top == -INFINITY ? 0.f : top) - kLift<DT>;
-            if (__any(top != m)) {
-                const float shrink = __builtin_amdgcn_exp2f(m - kLift<DT> - base);
-                l *= shrink;
-#pragma unroll
-                for (int j = 0; j < PW; ++j) o[j] *= shrink;
-                m = top;
-            }
-            float p[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                p[i] = __builtin_amdgcn_exp2f(sc[i / 4][i % 4] - base);
-                l += p[i];
-            }
-            // Probabilities in two 16-bit terms: one alone would cost as much accuracy as the rounding of the result, and the
-            // matrix unit has time to spare.
-            uint32_t hi[4], lo[4];
+        for (int j = 0; j < PW; ++j) {
+            uint32_t f[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                hi[i] = Elem<DT>::pack2(p[2 * i], p[2 * i + 1]);
-                lo[i] = Elem<DT>::pack2(p[2 * i] - Elem<DT>::to_float((uint16_t)hi[i]), p[2 * i + 1] - Elem<DT>::to_float((uint16_t)(hi[i] >> 16)));
-            }
-            // ---- values
-#pragma unroll
-            for (int j = 0; j < PW; ++j) {
-                uint32_t f[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (F8) {
-                        // byte j of both rows next to each other, then widened together
-                        const uint32_t both = __builtin_amdgcn_perm(vx[2 * i + 1][j / 4 / VN][j / 4 % VN], vx[2 * i][j / 4 / VN][j / 4 % VN],
-                                                                    0x0c0c0400u + (uint32_t)(j % 4) * 0x0101u);
-                        f[i] = widen<DT, false>(both);
-                    } else {
-                        f[i] = __builtin_amdgcn_perm(vx[2 * i + 1][j / 2 / VN][j / 2 % VN], vx[2 * i][j / 2 / VN][j / 2 % VN],
-                                                     j % 2 ? 0x07060302u : 0x05040100u);
-                    }
+                const int k = j / E, x = j % E;
+                if (F8) {
+                    // byte x of both rows next to each other, then widened together
+                    const uint32_t both = __builtin_amdgcn_perm(vx[2 * i + 1][k][x / 4], vx[2 * i][k][x / 4], 0x0c0c0400u + (uint32_t)(x % 4) * 0x0101u);
+                    f[i] = widen<DT, false>(both);
+                } else {
+                    f[i] = __builtin_amdgcn_perm(vx[2 * i + 1][k][x / 2], vx[2 * i][k][x / 2], x % 2 ? 0x07060302u : 0x05040100u);
                 }
-                const u32x4 v = {f[0], f[1], f[2], f[3]};
-                o[j] = Elem<DT>::mfma(v, u32x4{hi[0], hi[1], hi[2], hi[3]}, o[j]);
-                o[j] = Elem<DT>::mfma(v, u32x4{lo[0], lo[1], lo[2], lo[3]}, o[j]);
             }
-            if (MORE) load_values();
-        };
-        int s = tile + wave;
-        if (s < last && len > first && a.pages > 0) {
-            constexpr int kStep = kPagedWaves * kPagedTile;
-            int t0 = start + s * kPagedTile;
-            look_up(t0);
-            load_keys();
-            load_values();
-            for (; s + kPagedWaves < last; s += kPagedWaves, t0 += kStep) {
-                look_up(t0 + kStep);
-                attend(std::true_type{}, t0);
-            }
-            attend(std::false_type{}, t0);
+            const u32x4 v = {f[0], f[1], f[2], f[3]};
+            o[j] = Elem<DT>::mfma(v, u32x4{hi[0], hi[1], hi[2], hi[3]}, o[j]);
+            o[j] = Elem<DT>::mfma(v, u32x4{lo[0], lo[1], lo[2], lo[3]}, o[j]);
         }
-        if (__any(poison)) l = NAN;
+        if (MORE) load_values(u);
+    };
 
-        // ---- join the wavefronts: lane (g, l16) has dimensions PW (4 g + i) + j of head l16
+    load_first(cur);
+    for (;;) {
+        const float to_log2 = a.scale * kLog2e * (F8 ? a.k.scale[cur.h] : 1.f);
+        m = -INFINITY; l = 0.f;
+#pragma unroll
+        for (int j = 0; j < PW; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (has_tile(cur)) {
+            constexpr int kStep = kPagedWaves * kPagedTile;
+            int s = cur.tile + wave, t0 = cur.start + s * kPagedTile;
+            for (; s + kPagedWaves < cur.last; s += kPagedWaves, t0 += kStep) {
+                look_up(cur, t0 + kStep);
+                attend(cur, std::true_type{}, t0, to_log2);
+            }
+            attend(cur, std::false_type{}, t0, to_log2);
+        }
+        if (__any(poison) || (a.pages == 0 && cur.len > cur.first)) l = NAN;
+        poison = false;
+        // the next unit's first tile is on its way while this one is finished
+        Unit next = cur;
+        const int64_t at = cur.at + (cur.last - cur.tile);
+        if (at < end) {
+            if (cur.unit + 1 < units) {
+                next = unit_of(cur.request, cur.unit + 1, 0, at, {cur.first, cur.len});
+            } else {
+                const Visible v = visible(a, cur.request + 1);
+                next = unit_of(cur.request + 1, 0, 0, at, {uniform(v.first), uniform(v.len)});
+            }
+            load_first(next);
+        }
+
+        // ---- join the wavefronts: lane (g, l16) has dimensions 16 E k + E (4 g + i) + x of head l16, j = E k + x
         constexpr int pitch = DC + 4;
-        const int busy = min(last - tile, kPagedWaves);
+        const int busy = min(cur.last - cur.tile, kPagedWaves);
         l = quad_column_sum(l);
         if (wave < busy) {
             if (g == 0) { wave_m[wave][l16] = m; wave_l[wave][l16] = l; }
-            if (l16 < rows) {
+            if (l16 < cur.rows) {
                 float *const mineo = lds + (wave * w.rows + l16) * pitch;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int j = 0; j < PW; j += 4) {
-                        const int d = PW * (4 * g + i) + j;
+                        const int d = 16 * E * (j / E) + E * (4 * g + i) + j % E;
                         if (SHAPE == kFull || d < a.dim) *(f32x4 *)(mineo + d) = f32x4{o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]};
                     }
             }
         }
-        __syncthreads();
-        const bool begun = tile == 0, done = last == n, whole = begun && done;
+        lds_barrier();
+        const bool begun = cur.tile == 0, done = cur.last == cur.n, whole = begun && done;
         const int slot = 2 * (int)group + (begun ? 1 : 0);
-        for (int x = 4 * (int)threadIdx.x; x < rows * DC; x += 4 * kPagedThreads) {
+        for (int x = 4 * (int)threadIdx.x; x < cur.rows * DC; x += 4 * kPagedThreads) {
             const int hd = x / DC, d = x % DC;
             if (d >= a.dim) continue;
             float top = -INFINITY, sum = 0.f;
@@ -422,9 +525,9 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
                 acc += f * *(const f32x4 *)(lds + (i * w.rows + hd) * pitch + d);
             }
             if (whole) {
-                const float f = len > first ? (F8 ? a.v.scale[h] : 1.f) / sum : 0.f;
-                if (len <= first) acc = f32x4{0.f, 0.f, 0.f, 0.f};
-                store_result<DT>(a.out + (q0 + hd) * a.out_head_bytes + request * a.out_row_bytes, d, a.dim, acc * f);
+                const float f = cur.len > cur.first ? (F8 ? a.v.scale[cur.h] : 1.f) / sum : 0.f;
+                if (cur.len <= cur.first) acc = f32x4{0.f, 0.f, 0.f, 0.f};
+                store_result<DT>(a.out + (cur.q0 + hd) * a.out_head_bytes + cur.request * a.out_row_bytes, d, a.dim, acc * f);
             } else {
                 *(f32x4 *)(w.sums + ((int64_t)slot * w.rows + hd) * w.pitch + d) = acc;
                 if (d == 0) w.parts[slot * kPagedHeads + hd] = {top, sum};
@@ -432,20 +535,14 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
         }
         if (begun) {
             // who has the unit's last tile
-            const int parts = done ? 0 : (int)(scaled(at - tile + n, groups, total) + (scaled(at - tile + n, groups, total) * total < (at - tile + n) * groups) - group);
-            join = {request, unit, (int)group, parts};
-            if (w.by_unit && threadIdx.x == 0) w.joins[(int64_t)request * units + unit] = join;
+            const int64_t stop = cur.at + cur.n;
+            const int parts = done ? 0 : (int)(scaled(stop, groups, total) + (scaled(stop, groups, total) * total < stop * groups) - group);
+            join = {cur.request, cur.unit, (int)group, parts};
+            if (w.by_unit && threadIdx.x == 0) w.joins[(int64_t)cur.request * units + cur.unit] = join;
         }
-        at += last - tile;
-        tile = 0;
-        if (++unit == units) {
-            unit = 0;
-            if (++request < a.requests) {
-                const Visible v = visible(a, request);
-                see = {uniform(v.first), uniform(v.len)};
-            }
-        }
-        __syncthreads();
+        if (at >= end) break;
+        lds_barrier();
+        cur = next;
     }
     if (!w.by_unit && threadIdx.x == 0) w.joins[group] = join;
 }
@@ -520,7 +617,7 @@ static PagedWork work_of(int64_t heads, int64_t group, int64_t dim, int64_t requ
     PagedWork w{};
     w.tiles_a_head = (int32_t)((group + kPagedHeads - 1) / kPagedHeads);
     w.rows = (int32_t)((group + w.tiles_a_head - 1) / w.tiles_a_head);
-    const int64_t resident = (int64_t)device_cu_count() * (dim_class(dim) == 64 ? 4 : dim_class(dim) == 128 ? 3 : 2);
+    const int64_t resident = (int64_t)device_cu_count() * resident_groups(dim_class(dim));
     const int64_t units = requests * heads * w.tiles_a_head;
     const double tiles = (double)units * ((double)width * page / kPagedTile + 1);
     w.groups = (int32_t)std::max<int64_t>(1, (int64_t)std::min<double>((double)resident, tiles / kPagedShare + 1));
