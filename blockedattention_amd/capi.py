@@ -25,6 +25,7 @@ SYMBOLS = (
 )
 MAILBOX_BYTES = 320
 STATIC_MAX_SEGMENTS = 4096   # BA_STATIC_MAX_SEGMENTS
+PAGED_COUNTERS = 4096        # BA_PAGED_COUNTERS
 
 
 class PlanInfo(ctypes.Structure):
@@ -130,7 +131,7 @@ def load():
     lib.ba_paged_attention_workspace.restype = ctypes.c_size_t
     lib.ba_paged_attention_workspace.argtypes = [cache, i64, i64, i64]
     lib.ba_paged_attention.restype = i32
-    lib.ba_paged_attention.argtypes = [cache, i32, vp, i64, i64, i64, i64, vp, i64, i64, vp, i64, f32, vp, i64, i64, vp,
+    lib.ba_paged_attention.argtypes = [cache, i32, vp, i64, i64, i64, i64, vp, i64, i64, vp, i64, f32, vp, i64, i64, vp, vp,
                                        ctypes.c_size_t, vp]
     _lib = lib
     return lib
@@ -371,12 +372,18 @@ def paged_append(cache, k, v, slots):
     check(st, "ba_paged_append")
 
 
-def paged_attention(cache, q, table, lens, out, scale=1.0, window=0):
+def paged_counters(device):
+    """The counters of paged_attention: calls on one stream may share them."""
+    return torch.zeros(PAGED_COUNTERS, dtype=torch.int32, device=device)
+
+
+def paged_attention(cache, q, table, lens, out, scale=1.0, window=0, counters=None):
     """out [heads, requests, dim] <- attention of q over the requests' pages (see ba_paged_attention)."""
+    counters = paged_counters(q.device) if counters is None else counters
     need = load().ba_paged_attention_workspace(ctypes.byref(cache), q.size(0), q.size(1), table.size(1))
     work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     st = load().ba_paged_attention(ctypes.byref(cache), dtype_code(q.dtype), _ptr(q), q.stride(0), q.stride(1), q.size(0), q.size(1),
                                    _ptr(table), table.stride(0), table.size(1), _ptr(lens), window, float(scale), _ptr(out),
-                                   out.stride(0), out.stride(1), _ptr(work), need, _stream())
+                                   out.stride(0), out.stride(1), _ptr(counters), _ptr(work), need, _stream())
     check(st, "ba_paged_attention")
     return out

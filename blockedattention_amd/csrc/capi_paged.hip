@@ -92,7 +92,7 @@ __attribute__((visibility("default"))) int ba_paged_append(const ba_paged_cache 
 __attribute__((visibility("default"))) size_t ba_paged_attention_workspace(const ba_paged_cache *cache, int64_t heads,
                                                                            int64_t requests, int64_t width) {
     if (check_cache(cache) != BA_OK || heads < 1 || heads % cache->heads || requests < 1 || width < 0) return 0;
-    return paged_attention_workspace(cache->heads, heads / cache->heads, cache->dim, requests, width, cache->page);
+    return paged_attention_workspace(cache->heads, heads / cache->heads, cache->dim, cache->dtype, requests, width, cache->page);
 }
 
 __attribute__((visibility("default"))) int ba_paged_attention(const ba_paged_cache *cache, int dtype, const void *q,
@@ -100,7 +100,7 @@ __attribute__((visibility("default"))) int ba_paged_attention(const ba_paged_cac
                                                               int64_t requests, const int32_t *table, int64_t table_stride,
                                                               int64_t width, const int64_t *lens, int64_t window,
                                                               float scale, void *out, int64_t out_head_stride,
-                                                              int64_t out_row_stride, void *workspace,
+                                                              int64_t out_row_stride, int32_t *counters, void *workspace,
                                                               size_t workspace_bytes, ba_stream_t stream) {
     const int st = check_cache(cache);
     if (st != BA_OK) return st;
@@ -110,7 +110,7 @@ __attribute__((visibility("default"))) int ba_paged_attention(const ba_paged_cac
     if (bad_stride(q_head_stride) || bad_stride(q_row_stride) || bad_stride(out_head_stride) || bad_stride(out_row_stride))
         return BA_ERR_INVALID_ARG;
     if (requests == 0) return BA_OK;
-    if (!q || !out || !lens || (width > 0 && !table)) return BA_ERR_INVALID_ARG;
+    if (!q || !out || !lens || !counters || (width > 0 && !table)) return BA_ERR_INVALID_ARG;
     if (requests > 1 && width > 0 && table_stride < width) return BA_ERR_INVALID_ARG;
     if (heads >= (1 << 20) || requests >= kTokenLimit / heads || width >= kTokenLimit / cache->page) return BA_ERR_UNSUPPORTED;
     const size_t need = ba_paged_attention_workspace(cache, heads, requests, width);
@@ -125,7 +125,7 @@ __attribute__((visibility("default"))) int ba_paged_attention(const ba_paged_cac
     a.dim = (int32_t)cache->dim; a.pages = (int32_t)cache->pages; a.width = (int32_t)width;
     a.window = (int32_t)std::min<int64_t>(window, kTokenLimit - 1);
     a.scale = scale; a.page = PageDiv::of((uint32_t)cache->page);
-    return launch_paged_attention(a, dtype, cache->dtype, workspace, (hipStream_t)stream);
+    return launch_paged_attention(a, dtype, cache->dtype, counters, workspace, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -103,7 +103,7 @@ template <int N> __device__ __forceinline__ void load_part(uint32_t (&x)[N], con
 size_t paged_tables_workspace(int64_t requests);
 int launch_paged_tables(const PagedTablesArgs &args, void *workspace, hipStream_t stream);
 int launch_paged_append(const PagedAppendArgs &args, int dtype, int cache_dtype, hipStream_t stream);
-size_t paged_attention_workspace(int64_t cache_heads, int64_t group, int64_t dim, int64_t requests, int64_t width, int64_t page);
-int launch_paged_attention(const PagedAttentionArgs &args, int dtype, int cache_dtype, void *workspace, hipStream_t stream);
+size_t paged_attention_workspace(int64_t cache_heads, int64_t group, int64_t dim, int cache_dtype, int64_t requests, int64_t width, int64_t page);
+int launch_paged_attention(const PagedAttentionArgs &args, int dtype, int cache_dtype, int32_t *counters, void *workspace, hipStream_t stream);
 
 }  // namespace ba

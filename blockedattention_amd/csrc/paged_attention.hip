@@ -8,7 +8,8 @@
 // the tiles of all units, in order, are dealt out to the workgroups in equal shares (the lengths are on the GPU only, so
 // every workgroup adds them up itself).  A workgroup goes through its share unit by unit, its four wavefronts taking every
 // fourth tile each; at the end of a unit their results are joined in LDS.  A unit that lies in one share is done
-// then; for others each workgroup leaves its maximum, sum and fp32 accumulators, and a second small kernel joins them.
+// then; for others each workgroup leaves its maximum, sum and fp32 accumulators in memory and counts itself in, and the
+// last one there joins them all, in the order of the tokens whoever it is.
 //
 // One tile.  Lanes that follow each other read bytes that follow each other, four lanes 64 of them and sixteen a row (of
 // 128 dimensions); nothing of the cache passes through LDS.  With lane = 16 g + 4 q + c:
@@ -25,6 +26,7 @@
 #include <type_traits>
 
 #include "ba_device.hpp"
+#include "ba_gemm_common.hpp"
 #include "ba_host.hpp"
 #include "paged.hpp"
 
@@ -35,6 +37,8 @@ constexpr int kPagedThreads = 64 * kPagedWaves;
 constexpr int kPagedTile = 32;               // tokens
 constexpr int kPagedHeads = 16;              // query heads of a unit at most
 constexpr int kPagedShare = kPagedWaves;     // tiles of a workgroup at least
+constexpr int kPagedFewParts = 8;            // parts of a unit, on the average, up to which the kernel itself joins them
+constexpr int kPagedJoins = 512;             // workgroups of the joining kernel, where it has a choice
 constexpr int kPagedWhole = 8;               // units of up to so many tiles are not split between workgroups
 
 // Probabilities are scaled by a power of two that keeps those of 2^-39 (and not 2^-24) of the largest apart from
@@ -48,23 +52,25 @@ template <int DT> constexpr float kLift = DT == 0 ? 14.f : 0.f;
 #define BA_O128 3
 #endif
 #ifndef BA_O256
-#define BA_O256 2
+#define BA_O256 1
 #endif
-constexpr int resident_groups(int dim_class) { return dim_class == 64 ? BA_O64 : dim_class == 128 ? BA_O128 : BA_O256; }
+constexpr int resident_groups(int dim_class, bool f8) { return dim_class == 64 ? BA_O64 : dim_class == 128 ? BA_O128 : f8 ? 2 : BA_O256; }
 
-struct PagedPart {                           // what a workgroup leaves for a unit that others work on too
+struct alignas(8) PagedPart {                // what a workgroup leaves for a unit that others work on too
     float m, l;
 };
-// Units of which a workgroup does the first tiles and not the last ones: who has to join what.
-struct PagedJoin {
-    int32_t request, unit, first, parts;     // parts 0: nothing to join; first: workgroup
+// A unit of which several workgroups did a part each: the one that has its first tile, how many they are (0: not split).
+struct Left {
+    int32_t begins, parts, request, h, q0, rows;
 };
 
 struct PagedWork {
-    PagedJoin *joins;                        // one entry a unit, or a workgroup where there are fewer of those
+    int32_t *counters;                       // [groups]: how many have left their part of the unit begun by a workgroup; 0 between calls; or
+    Left *split;                             // (counters NULL) one entry a unit, or a workgroup where there are fewer of those
+    int32_t by_unit;
     PagedPart *parts;                        // [2 * groups][kPagedHeads]
     float *sums;                             // [2 * groups][rows][pitch]
-    int32_t groups, by_unit, tiles_a_head, rows, pitch;   // tiles_a_head: units of a key head; rows: query heads of the largest unit
+    int32_t groups, tiles_a_head, rows, pitch;     // tiles_a_head: units of a key head; rows: query heads of the largest unit
 };
 
 // Two e4m3 values (HI: the upper two bytes) as two 16-bit numbers: exact in either type.
@@ -111,10 +117,33 @@ template <int DT, bool F8, int E, int N> __device__ __forceinline__ f32x4 produc
 }
 
 // Whether keys are loaded in whole lines (see above).
+#ifndef BA_QP
+#define BA_QP false
+#endif
 #ifndef BA_QUAD16
 #define BA_QUAD16 false
 #endif
-template <bool F8, int DC, Shape SHAPE> constexpr bool quad_keys = SHAPE != kAny && (F8 || BA_QUAD16);
+template <bool F8, int DC, Shape SHAPE> constexpr bool quad_keys = SHAPE != kAny && (F8 || BA_QUAD16 || (BA_QP && SHAPE == kPieces));
+
+// Loads through a buffer descriptor: the base in scalar registers, one offset a lane, and what is past the range reads as zeros.
+constexpr uint32_t kNowhere = 0x80000000u;
+constexpr int kStreamAux = 2;                // past the caches, as load_stream
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t stream_resource(const char *base) {
+    return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, 0x7fffffff, kRsrcFlags);
+}
+template <int N> __device__ __forceinline__ void buffer_stream(uint32_t (&x)[N], __amdgpu_buffer_rsrc_t res, uint32_t off, int soff) {
+    static_assert(N == 1 || N == 2 || N == 4);
+    if constexpr (N == 4) {
+        const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(res, off, soff, kStreamAux);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = v[i];
+    } else if constexpr (N == 2) {
+        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(res, off, soff, kStreamAux);
+        x[0] = v[0]; x[1] = v[1];
+    } else {
+        x[0] = __builtin_amdgcn_raw_buffer_load_b32(res, off, soff, kStreamAux);
+    }
+}
 
 // Barrier that waits for this wavefront's LDS traffic only (the loads of the next unit stay in flight).
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -144,9 +173,107 @@ __device__ __forceinline__ int64_t scaled(int64_t x, int64_t y, int64_t z) {
     return ((uint64_t)p | (uint64_t)z) >> 32 ? p / z : (int64_t)((uint32_t)p / (uint32_t)z);
 }
 
+// x y / z, rounded up.
+__device__ __forceinline__ int64_t scaled_up(int64_t x, int64_t y, int64_t z) {
+    const int64_t q = scaled(x, y, z);
+    return q + (q * z < x * y);
+}
+
+// Parts travel between workgroups of different dies, whose caches know nothing of each other.  Fences for that write back and
+// drop a whole cache (measured: 70 us more for a call of 100); stores and loads that go to where all meet by
+// themselves only have to be in order, so a workgroup waits for its stores before it counts itself in.
+constexpr int kSharedAux = 16;               // scope of the device
+struct Shared {
+    __amdgpu_buffer_rsrc_t parts, sums;
+    int rows, pitch;
+    __device__ __forceinline__ uint32_t part_at(int slot, int hd) const { return (uint32_t)((slot * kPagedHeads + hd) * sizeof(PagedPart)); }
+    __device__ __forceinline__ uint32_t sum_at(int slot, int hd, int d) const { return (uint32_t)((slot * rows + hd) * pitch + d) * 4u; }
+    __device__ __forceinline__ void store(int slot, int hd, int d, f32x4 x) const {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), sums, sum_at(slot, hd, d), 0, kSharedAux);
+    }
+    __device__ __forceinline__ void store(int slot, int hd, PagedPart x) const {
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, x), parts, part_at(slot, hd), 0, kSharedAux);
+    }
+    __device__ __forceinline__ f32x4 sum(int slot, int hd, int d) const {
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sums, sum_at(slot, hd, d), 0, kSharedAux));
+    }
+    __device__ __forceinline__ PagedPart part(int slot, int hd) const {
+        return __builtin_bit_cast(PagedPart, __builtin_amdgcn_raw_buffer_load_b64(parts, part_at(slot, hd), 0, kSharedAux));
+    }
+};
+__device__ __forceinline__ Shared shared_of(const PagedWork &w) {
+    return {__builtin_amdgcn_make_buffer_rsrc(w.parts, 0, 2 * w.groups * kPagedHeads * (int)sizeof(PagedPart), kRsrcFlags),
+            __builtin_amdgcn_make_buffer_rsrc(w.sums, 0, 2 * w.groups * w.rows * w.pitch * 4, kRsrcFlags), w.rows, w.pitch};
+}
+
+// Joins the parts of a unit for its query heads [hd0, hd1), by a whole workgroup.  DC / 4 threads read a row of partial sums;
+// the rest of the threads take other heads, or every so manieth part of the same ones.
+template <int DT, int DC>
+__device__ __forceinline__ void join_parts(const PagedAttentionArgs &a, const PagedWork &w, const Left &u, int hd0, int hd1, float v_scale) {
+    constexpr int kLanes = DC / 4, kRows = kPagedThreads / kLanes, kAhead = DC == 64 ? 8 : 16;
+    __shared__ float rest_m[kRows], rest_l[kRows];
+    __shared__ f32x4 rest_acc[kRows][kLanes];
+    const int begins = u.begins, parts = u.parts, rows = min(u.rows, hd1);
+    const Shared shared = shared_of(w);
+    int heads = 1;
+    while (heads < rows - hd0 && heads < kRows) heads *= 2;
+    const int mine = (int)threadIdx.x / kLanes, d = 4 * ((int)threadIdx.x % kLanes), deep = kRows / heads, sub = mine / heads;
+    for (int hd = hd0 + mine % heads; hd < hd0 + (rows - hd0 + heads - 1) / heads * heads; hd += heads) {
+        float m = -INFINITY, l = 0.f;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        if (hd < rows && d < a.dim)
+            for (int p0 = sub; p0 < parts; p0 += kAhead * deep) {
+                PagedPart x[kAhead];
+                f32x4 y[kAhead];
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    const int p = p0 + i * deep;
+                    x[i] = {-INFINITY, 0.f};
+                    y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    if (p < parts) {
+                        const int slot = 2 * (begins + p) + (p == 0 ? 1 : 0);
+                        x[i] = shared.part(slot, hd);
+                        y[i] = shared.sum(slot, hd, d);
+                    }
+                }
+                float top = m;
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) top = fmaxf(top, x[i].m);
+                const float base = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f(m - base);
+                l *= old;
+                acc *= old;
+                m = top;
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    const float f = __builtin_amdgcn_exp2f(x[i].m - base);
+                    l += f * x[i].l;
+                    acc += f * y[i];
+                }
+            }
+        if (deep > 1) {
+            rest_acc[mine][d / 4] = acc;
+            if (d == 0) { rest_m[mine] = m; rest_l[mine] = l; }
+            __syncthreads();
+            float top = m;
+            for (int i = 1; i < deep && sub == 0; ++i) top = fmaxf(top, rest_m[mine + i * heads]);
+            const float base = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f(m - base);
+            l *= old;
+            acc *= old;
+            for (int i = 1; i < deep && sub == 0; ++i) {
+                const float f = __builtin_amdgcn_exp2f(rest_m[mine + i * heads] - base);
+                l += f * rest_l[mine + i * heads];
+                acc += f * rest_acc[mine + i * heads][d / 4];
+            }
+        }
+        if (deep > 1) __syncthreads();
+        if (sub == 0 && hd < rows && d < a.dim)
+            store_result<DT>(a.out + (u.q0 + hd) * a.out_head_bytes + u.request * a.out_row_bytes, d, a.dim, acc * (v_scale / l));
+    }
+}
+
 // DC: dimensions that the registers hold (64, 128, 256).
 template <int DT, bool F8, int DC, Shape SHAPE, Pages PAGES>
-__global__ void __launch_bounds__(kPagedThreads, resident_groups(DC))
+__global__ void __launch_bounds__(kPagedThreads, resident_groups(DC, F8))
 paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
     constexpr int EB = F8 ? 1 : 2;           // bytes of an element
     constexpr int PW = DC / 16;              // dimensions of a row that a lane holds
@@ -156,7 +283,6 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
     constexpr int PARTS = QUAD && E > 8 ? E / 8 : 1;           // matrix instructions that a load of a key feeds (for each c')
     constexpr int KR = QUAD ? 8 : 2, KL = QUAD ? L : DC * EB / 64, KN = QUAD ? N : 4;      // a lane's tokens of a tile, loads of each, dwords
     constexpr int QC = QUAD ? 4 : 1, QK = QUAD ? L * PARTS : DC / 32;                    // operands of the queries
-    constexpr int NPK = PAGES == kTokens && QUAD ? 8 : 2, NPV = PAGES == kHalves ? 0 : PAGES == kFours ? 2 : 8;
     const int lane = lane_id(), l16 = lane & 15, g = lane >> 4, q4 = l16 >> 2, c4 = l16 & 3, wave = uniform((int)threadIdx.x >> 6);
     const int units = a.heads * w.tiles_a_head;
 
@@ -164,6 +290,10 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
     __shared__ int64_t scan[kPagedWaves];
     __shared__ Place places[2];
     __shared__ float wave_m[kPagedWaves][kPagedHeads], wave_l[kPagedWaves][kPagedHeads];
+    __shared__ Left left[2];
+    __shared__ bool joins[2];
+    int unfinished = 0;
+    Left mine_split = {0, 0, 0, 0, 0, 0};
 
     // ---- the share.  Thread i adds up the tiles of requests [i c, (i + 1) c).
     const int c = (a.requests + kPagedThreads - 1) / kPagedThreads, r0 = (int)threadIdx.x * c;
@@ -188,7 +318,7 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
     const int64_t groups = min((int64_t)w.groups, (total + kPagedShare - 1) / kPagedShare);
     const int64_t group = blockIdx.x;
     if (group >= groups) {
-        if (!w.by_unit && threadIdx.x == 0) w.joins[group].parts = 0;
+        if (w.split && !w.by_unit && threadIdx.x == 0) w.split[group].parts = 0;
         return;
     }
 #pragma unroll
@@ -238,9 +368,8 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
         return u;
     };
     const Place place = places[0];
-    PagedJoin join = {0, 0, 0, 0};
     if (place.at >= end) {
-        if (!w.by_unit && threadIdx.x == 0) w.joins[group] = join;
+        if (w.split && !w.by_unit && threadIdx.x == 0) w.split[group].parts = 0;
         return;
     }
     Unit cur = unit_of(uniform(place.request), uniform(place.unit), uniform(place.tile), uniform64(place.at),
@@ -266,98 +395,113 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
             }
     };
 
-    // Pages and lines of a tile.  Tokens that are not seen may have no page (any more): a half, a group of four or a token
-    // without any that is seen borrows the place of one with.  Page numbers outside the cache become page 0 and poison
-    // the result.
-    int32_t page[NPK + NPV], line[NPK + NPV];
-    bool poison = false;
-    auto look_up = [&](const Unit &u, int t0) {
-        if (PAGES == kHalves) {
-            typedef const __attribute__((address_space(4))) int32_t *Row;      // the same for all lanes: scalar loads
-            const Row row = (Row)(uintptr_t)(a.table + u.request * a.table_stride);
-            int t[2] = {t0, t0 + 16};
-            if (t[1] >= u.len) t[1] = t[0];
-            if (t[0] + 16 <= u.first) t[0] = t[1];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t c = a.page.div((uint32_t)t[i]);
-                page[i] = row[c];
-                line[i] = t[i] - (int)(c * a.page.d);
-            }
-        } else {
-            constexpr int four = PAGES == kFours ? 3 : 0;
-#pragma unroll
-            for (int i = 0; i < NPK + NPV; ++i) {
-                const int k = i < NPK ? i : i - NPK, x = i < NPK ? q4 : g;
-                const int mine = i < NPK && !QUAD ? t0 + 16 * k + l16 : PAGES == kFours ? t0 + 16 * k + 4 * x : t0 + 16 * (k / 4) + 4 * x + k % 4;
-                const int t = min(max(mine & ~four, u.first & ~four), (u.len - 1) & ~four) + (mine & four);
-                const uint32_t c = a.page.div((uint32_t)t);
-                page[i] = a.table[u.request * a.table_stride + c];
-                line[i] = t - (int)(c * a.page.d);
-            }
-        }
+    // Pages of a tile.  Tokens that are not seen may have no page (any more): a half, a group of four or a token
+    // without any that is seen borrows the place of the nearest one with (so tiles past the unit's last may be asked for).
+    // Page numbers outside the cache become page 0 and poison the result.
+    // kHalves: the pages of both halves, the same in all lanes; else lane i has that of the i-th group of four or token.
+    struct Spot {
+        int32_t page[PAGES == kHalves ? 2 : 1];
     };
-    // Where token line[i] of page[i] lies in an array, for a head.
-    auto place_of = [&](const PagedArray &array, int h, int i) {
-        int32_t p = page[i], ln = line[i];
-        if (PAGES == kHalves) { p = uniform(p); ln = uniform(ln); }
+    bool poison = false;
+    constexpr int low = PAGES == kHalves ? 15 : PAGES == kFours ? 3 : 0;
+    auto borrowed = [&](const Unit &u, int t) { return min(max(t & ~low, u.first & ~low), (u.len - 1) & ~low) + (t & low); };
+    auto look_up = [&](const Unit &u, int t0) {
+        Spot s;
+        const int32_t *const row = a.table + u.request * a.table_stride;
+        if (PAGES == kHalves) {
+            typedef const __attribute__((address_space(4))) int32_t *Row;      // scalar loads
+#pragma unroll
+            for (int i = 0; i < 2; ++i) s.page[i] = ((Row)(uintptr_t)row)[a.page.div((uint32_t)borrowed(u, t0 + 16 * i))];
+        } else {
+            s.page[0] = row[a.page.div((uint32_t)borrowed(u, t0 + (PAGES == kFours ? 4 * (lane & 7) : lane & 31)))];
+        }
+        return s;
+    };
+    // Where token t0 + i lies in an array, from the first token of the head on.
+    auto place_of = [&](const PagedArray &array, const Unit &u, const Spot &s, int t0, int i) {
+        const uint32_t t = (uint32_t)borrowed(u, t0 + i);
+        const int32_t p = PAGES == kHalves ? uniform(s.page[i / 16 % 2]) : __shfl(s.page[0], PAGES == kFours ? i / 4 : i);
+        const int32_t line = (int)(t - a.page.div(t) * a.page.d);
         const bool bad = (uint32_t)p >= (uint32_t)a.pages;
         poison |= bad;
-        return array.base + h * array.head_bytes + (bad ? 0 : p) * array.page_bytes + (int64_t)ln * array.token_bytes;
+        return (bad ? 0 : p) * array.page_bytes + (int64_t)line * array.token_bytes;
     };
-    // Pieces that are not there (kPieces) are loaded from the row's front: those of a key count as zeros, those of a value
-    // make results that nobody stores.
+    // The rows of a tile.  With kHalves and kFours through descriptors, whose range check reads pieces that are not there as zeros.
     uint32_t kx[KR][KL][KN], vx[8][L][N];
-    auto load_keys = [&](const Unit &u) {
-        if (QUAD) {
+    auto may_miss = [](int k, int loads) { return SHAPE == kPieces && (DC == 64 || 2 * k + 1 >= loads); };      // (more than half of DC there are always)
+    auto load_keys = [&](const Unit &u, const Spot &s, int t0) {
+        constexpr int kNext = QUAD ? 16 * EB * E : 64;
+        const int b = QUAD ? EB * E * (4 * g + c4) : 16 * g, row = EB * a.dim;
+        const char *const base = a.k.base + u.h * a.k.head_bytes;
+        if (PAGES == kTokens) {
+            const char *p[KR];
+#pragma unroll
+            for (int i = 0; i < KR; ++i) p[i] = base + place_of(a.k, u, s, t0, 16 * i + l16);
+#pragma unroll
+            for (int k = 0; k < KL; ++k)
+#pragma unroll
+                for (int i = 0; i < KR; ++i) load_part<KN>(kx[i][k], p[i] + b + kNext * k, row - b - kNext * k);
+            return;
+        }
+        __amdgpu_buffer_rsrc_t res[2];
+        uint32_t off[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int64_t at = place_of(a.k, u, s, t0, 16 * i + (PAGES == kHalves ? 0 : QUAD ? 4 * q4 : l16));
+            res[i] = stream_resource(PAGES == kHalves ? base + at : base);
+            off[i] = b + (PAGES == kHalves ? (uint32_t)((QUAD ? 4 * q4 : l16) * a.k.token_bytes) : (uint32_t)at);
+        }
+#pragma unroll
+        for (int k = 0; k < KL; ++k)
 #pragma unroll
             for (int i = 0; i < KR; ++i) {
-                const char *const base = place_of(a.k, u.h, PAGES == kTokens ? i : i / 4);
-                const uint32_t mine = PAGES == kHalves ? (uint32_t)((4 * q4 + i % 4) * a.k.token_bytes) : PAGES == kFours ? (uint32_t)(i % 4 * a.k.token_bytes) : 0u;
-#pragma unroll
-                for (int k = 0; k < KL; ++k) {
-                    const uint32_t b = EB * E * (16 * k + 4 * g + c4);
-                    if (SHAPE == kPieces) load_stream<KN>(kx[i][k], base + (mine + ((int)b < EB * a.dim ? b : 0u)));
-                    else load_stream<KN>(kx[i][k], base + (mine + (uint32_t)(EB * E * (4 * g + c4))) + EB * E * 16 * k);
-                }
+                const int half = QUAD ? i / 4 : i;
+                buffer_stream<KN>(kx[i][k], res[half], may_miss(k, KL) && b + kNext * k >= row ? kNowhere : off[half] + kNext * k, QUAD ? i % 4 * a.k.token_bytes : 0);
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < KR; ++i) {
-                const char *const base = place_of(a.k, u.h, i);
-                const uint32_t mine = PAGES == kHalves ? (uint32_t)(l16 * a.k.token_bytes) : 0u;
-#pragma unroll
-                for (int k = 0; k < KL; ++k) {
-                    const uint32_t b = 64 * k + 16 * g;
-                    if (SHAPE == kAny) load_part<KN>(kx[i][k], base + (mine + b), EB * a.dim - (int)b);
-                    else if (SHAPE == kPieces) load_stream<KN>(kx[i][k], base + (mine + ((int)b < EB * a.dim ? b : 0u)));
-                    else load_stream<KN>(kx[i][k], base + (mine + 16u * g) + 64 * k);
-                }
-            }
-        }
     };
-    auto load_values = [&](const Unit &u) {
+    auto load_values = [&](const Unit &u, const Spot &s, int t0) {
+        constexpr int kNext = 16 * EB * E;
+        const int b = EB * E * l16, row = EB * a.dim;
+        const char *const base = a.v.base + u.h * a.v.head_bytes;
+        if (PAGES == kTokens) {
+            const char *p[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const char *const base = place_of(a.v, u.h, PAGES == kHalves ? i / 4 : PAGES == kFours ? NPK + i / 4 : NPK + i);
-            const uint32_t mine = PAGES == kHalves ? (uint32_t)((4 * g + i % 4) * a.v.token_bytes) : PAGES == kFours ? (uint32_t)(i % 4 * a.v.token_bytes) : 0u;
+            for (int i = 0; i < 8; ++i) p[i] = base + place_of(a.v, u, s, t0, 16 * (i / 4) + 4 * g + i % 4);
 #pragma unroll
-            for (int k = 0; k < L; ++k) {
-                const uint32_t b = EB * E * (16 * k + l16);
-                if (SHAPE == kAny) load_part<N>(vx[i][k], base + (mine + b), EB * a.dim - (int)b);
-                else if (SHAPE == kPieces) load_stream<N>(vx[i][k], base + (mine + ((int)b < EB * a.dim ? b : 0u)));
-                else load_stream<N>(vx[i][k], base + (mine + (uint32_t)(EB * E * l16)) + EB * E * 16 * k);
-            }
+            for (int k = 0; k < L; ++k)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) load_part<N>(vx[i][k], p[i] + b + kNext * k, row - b - kNext * k);
+            return;
         }
+        __amdgpu_buffer_rsrc_t res[2];
+        uint32_t off[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int64_t at = place_of(a.v, u, s, t0, 16 * i + (PAGES == kHalves ? 0 : 4 * g));
+            res[i] = stream_resource(PAGES == kHalves ? base + at : base);
+            off[i] = b + (PAGES == kHalves ? (uint32_t)(4 * g * a.v.token_bytes) : (uint32_t)at);
+        }
+#pragma unroll
+        for (int k = 0; k < L; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                buffer_stream<N>(vx[i][k], res[i / 4], may_miss(k, L) && b + kNext * k >= row ? kNowhere : off[i / 4] + kNext * k, i % 4 * a.v.token_bytes);
     };
-    // The wavefront's first tile of a unit.
+    // The wavefront's first tile of a unit.  Loads come back in the order in which they were asked for, so page numbers are asked
+    // for before the loads that others wait for: those of a tile two tiles ahead.
+    constexpr int kStep = kPagedWaves * kPagedTile;
+    Spot ahead;
     auto has_tile = [&](const Unit &u) { return u.tile + wave < u.last && u.len > u.first && a.pages > 0; };
     auto load_first = [&](const Unit &u) {
         load_queries(u);
         if (has_tile(u)) {
-            look_up(u, u.start + (u.tile + wave) * kPagedTile);
-            load_keys(u);
-            load_values(u);
+            const int t0 = u.start + (u.tile + wave) * kPagedTile;
+            const Spot s = look_up(u, t0);
+            ahead = look_up(u, t0 + kStep);
+            __builtin_amdgcn_sched_barrier(0);
+            load_keys(u, s, t0);
+            __builtin_amdgcn_sched_barrier(0);
+            load_values(u, s, t0);
         }
     };
 
@@ -367,18 +511,8 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
     // as the scores have used this one's, and its values likewise.
     auto attend = [&](const Unit &u, auto more, int t0, float to_log2) {
         constexpr bool MORE = decltype(more)::value;
-        if (SHAPE == kPieces) {
-#pragma unroll
-            for (int k = 0; k < KL; ++k) {
-                const int b = QUAD ? EB * E * (16 * k + 4 * g + c4) : 64 * k + 16 * g;
-                if ((QUAD ? EB * E * 16 : 64) * (k + 1) > EB * a.dim) {
-#pragma unroll
-                    for (int i = 0; i < KR; ++i)
-#pragma unroll
-                        for (int x = 0; x < KN; ++x) kx[i][k][x] = b < EB * a.dim ? kx[i][k][x] : 0u;
-                }
-            }
-        }
+        Spot after;
+        if (MORE) after = look_up(u, t0 + 2 * kStep);
         // ---- scores of tokens t0 + 16 i + 4 g + j
         f32x4 sc[2];
         if (QUAD) {
@@ -402,7 +536,10 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
                 sc[i % 2] = s * to_log2;
             }
         }
-        if (MORE) load_keys(u);
+        if (MORE) {
+            load_keys(u, ahead, t0 + kStep);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         if (t0 < u.first || t0 + kPagedTile > u.len) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -459,7 +596,10 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
             o[j] = Elem<DT>::mfma(v, u32x4{hi[0], hi[1], hi[2], hi[3]}, o[j]);
             o[j] = Elem<DT>::mfma(v, u32x4{lo[0], lo[1], lo[2], lo[3]}, o[j]);
         }
-        if (MORE) load_values(u);
+        if (MORE) {
+            load_values(u, ahead, t0 + kStep);
+            ahead = after;
+        }
     };
 
     load_first(cur);
@@ -469,12 +609,8 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
 #pragma unroll
         for (int j = 0; j < PW; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (has_tile(cur)) {
-            constexpr int kStep = kPagedWaves * kPagedTile;
             int s = cur.tile + wave, t0 = cur.start + s * kPagedTile;
-            for (; s + kPagedWaves < cur.last; s += kPagedWaves, t0 += kStep) {
-                look_up(cur, t0 + kStep);
-                attend(cur, std::true_type{}, t0, to_log2);
-            }
+            for (; s + kPagedWaves < cur.last; s += kPagedWaves, t0 += kStep) attend(cur, std::true_type{}, t0, to_log2);
             attend(cur, std::false_type{}, t0, to_log2);
         }
         if (__any(poison) || (a.pages == 0 && cur.len > cur.first)) l = NAN;
@@ -529,116 +665,85 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
                 if (cur.len <= cur.first) acc = f32x4{0.f, 0.f, 0.f, 0.f};
                 store_result<DT>(a.out + (cur.q0 + hd) * a.out_head_bytes + cur.request * a.out_row_bytes, d, a.dim, acc * f);
             } else {
-                *(f32x4 *)(w.sums + ((int64_t)slot * w.rows + hd) * w.pitch + d) = acc;
-                if (d == 0) w.parts[slot * kPagedHeads + hd] = {top, sum};
+                const Shared shared = shared_of(w);
+                shared.store(slot, hd, d, acc);
+                if (d == 0) shared.store(slot, hd, PagedPart{top, sum});
             }
         }
-        if (begun) {
-            // who has the unit's last tile
-            const int64_t stop = cur.at + cur.n;
-            const int parts = done ? 0 : (int)(scaled(stop, groups, total) + (scaled(stop, groups, total) * total < stop * groups) - group);
-            join = {cur.request, cur.unit, (int)group, parts};
-            if (w.by_unit && threadIdx.x == 0) w.joins[(int64_t)cur.request * units + cur.unit] = join;
+        // the workgroups that have the unit's first and last tile
+        Left u = {0, 0, cur.request, cur.h, cur.q0, cur.rows};
+        if (!whole) {
+            const int64_t from = cur.at - cur.tile;
+            u.begins = begun ? (int)group : (int)scaled_up(from + 1, groups, total) - 1;
+            u.parts = (int)scaled_up(from + cur.n, groups, total) - u.begins;
+        }
+        if (w.split) {
+            if (begun) {
+                mine_split = u;
+                if (w.by_unit && threadIdx.x == 0) w.split[(int64_t)cur.request * units + cur.unit] = u;
+            }
+        } else if (!whole) {
+            if (threadIdx.x == 0) left[unfinished] = u;
+            ++unfinished;                    // (the first unit of the share at most, and its last)
         }
         if (at >= end) break;
         lds_barrier();
         cur = next;
     }
-    if (!w.by_unit && threadIdx.x == 0) w.joins[group] = join;
+    if (w.split) {
+        if (!w.by_unit && threadIdx.x == 0) w.split[group] = mine_split;
+        return;
+    }
+    if (unfinished == 0) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0)
+        for (int i = 0; i < unfinished; ++i) {
+            int32_t *const counter = w.counters + left[i].begins;
+            joins[i] = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == left[i].parts - 1;
+            if (joins[i]) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    __syncthreads();
+    for (int i = 0; i < unfinished; ++i)
+        if (joins[i]) join_parts<DT, DC>(a, w, left[i], 0, w.rows, F8 ? a.v.scale[left[i].h] : 1.f);
 }
 
-// Joins units that were split: grid (entries of the list, query heads / `heads`).  DC / 4 threads read a row of
-// partial sums; the rest of a workgroup's threads take other heads, or every so manieth part of the same ones.
+// The same as a kernel of its own: grid (entries of the list, query heads / `heads`).
 template <int DT, int DC> __global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(PagedAttentionArgs a, PagedWork w, int heads) {
-    constexpr int kLanes = DC / 4, kRows = kPagedThreads / kLanes, kAhead = 4;
-    const PagedJoin join = w.joins[blockIdx.x];
-    if (join.parts == 0) return;
-    __shared__ float rest_m[kRows], rest_l[kRows];
-    __shared__ f32x4 rest_acc[kRows][kLanes];
-    const int mine = (int)threadIdx.x / kLanes, d = 4 * ((int)threadIdx.x % kLanes), deep = kRows / heads;
-    const int hd = (int)blockIdx.y * heads + mine % heads, sub = mine / heads;
-    const int h = join.unit / w.tiles_a_head, q = h * a.group + (join.unit - h * w.tiles_a_head) * w.rows + hd;
-    const bool there = hd < w.rows && q < (h + 1) * a.group && d < a.dim;
-    float m = -INFINITY, l = 0.f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    if (there)
-        for (int p0 = sub; p0 < join.parts; p0 += kAhead * deep) {
-            PagedPart x[kAhead];
-            f32x4 y[kAhead];
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                const int p = p0 + i * deep;
-                x[i] = {-INFINITY, 0.f};
-                y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (p < join.parts) {
-                    const int64_t slot = 2 * (int64_t)(join.first + p) + (p == 0 ? 1 : 0);
-                    x[i] = w.parts[slot * kPagedHeads + hd];
-                    y[i] = *(const f32x4 *)(w.sums + (slot * w.rows + hd) * w.pitch + d);
-                }
-            }
-            float top = m;
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) top = fmaxf(top, x[i].m);
-            const float base = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f(m - base);
-            l *= old;
-            acc *= old;
-            m = top;
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                const float f = __builtin_amdgcn_exp2f(x[i].m - base);
-                l += f * x[i].l;
-                acc += f * y[i];
-            }
-        }
-    if (deep > 1) {
-        rest_acc[mine][d / 4] = acc;
-        if (d == 0) { rest_m[mine] = m; rest_l[mine] = l; }
-        __syncthreads();
-        if (sub) return;
-        float top = m;
-        for (int i = 1; i < deep; ++i) top = fmaxf(top, rest_m[mine + i * heads]);
-        const float base = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f(m - base);
-        l *= old;
-        acc *= old;
-        for (int i = 1; i < deep; ++i) {
-            const float f = __builtin_amdgcn_exp2f(rest_m[mine + i * heads] - base);
-            l += f * rest_l[mine + i * heads];
-            acc += f * rest_acc[mine + i * heads][d / 4];
-        }
-    }
-    if (there) store_result<DT>(a.out + q * a.out_head_bytes + join.request * a.out_row_bytes, d, a.dim, acc * ((a.v.scale ? a.v.scale[h] : 1.f) / l));
+    const Left u = w.split[blockIdx.x];
+    const int hd = (int)blockIdx.y * heads;
+    if (u.parts && hd < u.rows) join_parts<DT, DC>(a, w, u, hd, hd + heads, a.v.scale ? a.v.scale[u.h] : 1.f);
 }
 
 // ------------------------------------------------------------------ host
 static int dim_class(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
 // Workgroups: as many as are resident, or fewer where the longest possible requests would not give each its least share.
-static PagedWork work_of(int64_t heads, int64_t group, int64_t dim, int64_t requests, int64_t width, int64_t page, void *workspace, size_t *bytes) {
+static PagedWork work_of(int64_t heads, int64_t group, int64_t dim, bool f8, int64_t requests, int64_t width, int64_t page, void *workspace, size_t *bytes) {
     PagedWork w{};
     w.tiles_a_head = (int32_t)((group + kPagedHeads - 1) / kPagedHeads);
     w.rows = (int32_t)((group + w.tiles_a_head - 1) / w.tiles_a_head);
-    const int64_t resident = (int64_t)device_cu_count() * resident_groups(dim_class(dim));
+    const int64_t resident = (int64_t)device_cu_count() * resident_groups(dim_class(dim), f8);
     const int64_t units = requests * heads * w.tiles_a_head;
     const double tiles = (double)units * ((double)width * page / kPagedTile + 1);
-    w.groups = (int32_t)std::max<int64_t>(1, (int64_t)std::min<double>((double)resident, tiles / kPagedShare + 1));
+    w.groups = (int32_t)std::max<int64_t>(1, std::min<int64_t>(BA_PAGED_COUNTERS, (int64_t)std::min<double>((double)resident, tiles / kPagedShare + 1)));
     w.by_unit = units <= w.groups;
-    const size_t entries = (size_t)(w.by_unit ? units : w.groups);
-    const size_t joins = (entries * sizeof(PagedJoin) + 255) & ~size_t(255);
+    const size_t split = ((size_t)(w.by_unit ? units : w.groups) * sizeof(Left) + 255) & ~size_t(255);
     const size_t parts = (2 * (size_t)w.groups * kPagedHeads * sizeof(PagedPart) + 255) & ~size_t(255);
     w.pitch = (int32_t)((dim + 3) & ~int64_t(3));
     const size_t sums = 2 * (size_t)w.groups * w.rows * w.pitch * sizeof(float);
-    if (bytes) *bytes = joins + parts + sums;
+    if (bytes) *bytes = split + parts + sums;
     if (workspace) {
-        w.joins = (PagedJoin *)workspace;
-        w.parts = (PagedPart *)((char *)workspace + joins);
-        w.sums = (float *)((char *)workspace + joins + parts);
+        w.split = (Left *)workspace;
+        w.parts = (PagedPart *)((char *)workspace + split);
+        w.sums = (float *)((char *)workspace + split + parts);
     }
     return w;
 }
 
-size_t paged_attention_workspace(int64_t heads, int64_t group, int64_t dim, int64_t requests, int64_t width, int64_t page) {
+size_t paged_attention_workspace(int64_t heads, int64_t group, int64_t dim, int cache_dtype, int64_t requests, int64_t width, int64_t page) {
     size_t bytes = 0;
-    work_of(heads, group, dim, requests, width, page, nullptr, &bytes);
+    work_of(heads, group, dim, cache_dtype == BA_F8_E4M3, requests, width, page, nullptr, &bytes);
     return bytes;
 }
 
@@ -652,22 +757,33 @@ static int launch_split(const PagedAttentionArgs &a, const PagedWork &w, hipStre
     }
     const size_t lds = (size_t)kPagedWaves * w.rows * (DC + 4) * sizeof(float);
     paged_attention_kernel<DT, F8, DC, SHAPE, PAGES><<<w.groups, kPagedThreads, lds, stream>>>(a, w);
-    // Few units have many parts each, and a workgroup joins one head of one; of many units most were not split, and a
-    // workgroup takes as many heads as it has threads for.
-    const int most = kPagedThreads / (DC / 4);
-    int heads = 1;
-    while (!w.by_unit && heads < most && heads < w.rows) heads *= 2;
-    const dim3 grid((unsigned)(w.by_unit ? a.requests * a.heads * w.tiles_a_head : w.groups), (unsigned)((w.rows + heads - 1) / heads));
-    paged_join_kernel<DT, DC><<<grid, kPagedThreads, 0, stream>>>(a, w, heads);
+    if (w.split) {
+        const int64_t entries = w.by_unit ? a.requests * (int64_t)a.heads * w.tiles_a_head : w.groups;
+        const int most = kPagedThreads / (DC / 4);
+        int heads = 1;
+        while (heads < most && heads < w.rows && entries * ((w.rows + heads - 1) / heads) > kPagedJoins) heads *= 2;
+        paged_join_kernel<DT, DC><<<dim3((unsigned)entries, (unsigned)((w.rows + heads - 1) / heads)), kPagedThreads, 0, stream>>>(a, w, heads);
+    }
     return hipGetLastError() == hipSuccess ? BA_OK : BA_ERR_LAUNCH;
 }
 
-// Pages of 16, 32, ... tokens and those of 4, 8, 12, 20, ... have builds of their own where rows are whole pieces; all else
-// runs through the build that takes every token and byte by itself.
+// Bytes from the first element of an array to the end of the last one of a head.
+static int64_t span(const PagedArray &x, const PagedAttentionArgs &a) {
+    return (a.pages - 1) * x.page_bytes + ((int64_t)a.page.d - 1) * x.token_bytes + 2 * a.dim;
+}
+
+// Rows of whole pieces at addresses that are multiples of 16 go through descriptors: pages of 16, 32, ... tokens with one a page,
+// pages of 4, 8, 12, 20, ... with one for all pages, whose offsets have 31 bits.  All else runs through the build that takes
+// every token and byte by itself.
 template <int DT, bool F8, int DC> static int launch_class(const PagedAttentionArgs &a, const PagedWork &w, hipStream_t stream) {
-    if (a.page.d % 4 || a.dim % (F8 ? 16 : 8)) return launch_split<DT, F8, DC, kAny, kTokens>(a, w, stream);
-    if (a.page.d % 16) return a.dim == DC ? launch_split<DT, F8, DC, kFull, kFours>(a, w, stream) : launch_split<DT, F8, DC, kPieces, kFours>(a, w, stream);
-    return a.dim == DC ? launch_split<DT, F8, DC, kFull, kHalves>(a, w, stream) : launch_split<DT, F8, DC, kPieces, kHalves>(a, w, stream);
+    const uint64_t bits = (uint64_t)a.k.base | (uint64_t)a.v.base | (uint64_t)a.k.page_bytes | (uint64_t)a.v.page_bytes | (uint64_t)a.k.head_bytes |
+                          (uint64_t)a.v.head_bytes | (uint64_t)a.k.token_bytes | (uint64_t)a.v.token_bytes;
+    const bool pieces = bits % 16 == 0 && a.dim % (F8 ? 16 : 8) == 0;
+    if (pieces && a.page.d % 16 == 0)
+        return a.dim == DC ? launch_split<DT, F8, DC, kFull, kHalves>(a, w, stream) : launch_split<DT, F8, DC, kPieces, kHalves>(a, w, stream);
+    if (pieces && a.page.d % 4 == 0 && span(a.k, a) < kNowhere && span(a.v, a) < kNowhere)
+        return a.dim == DC ? launch_split<DT, F8, DC, kFull, kFours>(a, w, stream) : launch_split<DT, F8, DC, kPieces, kFours>(a, w, stream);
+    return launch_split<DT, F8, DC, kAny, kTokens>(a, w, stream);
 }
 
 template <int DT, bool F8> static int launch_dtype(const PagedAttentionArgs &a, const PagedWork &w, hipStream_t stream) {
@@ -678,9 +794,13 @@ template <int DT, bool F8> static int launch_dtype(const PagedAttentionArgs &a, 
     }
 }
 
-int launch_paged_attention(const PagedAttentionArgs &a, int dtype, int cache_dtype, void *workspace, hipStream_t stream) {
-    const PagedWork w = work_of(a.heads, a.group, a.dim, a.requests, a.width, a.page.d, workspace, nullptr);
+int launch_paged_attention(const PagedAttentionArgs &a, int dtype, int cache_dtype, int32_t *counters, void *workspace, hipStream_t stream) {
     const bool f8 = cache_dtype == BA_F8_E4M3;
+    PagedWork w = work_of(a.heads, a.group, a.dim, f8, a.requests, a.width, a.page.d, workspace, nullptr);
+    w.counters = counters;
+    // Joining within the kernel saves the second launch (about 3 us), but one workgroup then reads all parts of a unit: at 32 parts
+    // of 8 heads it takes 5 us more than a kernel that spreads them, at 96 parts 14 us.
+    if (w.groups <= kPagedFewParts * a.requests * (int64_t)a.heads * w.tiles_a_head) w.split = nullptr;
     if (dtype == BA_F16) return f8 ? launch_dtype<0, true>(a, w, stream) : launch_dtype<0, false>(a, w, stream);
     return f8 ? launch_dtype<1, true>(a, w, stream) : launch_dtype<1, false>(a, w, stream);
 }

@@ -25,6 +25,7 @@
 // pointers, which the version counters cannot see).
 #include <array>
 #include <deque>
+#include <map>
 #include <memory>
 #include <mutex>
 
@@ -751,6 +752,29 @@ void pagedAppend_op(const Tensor &k, const Tensor &v, const Tensor &k_cache, con
     written(k_cache); written(v_cache);
 }
 
+// The counters of ba_paged_attention, zeros that every call leaves as zeros: kept for each of PyTorch's own streams, on
+// which calls follow each other (and which live as long as the process).  A call that is being captured may be replayed on
+// any stream, and a stream from elsewhere may end and its handle come back while its work still runs: those get
+// counters of their own.
+Tensor paged_counters(const Tensor &like) {
+    const auto opts = at::TensorOptions().dtype(at::kInt).device(like.device());
+    const c10::hip::HIPStream stream = c10::hip::getCurrentHIPStream(like.device().index());
+    hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+    const int64_t id = stream.unwrap().id();
+    const bool foreign = id != 0 && (id & 1) == 0;           // such ids are the stream's address
+    if (foreign || hipStreamIsCapturing(stream.stream(), &capturing) != hipSuccess || capturing != hipStreamCaptureStatusNone)
+        return at::zeros({BA_PAGED_COUNTERS}, opts);
+    static std::mutex mu;
+    static auto *kept = new std::map<std::pair<int, int64_t>, Tensor>;       // never taken down: the GPU may be gone by then
+    std::lock_guard<std::mutex> lock(mu);
+    Tensor &t = (*kept)[{(int)like.device().index(), id}];
+    if (!t.defined()) {
+        c10::InferenceMode normal_tensors(false);
+        t = at::zeros({BA_PAGED_COUNTERS}, opts);
+    }
+    return t;
+}
+
 Tensor pagedAttention_op(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &table, const Tensor &lens,
                          double scale, int64_t window, const OptTensor &k_scale, const OptTensor &v_scale) {
     const ba_paged_cache c = cache_of(k_cache, v_cache, k_scale, v_scale);
@@ -769,9 +793,10 @@ Tensor pagedAttention_op(const Tensor &q, const Tensor &k_cache, const Tensor &v
     const size_t bytes = ba_paged_attention_workspace(&c, qr.heads, qr.rows, table.size(1));
     Tensor work;
     if (bytes) work = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+    const Tensor counters = paged_counters(q);
     check_status(ba_paged_attention(&c, dtype_code(q, "pagedAttention"), q.data_ptr(), qr.head_stride, qr.row_stride, qr.heads, qr.rows,
                                     table.data_ptr<int32_t>(), table.stride(0), table.size(1), lens.data_ptr<int64_t>(), window, (float)scale,
-                                    out.data_ptr(), outr.head_stride, outr.row_stride, bytes ? work.data_ptr() : nullptr, bytes,
+                                    out.data_ptr(), outr.head_stride, outr.row_stride, counters.data_ptr<int32_t>(), bytes ? work.data_ptr() : nullptr, bytes,
                                     current_stream(q)),
                  "ba_paged_attention");
     return out;

@@ -19,9 +19,9 @@ def a_cache(**changes):
 P = ctypes.c_void_p(256)          # an address that nothing reads
 
 
-def attention(cache, dtype=0, q=P, heads=4, requests=3, table=P, table_stride=9, width=9, lens=P, window=0, out=P, work=P, room=1 << 30, stride=64):
+def attention(cache, dtype=0, q=P, heads=4, requests=3, table=P, table_stride=9, width=9, lens=P, window=0, out=P, counters=P, work=P, room=1 << 30, stride=64):
     return capi.load().ba_paged_attention(cache, dtype, q, stride, 256, heads, requests, table, table_stride, width, lens, window, 1.0, out, 64, 256,
-                                          work, room, None)
+                                          counters, work, room, None)
 
 
 def append(cache, dtype=0, k=P, v=P, slots=P, tokens=5, stride=64):
@@ -41,7 +41,7 @@ def test_caches(changes, status):
 def test_attention_arguments():
     c = a_cache()
     assert attention(None) == 1
-    for bad in (dict(q=None), dict(out=None), dict(lens=None), dict(table=None), dict(heads=3), dict(heads=0), dict(requests=-1), dict(width=-1),
+    for bad in (dict(q=None), dict(out=None), dict(counters=None), dict(lens=None), dict(table=None), dict(heads=3), dict(heads=0), dict(requests=-1), dict(width=-1),
                 dict(window=-1), dict(table_stride=8), dict(stride=-64)):
         assert attention(c, **bad) == 1, bad
     assert attention(c, dtype=1) == 3 and attention(c, dtype=2) == 3
