@@ -133,6 +133,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t stream_resource(const char *ba
 }
 template <int N> __device__ __forceinline__ void buffer_stream(uint32_t (&x)[N], __amdgpu_buffer_rsrc_t res, uint32_t off, int soff) {
     static_assert(N == 1 || N == 2 || N == 4);
+    soff = uniform(soff);                    // (in a vector register it would make the load a loop)
     if constexpr (N == 4) {
         const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(res, off, soff, kStreamAux);
 #pragma unroll
