@@ -393,7 +393,7 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
     // Page numbers outside the cache become page 0 and poison the result.
     // kHalves: the pages of both halves, the same in all lanes; else lane i has that of the i-th group of four or token.
     struct Spot {
-        int32_t page[PAGES == kHalves ? 2 : 1];
+        int32_t page[PAGES == kHalves ? 2 : 1], line[PAGES == kHalves ? 2 : 1];      // (line: kHalves only)
     };
     bool poison = false;
     constexpr int low = PAGES == kHalves ? 15 : PAGES == kFours ? 3 : 0;
@@ -404,16 +404,33 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
         if (PAGES == kHalves) {
             typedef const __attribute__((address_space(4))) int32_t *Row;      // scalar loads
 #pragma unroll
-            for (int i = 0; i < 2; ++i) s.page[i] = ((Row)(uintptr_t)row)[a.page.div((uint32_t)borrowed(u, t0 + 16 * i))];
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t t = (uint32_t)borrowed(u, t0 + 16 * i), c = a.page.div(t);
+                s.page[i] = ((Row)(uintptr_t)row)[c];
+                s.line[i] = (int)(t - c * a.page.d);
+            }
         } else {
             s.page[0] = row[a.page.div((uint32_t)borrowed(u, t0 + (PAGES == kFours ? 4 * (lane & 7) : lane & 31)))];
         }
         return s;
     };
-    // Where token t0 + i lies in an array, from the first token of the head on.
+    // kHalves: the page numbers, once they are there.
+    auto check = [&](Spot &s) {
+        if (PAGES != kHalves) return;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            s.page[i % 2] = uniform(s.page[i % 2]);
+            const bool bad = (uint32_t)s.page[i % 2] >= (uint32_t)a.pages;
+            poison |= bad;
+            s.page[i % 2] = bad ? 0 : s.page[i % 2];
+        }
+    };
+    // Where token t0 + i (kHalves: half i of the tile) lies in an array, from the first token of the head on.
     auto place_of = [&](const PagedArray &array, const Unit &u, const Spot &s, int t0, int i) {
+        if (PAGES == kHalves)
+            return (int64_t)((uint64_t)(uint32_t)s.page[i % 2] * (uint32_t)array.page_bytes + (uint32_t)(uniform(s.line[i % 2]) * array.token_bytes));
         const uint32_t t = (uint32_t)borrowed(u, t0 + i);
-        const int32_t p = PAGES == kHalves ? uniform(s.page[i / 16 % 2]) : __shfl(s.page[0], PAGES == kFours ? i / 4 : i);
+        const int32_t p = __shfl(s.page[0], PAGES == kFours ? i / 4 : i);
         const int32_t line = (int)(t - a.page.div(t) * a.page.d);
         const bool bad = (uint32_t)p >= (uint32_t)a.pages;
         poison |= bad;
@@ -440,7 +457,7 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
         uint32_t off[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int64_t at = place_of(a.k, u, s, t0, 16 * i + (PAGES == kHalves ? 0 : QUAD ? 4 * q4 : l16));
+            const int64_t at = place_of(a.k, u, s, t0, PAGES == kHalves ? i : 16 * i + (QUAD ? 4 * q4 : l16));
             res[i] = stream_resource(PAGES == kHalves ? base + at : base);
             off[i] = b + (PAGES == kHalves ? (uint32_t)((QUAD ? 4 * q4 : l16) * a.k.token_bytes) : (uint32_t)at);
         }
@@ -470,7 +487,7 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
         uint32_t off[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int64_t at = place_of(a.v, u, s, t0, 16 * i + (PAGES == kHalves ? 0 : 4 * g));
+            const int64_t at = place_of(a.v, u, s, t0, PAGES == kHalves ? i : 16 * i + 4 * g);
             res[i] = stream_resource(PAGES == kHalves ? base + at : base);
             off[i] = b + (PAGES == kHalves ? (uint32_t)(4 * g * a.v.token_bytes) : (uint32_t)at);
         }
@@ -489,8 +506,9 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
         load_queries(u);
         if (has_tile(u)) {
             const int t0 = u.start + (u.tile + wave) * kPagedTile;
-            const Spot s = look_up(u, t0);
+            Spot s = look_up(u, t0);
             ahead = look_up(u, t0 + kStep);
+            check(s);
             __builtin_amdgcn_sched_barrier(0);
             load_keys(u, s, t0);
             __builtin_amdgcn_sched_barrier(0);
@@ -529,6 +547,7 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
                 }
             }
         if (MORE) {
+            check(ahead);
             load_keys(u, ahead, t0 + kStep);
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -757,7 +776,8 @@ static int64_t span(const PagedArray &x, const PagedAttentionArgs &a) {
 template <int DT, bool F8, int DC, int SETS> static int launch_class(const PagedAttentionArgs &a, const PagedWork &w, hipStream_t stream) {
     const uint64_t bits = (uint64_t)a.k.base | (uint64_t)a.v.base | (uint64_t)a.k.page_bytes | (uint64_t)a.v.page_bytes | (uint64_t)a.k.head_bytes |
                           (uint64_t)a.v.head_bytes | (uint64_t)a.k.token_bytes | (uint64_t)a.v.token_bytes;
-    const bool pieces = bits % 16 == 0 && a.dim % (F8 ? 16 : 8) == 0;
+    // (the page stride as 32 bits: one scalar multiplication less a tile and array)
+    const bool pieces = bits % 16 == 0 && ((uint64_t)a.k.page_bytes | (uint64_t)a.v.page_bytes) >> 32 == 0 && a.dim % (F8 ? 16 : 8) == 0;
     if (pieces && a.page.d % 16 == 0)
         return a.dim == DC ? launch_split<DT, F8, DC, SETS, kFull, kHalves>(a, w, stream) : launch_split<DT, F8, DC, SETS, kPieces, kHalves>(a, w, stream);
     if (pieces && a.page.d % 4 == 0 && span(a.k, a) < kNowhere && span(a.v, a) < kNowhere)
