@@ -8,20 +8,29 @@
 // the tiles of all units, in order, are dealt out to the workgroups in equal shares (the lengths are on the GPU only, so
 // every workgroup adds them up itself).  A workgroup goes through its share unit by unit, its four wavefronts taking every
 // fourth tile each; at the end of a unit their results are joined in LDS.  A unit that lies in one share is done
-// then; for others each workgroup leaves its maximum, sum and fp32 accumulators in memory and counts itself in, and the
-// last one there joins them all, in the order of the tokens whoever it is.
+// then; for others each workgroup leaves its maximum, sum and fp32 accumulators in memory.  Where units have few parts, each
+// counts itself in and the last one there joins them all, in the order of the tokens whoever it is; else a second kernel does.
 //
-// One tile.  Lanes that follow each other read bytes that follow each other, four lanes 64 of them and sixteen a row (of
-// 128 dimensions); nothing of the cache passes through LDS.  With lane = 16 g + 4 q + c:
-//   Scores, S[token][head] = K Q^T on the 16 x 16 x 32 matrix instruction.  It wants a lane to hold dimensions of token
-//   lane % 16, but loaded so every lane would be a memory access of its own and every line be asked for twice.  Instead
-//   load j gives the lane piece 4 g + c of token 4 q + j.  Multiplied with piece 4 g + c' of the queries, for c' = 0 .. 3,
-//   the rows 4 q + c of the result are right where c = c', and those lie in register c of the lanes that hold the rows of q:
-//   the score is the sum of register c' of product c'.  Four times the products, of which the matrix unit has plenty.
+// One tile; nothing of the cache passes through LDS.  With lane = 16 g + 4 q + c:
+//   Scores, S[token][head] = K Q^T on the 16 x 16 x 32 matrix instruction, tokens as rows.
+//     16-bit caches: a lane loads 16 bytes of tokens lane % 16 and 16 + lane % 16, which is what the instruction wants.
+//     8-bit caches: so loaded every lane is a memory access of its own for few bytes, and every line is asked for twice.
+//     Instead load j gives the lane piece 4 g + c of token 4 q + j, four lanes 32 bytes in a row.  Multiplied with piece 4 g + c'
+//     of the queries, for c' = 0 .. 3, the rows 4 q + c of the result are right where c = c', and those lie in register c
+//     of the lanes that hold the rows of q: the score is the sum of register c' of product c'.  Four times the products:
+//     96 requests of up to 8192 tokens, 128 dimensions 165 us against 191; in 16 bits, 128 requests of up to 16384, 603
+//     against 588, so there it is not done.
 //   A lane then holds the scores of tokens 4 g + j of both halves of the tile for head lane % 16: packed to 16 bits these
 //   are, as they are, its operand of the second product if that runs over the tokens in the order (half, g, j).
-//   Values, O[d][head] = V^T P.  A lane loads a piece of its eight tokens and turns the small matrix in registers: the
-//   operand of dimension j is made of the j-th halves of its eight rows.
+//   Values, O[d][head] = V^T P.  A lane loads a piece of its eight tokens, sixteen lanes a row, and turns the small matrix in
+//   registers: the operand of dimension j is made of the j-th halves of its eight rows.
+//   The next tile's keys are asked for as soon as the scores have used this one's, its values behind the second product, and the
+//   page numbers of the tile after that before both: loads come back in order.
+//
+// Bound and figures.  Loads that pass the caches reach 7.05 TB/s here, others 6.2.  128 requests of 1 to 16384 tokens, 32 query
+// heads on 8, 128 dimensions, bf16 (3.8 GB): 581 us, 6.6 TB/s; 64 requests of up to 4096 (500 MB): 92 us, 5.4 TB/s, of which
+// about 12 us do not depend on the lengths (launch, adding up the lengths, first loads, joining).  8-bit caches are bound by
+// instructions as much as by memory: 96 requests of up to 8192 tokens (876 MB) 165 us, 5.3 TB/s, and the same time at 64 dimensions.
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -37,7 +46,7 @@ constexpr int kPagedWaves = 4;
 constexpr int kPagedThreads = 64 * kPagedWaves;
 constexpr int kPagedTile = 32;               // tokens
 constexpr int kPagedHeads = 16;              // query heads of an operand of the matrix instruction; a unit has one or two such sets
-constexpr int kPagedShare = kPagedWaves;     // tiles of a workgroup at least
+constexpr int kPagedShare = kPagedWaves;     // tiles of a workgroup at least: one a wavefront
 constexpr int kPagedFewParts = 8;            // parts of a unit, on the average, up to which the kernel itself joins them
 constexpr int kPagedJoins = 512;             // workgroups of the joining kernel, where it has a choice
 constexpr int kPagedWhole = 8;               // units of up to so many tiles are not split between workgroups
@@ -46,7 +55,9 @@ constexpr int kPagedWhole = 8;               // units of up to so many tiles are
 // zero in fp16; it is in the sums as well and drops out.
 template <int DT> constexpr float kLift = DT == 0 ? 14.f : 0.f;
 
-// Workgroups of a compute unit, by the registers that the tiles in flight and the results take.
+// Workgroups of a compute unit, by the registers that the tiles in flight and the results take.  (One or two less: 128 dimensions
+// 94 -> 97 us for 64 requests of up to 4096 tokens; one more, 8-bit, 167 -> 198; 256 dimensions in 16 bits at two, with registers in
+// memory, 244 against 183.)
 constexpr int resident_groups(int dim_class, bool f8, int sets) {
     return dim_class == 64 ? (sets == 2 ? 3 : 4) : dim_class == 128 ? (sets == 2 ? 2 : 3) : f8 && sets == 1 ? 2 : 1;
 }
@@ -60,8 +71,8 @@ struct Left {
 };
 
 struct PagedWork {
-    int32_t *counters;                       // [groups]: how many have left their part of the unit begun by a workgroup; 0 between calls; or
-    Left *split;                             // (counters NULL) one entry a unit, or a workgroup where there are fewer of those
+    int32_t *counters;                       // [groups]: how many have left their part of the unit begun by a workgroup; 0 between calls
+    Left *split;                             // not NULL: instead of counting, one entry a unit (by_unit) or a workgroup for the joining kernel
     int32_t by_unit;
     PagedPart *parts;                        // [2 * groups][rows]
     float *sums;                             // [2 * groups][rows][pitch]
