@@ -18,14 +18,31 @@ struct AppendShape {
     int32_t tokens, heads_inner;             // tokens of a workgroup; whether it takes all heads of them
 };
 
+// x / scale, limited to +-448; a NaN stays one.  With r the nearest number to 1 / scale and q = x r, one correction by the residual
+// gives the nearest number to x / scale (Markstein's theorem; infinities and zeros stay as they are).  `plain`: a
+// scale for which nothing on the way leaves fp32's range (what does has a result that rounds to 0 or 448 all the same);
+// others are divided.  30 000 tokens of 8 x 64: 24 us with a division each, which costs twice the instructions.
+__device__ __forceinline__ float scaled_down(float x, float scale, float r, bool plain) {
+    float q = x * r;
+    if (plain) {
+        const float better = fmaf(fmaf(-q, scale, x), r, q);
+        q = __builtin_amdgcn_classf(q, 0x198) ? better : q;      // finite and not 0 (which would lose its sign)
+    } else {
+        q = x / scale;
+    }
+    const float y = __builtin_amdgcn_fmed3f(q, -448.f, 448.f);
+    return q == q ? y : q;
+}
+
 template <int DT, bool F8, bool WHOLE> __device__ __forceinline__ void store_piece(char *dst, const uint32_t (&x)[4], float scale, int left) {
     if (F8) {
         uint32_t y[2] = {0, 0};
+        const float r = 1.f / scale, size = fabsf(scale);
+        const bool plain = size > 0x1p-100f && size < 0x1p100f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float lo = Elem<DT>::to_float((uint16_t)x[i]) / scale, hi = Elem<DT>::to_float((uint16_t)(x[i] >> 16)) / scale;
-            lo = lo > 448.f ? 448.f : lo < -448.f ? -448.f : lo;      // (a NaN stays one)
-            hi = hi > 448.f ? 448.f : hi < -448.f ? -448.f : hi;
+            const float lo = scaled_down(Elem<DT>::to_float((uint16_t)x[i]), scale, r, plain);
+            const float hi = scaled_down(Elem<DT>::to_float((uint16_t)(x[i] >> 16)), scale, r, plain);
             if (i % 2) y[i / 2] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, (int)y[i / 2], true);
             else y[i / 2] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, (int)y[i / 2], false);
         }
