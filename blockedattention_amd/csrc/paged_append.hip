@@ -10,7 +10,7 @@
 namespace ba {
 
 constexpr int kAppendThreads = 256;
-constexpr int kAppendPieces = 4;             // of a thread, their loads in flight together
+constexpr int kAppendPieces = 2;             // of a thread, their loads in flight together (with 4: 22.6 us for 22.1, with 8: 26.2)
 constexpr int kPieceElems = 8;
 
 struct AppendShape {
