@@ -9,12 +9,12 @@ extern template int launch_paged_dtype<0, true>(const PagedAttentionArgs &a, con
 extern template int launch_paged_dtype<1, true>(const PagedAttentionArgs &a, const PagedWork &w, hipStream_t stream);
 
 // Workgroups: as many as are resident, or fewer where the longest possible requests would not give each its least share.
-static PagedWork work_of(int64_t heads, int64_t group, int64_t dim, bool f8, int64_t requests, int64_t width, int64_t page, void *workspace, size_t *bytes) {
+static PagedWork work_of(int64_t heads, int64_t group, int64_t dim, bool f8, bool any, int64_t requests, int64_t width, int64_t page, void *workspace, size_t *bytes) {
     PagedWork w{};
     const int sets = group > kPagedHeads ? 2 : 1;
     w.tiles_a_head = (int32_t)((group + sets * kPagedHeads - 1) / (sets * kPagedHeads));
     w.rows = (int32_t)((group + w.tiles_a_head - 1) / w.tiles_a_head);
-    const int64_t resident = (int64_t)device_cu_count() * resident_groups(dim_class(dim), f8, sets);
+    const int64_t resident = (int64_t)device_cu_count() * resident_groups(dim_class(dim), f8, sets, any);
     const int64_t units = requests * heads * w.tiles_a_head;
     const double tiles = (double)units * ((double)width * page / kPagedTile + 1);
     w.groups = (int32_t)std::max<int64_t>(1, std::min<int64_t>(BA_PAGED_COUNTERS, (int64_t)std::min<double>((double)resident, tiles / kPagedShare + 1)));
@@ -33,14 +33,14 @@ static PagedWork work_of(int64_t heads, int64_t group, int64_t dim, bool f8, int
 }
 
 size_t paged_attention_workspace(int64_t heads, int64_t group, int64_t dim, int cache_dtype, int64_t requests, int64_t width, int64_t page) {
-    size_t bytes = 0;
-    work_of(heads, group, dim, cache_dtype == BA_F8_E4M3, requests, width, page, nullptr, &bytes);
+    size_t bytes = 0;                        // (rows at any address have fewer workgroups, which need no more)
+    work_of(heads, group, dim, cache_dtype == BA_F8_E4M3, false, requests, width, page, nullptr, &bytes);
     return bytes;
 }
 
 int launch_paged_attention(const PagedAttentionArgs &a, int dtype, int cache_dtype, int32_t *counters, void *workspace, hipStream_t stream) {
     const bool f8 = cache_dtype == BA_F8_E4M3;
-    PagedWork w = work_of(a.heads, a.group, a.dim, f8, a.requests, a.width, a.page.d, workspace, nullptr);
+    PagedWork w = work_of(a.heads, a.group, a.dim, f8, build_of(a, f8).shape != kFull, a.requests, a.width, a.page.d, workspace, nullptr);
     w.counters = counters;
     // Joining within the kernel saves the second launch (about 3 us), but one workgroup then reads all parts of a unit: at 32 parts
     // of 8 heads it takes 5 us more than a kernel that spreads them, at 96 parts 14 us.

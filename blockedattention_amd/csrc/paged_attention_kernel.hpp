@@ -58,7 +58,11 @@ template <int DT> constexpr float kLift = DT == 0 ? 14.f : 0.f;
 // Workgroups of a compute unit, by the registers that the tiles in flight and the results take.  (One or two less: 128 dimensions
 // 94 -> 97 us for 64 requests of up to 4096 tokens; one more, 8-bit, 167 -> 198; 256 dimensions in 16 bits at two, with registers in
 // memory, 244 against 183.)
-constexpr int resident_groups(int dim_class, bool f8, int sets) {
+// `any`: rows at any address, whose addresses and shifting take more (64 requests of up to 4096 tokens, 100 dimensions 140 us,
+// with a workgroup more 169; but 8-bit, 96 of up to 8192, 276 us with three, 282 with two, and 200 dimensions 437 with two, 504 with one).
+constexpr int resident_groups(int dim_class, bool f8, int sets, bool any) {
+    if (any)
+        return dim_class == 64 ? (sets == 2 ? 2 : 3) : dim_class == 128 ? (f8 && sets == 1 ? 3 : 2) : f8 && sets == 1 ? 2 : 1;
     return dim_class == 64 ? (sets == 2 ? 3 : 4) : dim_class == 128 ? (sets == 2 ? 2 : 3) : f8 && sets == 1 ? 2 : 1;
 }
 
@@ -97,8 +101,9 @@ template <int DT> __device__ __forceinline__ void store_result(char *row, int d,
     }
 }
 
-// What is known of the head dimension: it fills the registers (64, 128, 256), it is whole pieces (16 bytes of a key), or neither.
-enum Shape { kFull, kPieces, kAny };
+// What is known of the rows: at multiples of 16 bytes they fill the registers (64, 128, 256) or are whole pieces (16 bytes of
+// a key); at any address they have 16 bytes or more, or fewer.
+enum Shape { kFull, kPieces, kAny, kShort };
 // What is known of the pages: whole halves of tiles, whole groups of four tokens, nothing.
 enum Pages { kHalves, kFours, kTokens };
 
@@ -122,8 +127,27 @@ template <int DT, bool F8, int E, int N> __device__ __forceinline__ f32x4 produc
     return Elem<DT>::mfma(u32x4{w[0], w[1], w[2], w[3]}, q, c);
 }
 
-// Whether keys are loaded in whole lines (see above).
-template <bool F8, int DC, Shape SHAPE> constexpr bool quad_keys = SHAPE != kAny && F8;
+// Whether keys are loaded in whole lines (see above; rows at any address take 509 us that way, 276 without).
+template <bool F8, int DC, Shape SHAPE> constexpr bool quad_keys = SHAPE != kAny && SHAPE != kShort && F8;
+
+// kAny: the piece of a row that its end cuts off is loaded from so many bytes before (nothing past the row is read), and brought
+// into place, zeros behind, when it is used.  `past` may be the whole piece and more.
+template <int N> __device__ __forceinline__ void shift_down(uint32_t (&x)[N], int past) {
+    if constexpr (N == 4) {
+        const bool two = past & 8;
+        x[0] = two ? x[2] : x[0]; x[1] = two ? x[3] : x[1]; x[2] = two ? 0u : x[2]; x[3] = two ? 0u : x[3];
+    }
+    if constexpr (N >= 2) {
+        const bool one = past & 4;
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = one ? (i + 1 < N ? x[(i + 1) % N] : 0u) : x[i];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        x[i] = __builtin_amdgcn_alignbyte(i + 1 < N ? x[(i + 1) % N] : 0u, x[i], past & 3);
+        x[i] = past >= 4 * N ? 0u : x[i];
+    }
+}
 
 // Loads through a buffer descriptor: the base in scalar registers, one offset a lane, and what is past the range reads as zeros.
 constexpr uint32_t kNowhere = 0x80000000u;
@@ -274,7 +298,7 @@ __device__ __forceinline__ void join_parts(const PagedAttentionArgs &a, const Pa
 
 // DC: dimensions that the registers hold (64, 128, 256).
 template <int DT, bool F8, int DC, int SETS, Shape SHAPE, Pages PAGES>
-__global__ void __launch_bounds__(kPagedThreads, resident_groups(DC, F8, SETS))
+__global__ void __launch_bounds__(kPagedThreads, resident_groups(DC, F8, SETS, SHAPE == kAny || SHAPE == kShort))
 paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
     constexpr int EB = F8 ? 1 : 2;           // bytes of an element
     constexpr int PW = DC / 16;              // dimensions of a row that a lane holds
@@ -392,7 +416,7 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
                     const int hd = kPagedHeads * z + l16;
                     const char *const p = a.q + (u.q0 + hd) * a.q_head_bytes + u.request * a.q_row_bytes + 2 * d;
                     if (hd < u.rows) {
-                        if (SHAPE == kAny) load_part<QN>(x, p, 2 * (a.dim - d));
+                        if (SHAPE == kAny || SHAPE == kShort) load_part<QN>(x, p, 2 * (a.dim - d));
                         else if (SHAPE == kFull || d < a.dim) load_stream<QN>(x, p);
                     }
                     qf[z][c][k] = u32x4{x[0], x[1], x[QN - 2], x[QN - 1]};
@@ -454,14 +478,18 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
         constexpr int kNext = QUAD ? 16 * EB * E : 64;
         const int b = QUAD ? EB * E * (4 * g + c4) : 16 * g, row = EB * a.dim;
         const char *const base = a.k.base + u.h * a.k.head_bytes;
-        if (PAGES == kTokens) {
+        if (SHAPE == kAny || SHAPE == kShort) {
             const char *p[KR];
 #pragma unroll
-            for (int i = 0; i < KR; ++i) p[i] = base + place_of(a.k, u, s, t0, 16 * i + l16);
+            for (int i = 0; i < KR; ++i)
+                p[i] = base + place_of(a.k, u, s, t0, PAGES == kHalves ? i : 16 * i + l16) + (PAGES == kHalves ? (uint32_t)(l16 * a.k.token_bytes) : 0u);
 #pragma unroll
             for (int k = 0; k < KL; ++k)
 #pragma unroll
-                for (int i = 0; i < KR; ++i) load_part<KN>(kx[i][k], p[i] + b + kNext * k, row - b - kNext * k);
+                for (int i = 0; i < KR; ++i) {
+                    if (SHAPE == kAny) load_stream<KN>(kx[i][k], p[i] + (uint32_t)min(b + kNext * k, row - 4 * KN));
+                    else load_part<KN>(kx[i][k], p[i] + b + kNext * k, row - b - kNext * k);
+                }
             return;
         }
         __amdgpu_buffer_rsrc_t res[2];
@@ -484,14 +512,19 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
         constexpr int kNext = 16 * EB * E;
         const int b = EB * E * l16, row = EB * a.dim;
         const char *const base = a.v.base + u.h * a.v.head_bytes;
-        if (PAGES == kTokens) {
+        if (SHAPE == kAny || SHAPE == kShort) {
             const char *p[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = base + place_of(a.v, u, s, t0, 16 * (i / 4) + 4 * g + i % 4);
+            for (int i = 0; i < 8; ++i)
+                p[i] = base + place_of(a.v, u, s, t0, PAGES == kHalves ? i / 4 : 16 * (i / 4) + 4 * g + i % 4) +
+                       (PAGES == kHalves ? (uint32_t)((4 * g + i % 4) * a.v.token_bytes) : 0u);
 #pragma unroll
             for (int k = 0; k < L; ++k)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) load_part<N>(vx[i][k], p[i] + b + kNext * k, row - b - kNext * k);
+                for (int i = 0; i < 8; ++i) {
+                    if (SHAPE == kAny) load_stream<N>(vx[i][k], p[i] + (uint32_t)min(b + kNext * k, row - 4 * N));
+                    else load_part<N>(vx[i][k], p[i] + b + kNext * k, row - b - kNext * k);
+                }
             return;
         }
         __amdgpu_buffer_rsrc_t res[2];
@@ -507,6 +540,26 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 buffer_stream<N>(vx[i][k], res[i / 4], may_miss(k, L) && b + kNext * k >= row ? kNowhere : off[i / 4] + kNext * k, i % 4 * a.v.token_bytes);
+    };
+    // kAny: pieces that the rows' end cuts off, once they are there.
+    auto settle_keys = [&]() {
+        if (SHAPE != kAny) return;
+        const int row = EB * a.dim;
+#pragma unroll
+        for (int k = 0; k < KL; ++k)
+            if (64 * (k + 1) > row)
+#pragma unroll
+                for (int i = 0; i < KR; ++i) shift_down<KN>(kx[i][k], max(16 * g + 64 * k - (row - 4 * KN), 0));
+    };
+    auto settle_values = [&]() {
+        if (SHAPE != kAny) return;
+        constexpr int kNext = 16 * EB * E;
+        const int row = EB * a.dim;
+#pragma unroll
+        for (int k = 0; k < L; ++k)
+            if (kNext * (k + 1) > row)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) shift_down<N>(vx[i][k], max(EB * E * l16 + kNext * k - (row - 4 * N), 0));
     };
     // The wavefront's first tile of a unit.  Loads come back in the order in which they were asked for, so page numbers are asked
     // for before the loads that others wait for: those of a tile two tiles ahead.
@@ -536,6 +589,7 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
         Spot after;
         if (MORE) after = look_up(u, t0 + 2 * kStep);
         // ---- scores of tokens t0 + 16 i + 4 g + j
+        settle_keys();
         f32x4 sc[SETS][2];
 #pragma unroll
         for (int z = 0; z < SETS; ++z)
@@ -562,6 +616,7 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
             load_keys(u, ahead, t0 + kStep);
             __builtin_amdgcn_sched_barrier(0);
         }
+        settle_values();
         if (t0 < u.first || t0 + kPagedTile > u.len) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -782,18 +837,32 @@ static int64_t span(const PagedArray &x, const PagedAttentionArgs &a) {
 }
 
 // Rows of whole pieces at addresses that are multiples of 16 go through descriptors: pages of 16, 32, ... tokens with one a page,
-// pages of 4, 8, 12, 20, ... with one for all pages, whose offsets have 31 bits.  All else runs through the build that takes
-// every token and byte by itself.
-template <int DT, bool F8, int DC, int SETS> static int launch_class(const PagedAttentionArgs &a, const PagedWork &w, hipStream_t stream) {
+// pages of 4, 8, 12, 20, ... with one for all pages, whose offsets have 31 bits.  All else runs through the builds for any
+// address, by page for pages of 16, 32, ..., else token by token; rows shorter than a load take byte by byte.
+struct PagedBuild {
+    Shape shape;                             // (kFull for kPieces as well)
+    Pages pages;
+};
+static inline PagedBuild build_of(const PagedAttentionArgs &a, bool f8) {
     const uint64_t bits = (uint64_t)a.k.base | (uint64_t)a.v.base | (uint64_t)a.k.page_bytes | (uint64_t)a.v.page_bytes | (uint64_t)a.k.head_bytes |
                           (uint64_t)a.v.head_bytes | (uint64_t)a.k.token_bytes | (uint64_t)a.v.token_bytes;
+    const bool pieces = bits % 16 == 0 && a.dim % (f8 ? 16 : 8) == 0;
     // (the page stride as 32 bits: one scalar multiplication less a tile and array)
-    const bool pieces = bits % 16 == 0 && ((uint64_t)a.k.page_bytes | (uint64_t)a.v.page_bytes) >> 32 == 0 && a.dim % (F8 ? 16 : 8) == 0;
-    if (pieces && a.page.d % 16 == 0)
+    const bool near = ((uint64_t)a.k.page_bytes | (uint64_t)a.v.page_bytes) >> 32 == 0;
+    if (near && a.page.d % 16 == 0 && a.dim * (f8 ? 1 : 2) >= 16) return {pieces ? kFull : kAny, kHalves};
+    if (near && pieces && a.page.d % 4 == 0 && span(a.k, a) < kNowhere && span(a.v, a) < kNowhere) return {kFull, kFours};
+    return {a.dim * (f8 ? 1 : 2) < 16 ? kShort : kAny, kTokens};
+}
+
+template <int DT, bool F8, int DC, int SETS> static int launch_class(const PagedAttentionArgs &a, const PagedWork &w, hipStream_t stream) {
+    const PagedBuild build = build_of(a, F8);
+    if (build.shape == kFull && build.pages == kHalves)
         return a.dim == DC ? launch_split<DT, F8, DC, SETS, kFull, kHalves>(a, w, stream) : launch_split<DT, F8, DC, SETS, kPieces, kHalves>(a, w, stream);
-    if (pieces && a.page.d % 4 == 0 && span(a.k, a) < kNowhere && span(a.v, a) < kNowhere)
+    if (build.shape == kFull)
         return a.dim == DC ? launch_split<DT, F8, DC, SETS, kFull, kFours>(a, w, stream) : launch_split<DT, F8, DC, SETS, kPieces, kFours>(a, w, stream);
-    return launch_split<DT, F8, DC, SETS, kAny, kTokens>(a, w, stream);
+    if constexpr (DC == 64)
+        if (build.shape == kShort) return launch_split<DT, F8, DC, SETS, kShort, kTokens>(a, w, stream);
+    return build.pages == kHalves ? launch_split<DT, F8, DC, SETS, kAny, kHalves>(a, w, stream) : launch_split<DT, F8, DC, SETS, kAny, kTokens>(a, w, stream);
 }
 
 template <int DT, bool F8> int launch_paged_dtype(const PagedAttentionArgs &a, const PagedWork &w, hipStream_t stream) {
