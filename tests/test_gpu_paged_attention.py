@@ -112,6 +112,24 @@ def test_rows_at_any_alignment(dev, fp8, dim, order):
     Batch([5, 0, 40, 129, 1], 3, 2, dim, 16, torch.bfloat16, fp8, order, seed=dim).check(dev, flat=True)
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dim", [3, 8, 9, 15, 16, 17, 33, 64, 65, 119, 128, 200, 255])
+@pytest.mark.parametrize("page,group,window", [(16, 3, 0), (24, 32, 40), (7, 1, 0), (64, 32, 0)])
+def test_rows_between_nan(dev, fp8, dim, page, group, window):
+    """Rows an odd number of elements apart; what lies between them is NaN."""
+    b = Batch([1, 0, 33, 700, 64], 2, group, dim, page, torch.float16, fp8, seed=dim + page)
+    ref, bound = b.expect(0.25, window)
+    caches = []
+    for c in (b.k, b.v):
+        wide = torch.full((*c.shape[:3], dim + 2 + dim % 2 + 1), float("nan"), dtype=b.dtype).to(c.dtype)
+        raw, mine = (wide.view(torch.uint8), c.view(torch.uint8)) if fp8 else (wide, c)
+        raw[..., 1:dim + 1] = mine
+        caches.append(wide.to(dev)[..., 1:dim + 1])
+    scales = [None if x is None else x.to(dev) for x in b.scales]
+    got = blockedAttention.pagedAttention(b.q.to(dev), *caches, b.table.to(dev), torch.tensor(b.lens).to(dev), 0.25, window, *scales)
+    assert ((got.double().cpu() - ref).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("page", [1, 2, 7, 8, 16, 24, 32, 48, 64, 100, 256])
 @pytest.mark.parametrize("order", ["heads", "tokens"])
 @pytest.mark.parametrize("fp8", [False, True])
