@@ -788,7 +788,10 @@ Tensor pagedAttention_op(const Tensor &q, const Tensor &k_cache, const Tensor &v
     TORCH_CHECK(qr.heads >= 1 && qr.heads % c.heads == 0, "q must have a multiple of the cache's ", c.heads, " heads, got ", qr.heads);
     TORCH_CHECK(table.size(0) == qr.rows, "q has ", qr.rows, " rows, table ", table.size(0));
     check_meta(lens, "lens", k_cache, qr.rows);
-    Tensor out = at::empty_like(q);                          // q's order of dimensions
+    // q's order of dimensions; but where rows of q overlap that may put the last dimension, which the kernel writes in one
+    // piece, outside another
+    Tensor out = at::empty_like(q);
+    if (out.size(-1) > 1 && out.stride(-1) != 1) out = at::empty(q.sizes(), q.options());
     const Rows outr = rows_of(out, "out", c.dim);
     const size_t bytes = ba_paged_attention_workspace(&c, qr.heads, qr.rows, table.size(1));
     Tensor work;

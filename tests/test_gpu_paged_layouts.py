@@ -1,0 +1,32 @@
+"""Operands of the paged cache's operators in unusual layouts: the same values in the usual one give the same bits."""
+import pytest
+import torch
+
+import blockedAttention
+from test_gpu_paged_attention import Batch
+
+pytestmark = pytest.mark.gpu
+
+# queries of four heads, three requests, dimension 16 as views of 400 numbers
+QUERIES = {
+    "rows one element apart": lambda x: x[:4 * 18].view(4, 18).unfold(-1, 16, 1),
+    "rows and heads one element apart": lambda x: x.as_strided((4, 3, 16), (1, 1, 1)),
+    "heads one element apart, rows inside": lambda x: x.as_strided((4, 3, 16), (1, 40, 1)),
+    "heads by dimensions one element apart": lambda x: x.as_strided((4, 48), (1, 1)),
+    "one row for all": lambda x: x[:16].expand(4, 3, 16),
+    "one head for all": lambda x: x[:48].expand(4, 48),
+    "requests outside": lambda x: x[:4 * 48].view(3, 4, 16).transpose(0, 1),
+    "padded": lambda x: x[:4 * 3 * 20].view(4, 3, 20)[..., 1:17],
+}
+
+
+@pytest.mark.parametrize("name", QUERIES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_queries(dev, name, dtype):
+    b = Batch([40, 0, 700], 2, 2, 16, 16, dtype, seed=3)
+    q = QUERIES[name]((torch.randn(400, generator=torch.Generator().manual_seed(1)) * 2).to(dtype).to(dev))
+    rest = (b.k.to(dev), b.v.to(dev), b.table.to(dev), torch.tensor(b.lens).to(dev), 0.25)
+    want = blockedAttention.pagedAttention(q.contiguous(), *rest)
+    got = blockedAttention.pagedAttention(q, *rest)
+    assert got.shape == q.shape and got.dtype == dtype
+    assert torch.equal(got, want)
