@@ -6,6 +6,7 @@
 #include <algorithm>
 
 #include "ba_device.hpp"
+#include "ba_host.hpp"
 #include "paged.hpp"
 
 namespace ba {
@@ -63,10 +64,12 @@ template <int DT, bool F8, bool WHOLE> __device__ __forceinline__ void store_pie
     }
 }
 
-// Grid (tokens, heads or 1, keys and values).  WHOLE: rows are whole pieces.
+// Grid (a row of token groups, heads or 1, rows of keys and values by turns): one row but for more groups than flat_grid() puts
+// into one.  WHOLE: rows are whole pieces.
 template <int DT, bool F8, bool WHOLE> __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedAppendArgs a, AppendShape s) {
-    const int which = (int)blockIdx.z;
-    const int64_t t0 = (int64_t)blockIdx.x * s.tokens;
+    const int which = (int)blockIdx.z & 1;
+    const int64_t t0 = ((int64_t)(blockIdx.z >> 1) * gridDim.x + blockIdx.x) * s.tokens;
+    if (t0 >= a.tokens) return;
     const uint32_t most = (uint32_t)(min((int64_t)s.tokens, a.tokens - t0) * s.per_token.d);
     for (uint32_t i0 = threadIdx.x; i0 < most; i0 += kAppendPieces * kAppendThreads) {
         int64_t slot[kAppendPieces];
@@ -114,7 +117,8 @@ int launch_paged_append(const PagedAppendArgs &a, int dtype, int cache_dtype, hi
     const int64_t planes = s.heads_inner ? 2 : 2 * a.heads;
     while (tokens > 1 && a.tokens * planes < 256 * tokens) tokens /= 2;
     s.tokens = (int32_t)tokens;
-    const dim3 grid((unsigned)((a.tokens + tokens - 1) / tokens), s.heads_inner ? 1u : (unsigned)a.heads, 2);
+    const dim3 flat = flat_grid((a.tokens + tokens - 1) / tokens);
+    const dim3 grid(flat.x, s.heads_inner ? 1u : (unsigned)a.heads, 2 * flat.y);
     if (cache_dtype != BA_F8_E4M3) launch_append<0, false>(a, s, grid, stream);
     else if (dtype == BA_F16) launch_append<0, true>(a, s, grid, stream);
     else launch_append<1, true>(a, s, grid, stream);
