@@ -112,7 +112,8 @@ __attribute__((visibility("default"))) int ba_paged_attention(const ba_paged_cac
     if (requests == 0) return BA_OK;
     if (!q || !out || !lens || !counters || (width > 0 && !table)) return BA_ERR_INVALID_ARG;
     if (requests > 1 && width > 0 && table_stride < width) return BA_ERR_INVALID_ARG;
-    if (heads >= (1 << 20) || requests >= kTokenLimit / heads || width >= kTokenLimit / cache->page) return BA_ERR_UNSUPPORTED;
+    if (heads >= (1 << 20) || requests >= kTokenLimit / heads || width >= kTokenLimit || width * cache->page >= kTokenLimit)
+        return BA_ERR_UNSUPPORTED;
     const size_t need = ba_paged_attention_workspace(cache, heads, requests, width);
     if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255)) return BA_ERR_WORKSPACE;
     PagedAttentionArgs a{};
