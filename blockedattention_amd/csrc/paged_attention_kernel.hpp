@@ -190,8 +190,9 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 struct Visible {
     int first, len;                          // tokens first .. len - 1 are seen
     __device__ __forceinline__ int start() const { return first & ~(kPagedTile - 1); }
-    // a request without tokens has one tile: its zeros are written by whoever gets it
-    __device__ __forceinline__ int tiles() const { return len > first ? (len - start() + kPagedTile - 1) / kPagedTile : 1; }
+    // a request without tokens has one tile: its zeros are written by whoever gets it.  (The tile of the last token less that of the
+    // first: lengths go up to 2^31 - 1.)
+    __device__ __forceinline__ int tiles() const { return len > first ? (int)((uint32_t)(len - 1) / kPagedTile - (uint32_t)first / kPagedTile) + 1 : 1; }
 };
 __device__ __forceinline__ Visible visible(const PagedAttentionArgs &a, int r) {
     const int64_t room = (int64_t)a.width * a.page.d, length = a.lens[r];
@@ -455,19 +456,21 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
     bool poison = false;
     constexpr int low = PAGES == kHalves ? 15 : PAGES == kFours ? 3 : 0;
     auto borrowed = [&](const Unit &u, int t) { return min(max(t & ~low, u.first & ~low), (u.len - 1) & ~low) + (t & low); };
-    auto look_up = [&](const Unit &u, int t0) {
+    // (Tiles are looked up ahead, past the last one too: with lengths up to 2^31 - 1 such a place may wrap round to below zero, where
+    // it borrows that of the first token.)
+    auto look_up = [&](const Unit &u, uint32_t t0) {
         Spot s;
         const int32_t *const row = a.table + u.request * a.table_stride;
         if (PAGES == kHalves) {
             typedef const __attribute__((address_space(4))) int32_t *Row;      // scalar loads
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const uint32_t t = (uint32_t)borrowed(u, t0 + 16 * i), c = a.page.div(t);
+                const uint32_t t = (uint32_t)borrowed(u, (int)(t0 + 16 * i)), c = a.page.div(t);
                 s.page[i] = ((Row)(uintptr_t)row)[c];
                 s.line[i] = (int)(t - c * a.page.d);
             }
         } else {
-            s.page[0] = row[a.page.div((uint32_t)borrowed(u, t0 + (PAGES == kFours ? 4 * (lane & 7) : lane & 31)))];
+            s.page[0] = row[a.page.div((uint32_t)borrowed(u, (int)(t0 + (PAGES == kFours ? 4 * (lane & 7) : lane & 31))))];
         }
         return s;
     };
@@ -593,7 +596,7 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
         if (has_tile(u)) {
             const int t0 = u.start + (u.tile + wave) * kPagedTile;
             Spot s = look_up(u, t0);
-            ahead = look_up(u, t0 + kStep);
+            ahead = look_up(u, (uint32_t)t0 + kStep);
             check(s);
             __builtin_amdgcn_sched_barrier(0);
             load_keys(u, s, t0);
@@ -609,7 +612,7 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
     auto attend = [&](const Unit &u, auto more, int t0, float to_log2) {
         constexpr bool MORE = decltype(more)::value;
         Spot after;
-        if (MORE) after = look_up(u, t0 + 2 * kStep);
+        if (MORE) after = look_up(u, (uint32_t)t0 + 2 * kStep);
         // ---- scores of tokens t0 + 16 i + 4 g + j
         settle_keys();
         f32x4 sc[SETS][2];
@@ -639,7 +642,7 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
             __builtin_amdgcn_sched_barrier(0);
         }
         settle_values();
-        if (t0 < u.first || t0 + kPagedTile > u.len) {
+        if (t0 < u.first || (uint32_t)t0 + kPagedTile > (uint32_t)u.len) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int t = t0 + 16 * (i / 4) + 4 * g + i % 4;
