@@ -38,13 +38,12 @@ __device__ __forceinline__ Change change_of(const PagedTablesArgs &a, int64_t o,
     return {max(d, 0), max(-d, 0), n > o ? n - o : 0, 0};
 }
 
-// What all requests together change, and the verdict on it.
+// What all requests together change, and the verdict on it (the state given may hold any two numbers).
 struct Totals {
-    int64_t count, take, drop, grow;
-    int verdict;
+    int64_t count, take, drop, grow, verdict;
 };
 __device__ __forceinline__ void judge(const PagedTablesArgs &a, Totals &t) {
-    if (t.count < 0 || t.count + t.drop > a.pool) t.verdict |= BA_PAGED_BAD_STATE;
+    if (t.count < 0 || t.count > a.pool - t.drop) t.verdict |= BA_PAGED_BAD_STATE;
     if (!t.verdict) t.verdict = (t.take > t.count + t.drop ? BA_PAGED_NO_PAGES : 0) | (t.grow > a.tokens ? BA_PAGED_NO_SLOTS : 0);
 }
 
@@ -155,7 +154,7 @@ template <int K> __global__ void __launch_bounds__(kTableThreads) paged_tables_k
     int32_t *const take = sums, *const drop = sums + a.requests, *const grow = drop + a.requests;
     const int c = (a.requests + kTableThreads - 1) / kTableThreads;
     const int r0 = min(a.requests, (int)threadIdx.x * c), r1 = min(a.requests, r0 + c);
-    Totals t = {a.state_in[0], 0, 0, 0, (int)a.state_in[1]};
+    Totals t = {a.state_in[0], 0, 0, 0, a.state_in[1]};
     // all lengths of the thread are asked for before the first is used
     int64_t o[kTableEach], n[kTableEach];
 #pragma unroll
@@ -198,7 +197,7 @@ struct TableSums {
 };
 __global__ void __launch_bounds__(1024) paged_table_sums_kernel(PagedTablesArgs a, TableSums *w) {
     __shared__ Change waves[16];
-    Totals t = {a.state_in[0], 0, 0, 0, (int)a.state_in[1]};
+    Totals t = {a.state_in[0], 0, 0, 0, a.state_in[1]};
     for (int first = 0; first < a.requests; first += 1024) {
         const int r = first + (int)threadIdx.x;
         Change all;
