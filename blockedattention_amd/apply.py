@@ -136,9 +136,10 @@ def pagedAttention(
 
     ``q`` is ``[heads, requests * dim]`` or ``[heads, requests, dim]`` with any strides of heads and requests; its heads
     are a multiple of the cache's, consecutive ones share a key head.  ``table`` and ``lens`` are those of
-    ``pagedResize``, the caches and scales those of ``pagedAppend``.  ``window`` > 0 looks at the last ``window`` tokens
-    only.  Requests of length 0 give zeros.  The result has the shape, dtype and order of dimensions of ``q`` (contiguous where
-    rows of ``q`` overlap so that they have no order).  Forward only; nothing synchronises with the host.
+    ``pagedResize`` (here a table may also be one row expanded over the requests), the caches and scales those of
+    ``pagedAppend``.  ``window`` > 0 looks at the last ``window`` tokens only.  Requests of length 0 give zeros.  The result
+    has the shape, dtype and order of dimensions of ``q`` (contiguous where rows of ``q`` overlap so that they have no
+    order).  Forward only; nothing synchronises with the host.
     """
     return blockAttention.pagedAttention(q, kCache, vCache, table, lens, float(scale), int(window), kScale, vScale)
 

@@ -111,7 +111,7 @@ __attribute__((visibility("default"))) int ba_paged_attention(const ba_paged_cac
         return BA_ERR_INVALID_ARG;
     if (requests == 0) return BA_OK;
     if (!q || !out || !lens || !counters || (width > 0 && !table)) return BA_ERR_INVALID_ARG;
-    if (requests > 1 && width > 0 && table_stride < width) return BA_ERR_INVALID_ARG;
+    if (requests > 1 && width > 0 && table_stride < width && table_stride != 0) return BA_ERR_INVALID_ARG;   // (0: a row for all, only read)
     if (heads >= (1 << 20) || requests >= kTokenLimit / heads || width >= kTokenLimit || width * cache->page >= kTokenLimit)
         return BA_ERR_UNSUPPORTED;
     const size_t need = ba_paged_attention_workspace(cache, heads, requests, width);

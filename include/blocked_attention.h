@@ -390,11 +390,11 @@ int ba_paged_append(const ba_paged_cache *cache, int dtype, const void *k, int64
  * query head, over the request's lens[r] tokens or, with window > 0, the last `window` of them; group = heads / cache
  * heads query heads share a key head.  Requests without tokens give zeros.  q and out are [heads][requests][dim] by the
  * strides given (in elements); dtype: BA_F16 or BA_BF16, the cache's own or with a BA_F8_E4M3 cache either.  Sums, row
- * maxima and the products' accumulators are fp32.  Tokens beyond the table's row do not exist; a page number outside the cache makes
- * the rows of its request NaN instead of being read.  `workspace`: ba_paged_attention_workspace bytes, 256-byte aligned;
- * its content does not matter.  `counters`: BA_PAGED_COUNTERS numbers that are 0 before the first call and that every
- * call leaves at 0 again.  Calls that may run at the same time need counters and workspaces of their own; calls on one
- * stream may share them.
+ * maxima and the products' accumulators are fp32.  Tokens beyond the table's row do not exist; with a table_stride of 0 all
+ * requests have the same row; a page number outside the cache makes the rows of its request NaN instead of being read.
+ * `workspace`: ba_paged_attention_workspace bytes, 256-byte aligned; its content does not matter.  `counters`:
+ * BA_PAGED_COUNTERS numbers that are 0 before the first call and that every call leaves at 0 again.  Calls that may run at
+ * the same time need counters and workspaces of their own; calls on one stream may share them.
  */
 #define BA_PAGED_COUNTERS 4096
 size_t ba_paged_attention_workspace(const ba_paged_cache *cache, int64_t heads, int64_t requests, int64_t width);

@@ -30,3 +30,16 @@ def test_queries(dev, name, dtype):
     got = blockedAttention.pagedAttention(q, *rest)
     assert got.shape == q.shape and got.dtype == dtype
     assert torch.equal(got, want)
+
+
+def test_a_table_row_that_all_requests_share(dev):
+    """One row of pages, expanded over the requests: a prefix that all of them have, seen to different lengths."""
+    b = Batch([300], 2, 4, 64, 16, torch.float16, seed=5)
+    q = torch.randn((8, 5, 64), generator=torch.Generator().manual_seed(2)).half().to(dev)
+    lens = torch.tensor([300, 0, 17, 128, 1], device=dev)
+    k, v, row = b.k.to(dev), b.v.to(dev), b.table.to(dev)
+    got = blockedAttention.pagedAttention(q, k, v, row.expand(5, -1), lens, 0.125)
+    assert torch.equal(got, blockedAttention.pagedAttention(q, k, v, row.repeat(5, 1), lens, 0.125))
+    with pytest.raises(RuntimeError):                                     # where rows are written they have to be apart
+        blockedAttention.pagedResize(row.expand(5, -1), torch.arange(9, dtype=torch.int32, device=dev), torch.tensor([9, 0], device=dev),
+                                     lens, lens, 16, 0)
