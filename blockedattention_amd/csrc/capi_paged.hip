@@ -10,9 +10,17 @@ constexpr int64_t kTokenLimit = int64_t(1) << 31;      // tokens, places and byt
 
 static bool bad_stride(int64_t s) { return s < 0 || s > (int64_t(1) << 40); }
 
-// BA_OK, or what a cache that no kernel takes is refused with.
-static int check_cache(const ba_paged_cache *c) {
-    if (!c || c->pages < 0 || c->heads < 1 || c->page < 1 || c->dim < 1) return BA_ERR_INVALID_ARG;
+// BA_OK, or what a cache that no kernel takes is refused with.  The stride of a dimension of one entry is used by nothing and may
+// be anything: `c` becomes the same cache with 0 there (in pages of one token with something in range, which still tells whether
+// the heads lie closer together).
+static int check_cache(const ba_paged_cache *given, ba_paged_cache *c) {
+    if (!given) return BA_ERR_INVALID_ARG;
+    *c = *given;
+    if (c->pages <= 1) c->k_page_stride = c->v_page_stride = 0;
+    if (c->heads == 1) c->k_head_stride = c->v_head_stride = 0;
+    if (c->page == 1)
+        for (int64_t *s : {&c->k_token_stride, &c->v_token_stride}) *s = std::clamp<int64_t>(*s, 0, 1 << 28);
+    if (c->pages < 0 || c->heads < 1 || c->page < 1 || c->dim < 1) return BA_ERR_INVALID_ARG;
     if (c->dtype != BA_F16 && c->dtype != BA_BF16 && c->dtype != BA_F8_E4M3) return BA_ERR_UNSUPPORTED;
     if ((c->dtype == BA_F8_E4M3) != (c->k_scale != nullptr) || (c->dtype == BA_F8_E4M3) != (c->v_scale != nullptr))
         return BA_ERR_INVALID_ARG;
@@ -69,8 +77,10 @@ __attribute__((visibility("default"))) int ba_paged_append(const ba_paged_cache 
                                                            int64_t k_head_stride, int64_t k_token_stride, const void *v,
                                                            int64_t v_head_stride, int64_t v_token_stride,
                                                            const int64_t *slots, int64_t tokens, ba_stream_t stream) {
-    const int st = check_cache(cache);
+    ba_paged_cache plain;
+    const int st = check_cache(cache, &plain);
     if (st != BA_OK) return st;
+    cache = &plain;
     if (dtype != BA_F16 && dtype != BA_BF16) return BA_ERR_UNSUPPORTED;
     if (cache->dtype != BA_F8_E4M3 && cache->dtype != dtype) return BA_ERR_UNSUPPORTED;
     if (tokens < 0 || bad_stride(k_head_stride) || bad_stride(k_token_stride) || bad_stride(v_head_stride) || bad_stride(v_token_stride))
@@ -91,7 +101,8 @@ __attribute__((visibility("default"))) int ba_paged_append(const ba_paged_cache 
 
 __attribute__((visibility("default"))) size_t ba_paged_attention_workspace(const ba_paged_cache *cache, int64_t heads,
                                                                            int64_t requests, int64_t width) {
-    if (check_cache(cache) != BA_OK || heads < 1 || heads % cache->heads || requests < 1 || width < 0) return 0;
+    ba_paged_cache plain;
+    if (check_cache(cache, &plain) != BA_OK || heads < 1 || heads % cache->heads || requests < 1 || width < 0) return 0;
     return paged_attention_workspace(cache->heads, heads / cache->heads, cache->dim, cache->dtype, requests, width, cache->page);
 }
 
@@ -102,8 +113,10 @@ __attribute__((visibility("default"))) int ba_paged_attention(const ba_paged_cac
                                                               float scale, void *out, int64_t out_head_stride,
                                                               int64_t out_row_stride, int32_t *counters, void *workspace,
                                                               size_t workspace_bytes, ba_stream_t stream) {
-    const int st = check_cache(cache);
+    ba_paged_cache plain;
+    const int st = check_cache(cache, &plain);
     if (st != BA_OK) return st;
+    cache = &plain;
     if (dtype != BA_F16 && dtype != BA_BF16) return BA_ERR_UNSUPPORTED;
     if (cache->dtype != BA_F8_E4M3 && cache->dtype != dtype) return BA_ERR_UNSUPPORTED;
     if (heads < 1 || heads % cache->heads || requests < 0 || width < 0 || window < 0 || table_stride < 0) return BA_ERR_INVALID_ARG;

@@ -336,6 +336,7 @@ int ba_static_read(ba_plan_info *host_info, ba_stream_t stream);
  * (strides in elements, any order of heads and tokens, the last dimension contiguous), page_number = table[r][t / page].
  * dtype: BA_F16, BA_BF16, or BA_F8_E4M3 with `k_scale` and `v_scale` (fp32, one per head): what is stored times the
  * head's scale is the value.  dim <= 256; the tokens of a page and head span less than 2^31 bytes.
+ * The stride of a dimension of one entry is not used.
  * The structure itself is host memory, the pointers in it are device pointers.
  */
 typedef struct ba_paged_cache {

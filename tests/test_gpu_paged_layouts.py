@@ -43,3 +43,25 @@ def test_a_table_row_that_all_requests_share(dev):
     with pytest.raises(RuntimeError):                                     # where rows are written they have to be apart
         blockedAttention.pagedResize(row.expand(5, -1), torch.arange(9, dtype=torch.int32, device=dev), torch.tensor([9, 0], device=dev),
                                      lens, lens, 16, 0)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_strides_of_dimensions_of_one(dev, fp8):
+    """Pages of one token, one page, one head: the stride of a dimension of one means nothing, however large."""
+    for lens, heads, page in (([5, 9], 2, 1), ([7], 2, 16), ([40, 3], 1, 16)):
+        b = Batch(lens, heads, 2, 32, page, torch.float16, fp8, seed=page, extra=0)
+        k, v, q, table, lens = b.k.to(dev), b.v.to(dev), b.q.to(dev), b.table.to(dev), torch.tensor(lens).to(dev)
+        scales = [None if s is None else s.to(dev) for s in b.scales]
+        want = blockedAttention.pagedAttention(q, k, v, table, lens, 0.25, 0, *scales)
+        far = [c.as_strided(c.shape, [(1 << 45) + 1 if n == 1 else s for n, s in zip(c.shape, c.stride())]) for c in (k, v)]
+        assert torch.equal(blockedAttention.pagedAttention(q, *far, table, lens, 0.25, 0, *scales), want)
+        x = torch.randn((heads, 1, 32), device=dev).half()
+        place = torch.tensor([page * k.size(0) - 1], device=dev)
+        blockedAttention.pagedAppend(x, 2 * x, k, v, place, *scales)
+        want = [c.clone().view(torch.uint8) for c in (k, v)]
+        for c in (k, v):
+            c.view(torch.uint8).zero_()
+        blockedAttention.pagedAppend(x, 2 * x, *far, place, *scales)
+        for c, w in zip((k, v), want):
+            last = (k.size(0) - 1, slice(None), page - 1)
+            assert torch.equal(c.view(torch.uint8)[last], w[last]) and c.view(torch.uint8)[last].any()
