@@ -121,8 +121,8 @@ def pagedAppend(
     ``k`` and ``v`` are ``[heads, tokens * dim]`` (the layout of ``blockFusedAttention``) or ``[heads, tokens, dim]`` with any
     strides of heads and tokens, the caches ``[pages, heads, page, dim]`` with any strides but the last.  The caches have
     the dtype of ``k`` and ``v`` (fp16 or bf16), or are ``float8_e4m3fn``: then ``kScale`` and ``vScale`` (fp32
-    ``[heads]``) are what stored values are multiplied with; values are divided by it, limited to +-448 and rounded to
-    the nearest.  Places below 0 are skipped; no place may occur twice.
+    ``[heads]``) are what stored values are multiplied with; values are divided by it in fp32, limited to +-448 and
+    the quotient is rounded to the nearest, ties to even.  Places below 0 are skipped; no place may occur twice.
     """
     blockAttention.pagedAppend(k, v, kCache, vCache, slots, kScale, vScale)
 

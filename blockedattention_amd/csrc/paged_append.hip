@@ -2,7 +2,7 @@
 // writes is its floor.  A thread takes pieces of eight elements (16 bytes of the source); within a workgroup the
 // pieces follow each other as they lie in the cache -- the tokens of a head or the heads of a token, whichever are closer --
 // so that adjacent lanes write whole lines.  16384 tokens, 8 heads of 128, fp16 (134 MB) 22.8 us, 5.9 TB/s, bound by memory;
-// 30011 tokens, 8 heads of 64, bf16 to e4m3 (92 MB) 22.1 us, 4.2 TB/s, bound by the exact quotients as well; 64 tokens 4.0 us, a launch.
+// 30011 tokens, 8 heads of 64, bf16 to e4m3 (92 MB) 22.1 us, 4.2 TB/s, bound by the quotients as well; 64 tokens 4.0 us, a launch.
 #include <algorithm>
 
 #include "ba_device.hpp"
@@ -20,10 +20,12 @@ struct AppendShape {
     int32_t tokens, heads_inner;             // tokens of a workgroup; whether it takes all heads of them
 };
 
-// x / scale, limited to +-448; a NaN stays one.  With r the nearest number to 1 / scale and q = x r, one correction by the residual
+// The fp32 quotient x / scale, limited to +-448; a NaN stays one.  With r the nearest number to 1 / scale and q = x r, one correction by the residual
 // gives the nearest number to x / scale (Markstein's theorem; infinities and zeros stay as they are).  `plain`: a
 // scale for which nothing on the way leaves fp32's range (what does has a result that rounds to 0 or 448 all the same);
-// others are divided.  30 000 tokens of 8 x 64: 24 us with a division each, which costs twice the instructions.
+// others are divided.  30 000 tokens of 8 x 64: 24 us with a division each, which costs
+// twice the instructions.  It is rounded once more, to e4m3, as fp32 code that divides and converts does: a quotient that fp32
+// makes a tie of goes to even, whichever side of it the exact one is.
 __device__ __forceinline__ float scaled_down(float x, float scale, float r, bool plain) {
     float q = x * r;
     if (plain) {

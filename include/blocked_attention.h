@@ -379,8 +379,9 @@ int ba_paged_resize(int32_t *table, int64_t table_stride, int64_t width, int32_t
 /*
  * Keys and values of new tokens into their places: token t of k and v ([heads][tokens][dim] by the strides given, in
  * elements) goes to place slots[t]; places below 0 or past the last page are skipped.  No place may occur twice.
- * dtype: BA_F16 or BA_BF16, the cache's own or, into a BA_F8_E4M3 cache, either: value / scale, limited to +-448, to
- * the nearest, ties to even.
+ * dtype: BA_F16 or BA_BF16, the cache's own or, into a BA_F8_E4M3 cache, either: the fp32 quotient value / scale, limited
+ * to +-448 and rounded to the nearest, ties to even (of the two roundings the first decides where it makes a tie).
+ * pages * page is below 2^31.
  */
 int ba_paged_append(const ba_paged_cache *cache, int dtype, const void *k, int64_t k_head_stride, int64_t k_token_stride,
                     const void *v, int64_t v_head_stride, int64_t v_token_stride, const int64_t *slots, int64_t tokens,
