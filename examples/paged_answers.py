@@ -5,12 +5,13 @@
 Every step some requests arrive with a prompt, some end, the others go on by one token:
 
     pagedResize          gives the prompts and the new tokens their places, and the ended requests' pages to others
-    blockFusedAttention  attends within the prompts (segments of different lengths back to back)
+    blockFusedAttention  attends within the prompts (segments of different lengths back to back), from every token to all of
+                         its prompt: it has no causal mask, so this is a prefix that is read in both directions
     pagedAppend          writes keys and values of both to their places
     pagedAttention       attends from each request's new token to all that it has
 
 The host makes the lengths; the GPU keeps pages and places, and nothing waits for it until the end, when the verdict of
-all steps is read.  The weights are random; every result is compared with the same attention over dense copies in fp32.
+all steps is read.  The weights are random; every result of either attention is compared with the same over dense copies in fp32.
 """
 import argparse
 import os
@@ -77,13 +78,19 @@ def main(cache="bf16", steps=40, seed=0):
         blockedAttention.pagedAppend(k, v, layer.k, layer.v, slots, *layer.scales)
         at = {r: sum(grown[:r]) for r in range(SLOTS)}
         if prompts:
-            # the prompts' own attention, over segments back to back; key heads are repeated for their query heads
+            # the prompts' own attention, over segments back to back; key heads are repeated for their query heads.  (It takes the
+            # keys and values as the projection gave them, not as a cache in 8 bits has them.)
             rows = torch.cat([torch.arange(at[r], at[r] + new[r]) for r in prompts]).to(dev)
             lengths = torch.tensor([new[r] for r in prompts], device=dev)
             flat = lambda t: t[:, rows].reshape(t.shape[0], -1).contiguous()  # noqa: E731
             wide = lambda t: t.repeat_interleave(GROUP, 0)  # noqa: E731
-            blockedAttention.blockFusedAttention(flat(q), flat(wide(k)), flat(wide(v)), lengths, lengths, torch.full_like(lengths, DIM),
-                                                 scale=DIM ** -0.5)
+            inside = blockedAttention.blockFusedAttention(flat(q), flat(wide(k)), flat(wide(v)), lengths, lengths,
+                                                          torch.full_like(lengths, DIM), scale=DIM ** -0.5)
+            inside = inside.view(HEADS * GROUP, -1, DIM).float().split([new[r] for r in prompts], 1)
+            for r, got in zip(prompts, inside):
+                qr, kr, vr = (t[:, at[r]:at[r] + new[r]].float() for t in (q, wide(k), wide(v)))
+                p = torch.softmax(qr @ kr.transpose(1, 2) * DIM ** -0.5, -1)
+                worst = max(worst, (p @ vr - got).abs().max().item())
         # one query per request that has tokens: its newest; ended and empty ones are rows of length 0
         newest = torch.tensor([max(at[r] + grown[r] - 1, 0) for r in range(SLOTS)], device=dev)
         out = blockedAttention.pagedAttention(q[:, newest], layer.k, layer.v, table, lens, scale=DIM ** -0.5,
