@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_gpu_paged_attention import Batch
+from test_gpu_paged_attention import FP8, U, Batch
 
 pytestmark = pytest.mark.gpu
 
@@ -27,3 +27,43 @@ def test_an_infinite_value_that_counts_makes_its_column_infinite(dev, dtype, dim
     # (NaN only where both signs meet)
     assert torch.equal(torch.nan_to_num(got[~finite], nan=0.5), torch.nan_to_num(ref[~finite], nan=0.5))
     assert ((got - ref).abs() <= bound)[finite].all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_a_probability_is_kept_to_more_than_16_bits(dev, dtype, fp8, dim):
+    """128 tokens whose signed values nearly cancel: the rounding of the result is small, that of the probabilities is not.
+
+    Bound, times P |V|: what two 16-bit terms lose of a probability, 2^-16 (bf16, 8 bits a term) or 2^-21 (fp16, 11 bits; those
+    here are far above its smallest number); 2 (2 + 8) 2^-24 max |scale| sum |q k| for scores of two non-zero products in fp32;
+    2^-20 for the exponentials; 80 additions of fp32 (a tile's 64 products, four wavefronts).  And the result's own rounding.
+    """
+    heads, n = 4, 128
+    b = Batch([n], heads, 1, dim, 16, dtype, fp8, seed=dim)
+    g = torch.Generator().manual_seed(dim + 1)
+    b.q[:] = 0
+    b.q[:, 0, :2] = torch.randn((heads, 2), generator=g).to(dtype)
+    k = torch.randint(-16, 17, (heads, n, dim), generator=g) / 8.0
+    q = b.q[:, 0].double()
+    p = torch.softmax(torch.matmul(k.double(), q[:, :, None])[..., 0], -1)                  # [heads, tokens]
+    v = torch.randint(8, 16, (heads, n, dim), generator=g) / 8.0
+    order, total = p.argsort(-1, descending=True), torch.zeros((heads, dim), dtype=torch.float64)
+    for i in range(n):                                                                      # signs that keep the sum near 0
+        at = (torch.arange(heads), order[:, i])
+        v[at] *= torch.where(total > 0, -1.0, 1.0)
+        total += p[at][:, None] * v[at]
+    for c, x in ((b.k, k), (b.v, v)):
+        raw, mine = (c.view(torch.uint8), x.to(FP8).view(torch.uint8)) if fp8 else (c, x.to(dtype))
+        for i in range(n // 16):
+            raw[int(b.table[0, i])] = mine[:, 16 * i:16 * i + 16]
+    if fp8:
+        b.scales = [torch.ones(heads), torch.ones(heads)]
+    got = b.run(dev, 1.0).double().cpu()[:, 0]
+    e = 10 * 2.0 ** -24 * (k.double().abs() * q.abs()[:, None]).sum(-1).amax(-1)
+    terms = 2.0 ** -16 if dtype == torch.bfloat16 else 2.0 ** -21
+    ref, size = (torch.matmul(p[:, None], x.double())[:, 0] for x in (v, v.abs()))
+    bound = U[dtype] * ref.abs() + (terms + 2 * e[:, None] + 2.0 ** -20 + 80 * 2.0 ** -24) * size + 2.0 ** -24
+    one = torch.matmul(p.to(dtype).double()[:, None], v.double())[:, 0]                     # with one 16-bit term each
+    assert ((one - ref).abs() > 2 * bound).any()
+    assert ((got - ref).abs() <= bound).all()
