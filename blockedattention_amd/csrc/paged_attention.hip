@@ -20,8 +20,8 @@ static PagedWork work_of(int64_t heads, int64_t group, int64_t dim, bool f8, boo
     const double longest = window > 0 ? std::min((double)width * page, (double)window + kPagedTile) : (double)width * page;
     const double most = std::max((double)units, (double)units * (longest / kPagedTile + 1) / kPagedShare + 1);
     w.groups = (int32_t)std::max<int64_t>(1, std::min<int64_t>(BA_PAGED_COUNTERS, (int64_t)std::min<double>((double)resident, most)));
-    w.by_unit = units <= w.groups;
-    const size_t split = ((size_t)(w.by_unit ? units : w.groups) * sizeof(Left) + 255) & ~size_t(255);
+    // (the list is only used where units are far fewer than workgroups, see below)
+    const size_t split = ((size_t)std::min<int64_t>(units, w.groups) * sizeof(Left) + 255) & ~size_t(255);
     const size_t parts = (2 * (size_t)w.groups * w.rows * sizeof(PagedPart) + 255) & ~size_t(255);
     w.pitch = (int32_t)((dim + 3) & ~int64_t(3));
     const size_t sums = 2 * (size_t)w.groups * w.rows * w.pitch * sizeof(float);

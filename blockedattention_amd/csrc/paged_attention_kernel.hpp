@@ -76,8 +76,10 @@ struct Left {
 
 struct PagedWork {
     int32_t *counters;                       // [groups]: how many have left their part of the unit begun by a workgroup; 0 between calls
-    Left *split;                             // not NULL: instead of counting, one entry a unit (by_unit) or a workgroup for the joining kernel
-    int32_t by_unit;
+    Left *split;                             // not NULL: instead of counting, one entry a unit for the joining kernel
+    // Brings what follows to a multiple of 32 bytes in the kernel's arguments.  Else the compiler fetches it in pieces with what is before,
+    // moves whole pieces to and from vector registers (367 moves for 144), and 64 dimensions take 64 us for 60.
+    int64_t pad;
     PagedPart *parts;                        // [2 * groups][rows]
     float *sums;                             // [2 * groups][rows][pitch]
     int32_t groups, tiles_a_head, rows, pitch;     // tiles_a_head: units of a key head; rows: query heads of the largest unit
@@ -142,7 +144,7 @@ template <int DT, bool F8, int E, int N> __device__ __forceinline__ f32x4 produc
 }
 
 // Whether keys are loaded in whole lines (see above; rows at any address take 509 us that way, 276 without).
-template <bool F8, int DC, Shape SHAPE> constexpr bool quad_keys = SHAPE != kAny && SHAPE != kShort && F8;
+template <bool F8, Shape SHAPE> constexpr bool quad_keys = SHAPE != kAny && SHAPE != kShort && F8;
 
 // kAny: the piece of a row that its end cuts off is loaded from so many bytes before (nothing past the row is read), and brought
 // into place, zeros behind, when it is used.  `past` may be the whole piece and more.
@@ -319,7 +321,7 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
     constexpr int PW = DC / 16;              // dimensions of a row that a lane holds
     constexpr int E = PW * EB < 16 ? PW : 16 / EB, N = E * EB / 4;      // those of one load, its dwords
     constexpr int L = PW / E;                // loads; load k of lane x of a row: dimensions 16 E k + E x ..
-    constexpr bool QUAD = quad_keys<F8, DC, SHAPE>;
+    constexpr bool QUAD = quad_keys<F8, SHAPE>;
     constexpr int PARTS = QUAD && E > 8 ? E / 8 : 1;           // matrix instructions that a load of a key feeds (for each c')
     constexpr int KR = QUAD ? 8 : 2, KL = QUAD ? L : DC * EB / 64, KN = QUAD ? N : 4;      // a lane's tokens of a tile, loads of each, dwords
     constexpr int QC = QUAD ? 4 : 1, QK = QUAD ? L * PARTS : DC / 32;                    // operands of the queries
@@ -328,47 +330,37 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
 
     extern __shared__ __attribute__((aligned(16))) float lds[];           // [waves][rows][DC + 4]
     __shared__ int64_t scan[kPagedWaves];
-    __shared__ int lives[kPagedWaves];
     __shared__ Place places[2];
     __shared__ float wave_m[kPagedWaves][SETS * kPagedHeads], wave_l[kPagedWaves][SETS * kPagedHeads];
     __shared__ Left left[2];
     __shared__ bool joins[2];
     int unfinished = 0;
-    Left mine_split = {0, 0, 0, 0, 0, 0};
 
     // ---- the share.  Thread i adds up the tiles of requests [i c, (i + 1) c).
     const int c = (a.requests + kPagedThreads - 1) / kPagedThreads, r0 = (int)threadIdx.x * c;
     const int r1 = min(a.requests, r0 + c);
     int64_t mine = 0;
-    int live = 0;
     Visible front = {0, 0};
     for (int r = r0; r < r1; ++r) {
         const Visible v = visible(a, r);
         if (r == r0) front = v;
         mine += v.tiles();
-        live += v.tiles() > 0;
     }
     int64_t upto = wave_inclusive_scan(mine);
-    live = wave_inclusive_scan(live);
-    if (lane == 63) { scan[wave] = upto; lives[wave] = live; }
+    if (lane == 63) scan[wave] = upto;
     __syncthreads();
     int64_t total = 0;
-    live = 0;
 #pragma unroll
     for (int i = 0; i < kPagedWaves; ++i) {
         if (i < wave) upto += scan[i];
         total += scan[i];
-        live += lives[i];
     }
     total = uniform64(total) * units;
     // (a workgroup for every unit while there are enough: a request of 5 tokens, 14 key heads of 80, 8-bit 7.7 us,
     // four units to a workgroup 17.4)
-    const int64_t groups = min((int64_t)w.groups, max((total + kPagedShare - 1) / kPagedShare, uniform64((int64_t)live) * units));
+    const int64_t groups = min((int64_t)w.groups, max((total + kPagedShare - 1) / kPagedShare, (int64_t)a.requests * units));
     const int64_t group = blockIdx.x;
-    if (group >= groups) {
-        if (w.split && !w.by_unit && threadIdx.x == 0) w.split[group].parts = 0;
-        return;
-    }
+    if (group >= groups) return;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         int64_t at = scaled(group + k, total, groups);
@@ -416,10 +408,7 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
         return u;
     };
     const Place place = places[0];
-    if (place.at >= end) {
-        if (w.split && !w.by_unit && threadIdx.x == 0) w.split[group].parts = 0;
-        return;
-    }
+    if (place.at >= end) return;
     Unit cur = unit_of(uniform(place.request), uniform(place.unit), uniform(place.tile), uniform64(place.at),
                        {uniform(place.see.first), uniform(place.see.len)});
 
@@ -797,10 +786,7 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
             u.parts = (int)scaled_up(from + cur.n, groups, total) - u.begins;
         }
         if (w.split) {
-            if (begun) {
-                mine_split = u;
-                if (w.by_unit && threadIdx.x == 0) w.split[(int64_t)cur.request * units + cur.unit] = u;
-            }
+            if (begun && threadIdx.x == 0) w.split[(int64_t)cur.request * units + cur.unit] = u;
         } else if (!whole) {
             if (threadIdx.x == 0) left[unfinished] = u;
             ++unfinished;                    // (the first unit of the share at most, and its last)
@@ -809,11 +795,7 @@ paged_attention_kernel(PagedAttentionArgs a, PagedWork w) {
         lds_barrier();
         cur = next;
     }
-    if (w.split) {
-        if (!w.by_unit && threadIdx.x == 0) w.split[group] = mine_split;
-        return;
-    }
-    if (unfinished == 0) return;
+    if (w.split || unfinished == 0) return;  // (with a list nothing is unfinished; said for the compiler, as the padding is)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0)
@@ -848,7 +830,7 @@ static int launch_split(const PagedAttentionArgs &a, const PagedWork &w, hipStre
     const size_t lds = (size_t)kPagedWaves * w.rows * (DC + 4) * sizeof(float);
     paged_attention_kernel<DT, F8, DC, SETS, SHAPE, PAGES><<<w.groups, kPagedThreads, lds, stream>>>(a, w);
     if (w.split) {
-        const int64_t entries = w.by_unit ? a.requests * (int64_t)a.heads * w.tiles_a_head : w.groups;
+        const int64_t entries = a.requests * (int64_t)a.heads * w.tiles_a_head;
         const int most = kPagedThreads / (DC / 4);
         int heads = 1;
         while (heads < most && heads < w.rows && entries * ((w.rows + heads - 1) / heads) > kPagedJoins) heads *= 2;
