@@ -67,3 +67,31 @@ def test_a_probability_is_kept_to_more_than_16_bits(dev, dtype, fp8, dim):
     one = torch.matmul(p.to(dtype).double()[:, None], v.double())[:, 0]                     # with one 16-bit term each
     assert ((one - ref).abs() > 2 * bound).any()
     assert ((got - ref).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("size", [2.0 ** 12, 3.0 * 2 ** 12, 2.0 ** 14, 3.0 * 2 ** 14, 60000.0])
+def test_scores_of_many_millions_find_their_token(dev, dtype, fp8, size):
+    """One key is far closer to the query than all others: the result is its value, whatever the scores' last digits are worth."""
+    b = Batch([1, 100, 700], 2, 2, 64, 16, dtype, fp8, seed=21)
+    b.q[:] = 0
+    b.q[..., :16] = size
+    b.scales = [torch.ones(2), torch.ones(2)] if fp8 else [None, None]
+    top = torch.tensor(448.0 if fp8 else size).to(b.k.dtype)
+    want = torch.zeros(b.q.shape, dtype=torch.float64)
+    for r, n in enumerate(b.lens):
+        for t in range(n):
+            at = (int(b.table[r, t // 16]), slice(None), t % 16)
+            row = torch.zeros((2, 64)).to(b.k.dtype)
+            for c in range(16 if t == n // 3 else t % 3):                 # 16 times the size, or not even a fifth of that
+                row.view(torch.uint8 if fp8 else torch.int16)[:, c] = top.view(torch.uint8 if fp8 else torch.int16)
+            b.k.view(row.view(torch.uint8).dtype if fp8 else torch.int16)[at] = row.view(torch.uint8 if fp8 else torch.int16)
+        v = b.tokens(b.v, b.scales[1], r, 0, n)
+        want[:, r] = v[:, n // 3].repeat_interleave(2, 0)
+    for scale, other in ((1.0, None), (0.125, None), (-1.0, 0)):
+        if other is None:
+            got = b.run(dev, scale).double().cpu()
+            assert torch.equal(got, want.to(dtype).double()), scale
+        else:
+            assert torch.isfinite(b.run(dev, scale)).all()
