@@ -662,8 +662,11 @@ Rows rows_of(const Tensor &t, const char *name, int64_t dim) {
     return {t.size(0), t.size(1) / dim, t.stride(0), dim};
 }
 
-void check_no_grad(std::initializer_list<const Tensor *> tensors, const char *op) {
-    for (const Tensor *t : tensors)
+void check_no_grad(std::initializer_list<const Tensor *> tensors, const OptTensor &k_scale, const OptTensor &v_scale, const char *op) {
+    std::vector<const Tensor *> all(tensors);
+    for (const OptTensor *s : {&k_scale, &v_scale})
+        if (s->has_value()) all.push_back(&**s);
+    for (const Tensor *t : all)
         TORCH_CHECK(!(at::GradMode::is_enabled() && t->requires_grad()), op, " has no backward pass: detach its operands or use torch.no_grad()");
 }
 
@@ -738,7 +741,7 @@ void pagedAppend_op(const Tensor &k, const Tensor &v, const Tensor &k_cache, con
                     const OptTensor &k_scale, const OptTensor &v_scale) {
     const ba_paged_cache c = cache_of(k_cache, v_cache, k_scale, v_scale);
     check_rows(k, "k", k_cache); check_rows(v, "v", k_cache);
-    check_no_grad({&k, &v, &k_cache, &v_cache}, "pagedAppend");
+    check_no_grad({&k, &v, &k_cache, &v_cache}, k_scale, v_scale, "pagedAppend");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
     check_cache_operand(k, "k", c);
     TORCH_CHECK(k.scalar_type() == v.scalar_type(), "k and v must have the same dtype");
@@ -780,7 +783,7 @@ Tensor pagedAttention_op(const Tensor &q, const Tensor &k_cache, const Tensor &v
     const ba_paged_cache c = cache_of(k_cache, v_cache, k_scale, v_scale);
     check_rows(q, "q", k_cache);
     check_table(table, k_cache);
-    check_no_grad({&q, &k_cache, &v_cache}, "pagedAttention");
+    check_no_grad({&q, &k_cache, &v_cache}, k_scale, v_scale, "pagedAttention");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
     check_cache_operand(q, "q", c);
     TORCH_CHECK(window >= 0, "window must not be negative (0: all tokens)");

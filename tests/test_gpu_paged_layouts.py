@@ -65,3 +65,19 @@ def test_strides_of_dimensions_of_one(dev, fp8):
         for c, w in zip((k, v), want):
             last = (k.size(0) - 1, slice(None), page - 1)
             assert torch.equal(c.view(torch.uint8)[last], w[last]) and c.view(torch.uint8)[last].any()
+
+
+def test_scales_that_want_gradients_are_refused(dev):
+    """There is no backward pass: a scale that is trained would silently get no gradient."""
+    b = Batch([20], 2, 2, 64, 16, torch.float16, True)
+    q, k, v, table, lens = b.q.to(dev), b.k.to(dev), b.v.to(dev), b.table.to(dev), torch.tensor(b.lens, device=dev)
+    plain, trained = b.scales[0].to(dev), b.scales[0].to(dev).requires_grad_()
+    x, slots = q[:2], torch.zeros(1, dtype=torch.int64, device=dev)
+    for scales in ((plain, trained), (trained, plain)):
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            blockedAttention.pagedAttention(q, k, v, table, lens, 0.1, 0, *scales)
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            blockedAttention.pagedAppend(x, x, k, v, slots, *scales)
+        with torch.no_grad():
+            blockedAttention.pagedAppend(x, x, k, v, slots, *scales)
+            blockedAttention.pagedAttention(q, k, v, table, lens, 0.1, 0, *scales)
