@@ -9,7 +9,7 @@ extern template int launch_paged_dtype<0, true>(const PagedAttentionArgs &a, con
 extern template int launch_paged_dtype<1, true>(const PagedAttentionArgs &a, const PagedWork &w, hipStream_t stream);
 
 // Workgroups: as many as are resident, or fewer where the longest possible requests would not give each its least share.
-// (The window counts: three requests that look at 69 tokens 7.2 us, with workgroups for the length and thus a joining kernel 15.)
+// (The window counts: three requests that look at 69 tokens 7.4 us, with workgroups for the length and thus a joining kernel 15.)
 static PagedWork work_of(int64_t heads, int64_t group, int64_t dim, bool f8, bool any, int64_t requests, int64_t width, int64_t page, int64_t window, void *workspace, size_t *bytes) {
     PagedWork w{};
     const int sets = group > kPagedHeads ? 2 : 1;

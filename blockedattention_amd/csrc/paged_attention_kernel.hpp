@@ -28,9 +28,9 @@
 //   page numbers of the tile after that before both: loads come back in order.
 //
 // Bound and figures.  Loads that pass the caches reach 7.05 TB/s here, others 6.2.  128 requests of 1 to 16384 tokens, 32 query
-// heads on 8, 128 dimensions, bf16 (3.8 GB): 581 us, 6.6 TB/s; 64 requests of up to 4096 (500 MB): 92 us, 5.4 TB/s, of which
+// heads on 8, 128 dimensions, bf16 (3.8 GB): 582 us, 6.6 TB/s; 64 requests of up to 4096 (500 MB): 92 us, 5.4 TB/s, of which
 // about 12 us do not depend on the lengths (launch, adding up the lengths, first loads, joining).  8-bit caches are bound by
-// instructions as much as by memory: 96 requests of up to 8192 tokens (876 MB) 165 us, 5.3 TB/s, and the same time at 64 dimensions.
+// instructions as much as by memory: 96 requests of up to 8192 tokens (876 MB) 164 us, 5.3 TB/s, and about the same time at 64 dimensions.
 #pragma once
 #include <algorithm>
 #include <type_traits>

@@ -18,7 +18,8 @@ constexpr int kTableThreads = 512;
 constexpr int kTableWaves = kTableThreads / 64;
 constexpr int kTableRequests = 4096;         // with so many requests every workgroup keeps the three sums in LDS
 // Workgroups: each makes the sums again, and a token is a chain of loads.  So one token a thread up to kTableGroups workgroups,
-// beyond those four at once (40 000 tokens of 2000 requests 8.2 us, with four 11.1; 250 000 of 64 prompts 6.2, with one 9.0).
+// beyond those four at once (49 495 tokens of 2000 requests 7.4 us, with four 9.4; 300 168 of 64 prompts 7.6, with one 7.5;
+// 1.2 million of 64 17.3, with one 19.6; 1.04 million of 1000 17.3, with one 21.3).
 constexpr int kTableGroups = 128;
 constexpr int kTableEach = kTableRequests / kTableThreads;      // requests of a thread at most
 
@@ -190,7 +191,8 @@ template <int K> __global__ void __launch_bounds__(kTableThreads) paged_tables_k
     fill<K>(a, t, take, drop, grow, (int64_t)blockIdx.x * kTableThreads + threadIdx.x, (int64_t)gridDim.x * kTableThreads);
 }
 
-// More requests: one workgroup makes the sums (grow: the accum result), a second launch reads them.
+// More requests: one workgroup makes the sums (grow: the accum result), a second launch reads them (5000 requests, 124 000 tokens
+// 32 + 16 us).
 struct TableSums {
     Totals totals;
     int64_t sums[];                                  // take, drop: [requests] each
