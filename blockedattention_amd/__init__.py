@@ -3,13 +3,15 @@
 ``blockGEMM`` / ``blockSoftmax`` keep the reference package's signatures;
 ``blockGEMMSoftmax`` is the fused pair, ``blockFusedAttention`` the one-pass
 ``softmax(scale q k^T) v``.  ``pagedResize``, ``pagedAppend`` and ``pagedAttention``
-keep a paged key-value cache and attend to it with one query per request.  ``capi`` exposes the C ABI directly.
+keep a paged key-value cache and attend to it with one query per request; ``pagedTree``, ``pagedTreeAttention`` and
+``pagedKeep`` answer several drafted tokens of a request at once, ``pagedFork`` and ``pagedCopy`` let rows of the cache
+go on from other rows.  ``capi`` exposes the C ABI directly.
 Importing the operators needs the in-tree build (``python -m
 blockedattention_amd.build``); nothing falls back to PyTorch or the CPU.
 """
 
 __all__ = ["blockGEMM", "blockSoftmax", "blockGEMMSoftmax", "blockFusedAttention", "pagedResize", "pagedAppend",
-           "pagedAttention", "set_schedule_cache", "schedule_cache_stats"]
+           "pagedAttention", "pagedTree", "pagedTreeAttention", "pagedKeep", "pagedFork", "pagedCopy", "set_schedule_cache", "schedule_cache_stats"]
 
 
 def __getattr__(name):

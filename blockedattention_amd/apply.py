@@ -144,6 +144,78 @@ def pagedAttention(
     return blockAttention.pagedAttention(q, kCache, vCache, table, lens, float(scale), int(window), kScale, vScale)
 
 
+def pagedTree(parents: torch.Tensor, accum: torch.Tensor, nodes: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """What the nodes of trees of drafted tokens see, and how deep they lie.
+
+    The nodes of request ``r`` are rows ``accum[r] .. accum[r + 1] - 1`` (int64, the ``tokenAccum`` of ``pagedResize``);
+    ``parents`` (int64, one entry a row) is the number of a node's parent within its request, which comes before it, or -1 for
+    the request's last token.  ``nodes`` (up to 1024) is the most that a request has.
+
+    Returns ``(mask, depth)``: int64 ``[rows, words]`` with bit ``j % 64`` of word ``j // 64`` set where the row's node goes
+    on from node ``j`` of its request or is it, and int64 ``[rows]``, the number of nodes it goes on from (so a node's
+    position is the request's length before the draft plus its depth).  Rows of no request, nodes beyond ``nodes`` and
+    nodes whose parent, or a parent's parent, does not come before its node get no bits and depth -1.
+    """
+    return tuple(blockAttention.pagedTree(parents, accum, int(nodes)))
+
+
+def pagedTreeAttention(
+    q: torch.Tensor, kCache: torch.Tensor, vCache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, accum: torch.Tensor,
+    mask: Optional[torch.Tensor] = None, scale: float = 1.0, window: int = 0,
+    kScale: Optional[torch.Tensor] = None, vScale: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``pagedAttention`` for several queries of a request: of all nodes of a tree of drafted tokens, or of a piece of a prompt.
+
+    ``q`` is ``[heads, tokens * dim]`` or ``[heads, tokens, dim]``; request ``r`` has its rows ``accum[r] .. accum[r + 1] - 1``,
+    whose keys and values are the last of its ``lens[r]`` tokens in the cache (``tokenAccum`` and ``lens`` as ``pagedResize``
+    returns them).  A row sees all tokens before those and, of those, the ones whose bits its row of ``mask`` has (int64
+    ``[tokens, words]``, of ``pagedTree`` or any other); without a mask those before it and itself.  ``window`` > 0 looks at the
+    last ``window`` tokens that a row sees.  Rows that see nothing give zeros, and so do rows of no request; what a
+    row does not see has no influence on it.  All else is as for ``pagedAttention``.
+    """
+    return blockAttention.pagedTreeAttention(q, kCache, vCache, table, lens, accum, mask, float(scale), int(window), kScale, vScale)
+
+
+def pagedKeep(kCache: torch.Tensor, vCache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, path: torch.Tensor) -> torch.Tensor:
+    """Moves the keys and values of accepted nodes to the front of their draft, in place.
+
+    ``lens`` (int64) are the requests' lengths before the draft, ``path`` (int64 ``[requests, depth]``) the accepted nodes in
+    their order, then -1: the token at ``lens[r] + path[r, i]`` comes to ``lens[r] + i``.  A path increases; it ends at the first entry
+    that does not, is below its own index, or lies outside the row.  Returns the lengths with the accepted nodes; ``pagedResize``
+    to those gives the other pages back.  Call it for every layer's cache.  Pages that are written must not be another row's
+    too (``pagedFork`` sees to that).
+    """
+    return blockAttention.pagedKeep(kCache, vCache, table, lens, path)
+
+
+def pagedFork(
+    table: torch.Tensor, free: torch.Tensor, state: torch.Tensor, shares: torch.Tensor, lens: torch.Tensor, origin: torch.Tensor, pageSize: int,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Row ``r`` of the table goes on from row ``origin[r]``: itself, another one whose tokens it has from then on, or -1 if it ends.
+
+    ``table``, ``free``, ``state`` and ``lens`` are those of ``pagedResize``; ``shares`` (int32, an entry for each page of the cache, zeros at
+    first) counts the rows that hold a page beyond the first.  Full pages are shared.  A last page that is not full stays
+    with the row itself if it goes on, else with the first row that goes on from it; the others get a fresh page each.  Pages that no row
+    holds any more go on the stack in ascending order, before fresh ones are taken from its end.  ``free`` is updated in
+    place.
+
+    Returns ``(table, lens, state, shares, source, target)``: the new table, lengths, state and counts, and for every row the page to be
+    copied and the fresh one it is copied to, or -1 (int32, for ``pagedCopy`` in every layer's cache).  A refused step changes
+    nothing and returns what came in; its verdict adds 32 (an origin that is no row) and 64 (pages and ``shares`` that do
+    not fit) to those of ``pagedResize``.  A row that shares pages may grow by ``pagedResize`` and shrink by it as far as
+    pages that it holds alone; it ends here, with origin -1.  Up to 8192 rows.
+    """
+    return tuple(blockAttention.pagedFork(table, free, state, shares, lens, origin, int(pageSize)))
+
+
+def pagedCopy(kCache: torch.Tensor, vCache: torch.Tensor, source: torch.Tensor, target: torch.Tensor) -> None:
+    """Pages ``source[i]`` of both caches into pages ``target[i]`` (int32), in place; entries below 0 are skipped.
+
+    No page may be a target twice, or a target and a source.
+    """
+    blockAttention.pagedCopy(kCache, vCache, source, target)
+
+
 def set_schedule_cache(capacity: int) -> None:
     """How many schedules the operators keep for metadata tensors they have seen (default 8; 0 = off).
 

@@ -22,6 +22,8 @@ SYMBOLS = (
     "ba_varlen_attention", "ba_attention_rows", "ba_varlen_attention_train", "ba_varlen_attention_backward",
     "ba_gemm_softmax_static", "ba_static_read", "ba_varlen_gemm_two",
     "ba_paged_resize_workspace", "ba_paged_resize", "ba_paged_append", "ba_paged_attention_workspace", "ba_paged_attention",
+    "ba_paged_tree", "ba_paged_tree_attention_workspace", "ba_paged_tree_attention", "ba_paged_keep", "ba_paged_fork_workspace", "ba_paged_fork",
+    "ba_paged_copy",
 )
 MAILBOX_BYTES = 320
 STATIC_MAX_SEGMENTS = 4096   # BA_STATIC_MAX_SEGMENTS
@@ -133,6 +135,21 @@ def load():
     lib.ba_paged_attention.restype = i32
     lib.ba_paged_attention.argtypes = [cache, i32, vp, i64, i64, i64, i64, vp, i64, i64, vp, i64, f32, vp, i64, i64, vp, vp,
                                        ctypes.c_size_t, vp]
+    lib.ba_paged_tree.restype = i32
+    lib.ba_paged_tree.argtypes = [vp, vp, i64, i64, i64, vp, vp, vp]
+    lib.ba_paged_tree_attention_workspace.restype = ctypes.c_size_t
+    lib.ba_paged_tree_attention_workspace.argtypes = [cache, i64, i64, i64, i64]
+    lib.ba_paged_tree_attention.restype = i32
+    lib.ba_paged_tree_attention.argtypes = [cache, i32, vp, i64, i64, i64, i64, vp, i64, i64, vp, vp, i64, vp, i64, i64, i64, f32, vp, i64, i64,
+                                            vp, vp, ctypes.c_size_t, vp]
+    lib.ba_paged_keep.restype = i32
+    lib.ba_paged_keep.argtypes = [cache, vp, i64, i64, vp, vp, i64, i64, i64, vp, vp]
+    lib.ba_paged_fork_workspace.restype = ctypes.c_size_t
+    lib.ba_paged_fork_workspace.argtypes = [i64, i64]
+    lib.ba_paged_fork.restype = i32
+    lib.ba_paged_fork.argtypes = [vp, i64, i64, vp, i64, vp, vp, i64, vp, vp, i64, i64, vp, i64, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp]
+    lib.ba_paged_copy.restype = i32
+    lib.ba_paged_copy.argtypes = [cache, vp, vp, i64, vp]
     _lib = lib
     return lib
 
@@ -387,3 +404,48 @@ def paged_attention(cache, q, table, lens, out, scale=1.0, window=0, counters=No
                                    out.stride(0), out.stride(1), _ptr(counters), _ptr(work), need, _stream())
     check(st, "ba_paged_attention")
     return out
+
+
+def paged_tree(parents, accum, nodes, mask, depth):
+    """What the nodes of trees of drafted tokens see, and how deep they lie (see ba_paged_tree)."""
+    st = load().ba_paged_tree(_ptr(parents), _ptr(accum), accum.numel() - 1, parents.numel(), nodes, _ptr(mask), _ptr(depth), _stream())
+    check(st, "ba_paged_tree")
+    return mask
+
+
+def paged_tree_attention(cache, q, table, lens, accum, out, mask=None, scale=1.0, window=0, counters=None):
+    """out [heads, tokens, dim] <- attention of all requests' rows of q over their pages (see ba_paged_tree_attention)."""
+    counters = paged_counters(q.device) if counters is None else counters
+    need = load().ba_paged_tree_attention_workspace(ctypes.byref(cache), q.size(0), q.size(1), lens.numel(), table.size(1))
+    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    st = load().ba_paged_tree_attention(ctypes.byref(cache), dtype_code(q.dtype), _ptr(q), q.stride(0), q.stride(1), q.size(0), q.size(1),
+                                        _ptr(table), table.stride(0), table.size(1), _ptr(lens), _ptr(accum), lens.numel(), _ptr(mask),
+                                        0 if mask is None else mask.stride(0), 0 if mask is None else mask.size(1), window, float(scale),
+                                        _ptr(out), out.stride(0), out.stride(1), _ptr(counters), _ptr(work), need, _stream())
+    check(st, "ba_paged_tree_attention")
+    return out
+
+
+def paged_keep(cache, table, lens, path, lens_out):
+    """Accepted paths to the front of their drafts (see ba_paged_keep)."""
+    st = load().ba_paged_keep(ctypes.byref(cache), _ptr(table), table.stride(0), table.size(1), _ptr(lens), _ptr(path), path.stride(0),
+                              lens.numel(), path.size(1), _ptr(lens_out), _stream())
+    check(st, "ba_paged_keep")
+    return lens_out
+
+
+def paged_fork(table, free, state, shares, lens, origin, page, table_out, lens_out, state_out, shares_out, source, target):
+    """Rows of a table that go on from other rows (see ba_paged_fork)."""
+    need = load().ba_paged_fork_workspace(lens.numel(), shares.numel())
+    work = torch.empty(need, dtype=torch.uint8, device=table.device)
+    st = load().ba_paged_fork(_ptr(table), table.stride(0), table.size(1), _ptr(free), free.numel(), _ptr(state), _ptr(shares), shares.numel(),
+                              _ptr(lens), _ptr(origin), lens.numel(), page, _ptr(table_out), table_out.stride(0), _ptr(lens_out), _ptr(state_out),
+                              _ptr(shares_out), _ptr(source), _ptr(target), _ptr(work), need, _stream())
+    check(st, "ba_paged_fork")
+    return table_out
+
+
+def paged_copy(cache, source, target):
+    """Pages of both arrays to other pages (see ba_paged_copy)."""
+    st = load().ba_paged_copy(ctypes.byref(cache), _ptr(source), _ptr(target), source.numel(), _stream())
+    check(st, "ba_paged_copy")

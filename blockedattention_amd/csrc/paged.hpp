@@ -62,6 +62,64 @@ struct PagedAttentionArgs {
     PageDiv page;
 };
 
+constexpr int kTreePadGroups = 8;            // workgroups for the rows that belong to no request
+
+struct PagedTreeArgs {
+    const int64_t *parents, *accum;
+    int64_t *mask, *depth;
+    int64_t tokens;
+    int32_t requests, nodes, words;
+};
+
+struct PagedTreeAttentionArgs {
+    PagedArray k, v;
+    const char *q;
+    char *out;
+    const int32_t *table;
+    const int64_t *lens, *accum, *mask;      // mask NULL: a node sees those before it and itself
+    int64_t q_head_bytes, q_row_bytes, out_head_bytes, out_row_bytes, table_stride, mask_stride, tokens;
+    int32_t requests, heads, group, dim, pages, width, words;
+    int32_t window;                          // tokens; 0: all
+    float scale;
+    PageDiv page;
+};
+
+struct PagedKeepArgs {
+    PagedArray arrays[2];
+    const int32_t *table;
+    const int64_t *lens, *path;
+    int64_t *lens_out;
+    int64_t table_stride, path_stride;
+    int32_t requests, heads, pages, width, depth, row_bytes;
+    int32_t group_heads, splits;             // heads of a workgroup, workgroups of a request
+    PageDiv page, per_row, per_entry, per_rest;              // pieces of a row, of an entry, of one in the last workgroup
+};
+
+// A page of one array as runs of bytes.
+struct PagedRuns {
+    char *base;
+    int64_t page_bytes, outer_bytes, inner_bytes, run_bytes;
+    PageDiv per_run, per_outer;              // pieces of a run, inner runs of an outer one
+    uint32_t pieces;                         // of a page
+};
+
+struct PagedCopyArgs {
+    PagedRuns runs[2];
+    const int32_t *source, *target;
+    int64_t copies;
+    int32_t pages, parts, part_pieces;       // workgroups of a page and their pieces
+};
+
+struct PagedForkArgs {
+    const int32_t *table, *shares;
+    int32_t *free_pages, *table_out, *shares_out, *source, *target;
+    const int64_t *state_in, *lens, *origin;
+    int64_t *lens_out, *state_out;
+    int64_t table_stride, table_out_stride, pool;
+    int32_t requests, width, pages;
+    PageDiv page;
+};
+
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
 typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint32_t u32_any __attribute__((aligned(1)));
@@ -105,5 +163,13 @@ int launch_paged_tables(const PagedTablesArgs &args, void *workspace, hipStream_
 int launch_paged_append(const PagedAppendArgs &args, int dtype, int cache_dtype, hipStream_t stream);
 size_t paged_attention_workspace(int64_t cache_heads, int64_t group, int64_t dim, int cache_dtype, int64_t requests, int64_t width, int64_t page);
 int launch_paged_attention(const PagedAttentionArgs &args, int dtype, int cache_dtype, int32_t *counters, void *workspace, hipStream_t stream);
+int launch_paged_tree(const PagedTreeArgs &args, hipStream_t stream);
+size_t paged_tree_attention_workspace(int64_t cache_heads, int64_t group, int64_t dim, int cache_dtype, int64_t tokens, int64_t requests,
+                                      int64_t width, int64_t page);
+int launch_paged_tree_attention(const PagedTreeAttentionArgs &args, int dtype, int cache_dtype, int32_t *counters, void *workspace, hipStream_t stream);
+int launch_paged_keep(PagedKeepArgs args, hipStream_t stream);
+int launch_paged_copy(PagedCopyArgs args, const PagedArray (&arrays)[2], int64_t heads, int64_t page, int64_t row_bytes, hipStream_t stream);
+size_t paged_fork_workspace(int64_t requests, int64_t pages);
+int launch_paged_fork(const PagedForkArgs &args, void *workspace, hipStream_t stream);
 
 }  // namespace ba

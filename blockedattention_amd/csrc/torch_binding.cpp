@@ -9,7 +9,8 @@
 // Additions that keep the reference behaviour when left at their defaults:
 //   sparseBlockedSoftmaxScaled(src, rowList, colList, srcAccum?, scale)
 //   sparseBlockedGEMMSoftmax(mat1, mat2, ..., scale, out_fp32)   fused pair, forward only
-//   pagedResize, pagedAppend, pagedAttention                     paged key-value cache, forward only; no schedule, no
+//   pagedResize, pagedAppend, pagedAttention, pagedTree, pagedTreeAttention, pagedKeep, pagedFork, pagedCopy
+//                                                                paged key-value cache, forward only; no schedule, no
 //                                                                host synchronisation
 //
 // Every precondition the reference leaves to assert() is a TORCH_CHECK here.
@@ -675,7 +676,8 @@ void written(const Tensor &t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
-ba_paged_cache cache_of(const Tensor &k, const Tensor &v, const OptTensor &k_scale, const OptTensor &v_scale) {
+// moved: what the cache holds is only moved, so nobody needs its scales.
+ba_paged_cache cache_of(const Tensor &k, const Tensor &v, const OptTensor &k_scale, const OptTensor &v_scale, bool moved = false) {
     check_rows(k, "kCache", k); check_rows(v, "vCache", k);
     TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes(), "kCache and vCache must both be [pages, heads, page, dim], got ", k.sizes(), " and ", v.sizes());
     TORCH_CHECK(k.scalar_type() == v.scalar_type(), "kCache and vCache must have the same dtype");
@@ -683,18 +685,18 @@ ba_paged_cache cache_of(const Tensor &k, const Tensor &v, const OptTensor &k_sca
     const bool f8 = k.scalar_type() == at::kFloat8_e4m3fn;
     TORCH_CHECK(f8 || k.scalar_type() == at::kHalf || k.scalar_type() == at::kBFloat16,
                 "a paged cache holds fp16, bf16 or float8_e4m3fn, got ", k.scalar_type());
-    TORCH_CHECK(k_scale.has_value() == f8 && v_scale.has_value() == f8,
+    TORCH_CHECK(moved || (k_scale.has_value() == f8 && v_scale.has_value() == f8),
                 f8 ? "a float8_e4m3fn cache needs kScale and vScale" : "kScale and vScale belong to a float8_e4m3fn cache");
     TORCH_CHECK(k.size(1) >= 1 && k.size(2) >= 1 && k.size(3) >= 1 && k.size(3) <= 256,
                 "a paged cache has at least one head, one token a page and 1 to 256 dimensions, got ", k.sizes());
-    if (f8)
+    if (f8 && !moved)
         for (const OptTensor *s : {&k_scale, &v_scale}) {
             check_data(**s, "kScale and vScale");
             TORCH_CHECK((*s)->scalar_type() == at::kFloat && (*s)->dim() == 1 && (*s)->numel() == k.size(1) && (*s)->device() == k.device(),
                         "kScale and vScale are fp32, one entry per head of the cache (", k.size(1), "), on its device");
         }
     c.k = k.data_ptr(); c.v = v.data_ptr();
-    c.k_scale = f8 ? k_scale->data_ptr<float>() : nullptr; c.v_scale = f8 ? v_scale->data_ptr<float>() : nullptr;
+    c.k_scale = f8 && !moved ? k_scale->data_ptr<float>() : nullptr; c.v_scale = f8 && !moved ? v_scale->data_ptr<float>() : nullptr;
     c.pages = k.size(0); c.heads = k.size(1); c.page = k.size(2); c.dim = k.size(3);
     c.k_page_stride = k.stride(0); c.k_head_stride = k.stride(1); c.k_token_stride = k.stride(2);
     c.v_page_stride = v.stride(0); c.v_head_stride = v.stride(1); c.v_token_stride = v.stride(2);
@@ -808,6 +810,112 @@ Tensor pagedAttention_op(const Tensor &q, const Tensor &k_cache, const Tensor &v
     return out;
 }
 
+std::vector<Tensor> pagedTree_op(const Tensor &parents, const Tensor &accum, int64_t nodes) {
+    check_data(accum, "accum");
+    TORCH_CHECK(accum.dim() == 1 && accum.numel() >= 1, "accum has one entry more than requests");
+    check_meta(accum, "accum", accum, accum.numel());
+    TORCH_CHECK(parents.dim() == 1, "parents must be 1-D");
+    check_meta(parents, "parents", accum, parents.numel());
+    TORCH_CHECK(nodes >= 1 && nodes <= BA_PAGED_TREE_NODES, "nodes must be 1 to ", BA_PAGED_TREE_NODES, ", got ", nodes);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(accum.device());
+    const int64_t T = parents.numel();
+    Tensor mask = at::empty({T, (nodes + 63) / 64}, accum.options()), depth = at::empty({T}, accum.options());
+    check_status(ba_paged_tree(parents.data_ptr<int64_t>(), accum.data_ptr<int64_t>(), accum.numel() - 1, T, nodes, mask.data_ptr<int64_t>(),
+                               depth.data_ptr<int64_t>(), current_stream(accum)),
+                 "ba_paged_tree");
+    return {mask, depth};
+}
+
+Tensor pagedTreeAttention_op(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache, const Tensor &table, const Tensor &lens,
+                             const Tensor &accum, const OptTensor &mask, double scale, int64_t window, const OptTensor &k_scale,
+                             const OptTensor &v_scale) {
+    const ba_paged_cache c = cache_of(k_cache, v_cache, k_scale, v_scale);
+    check_rows(q, "q", k_cache);
+    check_table(table, k_cache);
+    check_no_grad({&q, &k_cache, &v_cache}, k_scale, v_scale, "pagedTreeAttention");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
+    check_cache_operand(q, "q", c);
+    TORCH_CHECK(window >= 0, "window must not be negative (0: all tokens)");
+    const Rows qr = rows_of(q, "q", c.dim);
+    TORCH_CHECK(qr.heads >= 1 && qr.heads % c.heads == 0, "q must have a multiple of the cache's ", c.heads, " heads, got ", qr.heads);
+    const int64_t R = table.size(0);
+    check_meta(lens, "lens", k_cache, R); check_meta(accum, "accum", k_cache, R + 1);
+    if (mask.has_value()) {
+        check_rows(*mask, "mask", k_cache);
+        TORCH_CHECK(mask->scalar_type() == at::kLong && mask->dim() == 2 && mask->size(0) == qr.rows && mask->size(1) >= 1,
+                    "mask must be int64 [", qr.rows, ", words], a row for each of q, got ", mask->sizes());
+    }
+    Tensor out = at::empty_like(q);
+    if (out.size(-1) > 1 && out.stride(-1) != 1) out = at::empty(q.sizes(), q.options());        // (as in pagedAttention)
+    const Rows outr = rows_of(out, "out", c.dim);
+    const size_t bytes = ba_paged_tree_attention_workspace(&c, qr.heads, qr.rows, R, table.size(1));
+    Tensor work;
+    if (bytes) work = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+    const Tensor counters = paged_counters(q);
+    check_status(ba_paged_tree_attention(&c, dtype_code(q, "pagedTreeAttention"), q.data_ptr(), qr.head_stride, qr.row_stride, qr.heads, qr.rows,
+                                         table.data_ptr<int32_t>(), table.stride(0), table.size(1), lens.data_ptr<int64_t>(),
+                                         accum.data_ptr<int64_t>(), R, mask.has_value() ? mask->data_ptr<int64_t>() : nullptr,
+                                         mask.has_value() ? mask->stride(0) : 0, mask.has_value() ? mask->size(1) : 0, window, (float)scale,
+                                         out.data_ptr(), outr.head_stride, outr.row_stride, counters.data_ptr<int32_t>(),
+                                         bytes ? work.data_ptr() : nullptr, bytes, current_stream(q)),
+                 "ba_paged_tree_attention");
+    return out;
+}
+
+Tensor pagedKeep_op(const Tensor &k_cache, const Tensor &v_cache, const Tensor &table, const Tensor &lens, const Tensor &path) {
+    const ba_paged_cache c = cache_of(k_cache, v_cache, {}, {}, true);
+    check_table(table, k_cache);
+    check_no_grad({&k_cache, &v_cache}, {}, {}, "pagedKeep");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
+    const int64_t R = table.size(0);
+    check_meta(lens, "lens", k_cache, R);
+    check_rows(path, "path", k_cache);
+    TORCH_CHECK(path.scalar_type() == at::kLong && path.dim() == 2 && path.size(0) == R, "path must be int64 [", R, ", nodes], got ", path.sizes());
+    Tensor out = at::empty({R}, lens.options());
+    check_status(ba_paged_keep(&c, table.data_ptr<int32_t>(), table.stride(0), table.size(1), lens.data_ptr<int64_t>(), path.data_ptr<int64_t>(),
+                               path.stride(0), R, path.size(1), out.data_ptr<int64_t>(), current_stream(k_cache)),
+                 "ba_paged_keep");
+    written(k_cache); written(v_cache);
+    return out;
+}
+
+std::vector<Tensor> pagedFork_op(const Tensor &table, const Tensor &free_pages, const Tensor &state, const Tensor &shares, const Tensor &lens,
+                                 const Tensor &origin, int64_t page) {
+    check_table(table, table);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(table.device());
+    const int64_t R = table.size(0);
+    TORCH_CHECK(page >= 1, "a page holds at least one token");
+    TORCH_CHECK(R <= BA_PAGED_FORK_ROWS, "pagedFork takes up to ", BA_PAGED_FORK_ROWS, " rows, got ", R);
+    check_data(free_pages, "free"); check_data(shares, "shares");
+    for (const Tensor *t : {&free_pages, &shares})
+        TORCH_CHECK(t->scalar_type() == at::kInt && t->dim() == 1 && t->device() == table.device(), "free and shares must be 1-D int32 on the table's device");
+    check_meta(state, "state", table, 2); check_meta(lens, "lens", table, R); check_meta(origin, "origin", table, R);
+    Tensor table_out = at::empty({R, table.size(1)}, table.options()), lens_out = at::empty({R}, lens.options()), state_out = at::empty({2}, lens.options());
+    Tensor shares_out = at::empty({shares.numel()}, shares.options()), source = at::empty({R}, table.options()), target = at::empty({R}, table.options());
+    const size_t bytes = ba_paged_fork_workspace(R, shares.numel());
+    Tensor work = at::empty({(int64_t)bytes}, table.options().dtype(at::kByte));
+    check_status(ba_paged_fork(table.data_ptr<int32_t>(), table.stride(0), table.size(1), free_pages.data_ptr<int32_t>(), free_pages.numel(),
+                               state.data_ptr<int64_t>(), shares.data_ptr<int32_t>(), shares.numel(), lens.data_ptr<int64_t>(),
+                               origin.data_ptr<int64_t>(), R, page, table_out.data_ptr<int32_t>(), table_out.stride(0), lens_out.data_ptr<int64_t>(),
+                               state_out.data_ptr<int64_t>(), shares_out.data_ptr<int32_t>(), source.data_ptr<int32_t>(), target.data_ptr<int32_t>(),
+                               work.data_ptr(), bytes, current_stream(table)),
+                 "ba_paged_fork");
+    written(free_pages);
+    return {table_out, lens_out, state_out, shares_out, source, target};
+}
+
+void pagedCopy_op(const Tensor &k_cache, const Tensor &v_cache, const Tensor &source, const Tensor &target) {
+    const ba_paged_cache c = cache_of(k_cache, v_cache, {}, {}, true);
+    check_no_grad({&k_cache, &v_cache}, {}, {}, "pagedCopy");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
+    check_data(source, "source"); check_data(target, "target");
+    for (const Tensor *t : {&source, &target})
+        TORCH_CHECK(t->scalar_type() == at::kInt && t->dim() == 1 && t->numel() == source.numel() && t->device() == k_cache.device(),
+                    "source and target must be 1-D int32 of one length on the cache's device");
+    check_status(ba_paged_copy(&c, source.data_ptr<int32_t>(), target.data_ptr<int32_t>(), source.numel(), current_stream(k_cache)), "ba_paged_copy");
+    written(k_cache); written(v_cache);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -819,6 +927,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("pagedResize", &pagedResize_op, "page tables and slots from the requests' lengths before and after");
     m.def("pagedAppend", &pagedAppend_op, "keys and values of new tokens into a paged cache, in place");
     m.def("pagedAttention", &pagedAttention_op, "one query per request over a paged cache");
+    m.def("pagedTree", &pagedTree_op, "what the nodes of trees of drafted tokens see, and how deep they lie");
+    m.def("pagedTreeAttention", &pagedTreeAttention_op, "several queries per request over a paged cache, of a tree of drafted tokens");
+    m.def("pagedKeep", &pagedKeep_op, "an accepted path's keys and values to consecutive places, in place");
+    m.def("pagedFork", &pagedFork_op, "rows of a page table that go on from other rows");
+    m.def("pagedCopy", &pagedCopy_op, "pages of a cache to other pages, in place");
     m.def("set_schedule_cache", &set_schedule_cache, "number of schedules kept for repeated metadata (0 = off)");
     m.def("schedule_cache_stats", &schedule_cache_stats, "[hits, misses, entries, capacity]");
 }

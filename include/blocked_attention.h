@@ -334,8 +334,8 @@ int ba_static_read(ba_plan_info *host_info, ba_stream_t stream);
  * the order of its tokens.  Token t of request r and key head h is the `dim` elements at
  *     base + page_number * page_stride + h * head_stride + (t % page) * token_stride
  * (strides in elements, any order of heads and tokens, the last dimension contiguous), page_number = table[r][t / page].
- * dtype: BA_F16, BA_BF16, or BA_F8_E4M3 with `k_scale` and `v_scale` (fp32, one per head): what is stored times the
- * head's scale is the value.  dim <= 256; the tokens of a page and head span less than 2^31 bytes.
+ * dtype: BA_F16, BA_BF16, or BA_F8_E4M3 with `k_scale` and `v_scale` (fp32, one per head; ba_paged_keep and ba_paged_copy need
+ * none): what is stored times the head's scale is the value.  dim <= 256; the tokens of a page and head span less than 2^31 bytes.
  * The stride of a dimension of one entry is not used.
  * The structure itself is host memory, the pointers in it are device pointers.
  */
@@ -405,6 +405,84 @@ int ba_paged_attention(const ba_paged_cache *cache, int dtype, const void *q, in
                        const int64_t *lens, int64_t window, float scale, void *out, int64_t out_head_stride,
                        int64_t out_row_stride, int32_t *counters, void *workspace, size_t workspace_bytes,
                        ba_stream_t stream);
+
+/*
+ * Drafted tokens.  A request may have several new tokens at once, the nodes of a tree: every node goes on from another node of
+ * its request that comes before it, or from the request's last token.  The nodes of request r are rows accum[r] .. accum[r + 1] - 1
+ * (int64 [requests + 1], the sums that ba_paged_resize gives) of the arrays below, in the order in which their keys and values lie
+ * behind the request's other tokens.
+ *
+ * ba_paged_tree: parents[i] is the number of a node's parent within its request, -1 for the request's last token.
+ * mask (int64 [tokens][words], words = nodes / 64 rounded up) gets a bit for every node that the row's node goes on from, and for itself: node
+ * j of the request is bit j % 64 of word j / 64.  depth (int64 [tokens]) gets the number of nodes it goes on from: its place among the
+ * request's tokens is the number of tokens before the draft plus that.  `nodes`, 1 to BA_PAGED_TREE_NODES, is the most that a
+ * request has.  Rows of no request, nodes beyond `nodes`, nodes whose parent does not come before them and those that go on
+ * from such: mask 0, depth -1.  The sums do not decrease; rows beyond `tokens` do not exist.
+ */
+#define BA_PAGED_TREE_NODES 1024
+int ba_paged_tree(const int64_t *parents, const int64_t *accum, int64_t requests, int64_t tokens, int64_t nodes, int64_t *mask,
+                  int64_t *depth, ba_stream_t stream);
+
+/*
+ * ba_paged_attention for several queries of a request: out[h][i] = sum over the tokens t that row i sees of softmax_t(scale *
+ * q[h][i] . K[r][h / group][t]) V[r][h / group][t].  lens[r] counts the nodes too, which are the last n = accum[r + 1] -
+ * accum[r] of the request's tokens.  A row sees all tokens before the draft and, of the draft, the nodes whose bits are set in
+ * its row of `mask` (int64, rows of mask_stride words, of which the first `words` count: nodes beyond are not seen); without a mask those
+ * before it and itself, so that a draft without branches, or a piece of a prompt, needs none.  With window > 0 it sees of these
+ * the last `window`.  Rows that see nothing, and rows of no request, give zeros; what a row does not see has no influence on it, whatever is there.
+ * q and out are [heads][tokens][dim] by the strides given (in elements).  The sums do not decrease; rows beyond `tokens` do not
+ * exist, and neither do tokens beyond the table's row.  A page number outside the cache makes the rows of its request NaN
+ * that look at it.  Types, table, counters and workspace (ba_paged_tree_attention_workspace bytes) are those of ba_paged_attention.
+ */
+size_t ba_paged_tree_attention_workspace(const ba_paged_cache *cache, int64_t heads, int64_t tokens, int64_t requests, int64_t width);
+int ba_paged_tree_attention(const ba_paged_cache *cache, int dtype, const void *q, int64_t q_head_stride, int64_t q_row_stride,
+                            int64_t heads, int64_t tokens, const int32_t *table, int64_t table_stride, int64_t width,
+                            const int64_t *lens, const int64_t *accum, int64_t requests, const int64_t *mask, int64_t mask_stride,
+                            int64_t words, int64_t window, float scale, void *out, int64_t out_head_stride,
+                            int64_t out_row_stride, int32_t *counters, void *workspace, size_t workspace_bytes,
+                            ba_stream_t stream);
+
+/*
+ * Keeps the accepted path of a draft: lens[r] is the number of tokens before it, path (int64, rows of path_stride entries, `depth` of them)
+ * the accepted nodes in their order.  Keys and values at place lens[r] + i become those at place lens[r] + path[r][i], as if
+ * all were read before any is written; lens_out[r] becomes lens[r] plus the number of accepted nodes (ba_paged_resize to that gives the
+ * rest of the pages back).  A path increases, so path[r][i] >= i; it ends at the first entry that is not above the
+ * one before it or is below i (as -1 is), or whose place is not in the row.  Tokens on page numbers outside the cache are not
+ * moved.  lens_out must not overlap lens.  No page of a place that is written may be another row's too.
+ */
+int ba_paged_keep(const ba_paged_cache *cache, const int32_t *table, int64_t table_stride, int64_t width, const int64_t *lens,
+                  const int64_t *path, int64_t path_stride, int64_t requests, int64_t depth, int64_t *lens_out, ba_stream_t stream);
+
+/* More verdicts, of ba_paged_fork. */
+#define BA_PAGED_BAD_ORIGIN 32 /* an origin is below -1 or no row */
+#define BA_PAGED_BAD_SHARES 64 /* a page number is outside the cache, or more rows hold a page than `shares` says */
+
+/*
+ * Row r of the table goes on from row origin[r] (int64; r itself: it stays; -1: it ends): table_out, lens_out (int64) get its
+ * pages and length.  Rows share pages from then on: shares (int32, one of each of the cache's `pages`) is the number of rows that hold a page
+ * beyond the first, 0 for pages that one row holds or none.  A last page that is not full stays with the row itself if it goes on, else with the
+ * first that goes on from it; the others get a fresh page each, numbered by row, and source[r], target[r] (int32) are that page's
+ * and the fresh one's numbers, for ba_paged_copy in every layer's cache (-1 where there is nothing to copy).  Pages that no row
+ * holds any more go on the stack, in ascending order, before the fresh ones are taken from its end.  So a row that shares
+ * its pages may always grow by ba_paged_resize, and shrink by it as far as pages that it holds alone; it ends with origin -1.
+ * Entries of table_out behind a row's pages are -1.  Stack, state and verdict as for ba_paged_resize: where the verdict is not 0 the
+ * stack is untouched, table_out, lens_out and shares_out are what came in, source and target -1.  BA_PAGED_NO_PAGES only where all
+ * else is valid.  Outputs must not overlap inputs; inputs are not changed (the stack beyond state_in[0] is), so the same call
+ * again writes the same.  At most BA_PAGED_FORK_ROWS rows.  `workspace`: ba_paged_fork_workspace bytes, 256-byte aligned.
+ */
+#define BA_PAGED_FORK_ROWS 8192
+size_t ba_paged_fork_workspace(int64_t requests, int64_t pages);
+int ba_paged_fork(const int32_t *table, int64_t table_stride, int64_t width, int32_t *free_pages, int64_t pool, const int64_t *state_in,
+                  const int32_t *shares, int64_t pages, const int64_t *lens, const int64_t *origin, int64_t requests, int64_t page,
+                  int32_t *table_out, int64_t table_out_stride, int64_t *lens_out, int64_t *state_out, int32_t *shares_out, int32_t *source,
+                  int32_t *target, void *workspace, size_t workspace_bytes, ba_stream_t stream);
+
+/*
+ * Page target[i] of both arrays becomes page source[i], all heads and tokens of it (int32, `copies` each).  Entries with a
+ * number outside the cache are skipped.  No page may be a target twice, or a target and a source.
+ * heads * page * (dim in 16-byte pieces, rounded up) is below 2^31.
+ */
+int ba_paged_copy(const ba_paged_cache *cache, const int32_t *source, const int32_t *target, int64_t copies, ba_stream_t stream);
 
 #ifdef __cplusplus
 }
