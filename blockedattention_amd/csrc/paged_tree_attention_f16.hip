@@ -1,0 +1,6 @@
+// Attention of drafted tokens: fp16 queries and cache.
+#include "paged_tree_attention_kernel.hpp"
+
+namespace ba {
+template int launch_tree_types<0, false>(const PagedTreeAttentionArgs &a, const TreeWork &w, bool any, int waves, hipStream_t stream);
+}  // namespace ba

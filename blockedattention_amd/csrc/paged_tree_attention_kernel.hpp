@@ -1,0 +1,782 @@
+// Attention of the drafted tokens of each request over a paged key-value cache.
+//
+// out[h][i] = sum_t softmax_t(scale q[h][i] . K[t]) V[t] over the tokens t that row i sees: those before the draft, of the draft
+// those with a bit in the row's mask, of these the last `window`.  A key takes part in one product for every row and query head that
+// shares it, n x group of them: up to about a hundred rows the cache's bytes are the floor, beyond that the products.
+#pragma once
+#include <algorithm>
+#include <type_traits>
+
+#include "ba_device.hpp"
+#include "ba_gemm_common.hpp"
+#include "ba_host.hpp"
+#include "paged.hpp"
+
+namespace ba {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char *LdsPtr;
+typedef __attribute__((address_space(3))) s16x4 *LdsPiece;
+
+constexpr int kTreeWaves = 4;
+constexpr int kTreeThreads = 64 * kTreeWaves;
+constexpr int kTreeShare = 2;                // tiles of a workgroup at least, unless units are shorter
+constexpr int kTreeWhole = 4;                // units of up to so many tiles are not split between workgroups
+constexpr int kTreeFewParts = 8;             // parts of a unit, on the average, up to which the kernel itself joins them
+
+// What is known when it is launched: what a workgroup's four wavefronts share out, and how much is in flight.
+//   rows   wavefronts side by side over 32 rows each; the others take other tokens of the same tile
+template <int DC, int WR> struct TreeTile {
+    static constexpr int kRows = 32 * WR, kGroups = kTreeWaves / WR;     // rows of a unit, groups of wavefronts with the same tokens
+    static constexpr int kMine = WR == 4 ? 64 : 32;                       // tokens of a wavefront in a tile
+    static constexpr int kTokens = kMine * kGroups;
+    static constexpr bool kAlone = WR == 1;                               // every wavefront loads its own tokens
+    static constexpr int kBuffers = kAlone ? 1 : 2;
+    // Bytes between rows in LDS: keys 16 more than whole lines of banks, so that sixteen rows' pieces lie side by side; values 64 more, so
+    // that four rows' 64 bytes do.
+    static constexpr int kPitchK = 2 * DC + 16, kPitchV = 2 * DC + 64;
+    static constexpr int kStaged = kAlone ? kMine : kTokens;              // tokens that are loaded together
+    static constexpr int kBuffer = kStaged * (kPitchK + kPitchV);
+    static constexpr int kLds = (kAlone ? kTreeWaves : kBuffers) * kBuffer;
+    static constexpr int kPitchO = DC + 4;                                // floats between rows where wavefronts are joined
+    static constexpr int kResident = DC == 64 ? 3 : DC == 128 ? 2 : 1;    // workgroups of a compute unit, by LDS and registers
+};
+
+struct alignas(8) TreePart {                 // what a workgroup leaves for a unit that others work on too
+    float m, l;
+};
+// A unit of which several workgroups did a part each: the one that has its first tile, how many they are (0: not split).
+struct TreeLeft {
+    int32_t begins, parts, request, h, block;
+};
+struct TreeWork {
+    int32_t *counters;                       // [groups]: how many have left their part of the unit begun by a workgroup; 0 between calls
+    TreeLeft *left;                          // not NULL: instead of counting, an entry a workgroup for the joining kernel
+    TreePart *parts;                         // [2 * groups][kRows]
+    float *sums;                             // [2 * groups][kRows][pitch]
+    PageDiv group;                           // query heads of a key head
+    int32_t groups, pitch;
+};
+
+// A request's draft.
+struct Draft {
+    int64_t node0;                           // number of the node of its first row
+    int32_t row0, rows;                      // rows of q and out
+    int32_t before, end;                     // tokens before the draft, tokens; as far as the table's row holds them
+    int32_t blocks, start, tiles;            // of kRows rows; first token of the first tile that may be seen, tiles
+};
+template <int DC, int WR> __device__ __forceinline__ Draft draft_of(const PagedTreeAttentionArgs &a, const PageDiv &, int r) {
+    typedef TreeTile<DC, WR> T;
+    constexpr int64_t kFar = int64_t(1) << 40;               // sums and lengths beyond any array
+    const int64_t a0 = min(max(a.accum[r], -kFar), kFar), a1 = min(max(a.accum[r + 1], -kFar), kFar), length = min(max(a.lens[r], (int64_t)0), kFar);
+    const int64_t n = max(a1 - a0, (int64_t)0), room = (int64_t)a.width * a.page.d;
+    const int64_t first = min(max(a0, (int64_t)0), a.tokens), last = min(max(a1, first), a.tokens);
+    Draft d;
+    d.row0 = (int)first;
+    d.rows = (int)(last - first);
+    d.node0 = first - a0;
+    d.end = (int)min(length, room);
+    d.before = (int)min(max(length - n, (int64_t)0), (int64_t)d.end);
+    d.blocks = (int)(((int64_t)d.rows * a.group + T::kRows - 1) / T::kRows);
+    d.start = a.window && d.before > a.window ? (d.before - a.window) & ~(T::kTokens - 1) : 0;
+    d.tiles = d.end > d.start ? (int)((uint32_t)(d.end - 1 - d.start) / T::kTokens) + 1 : 1;
+    return d;
+}
+
+// x y / z, rounded down and up, z > 0
+__device__ __forceinline__ int64_t tree_scaled(int64_t x, int64_t y, int64_t z) {
+    const int64_t p = x * y;
+    return ((uint64_t)p | (uint64_t)z) >> 32 ? p / z : (int64_t)((uint32_t)p / (uint32_t)z);
+}
+__device__ __forceinline__ int64_t tree_scaled_up(int64_t x, int64_t y, int64_t z) {
+    const int64_t q = tree_scaled(x, y, z);
+    return q + (q * z < x * y);
+}
+
+// Parts travel between workgroups of different dies: stores and loads that go to where all meet (fences would write back and
+// drop whole caches), in order because a workgroup waits for its stores before it counts itself in.
+constexpr int kTreeAux = 16;                 // scope of the device
+template <int ROWS> struct TreeShared {
+    __amdgpu_buffer_rsrc_t parts, sums;
+    int pitch;
+    __device__ __forceinline__ explicit TreeShared(const TreeWork &w) : pitch(w.pitch) {
+        parts = __builtin_amdgcn_make_buffer_rsrc(w.parts, 0, 2 * w.groups * ROWS * (int)sizeof(TreePart), kRsrcFlags);
+        sums = __builtin_amdgcn_make_buffer_rsrc(w.sums, 0, 2 * w.groups * ROWS * w.pitch * 4, kRsrcFlags);
+    }
+    __device__ __forceinline__ uint32_t sum_at(int slot, int row, int d) const { return (uint32_t)((slot * ROWS + row) * pitch + d) * 4u; }
+    __device__ __forceinline__ void store(int slot, int row, int d, f32x4 x) const {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), sums, sum_at(slot, row, d), 0, kTreeAux);
+    }
+    __device__ __forceinline__ void store(int slot, int row, TreePart x) const {
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, x), parts, (uint32_t)((slot * ROWS + row) * sizeof(TreePart)), 0, kTreeAux);
+    }
+    __device__ __forceinline__ f32x4 sum(int slot, int row, int d) const {
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sums, sum_at(slot, row, d), 0, kTreeAux));
+    }
+    __device__ __forceinline__ TreePart part(int slot, int row) const {
+        return __builtin_bit_cast(TreePart, __builtin_amdgcn_raw_buffer_load_b64(parts, (uint32_t)((slot * ROWS + row) * sizeof(TreePart)), 0, kTreeAux));
+    }
+};
+
+// Dimensions d .. d + 3 of a result, as far as there are `dim`.
+template <int DT> __device__ __forceinline__ void tree_store(char *row, int d, int dim, f32x4 x) {
+    u16_any *const p = (u16_any *)row + d;
+    if (d + 4 <= dim) {
+        *(u32x2_any *)p = u32x2_any{Elem<DT>::pack2(x[0], x[1]), Elem<DT>::pack2(x[2], x[3])};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (d + i < dim) p[i] = Elem<DT>::from_float(x[i]);
+    }
+}
+
+// Row `x` of a unit: a row of q and out, and one of the query heads.
+struct TreeRow {
+    int node, head;                          // number within the request's rows, query head
+    bool there;
+};
+__device__ __forceinline__ TreeRow tree_row(const PagedTreeAttentionArgs &a, const TreeWork &w, const Draft &d, int h, int64_t x) {
+    TreeRow t;
+    t.there = x < (int64_t)d.rows * a.group;
+    const uint32_t y = t.there ? (uint32_t)x : 0u;
+    t.node = (int)w.group.div(y);
+    t.head = h * a.group + (int)(y - (uint32_t)t.node * w.group.d);
+    return t;
+}
+template <int DT>
+__device__ __forceinline__ void tree_result(const PagedTreeAttentionArgs &a, const Draft &d, const TreeRow &t, int dim0, f32x4 acc, float l, float v_scale) {
+    if (dim0 >= a.dim) return;
+    const float f = l == 0.f ? 0.f : v_scale / l;            // (rows that see nothing: zeros)
+    if (l == 0.f) acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    tree_store<DT>(a.out + t.head * a.out_head_bytes + (int64_t)(d.row0 + t.node) * a.out_row_bytes, dim0, a.dim, acc * f);
+}
+
+// Joins the parts of a unit for its rows [row0, row1), by a whole workgroup: DC / 4 threads a row.
+template <int DT, int DC, int WR>
+__device__ __forceinline__ void tree_join(const PagedTreeAttentionArgs &a, const TreeWork &w, const TreeLeft &u, int row0, int row1, float v_scale) {
+    typedef TreeTile<DC, WR> T;
+    constexpr int kLanes = DC / 4, kAtOnce = kTreeThreads / kLanes, kAhead = 8;
+    const Draft d = draft_of<DC, WR>(a, w.group, u.request);
+    const TreeShared<T::kRows> shared(w);
+    const int dim0 = 4 * ((int)threadIdx.x % kLanes);
+    for (int x = row0 + (int)threadIdx.x / kLanes; x < row1; x += kAtOnce) {
+        const TreeRow t = tree_row(a, w, d, u.h, (int64_t)u.block * T::kRows + x);
+        if (!t.there || dim0 >= a.dim) continue;
+        float m = -INFINITY, l = 0.f;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int p0 = 0; p0 < u.parts; p0 += kAhead) {
+            TreePart part[kAhead];
+            f32x4 sum[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                part[i] = {-INFINITY, 0.f};
+                sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (p0 + i < u.parts) {
+                    const int slot = 2 * (u.begins + p0 + i) + (p0 + i == 0 ? 1 : 0);
+                    part[i] = shared.part(slot, x);
+                    sum[i] = shared.sum(slot, x, dim0);
+                }
+            }
+            float top = m;
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) top = fmaxf(top, part[i].m);
+            const float base = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f(m - base);
+            l *= old;
+            acc *= old;
+            m = top;
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const float f = __builtin_amdgcn_exp2f(part[i].m - base);
+                l += f * part[i].l;
+                acc += f * sum[i];
+            }
+        }
+        tree_result<DT>(a, d, t, dim0, acc, l, v_scale);
+    }
+}
+
+template <int DT> struct TreeElem;
+template <> struct TreeElem<0> {
+    static constexpr uint32_t kExponent = 0x7c00u;
+    // Probabilities are lifted by a power of two, so that small ones stay apart from zero in fp16.  A maximum that is kept though a
+    // larger one has come (by up to 2^7, see kTreeLag) leaves them below 2^13, and with scores so large that neighbouring fp32
+    // numbers lie 2, 4 or 8 apart, where the difference rounds, below 2^15.
+    static constexpr float kLift = 6.f;
+    static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+template <> struct TreeElem<1> {
+    static constexpr uint32_t kExponent = 0x7f80u;
+    static constexpr float kLift = 0.f;
+    static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+constexpr float kTreeLag = 7.f;
+
+// Two e4m3 values (HI: the upper two bytes) as two 16-bit numbers: exact in either type.
+template <int DT, bool HI> __device__ __forceinline__ uint32_t tree_widen(uint32_t x) {
+    if (DT == 0) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)x, 1.f, HI));
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)x, 1.f, HI));
+}
+
+// A 16-byte piece that was loaded from `past` bytes before its place (the row's end would have cut it off), brought into place.
+__device__ __forceinline__ void tree_shift(uint32_t (&x)[4], int past) {
+    const bool two = past & 8, one = past & 4;
+    x[0] = two ? x[2] : x[0]; x[1] = two ? x[3] : x[1]; x[2] = two ? 0u : x[2]; x[3] = two ? 0u : x[3];
+    x[0] = one ? x[1] : x[0]; x[1] = one ? x[2] : x[1]; x[2] = one ? x[3] : x[2]; x[3] = one ? 0u : x[3];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = past >= 16 ? 0u : __builtin_amdgcn_alignbyte(i < 3 ? x[i + 1] : 0u, x[i], past & 3);
+}
+
+// Greatest and sum over a lane and its partner, 32 lanes on.
+__device__ __forceinline__ float pair_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ __forceinline__ float pair_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+
+// Barrier that waits for this wavefront's LDS traffic only (loads of the next tile stay in flight).
+__device__ __forceinline__ void tree_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ int64_t shuffle64(int64_t v, int lane) {
+    const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)v, lane), hi = (uint32_t)__shfl((int)(uint32_t)((uint64_t)v >> 32), lane);
+    return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+
+// DC: dimensions that the registers hold (64, 128, 256).  ANY: rows at any address.
+template <int DT, bool F8, int DC, int WR, bool ANY>
+__global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) paged_tree_attention_kernel(PagedTreeAttentionArgs a, TreeWork w) {
+    typedef TreeTile<DC, WR> T;
+    typedef TreeElem<DT> E;
+    constexpr int EB = F8 ? 1 : 2, kPieces = DC * EB / 16;   // bytes of an element, 16-byte pieces of a row
+    constexpr int kLoaders = T::kAlone ? 64 : kTreeThreads, kAtOnce = kLoaders / kPieces, kPasses = T::kStaged / kAtOnce;
+    constexpr int KS = DC / 16, DB = DC / 32, SUBS = T::kMine / 32;
+    static_assert(kLoaders % kPieces == 0 && T::kStaged % kAtOnce == 0);
+    const int lane = lane_id(), l32 = lane & 31, half = lane >> 5, wave = uniform((int)threadIdx.x >> 6), wr = wave % WR, wt = wave / WR;
+
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ int64_t scan[kTreeWaves];
+    struct Place {
+        int32_t request, unit, tile;
+        int64_t at;
+    };
+    __shared__ Place places[2];
+    __shared__ float wave_m[kTreeWaves][32], wave_l[kTreeWaves][32];
+    __shared__ TreeLeft left[2];
+    __shared__ bool joins[2];
+    __shared__ int32_t odd[T::kAlone ? kTreeWaves : T::kBuffers];        // number of the last tile there with values that are not finite
+    int unfinished = 0;
+
+    // ---- rows of no request: zeros
+    {
+        const int64_t head = a.requests ? min(max(a.accum[0], (int64_t)0), a.tokens) : a.tokens;
+        const int64_t tail = a.requests ? min(max(a.accum[a.requests], head), a.tokens) : a.tokens;
+        const int64_t none = head + a.tokens - tail;
+        const int heads = a.heads * a.group;
+        for (int64_t i = blockIdx.x; i < none * heads; i += gridDim.x) {
+            const int64_t row = i / heads;
+            char *const out = a.out + (i - row * heads) * a.out_head_bytes + (row < head ? row : tail + (row - head)) * a.out_row_bytes;
+            for (int d = (int)threadIdx.x; d < a.dim; d += kTreeThreads) ((u16_any *)out)[d] = 0;
+        }
+    }
+    if (threadIdx.x < sizeof(odd) / sizeof(odd[0])) odd[threadIdx.x] = 0;
+
+    // ---- the share: tiles of all units in the order of requests, key heads, blocks of rows.  Thread i adds up requests [i c, (i + 1) c).
+    const int c = (a.requests + kTreeThreads - 1) / kTreeThreads, r0 = (int)threadIdx.x * c, r1 = min(a.requests, r0 + c);
+    int64_t mine = 0, units = 0;
+    for (int r = r0; r < r1; ++r) {
+        const Draft d = draft_of<DC, WR>(a, w.group, r);
+        mine += (int64_t)a.heads * d.blocks * d.tiles;
+        units += (int64_t)a.heads * d.blocks;
+    }
+    int64_t upto = wave_inclusive_scan(mine);
+    const int64_t some = wave_inclusive_scan(units);
+    __shared__ int64_t scan_units[kTreeWaves];
+    if (lane == 63) { scan[wave] = upto; scan_units[wave] = some; }
+    __syncthreads();
+    int64_t total = 0;
+    units = 0;
+#pragma unroll
+    for (int i = 0; i < kTreeWaves; ++i) {
+        if (i < wave) upto += scan[i];
+        total += scan[i];
+        units += scan_units[i];
+    }
+    total = uniform64(total);
+    units = uniform64(units);
+    const int64_t groups = min((int64_t)w.groups, max((total + kTreeShare - 1) / kTreeShare, units));
+    const int64_t group = blockIdx.x;
+    if (w.left && threadIdx.x == 0) w.left[group].parts = 0;
+    if (group >= groups || total == 0) return;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        int64_t at = tree_scaled(group + k, total, groups);
+        if (at >= total) {
+            if (threadIdx.x == 0) places[k] = {a.requests, 0, 0, total};
+        } else if (at < upto && at >= upto - mine) {
+            int64_t before = upto - mine;
+            int r = r0;
+            Draft d = draft_of<DC, WR>(a, w.group, r);
+            while (at >= before + (int64_t)a.heads * d.blocks * d.tiles) {
+                before += (int64_t)a.heads * d.blocks * d.tiles;
+                d = draft_of<DC, WR>(a, w.group, ++r);
+            }
+            int unit = (int)tree_scaled(at - before, 1, d.tiles), tile = (int)((at - before) - (int64_t)unit * d.tiles);
+            if (d.tiles <= kTreeWhole && tile) {             // short units go where most of them lies
+                at -= tile;
+                if (2 * tile > d.tiles) {
+                    at += d.tiles;
+                    if (++unit == a.heads * d.blocks) {
+                        unit = 0;
+                        ++r;
+                    }
+                }
+                tile = 0;
+            }
+            places[k] = {r, unit, tile, at};
+        }
+    }
+    __syncthreads();
+    const int64_t end = uniform64(places[1].at);
+    int64_t at = uniform64(places[0].at);
+    int request = uniform(places[0].request), unit = uniform(places[0].unit), tile = uniform(places[0].tile);
+
+    char *const ours = lds + (T::kAlone ? wave * T::kBuffer : 0);
+    const int loader = T::kAlone ? lane : (int)threadIdx.x, piece = loader % kPieces, line = loader / kPieces;
+    const int row_bytes = EB * a.dim;
+    const bool has_piece = 16 * piece < row_bytes;
+    // what no load ever fills: the dimensions behind the row's end
+    if (16 * kPieces > row_bytes) {
+        for (int b = 0; b < (T::kAlone ? 1 : T::kBuffers); ++b)
+            for (int x = 16 * loader; x < T::kBuffer; x += 16 * kLoaders) *(u32x4 *)(ours + b * T::kBuffer + x) = u32x4{0u, 0u, 0u, 0u};
+        __syncthreads();
+    }
+    int number = 0;                                          // of the tile, over all units
+
+    while (at < end) {
+        // ---- a unit's part: tiles [tile, last)
+        Draft d = draft_of<DC, WR>(a, w.group, request);
+        while (d.blocks == 0) d = draft_of<DC, WR>(a, w.group, ++request);
+        d.row0 = uniform(d.row0); d.rows = uniform(d.rows); d.before = uniform(d.before); d.end = uniform(d.end); d.blocks = uniform(d.blocks);
+        d.start = uniform(d.start); d.tiles = uniform(d.tiles); d.node0 = uniform64(d.node0);
+        const int h = unit / d.blocks, block = unit - h * d.blocks, last = (int)min((int64_t)d.tiles, tile + (end - at));
+        const int32_t *const row = a.table + request * a.table_stride;
+        const char *const kbase = a.k.base + h * a.k.head_bytes, *const vbase = a.v.base + h * a.v.head_bytes;
+        const TreeRow mine_row = tree_row(a, w, d, h, (int64_t)block * T::kRows + 32 * wr + l32);
+
+        // queries: column l32 of the scores
+        u32x4 q[KS];
+        {
+            const char *const p = a.q + mine_row.head * a.q_head_bytes + (int64_t)(d.row0 + mine_row.node) * a.q_row_bytes;
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                uint32_t x[4] = {0, 0, 0, 0};
+                const int d0 = 16 * k + 8 * half;
+                if (mine_row.there) load_part<4>(x, p + 2 * d0, 2 * (a.dim - d0));
+                q[k] = u32x4{x[0], x[1], x[2], x[3]};
+            }
+        }
+        // what the row sees: tokens from `from` on that lie before the draft or have their bit
+        const int64_t *const bits = a.mask ? a.mask + (int64_t)(d.row0 + mine_row.node) * a.mask_stride : nullptr;
+        const int drafted = d.end - d.before, counted = a.mask ? (int)min((int64_t)drafted, 64 * (int64_t)a.words) : drafted;
+        const int chain = (int)min(d.node0 + mine_row.node + 1, (int64_t)drafted);       // without a mask: nodes it sees
+        int from = 0;
+        if (a.window) {
+            int seen = chain;
+            if (bits) {
+                seen = 0;
+                for (int j = 0; j < counted; j += 64)
+                    seen += __builtin_popcountll((uint64_t)bits[j >> 6] & (counted - j >= 64 ? ~0ull : (1ull << (counted - j)) - 1));
+            }
+            if (seen <= a.window) {
+                from = d.before > a.window - seen ? d.before - (a.window - seen) : 0;
+            } else if (!bits) {
+                from = d.before + (seen - a.window);
+            } else {
+                int skip = seen - a.window, j = 0;           // nodes that it sees no more
+                for (;; j += 64) {
+                    uint64_t x = (uint64_t)bits[j >> 6];
+                    const int n = __builtin_popcountll(x);
+                    if (n <= skip) {
+                        skip -= n;
+                        continue;
+                    }
+                    for (; skip > 0; --skip) x &= x - 1;
+                    from = d.before + j + __builtin_ctzll(x);
+                    break;
+                }
+            }
+        }
+        // tiles from here on are seen by all rows as far as they lie before the draft
+        const int all_from = a.window ? max(d.before - a.window + min(drafted, a.window), 0) : 0;
+        auto visible = [&](int t0) {                         // bit i: token t0 + i
+            const int j0 = t0 - d.before;
+            uint32_t m = low_bits(-j0);
+            if (j0 > -32 && drafted > 0) {
+                if (bits) {
+                    const int j = max(j0, 0);
+                    uint64_t x = 0;
+                    if (j < counted) {
+                        x = (uint64_t)bits[j >> 6] >> (j & 63);
+                        if ((j & 63) > 32 && (j >> 6) + 1 < a.words) x |= (uint64_t)bits[(j >> 6) + 1] << (64 - (j & 63));
+                    }
+                    m |= j0 >= 0 ? (uint32_t)x : (uint32_t)x << -j0;
+                    m &= low_bits(counted - j0);
+                } else {
+                    m |= low_bits(chain - j0);
+                }
+            }
+            m &= low_bits(d.end - t0) & ~low_bits(from - t0);
+            return mine_row.there ? m : 0u;
+        };
+
+        // Places of a tile's tokens: lane i has that of token i, and hands it to those that load the token.  Tokens that are not there, or
+        // whose page number is outside the cache, have none: their keys are NaN (which is the result of rows that see them), their values zeros.
+        const int mine_at = T::kAlone ? lane & (T::kStaged - 1) : lane;
+        auto first_of = [&](int i) { return d.start + i * T::kTokens + (T::kAlone ? wave * T::kMine : 0); };
+        auto look_up = [&](int i) {
+            const int64_t t = (int64_t)d.start + (int64_t)i * T::kTokens + (T::kAlone ? wave * T::kMine : 0) + mine_at;
+            return i < last && t < d.end ? row[a.page.div((uint32_t)t)] : -1;
+        };
+        uint32_t kx[kPasses][4], vx[kPasses][4];
+        uint32_t missing = 0;                                // bit p: the token of pass p is not there
+        auto load = [&](int i, int32_t page) {
+            const uint32_t t = (uint32_t)(first_of(i) + mine_at), in = t - a.page.div(t) * a.page.d;
+            const bool none = (uint32_t)page >= (uint32_t)a.pages;
+            const int64_t k_at = none ? -1 : (int64_t)page * a.k.page_bytes + (int64_t)in * a.k.token_bytes;
+            const int64_t v_at = none ? -1 : (int64_t)page * a.v.page_bytes + (int64_t)in * a.v.token_bytes;
+            missing = 0;
+#pragma unroll
+            for (int p = 0; p < kPasses; ++p) {
+                const int64_t ko = shuffle64(k_at, p * kAtOnce + line), vo = shuffle64(v_at, p * kAtOnce + line);
+                missing |= ko < 0 ? 1u << p : 0u;
+                if (has_piece) {
+                    // (a.q: somewhere that can be read)
+                    const char *const kp = ko < 0 ? a.q : kbase + ko, *const vp = ko < 0 ? a.q : vbase + vo;
+                    if (ANY) {
+                        if (row_bytes >= 16) {
+                            const int b = min(16 * piece, row_bytes - 16);
+                            load_stream<4>(kx[p], kp + b);
+                            load_stream<4>(vx[p], vp + b);
+                        } else {
+                            load_part<4>(kx[p], kp, row_bytes);
+                            load_part<4>(vx[p], vp, row_bytes);
+                        }
+                    } else {
+                        load_stream<4>(kx[p], kp + 16 * piece);
+                        load_stream<4>(vx[p], vp + 16 * piece);
+                    }
+                }
+            }
+        };
+        auto put = [&](char *to, const uint32_t (&x)[4]) {   // a piece into LDS, in 16 bits
+            if (F8) {
+                const uint32_t y[8] = {tree_widen<DT, false>(x[0]), tree_widen<DT, true>(x[0]), tree_widen<DT, false>(x[1]), tree_widen<DT, true>(x[1]),
+                                       tree_widen<DT, false>(x[2]), tree_widen<DT, true>(x[2]), tree_widen<DT, false>(x[3]), tree_widen<DT, true>(x[3])};
+                *(u32x4 *)to = u32x4{y[0], y[1], y[2], y[3]};
+                *(u32x4 *)(to + 16) = u32x4{y[4], y[5], y[6], y[7]};
+            } else {
+                *(u32x4 *)to = u32x4{x[0], x[1], x[2], x[3]};
+            }
+        };
+        // a tile that not all rows see all of
+        auto partial = [&](int i) { return first_of(i) + T::kStaged > d.before || first_of(i) < all_from; };
+        auto write = [&](int i, char *buf, int slot) {
+            char *const kt = buf + line * T::kPitchK + (F8 ? 32 : 16) * piece, *const vt = buf + T::kStaged * T::kPitchK + line * T::kPitchV + (F8 ? 32 : 16) * piece;
+            if (ANY && row_bytes >= 16 && 16 * piece + 16 > row_bytes && has_piece) {
+                const int past = 16 * piece - (row_bytes - 16);
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p) { tree_shift(kx[p], past); tree_shift(vx[p], past); }
+            }
+            if (__any(missing)) {
+                // (a NaN in either type; behind the row's end zeros stay zeros, so that the queries' zeros there make none)
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p)
+                    if (missing >> p & 1) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const int bytes = row_bytes - 16 * piece - 4 * x;
+                            const uint32_t keep = bytes >= 4 ? 0xffffffffu : bytes <= 0 ? 0u : (1u << (8 * bytes)) - 1u;
+                            kx[p][x] = (F8 ? 0x7f7f7f7fu : 0x7fff7fffu) & keep;
+                            vx[p][x] = 0u;
+                        }
+                    }
+            }
+            if (partial(i)) {
+                bool not_finite = false;
+                if (has_piece)
+#pragma unroll
+                    for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const uint32_t y = vx[p][x];
+                            constexpr int kWidth = F8 ? 8 : 16;
+                            constexpr uint32_t kTop = F8 ? 0x7fu : E::kExponent, kAll = F8 ? 0xffu : 0xffffu;
+#pragma unroll
+                            for (int b = 0; b < 32; b += kWidth)
+                                if ((y >> b & kTop) == kTop) {
+                                    not_finite = true;
+                                    vx[p][x] &= ~(kAll << b);
+                                }
+                        }
+                if (__any(not_finite) && lane == 0) odd[slot] = number + 1;
+            }
+            if (has_piece)
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p) {
+                    put(kt + p * kAtOnce * T::kPitchK, kx[p]);
+                    put(vt + p * kAtOnce * T::kPitchV, vx[p]);
+                }
+        };
+
+        const float to_log2 = a.scale * kLog2e * (F8 ? a.k.scale[h] : 1.f);
+        f32x16 o[DB];
+#pragma unroll
+        for (int j = 0; j < DB; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[j][i] = 0.f;
+        float m = -INFINITY, l = 0.f;
+
+        auto attend = [&](int i, const char *buf, int slot) {
+            const char *const kt = buf + (T::kAlone ? 0 : wt * T::kMine) * T::kPitchK + l32 * T::kPitchK + 16 * half;
+            const int t0 = first_of(i) + (T::kAlone ? 0 : wt * T::kMine);
+            f32x16 s[SUBS];
+#pragma unroll
+            for (int u = 0; u < SUBS; ++u) {
+#pragma unroll
+                for (int x = 0; x < 16; ++x) s[u][x] = 0.f;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) s[u] = E::mfma(*(const u32x4 *)(kt + 32 * u * T::kPitchK + 32 * k), q[k], s[u]);
+            }
+            // scores of tokens t0 + 32 u + 8 (x / 4) + 4 half + x % 4
+#pragma unroll
+            for (int u = 0; u < SUBS; ++u) s[u] *= to_log2;
+            const bool some_hidden = partial(i);
+            uint32_t see[SUBS];
+            if (some_hidden) {
+#pragma unroll
+                for (int u = 0; u < SUBS; ++u) {
+                    see[u] = visible(t0 + 32 * u) >> (4 * half);
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) s[u][x] = see[u] >> (8 * (x / 4) + x % 4) & 1 ? s[u][x] : -INFINITY;
+                }
+            }
+            float top = m;
+#pragma unroll
+            for (int u = 0; u < SUBS; ++u)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) top = fmaxf(top, s[u][x]);
+            top = pair_max(top);
+            if (__any(top > m + kTreeLag)) {                 // (also the first that is seen: m is -inf)
+                const float base = top == -INFINITY ? 0.f : top, shrink = __builtin_amdgcn_exp2f(m - base);
+                l *= shrink;
+#pragma unroll
+                for (int j = 0; j < DB; ++j) o[j] *= shrink;
+                m = top;
+            }
+            const float base = (m == -INFINITY ? 0.f : m) - E::kLift;
+            u32x4 p[2 * SUBS];
+#pragma unroll
+            for (int u = 0; u < SUBS; ++u)
+#pragma unroll
+                for (int x = 0; x < 16; x += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(s[u][x] - base), p1 = __builtin_amdgcn_exp2f(s[u][x + 1] - base);
+                    l += p0 + p1;
+                    p[2 * u + x / 8][x % 8 / 2] = Elem<DT>::pack2(p0, p1);
+                }
+            // ---- values: lane (dimension 32 j + l32, half) has tokens 16 k + 4 half + 0 .. 3 and 8 behind those
+            const char *const vt = buf + T::kStaged * T::kPitchK + ((T::kAlone ? 0 : wt * T::kMine) + 4 * half + (lane & 15) / 4) * T::kPitchV + 32 * (lane >> 4 & 1) + 8 * (lane & 3);
+            auto values = [&](int k, int j) {
+                const LdsPtr at = (LdsPtr)const_cast<char *>(vt) + 16 * k * T::kPitchV + 64 * j;
+                const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPiece)at));
+                const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPiece)(at + 8 * T::kPitchV)));
+                return u32x4{lo[0], lo[1], hi[0], hi[1]};
+            };
+#pragma unroll
+            for (int k = 0; k < 2 * SUBS; ++k)
+#pragma unroll
+                for (int j = 0; j < DB; ++j) o[j] = E::mfma(values(k, j), p[k], o[j]);
+            // Values that are not finite, in a tile of which not every row sees every token, are zeros in LDS (a probability of 0 times them would
+            // be NaN); rows that see them get them here, as they are: an infinity or NaN of any size is the same.
+            if (some_hidden && odd[slot] == number + 1) {
+#pragma nounroll
+                for (int t = t0; t < min(t0 + T::kMine, d.end); ++t) {
+                    const uint32_t page = (uint32_t)row[a.page.div((uint32_t)t)];
+                    if (page >= (uint32_t)a.pages) continue;
+                    const char *const v = vbase + page * a.v.page_bytes + (int64_t)((uint32_t)t - a.page.div((uint32_t)t) * a.page.d) * a.v.token_bytes;
+                    const bool sees = (visible(t) & 1) != 0;
+#pragma unroll
+                    for (int j = 0; j < DB; ++j)
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) {
+                            const int dim = 32 * j + 8 * (x / 4) + 4 * half + x % 4, in = min(dim, a.dim - 1);      // (behind the end: not stored)
+                            const uint32_t y = F8 ? ((const uint8_t *)v)[in] : ((const u16_any *)v)[in];
+                            const bool hit = F8 ? (y & 0x7f) == 0x7f : (y & E::kExponent) == E::kExponent;
+                            const float add = sees && hit ? (F8 ? NAN : Elem<DT>::to_float((uint16_t)y)) : 0.f;
+                            o[j][x] += add;
+                        }
+                }
+            }
+        };
+
+        // ---- tiles: while one is worked on the next one's rows are on their way, and the page numbers of the one behind it
+        int32_t page_next;
+        {
+            const int32_t page = look_up(tile);
+            page_next = look_up(tile + 1);
+            load(tile, page);
+        }
+        for (int i = tile; i < last; ++i, ++number) {
+            const int slot = T::kAlone ? wave : number & 1;
+            char *const buf = ours + (T::kAlone ? 0 : (number & 1) * T::kBuffer);
+            write(i, buf, slot);
+            if (i + 1 < last) {
+                load(i + 1, page_next);
+                page_next = look_up(i + 2);
+            }
+            if (!T::kAlone) tree_barrier();
+            attend(i, buf, slot);
+        }
+        l = pair_sum(l);
+
+        // ---- the unit's end: join the wavefronts, give out the result or leave a part
+        const bool begun = tile == 0, done = last == d.tiles, whole = begun && done;
+        const int part_slot = 2 * (int)group + (begun ? 1 : 0);
+        const float v_scale = F8 ? a.v.scale[h] : 1.f;
+        const TreeShared<T::kRows> shared(w);
+        if (T::kGroups == 1) {
+            const int x = 32 * wr + l32;
+            if (mine_row.there) {
+#pragma unroll
+                for (int j = 0; j < DB; ++j)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int dim0 = 32 * j + 8 * g + 4 * half;
+                        const f32x4 acc = {o[j][4 * g], o[j][4 * g + 1], o[j][4 * g + 2], o[j][4 * g + 3]};
+                        if (whole) tree_result<DT>(a, d, mine_row, dim0, acc, l, v_scale);
+                        else if (dim0 < a.dim) shared.store(part_slot, x, dim0, acc);
+                    }
+                if (!whole && half == 0) shared.store(part_slot, x, TreePart{m, l});
+            }
+        } else {
+            if (!T::kAlone) tree_barrier();                  // (else a wavefront's part lies where its own tokens did)
+            float *const mineo = (float *)(T::kAlone ? ours : lds + wave * 32 * T::kPitchO * 4) + l32 * T::kPitchO;
+            static_assert(32 * T::kPitchO * 4 <= (T::kAlone ? T::kBuffer : T::kLds / kTreeWaves));
+            if (half == 0) { wave_m[wave][l32] = m; wave_l[wave][l32] = l; }
+#pragma unroll
+            for (int j = 0; j < DB; ++j)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *(f32x4 *)(mineo + 32 * j + 8 * g + 4 * half) = f32x4{o[j][4 * g], o[j][4 * g + 1], o[j][4 * g + 2], o[j][4 * g + 3]};
+            tree_barrier();
+            for (int e = (int)threadIdx.x; e < T::kRows * (DC / 4); e += kTreeThreads) {
+                const int x = e / (DC / 4), dim0 = 4 * (e % (DC / 4));
+                const TreeRow t = tree_row(a, w, d, h, (int64_t)block * T::kRows + x);
+                if (!t.there || dim0 >= a.dim) continue;
+                float top = -INFINITY, sum = 0.f;
+                f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < T::kGroups; ++i) top = fmaxf(top, wave_m[i * WR + x / 32][x % 32]);
+                const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+                for (int i = 0; i < T::kGroups; ++i) {
+                    const int v = i * WR + x / 32;
+                    const float f = __builtin_amdgcn_exp2f(wave_m[v][x % 32] - base);
+                    sum += f * wave_l[v][x % 32];
+                    acc += f * *(const f32x4 *)((const float *)(lds + v * (T::kAlone ? T::kBuffer : 32 * T::kPitchO * 4)) + (x % 32) * T::kPitchO + dim0);
+                }
+                if (whole) {
+                    tree_result<DT>(a, d, t, dim0, acc, sum, v_scale);
+                } else {
+                    shared.store(part_slot, x, dim0, acc);
+                    if (dim0 == 0) shared.store(part_slot, x, TreePart{top, sum});
+                }
+            }
+        }
+        if (!whole) {
+            const int64_t first = at - tile;
+            TreeLeft u = {begun ? (int)group : (int)tree_scaled_up(first + 1, groups, total) - 1, 0, request, h, block};
+            u.parts = (int)tree_scaled_up(first + d.tiles, groups, total) - u.begins;
+            if (w.left) {
+                if (begun && threadIdx.x == 0) w.left[group] = u;
+            } else {
+                if (threadIdx.x == 0) left[unfinished] = u;
+                ++unfinished;                                // (the first unit of the share at most, and its last)
+            }
+        }
+        at += last - tile;
+        tile = 0;
+        if (++unit == a.heads * d.blocks) {
+            unit = 0;
+            ++request;
+        }
+        if (at < end) {
+            tree_barrier();
+            // (what the joining has put over the dimensions that no load fills)
+            if (T::kGroups > 1 && 16 * kPieces > row_bytes) {
+                for (int b = 0; b < (T::kAlone ? 1 : T::kBuffers); ++b)
+                    for (int x = 16 * loader; x < T::kBuffer; x += 16 * kLoaders) *(u32x4 *)(ours + b * T::kBuffer + x) = u32x4{0u, 0u, 0u, 0u};
+                if (!T::kAlone) tree_barrier();
+            }
+        }
+    }
+    if (w.left || unfinished == 0) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0)
+        for (int i = 0; i < unfinished; ++i) {
+            int32_t *const counter = w.counters + left[i].begins;
+            joins[i] = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == left[i].parts - 1;
+            if (joins[i]) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    __syncthreads();
+    for (int i = 0; i < unfinished; ++i)
+        if (joins[i]) tree_join<DT, DC, WR>(a, w, left[i], 0, T::kRows, F8 ? a.v.scale[left[i].h] : 1.f);
+}
+
+// The joining as a kernel of its own: grid (workgroups of the other, blocks of rows).
+template <int DT, int DC, int WR> __global__ void __launch_bounds__(kTreeThreads) paged_tree_join_kernel(PagedTreeAttentionArgs a, TreeWork w, int rows) {
+    const TreeLeft u = w.left[blockIdx.x];
+    const int row0 = (int)blockIdx.y * rows;
+    if (u.parts) tree_join<DT, DC, WR>(a, w, u, row0, row0 + rows, a.v.scale ? a.v.scale[u.h] : 1.f);
+}
+
+// ------------------------------------------------------------------ host
+// Which build takes a call: dimensions that its registers hold, wavefronts side by side over the rows.
+static inline int tree_dims(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+static inline int tree_waves(int64_t tokens, int64_t requests, int64_t group) { return tokens * group <= 32 * std::max<int64_t>(1, requests) ? 1 : 4; }
+
+template <int DT, bool F8, int DC, int WR, bool ANY> static int launch_tree_build(const PagedTreeAttentionArgs &a, const TreeWork &w, hipStream_t stream) {
+    typedef TreeTile<DC, WR> T;
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&paged_tree_attention_kernel<DT, F8, DC, WR, ANY>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds);
+    if (attr != hipSuccess) return BA_ERR_LAUNCH;
+    paged_tree_attention_kernel<DT, F8, DC, WR, ANY><<<w.groups, kTreeThreads, T::kLds, stream>>>(a, w);
+    if (w.left) {
+        constexpr int kRows = kTreeThreads / (DC / 4);
+        paged_tree_join_kernel<DT, DC, WR><<<dim3((unsigned)w.groups, T::kRows / kRows), kTreeThreads, 0, stream>>>(a, w, kRows);
+    }
+    return hipGetLastError() == hipSuccess ? BA_OK : BA_ERR_LAUNCH;
+}
+
+template <int DT, bool F8, int DC> static int launch_tree_dims(const PagedTreeAttentionArgs &a, const TreeWork &w, bool any, int waves, hipStream_t stream) {
+    if (waves == 1) return any ? launch_tree_build<DT, F8, DC, 1, true>(a, w, stream) : launch_tree_build<DT, F8, DC, 1, false>(a, w, stream);
+    return any ? launch_tree_build<DT, F8, DC, 4, true>(a, w, stream) : launch_tree_build<DT, F8, DC, 4, false>(a, w, stream);
+}
+
+template <int DT, bool F8> int launch_tree_types(const PagedTreeAttentionArgs &a, const TreeWork &w, bool any, int waves, hipStream_t stream) {
+    switch (tree_dims(a.dim)) {
+        case 64: return launch_tree_dims<DT, F8, 64>(a, w, any, waves, stream);
+        case 128: return launch_tree_dims<DT, F8, 128>(a, w, any, waves, stream);
+        default: return launch_tree_dims<DT, F8, 256>(a, w, any, waves, stream);
+    }
+}
+
+}  // namespace ba
