@@ -16,7 +16,7 @@ static TreeWork tree_work(int64_t heads, int64_t group, int64_t dim, int64_t tok
                           void *workspace, size_t *bytes) {
     TreeWork w{};
     const int waves = tree_waves(tokens, requests, group), dims = tree_dims(dim);
-    const int64_t rows = 32 * waves, tile = waves == 4 ? 64 : 128;
+    const int64_t rows = 32 * waves, tile = waves == 1 ? 128 : dims == 256 ? 32 : 64;
     const int64_t resident = (int64_t)device_cu_count() * resident_of(dims);
     const double units = (double)heads * (tokens * group / rows + requests);
     const double longest = window > 0 ? std::min((double)width * page, (double)window + tokens + tile) : (double)width * page;

@@ -29,7 +29,7 @@ constexpr int kTreeFewParts = 8;             // parts of a unit, on the average,
 //   rows   wavefronts side by side over 32 rows each; the others take other tokens of the same tile
 template <int DC, int WR> struct TreeTile {
     static constexpr int kRows = 32 * WR, kGroups = kTreeWaves / WR;     // rows of a unit, groups of wavefronts with the same tokens
-    static constexpr int kMine = WR == 4 ? 64 : 32;                       // tokens of a wavefront in a tile
+    static constexpr int kMine = WR == 4 && DC < 256 ? 64 : 32;           // tokens of a wavefront in a tile
     static constexpr int kTokens = kMine * kGroups;
     static constexpr bool kAlone = WR == 1;                               // every wavefront loads its own tokens
     static constexpr int kBuffers = kAlone ? 1 : 2;
@@ -66,10 +66,13 @@ struct Draft {
     int32_t before, end;                     // tokens before the draft, tokens; as far as the table's row holds them
     int32_t blocks, start, tiles;            // of kRows rows; first token of the first tile that may be seen, tiles
 };
-template <int DC, int WR> __device__ __forceinline__ Draft draft_of(const PagedTreeAttentionArgs &a, const PageDiv &, int r) {
+// UNIFORM: r is the same in all lanes (scalar loads).
+template <int DC, int WR, bool UNIFORM> __device__ __forceinline__ Draft draft_of(const PagedTreeAttentionArgs &a, int r) {
     typedef TreeTile<DC, WR> T;
+    typedef typename std::conditional<UNIFORM, ConstI64, const int64_t *>::type Numbers;
+    const Numbers accum = (Numbers)(uintptr_t)a.accum, lens = (Numbers)(uintptr_t)a.lens;
     constexpr int64_t kFar = int64_t(1) << 40;               // sums and lengths beyond any array
-    const int64_t a0 = min(max(a.accum[r], -kFar), kFar), a1 = min(max(a.accum[r + 1], -kFar), kFar), length = min(max(a.lens[r], (int64_t)0), kFar);
+    const int64_t a0 = min(max(accum[r], -kFar), kFar), a1 = min(max(accum[r + 1], -kFar), kFar), length = min(max(lens[r], (int64_t)0), kFar);
     const int64_t n = max(a1 - a0, (int64_t)0), room = (int64_t)a.width * a.page.d;
     const int64_t first = min(max(a0, (int64_t)0), a.tokens), last = min(max(a1, first), a.tokens);
     Draft d;
@@ -84,15 +87,16 @@ template <int DC, int WR> __device__ __forceinline__ Draft draft_of(const PagedT
     return d;
 }
 
-// x y / z, rounded down and up, z > 0
-__device__ __forceinline__ int64_t tree_scaled(int64_t x, int64_t y, int64_t z) {
+// x y / z, rounded down and up, for 0 <= x y < 2^62 and 0 < z: the quotient of fp64 numbers is off by one at most while it is below 2^51
+// (a division of 64-bit integers is ten times the code).
+__device__ __forceinline__ int64_t tree_ratio(int64_t x, int64_t y, int64_t z) {
     const int64_t p = x * y;
-    return ((uint64_t)p | (uint64_t)z) >> 32 ? p / z : (int64_t)((uint32_t)p / (uint32_t)z);
+    int64_t q = (int64_t)((double)p / (double)z);
+    q -= q * z > p ? 1 : 0;
+    q += p - q * z >= z ? 1 : 0;
+    return q;
 }
-__device__ __forceinline__ int64_t tree_scaled_up(int64_t x, int64_t y, int64_t z) {
-    const int64_t q = tree_scaled(x, y, z);
-    return q + (q * z < x * y);
-}
+__device__ __forceinline__ int64_t tree_ratio_up(int64_t x, int64_t y, int64_t z) { return tree_ratio(x, y, z) + (tree_ratio(x, y, z) * z < x * y); }
 
 // Parts travel between workgroups of different dies: stores and loads that go to where all meet (fences would write back and
 // drop whole caches), in order because a workgroup waits for its stores before it counts itself in.
@@ -157,7 +161,7 @@ template <int DT, int DC, int WR>
 __device__ __forceinline__ void tree_join(const PagedTreeAttentionArgs &a, const TreeWork &w, const TreeLeft &u, int row0, int row1, float v_scale) {
     typedef TreeTile<DC, WR> T;
     constexpr int kLanes = DC / 4, kAtOnce = kTreeThreads / kLanes, kAhead = 8;
-    const Draft d = draft_of<DC, WR>(a, w.group, u.request);
+    const Draft d = draft_of<DC, WR, false>(a, u.request);
     const TreeShared<T::kRows> shared(w);
     const int dim0 = 4 * ((int)threadIdx.x % kLanes);
     for (int x = row0 + (int)threadIdx.x / kLanes; x < row1; x += kAtOnce) {
@@ -248,7 +252,59 @@ __device__ __forceinline__ int64_t shuffle64(int64_t v, int lane) {
     const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)v, lane), hi = (uint32_t)__shfl((int)(uint32_t)((uint64_t)v >> 32), lane);
     return (int64_t)(((uint64_t)hi << 32) | lo);
 }
-__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+__device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
+
+// What a row sees of the tokens from a place on.
+struct Sight {
+    const int64_t *bits;                     // its row of the mask, or NULL
+    int counted, chain, from;                // nodes that have bits; without a mask nodes that it sees; first token of the window
+    bool there;
+    // bit i: token t0 + i
+    __device__ __forceinline__ uint64_t operator()(const Draft &d, int words, uint32_t t0) const {
+        if (!there || t0 >= (uint32_t)d.end) return 0;
+        const int j0 = (int)t0 - d.before, j = max(j0, 0);   // node of the first token; the first node
+        uint64_t x = low_bits(chain - j);
+        if (bits) {
+            x = 0;
+            if (j < counted) {
+                x = (uint64_t)bits[j >> 6] >> (j & 63);
+                if ((j & 63) && (j >> 6) + 1 < words) x |= (uint64_t)bits[(j >> 6) + 1] << (64 - (j & 63));
+            }
+        }
+        const int before = j - j0;                           // tokens that lie before the draft
+        x = before >= 64 ? ~0ull : x << before | low_bits(before);
+        return x & low_bits(d.end - (int)t0) & ~low_bits(from - (int)t0);
+    }
+};
+__device__ __forceinline__ Sight sight_of(const PagedTreeAttentionArgs &a, const Draft &d, const TreeRow &t, int from) {
+    const int drafted = d.end - d.before;
+    Sight s;
+    s.bits = a.mask ? a.mask + (int64_t)(d.row0 + t.node) * a.mask_stride : nullptr;
+    s.counted = a.mask ? (int)min((int64_t)drafted, 64 * (int64_t)a.words) : drafted;
+    s.chain = (int)min(d.node0 + t.node + 1, (int64_t)drafted);
+    s.from = from;
+    s.there = t.there;
+    return s;
+}
+// The first token that the window leaves of what a row sees.
+__device__ __forceinline__ int window_from(const PagedTreeAttentionArgs &a, const Draft &d, const Sight &s) {
+    int skip = s.chain - a.window, j = 0;                    // nodes that it sees no more
+    if (s.bits) {
+        skip = -a.window;
+        for (j = 0; j < s.counted; j += 64) skip += __builtin_popcountll((uint64_t)s.bits[j >> 6] & low_bits(s.counted - j));
+    }
+    if (skip <= 0) return max(d.before + skip, 0);
+    if (!s.bits) return d.before + skip;
+    for (j = 0;; j += 64) {
+        uint64_t x = (uint64_t)s.bits[j >> 6];
+        const int n = __builtin_popcountll(x);
+        if (n > skip) {
+            for (; skip > 0; --skip) x &= x - 1;
+            return d.before + j + __builtin_ctzll(x);
+        }
+        skip -= n;
+    }
+}
 
 // DC: dimensions that the registers hold (64, 128, 256).  ANY: rows at any address.
 template <int DT, bool F8, int DC, int WR, bool ANY>
@@ -258,48 +314,33 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
     constexpr int EB = F8 ? 1 : 2, kPieces = DC * EB / 16;   // bytes of an element, 16-byte pieces of a row
     constexpr int kLoaders = T::kAlone ? 64 : kTreeThreads, kAtOnce = kLoaders / kPieces, kPasses = T::kStaged / kAtOnce;
     constexpr int KS = DC / 16, DB = DC / 32, SUBS = T::kMine / 32;
-    static_assert(kLoaders % kPieces == 0 && T::kStaged % kAtOnce == 0);
+    static_assert(kLoaders % kPieces == 0 && T::kStaged % kAtOnce == 0 && T::kStaged <= 64);
     const int lane = lane_id(), l32 = lane & 31, half = lane >> 5, wave = uniform((int)threadIdx.x >> 6), wr = wave % WR, wt = wave / WR;
 
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    __shared__ int64_t scan[kTreeWaves];
     struct Place {
         int32_t request, unit, tile;
         int64_t at;
     };
     __shared__ Place places[2];
+    __shared__ int64_t scan[2 * kTreeWaves];
     __shared__ float wave_m[kTreeWaves][32], wave_l[kTreeWaves][32];
     __shared__ TreeLeft left[2];
-    __shared__ bool joins[2];
-    __shared__ int32_t odd[T::kAlone ? kTreeWaves : T::kBuffers];        // number of the last tile there with values that are not finite
+    __shared__ int32_t joins[2], row_from[T::kRows], odd;    // odd: whether a part's hidden tiles have values that are not finite
     int unfinished = 0;
-
-    // ---- rows of no request: zeros
-    {
-        const int64_t head = a.requests ? min(max(a.accum[0], (int64_t)0), a.tokens) : a.tokens;
-        const int64_t tail = a.requests ? min(max(a.accum[a.requests], head), a.tokens) : a.tokens;
-        const int64_t none = head + a.tokens - tail;
-        const int heads = a.heads * a.group;
-        for (int64_t i = blockIdx.x; i < none * heads; i += gridDim.x) {
-            const int64_t row = i / heads;
-            char *const out = a.out + (i - row * heads) * a.out_head_bytes + (row < head ? row : tail + (row - head)) * a.out_row_bytes;
-            for (int d = (int)threadIdx.x; d < a.dim; d += kTreeThreads) ((u16_any *)out)[d] = 0;
-        }
-    }
-    if (threadIdx.x < sizeof(odd) / sizeof(odd[0])) odd[threadIdx.x] = 0;
 
     // ---- the share: tiles of all units in the order of requests, key heads, blocks of rows.  Thread i adds up requests [i c, (i + 1) c).
     const int c = (a.requests + kTreeThreads - 1) / kTreeThreads, r0 = (int)threadIdx.x * c, r1 = min(a.requests, r0 + c);
     int64_t mine = 0, units = 0;
     for (int r = r0; r < r1; ++r) {
-        const Draft d = draft_of<DC, WR>(a, w.group, r);
+        const Draft d = draft_of<DC, WR, false>(a, r);
         mine += (int64_t)a.heads * d.blocks * d.tiles;
         units += (int64_t)a.heads * d.blocks;
     }
     int64_t upto = wave_inclusive_scan(mine);
-    const int64_t some = wave_inclusive_scan(units);
-    __shared__ int64_t scan_units[kTreeWaves];
-    if (lane == 63) { scan[wave] = upto; scan_units[wave] = some; }
+    units = wave_inclusive_scan(units);
+    if (lane == 63) { scan[wave] = upto; scan[kTreeWaves + wave] = units; }
+    if (threadIdx.x == 0) odd = 0;
     __syncthreads();
     int64_t total = 0;
     units = 0;
@@ -307,28 +348,40 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
     for (int i = 0; i < kTreeWaves; ++i) {
         if (i < wave) upto += scan[i];
         total += scan[i];
-        units += scan_units[i];
+        units += scan[kTreeWaves + i];
     }
     total = uniform64(total);
-    units = uniform64(units);
-    const int64_t groups = min((int64_t)w.groups, max((total + kTreeShare - 1) / kTreeShare, units));
-    const int64_t group = blockIdx.x;
+    const int64_t groups = uniform64(min((int64_t)w.groups, max((total + kTreeShare - 1) / kTreeShare, units)));
+    const int group = (int)blockIdx.x;
     if (w.left && threadIdx.x == 0) w.left[group].parts = 0;
-    if (group >= groups || total == 0) return;
-#pragma unroll
+    // rows of no request: zeros
+    {
+        const int64_t head = a.requests ? min(max(a.accum[0], (int64_t)0), a.tokens) : a.tokens;
+        const int64_t tail = a.requests ? min(max(a.accum[a.requests], head), a.tokens) : a.tokens;
+        for (int64_t i = group; i < head + a.tokens - tail; i += gridDim.x) {
+            char *const out = a.out + (i < head ? i : tail + (i - head)) * a.out_row_bytes;
+            for (int x = (int)threadIdx.x; x < a.heads * a.group * a.dim; x += kTreeThreads) {
+                const int head_of = x / a.dim;
+                *(u16_any *)(out + head_of * a.out_head_bytes + 2 * (x - head_of * a.dim)) = 0;
+            }
+        }
+    }
+    if (group >= groups) return;
+#pragma nounroll
     for (int k = 0; k < 2; ++k) {
-        int64_t at = tree_scaled(group + k, total, groups);
+        int64_t at = tree_ratio(group + k, total, groups);
         if (at >= total) {
             if (threadIdx.x == 0) places[k] = {a.requests, 0, 0, total};
         } else if (at < upto && at >= upto - mine) {
-            int64_t before = upto - mine;
-            int r = r0;
-            Draft d = draft_of<DC, WR>(a, w.group, r);
-            while (at >= before + (int64_t)a.heads * d.blocks * d.tiles) {
-                before += (int64_t)a.heads * d.blocks * d.tiles;
-                d = draft_of<DC, WR>(a, w.group, ++r);
+            int64_t before = upto - mine, all;
+            int r = r0 - 1;
+            Draft d;
+            for (all = 0;; before += all) {
+                d = draft_of<DC, WR, false>(a, ++r);
+                all = (int64_t)a.heads * d.blocks * d.tiles;
+                if (at < before + all) break;
             }
-            int unit = (int)tree_scaled(at - before, 1, d.tiles), tile = (int)((at - before) - (int64_t)unit * d.tiles);
+            int unit = (int)tree_ratio(at - before, 1, d.tiles), tile = (int)((at - before) - (int64_t)unit * d.tiles);
             if (d.tiles <= kTreeWhole && tile) {             // short units go where most of them lies
                 at -= tile;
                 if (2 * tile > d.tiles) {
@@ -352,189 +405,36 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
     const int loader = T::kAlone ? lane : (int)threadIdx.x, piece = loader % kPieces, line = loader / kPieces;
     const int row_bytes = EB * a.dim;
     const bool has_piece = 16 * piece < row_bytes;
-    // what no load ever fills: the dimensions behind the row's end
-    if (16 * kPieces > row_bytes) {
-        for (int b = 0; b < (T::kAlone ? 1 : T::kBuffers); ++b)
-            for (int x = 16 * loader; x < T::kBuffer; x += 16 * kLoaders) *(u32x4 *)(ours + b * T::kBuffer + x) = u32x4{0u, 0u, 0u, 0u};
-        __syncthreads();
-    }
-    int number = 0;                                          // of the tile, over all units
 
     while (at < end) {
         // ---- a unit's part: tiles [tile, last)
-        Draft d = draft_of<DC, WR>(a, w.group, request);
-        while (d.blocks == 0) d = draft_of<DC, WR>(a, w.group, ++request);
-        d.row0 = uniform(d.row0); d.rows = uniform(d.rows); d.before = uniform(d.before); d.end = uniform(d.end); d.blocks = uniform(d.blocks);
-        d.start = uniform(d.start); d.tiles = uniform(d.tiles); d.node0 = uniform64(d.node0);
+        Draft d = draft_of<DC, WR, true>(a, request);
+        while (d.blocks == 0) d = draft_of<DC, WR, true>(a, ++request);
         const int h = unit / d.blocks, block = unit - h * d.blocks, last = (int)min((int64_t)d.tiles, tile + (end - at));
         const int32_t *const row = a.table + request * a.table_stride;
         const char *const kbase = a.k.base + h * a.k.head_bytes, *const vbase = a.v.base + h * a.v.head_bytes;
         const TreeRow mine_row = tree_row(a, w, d, h, (int64_t)block * T::kRows + 32 * wr + l32);
 
-        // queries: column l32 of the scores
-        u32x4 q[KS];
-        {
-            const char *const p = a.q + mine_row.head * a.q_head_bytes + (int64_t)(d.row0 + mine_row.node) * a.q_row_bytes;
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                uint32_t x[4] = {0, 0, 0, 0};
-                const int d0 = 16 * k + 8 * half;
-                if (mine_row.there) load_part<4>(x, p + 2 * d0, 2 * (a.dim - d0));
-                q[k] = u32x4{x[0], x[1], x[2], x[3]};
-            }
+        // queries, by way of LDS: column l32 of the scores
+        for (int x = loader; x < (T::kAlone ? 32 : T::kRows) * (DC / 8); x += kLoaders) {
+            const int i = x / (DC / 8), d0 = 8 * (x % (DC / 8));
+            const TreeRow t = tree_row(a, w, d, h, (int64_t)block * T::kRows + i);
+            uint32_t y[4] = {0, 0, 0, 0};
+            if (t.there) load_part<4>(y, a.q + t.head * a.q_head_bytes + (int64_t)(d.row0 + t.node) * a.q_row_bytes + 2 * d0, 2 * (a.dim - d0));
+            *(u32x4 *)(ours + i * T::kPitchK + 2 * d0) = u32x4{y[0], y[1], y[2], y[3]};
         }
-        // what the row sees: tokens from `from` on that lie before the draft or have their bit
-        const int64_t *const bits = a.mask ? a.mask + (int64_t)(d.row0 + mine_row.node) * a.mask_stride : nullptr;
-        const int drafted = d.end - d.before, counted = a.mask ? (int)min((int64_t)drafted, 64 * (int64_t)a.words) : drafted;
-        const int chain = (int)min(d.node0 + mine_row.node + 1, (int64_t)drafted);       // without a mask: nodes it sees
-        int from = 0;
-        if (a.window) {
-            int seen = chain;
-            if (bits) {
-                seen = 0;
-                for (int j = 0; j < counted; j += 64)
-                    seen += __builtin_popcountll((uint64_t)bits[j >> 6] & (counted - j >= 64 ? ~0ull : (1ull << (counted - j)) - 1));
-            }
-            if (seen <= a.window) {
-                from = d.before > a.window - seen ? d.before - (a.window - seen) : 0;
-            } else if (!bits) {
-                from = d.before + (seen - a.window);
-            } else {
-                int skip = seen - a.window, j = 0;           // nodes that it sees no more
-                for (;; j += 64) {
-                    uint64_t x = (uint64_t)bits[j >> 6];
-                    const int n = __builtin_popcountll(x);
-                    if (n <= skip) {
-                        skip -= n;
-                        continue;
-                    }
-                    for (; skip > 0; --skip) x &= x - 1;
-                    from = d.before + j + __builtin_ctzll(x);
-                    break;
-                }
-            }
-        }
+        static_assert((T::kAlone ? 32 : T::kRows) * T::kPitchK <= (T::kAlone ? T::kBuffer : T::kLds));
+        Sight sight = sight_of(a, d, mine_row, 0);
+        if (a.window) sight.from = window_from(a, d, sight);
+        if (wt == 0 && half == 0) row_from[32 * wr + l32] = sight.from;
         // tiles from here on are seen by all rows as far as they lie before the draft
-        const int all_from = a.window ? max(d.before - a.window + min(drafted, a.window), 0) : 0;
-        auto visible = [&](int t0) {                         // bit i: token t0 + i
-            const int j0 = t0 - d.before;
-            uint32_t m = low_bits(-j0);
-            if (j0 > -32 && drafted > 0) {
-                if (bits) {
-                    const int j = max(j0, 0);
-                    uint64_t x = 0;
-                    if (j < counted) {
-                        x = (uint64_t)bits[j >> 6] >> (j & 63);
-                        if ((j & 63) > 32 && (j >> 6) + 1 < a.words) x |= (uint64_t)bits[(j >> 6) + 1] << (64 - (j & 63));
-                    }
-                    m |= j0 >= 0 ? (uint32_t)x : (uint32_t)x << -j0;
-                    m &= low_bits(counted - j0);
-                } else {
-                    m |= low_bits(chain - j0);
-                }
-            }
-            m &= low_bits(d.end - t0) & ~low_bits(from - t0);
-            return mine_row.there ? m : 0u;
-        };
-
-        // Places of a tile's tokens: lane i has that of token i, and hands it to those that load the token.  Tokens that are not there, or
-        // whose page number is outside the cache, have none: their keys are NaN (which is the result of rows that see them), their values zeros.
-        const int mine_at = T::kAlone ? lane & (T::kStaged - 1) : lane;
-        auto first_of = [&](int i) { return d.start + i * T::kTokens + (T::kAlone ? wave * T::kMine : 0); };
-        auto look_up = [&](int i) {
-            const int64_t t = (int64_t)d.start + (int64_t)i * T::kTokens + (T::kAlone ? wave * T::kMine : 0) + mine_at;
-            return i < last && t < d.end ? row[a.page.div((uint32_t)t)] : -1;
-        };
-        uint32_t kx[kPasses][4], vx[kPasses][4];
-        uint32_t missing = 0;                                // bit p: the token of pass p is not there
-        auto load = [&](int i, int32_t page) {
-            const uint32_t t = (uint32_t)(first_of(i) + mine_at), in = t - a.page.div(t) * a.page.d;
-            const bool none = (uint32_t)page >= (uint32_t)a.pages;
-            const int64_t k_at = none ? -1 : (int64_t)page * a.k.page_bytes + (int64_t)in * a.k.token_bytes;
-            const int64_t v_at = none ? -1 : (int64_t)page * a.v.page_bytes + (int64_t)in * a.v.token_bytes;
-            missing = 0;
+        const int all_from = a.window ? max(d.before - a.window + min(d.end - d.before, a.window), 0) : 0;
+        auto hidden = [&](uint32_t t) { return t + T::kStaged > (uint32_t)d.before || t < (uint32_t)all_from; };        // staged tokens from t on: not all rows see all
+        if (!T::kAlone) tree_barrier();
+        u32x4 q[KS];
 #pragma unroll
-            for (int p = 0; p < kPasses; ++p) {
-                const int64_t ko = shuffle64(k_at, p * kAtOnce + line), vo = shuffle64(v_at, p * kAtOnce + line);
-                missing |= ko < 0 ? 1u << p : 0u;
-                if (has_piece) {
-                    // (a.q: somewhere that can be read)
-                    const char *const kp = ko < 0 ? a.q : kbase + ko, *const vp = ko < 0 ? a.q : vbase + vo;
-                    if (ANY) {
-                        if (row_bytes >= 16) {
-                            const int b = min(16 * piece, row_bytes - 16);
-                            load_stream<4>(kx[p], kp + b);
-                            load_stream<4>(vx[p], vp + b);
-                        } else {
-                            load_part<4>(kx[p], kp, row_bytes);
-                            load_part<4>(vx[p], vp, row_bytes);
-                        }
-                    } else {
-                        load_stream<4>(kx[p], kp + 16 * piece);
-                        load_stream<4>(vx[p], vp + 16 * piece);
-                    }
-                }
-            }
-        };
-        auto put = [&](char *to, const uint32_t (&x)[4]) {   // a piece into LDS, in 16 bits
-            if (F8) {
-                const uint32_t y[8] = {tree_widen<DT, false>(x[0]), tree_widen<DT, true>(x[0]), tree_widen<DT, false>(x[1]), tree_widen<DT, true>(x[1]),
-                                       tree_widen<DT, false>(x[2]), tree_widen<DT, true>(x[2]), tree_widen<DT, false>(x[3]), tree_widen<DT, true>(x[3])};
-                *(u32x4 *)to = u32x4{y[0], y[1], y[2], y[3]};
-                *(u32x4 *)(to + 16) = u32x4{y[4], y[5], y[6], y[7]};
-            } else {
-                *(u32x4 *)to = u32x4{x[0], x[1], x[2], x[3]};
-            }
-        };
-        // a tile that not all rows see all of
-        auto partial = [&](int i) { return first_of(i) + T::kStaged > d.before || first_of(i) < all_from; };
-        auto write = [&](int i, char *buf, int slot) {
-            char *const kt = buf + line * T::kPitchK + (F8 ? 32 : 16) * piece, *const vt = buf + T::kStaged * T::kPitchK + line * T::kPitchV + (F8 ? 32 : 16) * piece;
-            if (ANY && row_bytes >= 16 && 16 * piece + 16 > row_bytes && has_piece) {
-                const int past = 16 * piece - (row_bytes - 16);
-#pragma unroll
-                for (int p = 0; p < kPasses; ++p) { tree_shift(kx[p], past); tree_shift(vx[p], past); }
-            }
-            if (__any(missing)) {
-                // (a NaN in either type; behind the row's end zeros stay zeros, so that the queries' zeros there make none)
-#pragma unroll
-                for (int p = 0; p < kPasses; ++p)
-                    if (missing >> p & 1) {
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const int bytes = row_bytes - 16 * piece - 4 * x;
-                            const uint32_t keep = bytes >= 4 ? 0xffffffffu : bytes <= 0 ? 0u : (1u << (8 * bytes)) - 1u;
-                            kx[p][x] = (F8 ? 0x7f7f7f7fu : 0x7fff7fffu) & keep;
-                            vx[p][x] = 0u;
-                        }
-                    }
-            }
-            if (partial(i)) {
-                bool not_finite = false;
-                if (has_piece)
-#pragma unroll
-                    for (int p = 0; p < kPasses; ++p)
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const uint32_t y = vx[p][x];
-                            constexpr int kWidth = F8 ? 8 : 16;
-                            constexpr uint32_t kTop = F8 ? 0x7fu : E::kExponent, kAll = F8 ? 0xffu : 0xffffu;
-#pragma unroll
-                            for (int b = 0; b < 32; b += kWidth)
-                                if ((y >> b & kTop) == kTop) {
-                                    not_finite = true;
-                                    vx[p][x] &= ~(kAll << b);
-                                }
-                        }
-                if (__any(not_finite) && lane == 0) odd[slot] = number + 1;
-            }
-            if (has_piece)
-#pragma unroll
-                for (int p = 0; p < kPasses; ++p) {
-                    put(kt + p * kAtOnce * T::kPitchK, kx[p]);
-                    put(vt + p * kAtOnce * T::kPitchV, vx[p]);
-                }
-        };
+        for (int k = 0; k < KS; ++k) q[k] = *(const u32x4 *)(ours + (T::kAlone ? l32 : 32 * wr + l32) * T::kPitchK + 32 * k + 16 * half);
+        if (!T::kAlone) tree_barrier();
 
         const float to_log2 = a.scale * kLog2e * (F8 ? a.k.scale[h] : 1.f);
         f32x16 o[DB];
@@ -544,9 +444,110 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
             for (int i = 0; i < 16; ++i) o[j][i] = 0.f;
         float m = -INFINITY, l = 0.f;
 
-        auto attend = [&](int i, const char *buf, int slot) {
-            const char *const kt = buf + (T::kAlone ? 0 : wt * T::kMine) * T::kPitchK + l32 * T::kPitchK + 16 * half;
-            const int t0 = first_of(i) + (T::kAlone ? 0 : wt * T::kMine);
+        // ---- tiles.  While one is worked on, the next one's rows are on their way, and the page numbers of the one behind it.
+        uint32_t kx[kPasses][4], vx[kPasses][4];
+        if (!has_piece)                                      // dimensions behind the rows' end
+#pragma unroll
+            for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) kx[p][x] = vx[p][x] = 0;
+        uint32_t missing = 0;                                // bit p: the token of pass p is not there
+        auto first_of = [&](int i) { return (uint32_t)d.start + (uint32_t)i * T::kTokens + (T::kAlone ? wave * T::kMine : 0); };
+        // Lane i looks after token i of what its wavefront or workgroup stages.
+        const int mine_at = lane & (T::kStaged - 1);
+        auto look_up = [&](int i) {
+            const uint32_t t = first_of(i) + (uint32_t)mine_at;
+            return i < last && t < (uint32_t)d.end ? row[a.page.div(t)] : -1;
+        };
+        int32_t page = look_up(tile);
+        for (int i = tile - 1; i < last; ++i) {
+            char *const buf = ours + (T::kAlone ? 0 : (i & 1) * T::kBuffer);
+            if (i >= tile) {
+                // -- the tile's rows, which have arrived, into LDS, in 16 bits
+                if (ANY && 16 * piece + 16 > row_bytes && has_piece && row_bytes >= 16) {
+                    const int past = 16 * piece - (row_bytes - 16);
+#pragma unroll
+                    for (int p = 0; p < kPasses; ++p) { tree_shift(kx[p], past); tree_shift(vx[p], past); }
+                }
+                if (__any(missing)) {
+                    // Tokens that are not there, or on a page outside the cache: values of zero; keys of NaN, which is the result of a row that
+                    // sees them (zeros behind the row's end: the queries' zeros there would make NaN of those as well).
+#pragma unroll
+                    for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const int bytes = ANY ? row_bytes - 16 * piece - 4 * x : 4;
+                            const uint32_t nan = (F8 ? 0x7f7f7f7fu : 0x7fff7fffu) & (bytes >= 4 ? 0xffffffffu : bytes <= 0 ? 0u : (1u << (8 * bytes)) - 1u);
+                            const bool none = missing >> p & 1;
+                            kx[p][x] = none && has_piece ? nan : kx[p][x];
+                            vx[p][x] = none ? 0u : vx[p][x];
+                        }
+                }
+                if (hidden(first_of(i))) {
+                    // Values that are not finite where not every row sees every token: a probability of 0 times them would be NaN.  They take part
+                    // as zeros, and rows that see them get them at the unit's end.
+                    constexpr int kWidth = F8 ? 8 : 16;
+                    constexpr uint32_t kTop = F8 ? 0x7fu : E::kExponent, kAll = F8 ? 0xffu : 0xffffu;
+                    bool found = false;
+#pragma unroll
+                    for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+#pragma unroll
+                            for (int b = 0; b < 32; b += kWidth) {
+                                const bool hit = (vx[p][x] >> b & kTop) == kTop;
+                                found |= hit;
+                                vx[p][x] &= hit ? ~(kAll << b) : 0xffffffffu;
+                            }
+                    if (found && has_piece) odd = 1;
+                }
+                char *const kt = buf + line * T::kPitchK + (F8 ? 32 : 16) * piece, *const vt = buf + T::kStaged * T::kPitchK + line * T::kPitchV + (F8 ? 32 : 16) * piece;
+                auto put = [&](char *to, const uint32_t (&x)[4]) {
+                    if (F8) {
+                        *(u32x4 *)to = u32x4{tree_widen<DT, false>(x[0]), tree_widen<DT, true>(x[0]), tree_widen<DT, false>(x[1]), tree_widen<DT, true>(x[1])};
+                        *(u32x4 *)(to + 16) = u32x4{tree_widen<DT, false>(x[2]), tree_widen<DT, true>(x[2]), tree_widen<DT, false>(x[3]), tree_widen<DT, true>(x[3])};
+                    } else {
+                        *(u32x4 *)to = u32x4{x[0], x[1], x[2], x[3]};
+                    }
+                };
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p) {
+                    put(kt + p * kAtOnce * T::kPitchK, kx[p]);
+                    put(vt + p * kAtOnce * T::kPitchV, vx[p]);
+                }
+            }
+            if (i + 1 < last) {
+                // -- the next tile's rows, where their pages are; the lane that looks after a token hands its place to those that load it
+                const uint32_t t = first_of(i + 1) + (uint32_t)mine_at, in = t - a.page.div(t) * a.page.d;
+                const bool none = (uint32_t)page >= (uint32_t)a.pages;
+                const int64_t k_at = none ? -1 : (int64_t)page * a.k.page_bytes + (int64_t)in * a.k.token_bytes;
+                const int64_t v_at = none ? -1 : (int64_t)page * a.v.page_bytes + (int64_t)in * a.v.token_bytes;
+                missing = 0;
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p) {
+                    const int64_t ko = shuffle64(k_at, p * kAtOnce + line), vo = shuffle64(v_at, p * kAtOnce + line);
+                    missing |= ko < 0 ? 1u << p : 0u;
+                    // (a.q: somewhere that can be read)
+                    const char *const kp = ko < 0 ? a.q : kbase + ko, *const vp = ko < 0 ? a.q : vbase + vo;
+                    if (has_piece) {
+                        if (ANY && row_bytes < 16) {
+                            load_part<4>(kx[p], kp, row_bytes);
+                            load_part<4>(vx[p], vp, row_bytes);
+                        } else {
+                            const int b = ANY ? min(16 * piece, row_bytes - 16) : 16 * piece;
+                            load_stream<4>(kx[p], kp + b);
+                            load_stream<4>(vx[p], vp + b);
+                        }
+                    }
+                }
+                page = look_up(i + 2);
+            }
+            if (i < tile) continue;
+            if (!T::kAlone) tree_barrier();
+
+            // -- scores of tokens t0 + 32 u + 8 (x / 4) + 4 half + x % 4
+            const uint32_t t0 = first_of(i) + (T::kAlone ? 0 : wt * T::kMine);
+            const char *const kt = buf + ((T::kAlone ? 0 : wt * T::kMine) + l32) * T::kPitchK + 16 * half;
             f32x16 s[SUBS];
 #pragma unroll
             for (int u = 0; u < SUBS; ++u) {
@@ -555,18 +556,14 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
 #pragma unroll
                 for (int k = 0; k < KS; ++k) s[u] = E::mfma(*(const u32x4 *)(kt + 32 * u * T::kPitchK + 32 * k), q[k], s[u]);
             }
-            // scores of tokens t0 + 32 u + 8 (x / 4) + 4 half + x % 4
 #pragma unroll
             for (int u = 0; u < SUBS; ++u) s[u] *= to_log2;
-            const bool some_hidden = partial(i);
-            uint32_t see[SUBS];
-            if (some_hidden) {
+            if (hidden(first_of(i))) {
+                const uint64_t see = sight(d, a.words, t0) >> (4 * half);
 #pragma unroll
-                for (int u = 0; u < SUBS; ++u) {
-                    see[u] = visible(t0 + 32 * u) >> (4 * half);
+                for (int u = 0; u < SUBS; ++u)
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) s[u][x] = see[u] >> (8 * (x / 4) + x % 4) & 1 ? s[u][x] : -INFINITY;
-                }
+                    for (int x = 0; x < 16; ++x) s[u][x] = (uint32_t)(see >> (32 * u)) >> (8 * (x / 4) + x % 4) & 1 ? s[u][x] : -INFINITY;
             }
             float top = m;
 #pragma unroll
@@ -575,7 +572,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
                 for (int x = 0; x < 16; ++x) top = fmaxf(top, s[u][x]);
             top = pair_max(top);
             if (__any(top > m + kTreeLag)) {                 // (also the first that is seen: m is -inf)
-                const float base = top == -INFINITY ? 0.f : top, shrink = __builtin_amdgcn_exp2f(m - base);
+                const float shrink = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
                 l *= shrink;
 #pragma unroll
                 for (int j = 0; j < DB; ++j) o[j] *= shrink;
@@ -591,68 +588,26 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
                     l += p0 + p1;
                     p[2 * u + x / 8][x % 8 / 2] = Elem<DT>::pack2(p0, p1);
                 }
-            // ---- values: lane (dimension 32 j + l32, half) has tokens 16 k + 4 half + 0 .. 3 and 8 behind those
-            const char *const vt = buf + T::kStaged * T::kPitchK + ((T::kAlone ? 0 : wt * T::kMine) + 4 * half + (lane & 15) / 4) * T::kPitchV + 32 * (lane >> 4 & 1) + 8 * (lane & 3);
-            auto values = [&](int k, int j) {
-                const LdsPtr at = (LdsPtr)const_cast<char *>(vt) + 16 * k * T::kPitchV + 64 * j;
-                const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPiece)at));
-                const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPiece)(at + 8 * T::kPitchV)));
-                return u32x4{lo[0], lo[1], hi[0], hi[1]};
-            };
+            // -- values: lane (dimension 32 j + l32, half) has tokens 16 k + 4 half + 0 .. 3 and 8 behind those
+            const LdsPtr vt = (LdsPtr)(buf + T::kStaged * T::kPitchK) + ((T::kAlone ? 0 : wt * T::kMine) + 4 * half + (lane & 15) / 4) * T::kPitchV +
+                              32 * (lane >> 4 & 1) + 8 * (lane & 3);
 #pragma unroll
             for (int k = 0; k < 2 * SUBS; ++k)
 #pragma unroll
-                for (int j = 0; j < DB; ++j) o[j] = E::mfma(values(k, j), p[k], o[j]);
-            // Values that are not finite, in a tile of which not every row sees every token, are zeros in LDS (a probability of 0 times them would
-            // be NaN); rows that see them get them here, as they are: an infinity or NaN of any size is the same.
-            if (some_hidden && odd[slot] == number + 1) {
-#pragma nounroll
-                for (int t = t0; t < min(t0 + T::kMine, d.end); ++t) {
-                    const uint32_t page = (uint32_t)row[a.page.div((uint32_t)t)];
-                    if (page >= (uint32_t)a.pages) continue;
-                    const char *const v = vbase + page * a.v.page_bytes + (int64_t)((uint32_t)t - a.page.div((uint32_t)t) * a.page.d) * a.v.token_bytes;
-                    const bool sees = (visible(t) & 1) != 0;
-#pragma unroll
-                    for (int j = 0; j < DB; ++j)
-#pragma unroll
-                        for (int x = 0; x < 16; ++x) {
-                            const int dim = 32 * j + 8 * (x / 4) + 4 * half + x % 4, in = min(dim, a.dim - 1);      // (behind the end: not stored)
-                            const uint32_t y = F8 ? ((const uint8_t *)v)[in] : ((const u16_any *)v)[in];
-                            const bool hit = F8 ? (y & 0x7f) == 0x7f : (y & E::kExponent) == E::kExponent;
-                            const float add = sees && hit ? (F8 ? NAN : Elem<DT>::to_float((uint16_t)y)) : 0.f;
-                            o[j][x] += add;
-                        }
+                for (int j = 0; j < DB; ++j) {
+                    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPiece)(vt + 16 * k * T::kPitchV + 64 * j)));
+                    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPiece)(vt + (16 * k + 8) * T::kPitchV + 64 * j)));
+                    o[j] = E::mfma(u32x4{lo[0], lo[1], hi[0], hi[1]}, p[k], o[j]);
                 }
-            }
-        };
-
-        // ---- tiles: while one is worked on the next one's rows are on their way, and the page numbers of the one behind it
-        int32_t page_next;
-        {
-            const int32_t page = look_up(tile);
-            page_next = look_up(tile + 1);
-            load(tile, page);
-        }
-        for (int i = tile; i < last; ++i, ++number) {
-            const int slot = T::kAlone ? wave : number & 1;
-            char *const buf = ours + (T::kAlone ? 0 : (number & 1) * T::kBuffer);
-            write(i, buf, slot);
-            if (i + 1 < last) {
-                load(i + 1, page_next);
-                page_next = look_up(i + 2);
-            }
-            if (!T::kAlone) tree_barrier();
-            attend(i, buf, slot);
         }
         l = pair_sum(l);
 
         // ---- the unit's end: join the wavefronts, give out the result or leave a part
         const bool begun = tile == 0, done = last == d.tiles, whole = begun && done;
-        const int part_slot = 2 * (int)group + (begun ? 1 : 0);
+        const int part_slot = 2 * group + (begun ? 1 : 0);
         const float v_scale = F8 ? a.v.scale[h] : 1.f;
         const TreeShared<T::kRows> shared(w);
-        if (T::kGroups == 1) {
-            const int x = 32 * wr + l32;
+        if constexpr (T::kGroups == 1) {
             if (mine_row.there) {
 #pragma unroll
                 for (int j = 0; j < DB; ++j)
@@ -661,14 +616,15 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
                         const int dim0 = 32 * j + 8 * g + 4 * half;
                         const f32x4 acc = {o[j][4 * g], o[j][4 * g + 1], o[j][4 * g + 2], o[j][4 * g + 3]};
                         if (whole) tree_result<DT>(a, d, mine_row, dim0, acc, l, v_scale);
-                        else if (dim0 < a.dim) shared.store(part_slot, x, dim0, acc);
+                        else if (dim0 < a.dim) shared.store(part_slot, 32 * wr + l32, dim0, acc);
                     }
-                if (!whole && half == 0) shared.store(part_slot, x, TreePart{m, l});
+                if (!whole && half == 0) shared.store(part_slot, 32 * wr + l32, TreePart{m, l});
             }
         } else {
             if (!T::kAlone) tree_barrier();                  // (else a wavefront's part lies where its own tokens did)
-            float *const mineo = (float *)(T::kAlone ? ours : lds + wave * 32 * T::kPitchO * 4) + l32 * T::kPitchO;
-            static_assert(32 * T::kPitchO * 4 <= (T::kAlone ? T::kBuffer : T::kLds / kTreeWaves));
+            constexpr int kPart = T::kAlone ? T::kBuffer : 32 * T::kPitchO * 4;
+            static_assert(32 * T::kPitchO * 4 <= kPart && kTreeWaves * kPart <= T::kLds);
+            float *const mineo = (float *)(lds + wave * kPart) + l32 * T::kPitchO;
             if (half == 0) { wave_m[wave][l32] = m; wave_l[wave][l32] = l; }
 #pragma unroll
             for (int j = 0; j < DB; ++j)
@@ -690,7 +646,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
                     const int v = i * WR + x / 32;
                     const float f = __builtin_amdgcn_exp2f(wave_m[v][x % 32] - base);
                     sum += f * wave_l[v][x % 32];
-                    acc += f * *(const f32x4 *)((const float *)(lds + v * (T::kAlone ? T::kBuffer : 32 * T::kPitchO * 4)) + (x % 32) * T::kPitchO + dim0);
+                    acc += f * *(const f32x4 *)((const float *)(lds + v * kPart) + (x % 32) * T::kPitchO + dim0);
                 }
                 if (whole) {
                     tree_result<DT>(a, d, t, dim0, acc, sum, v_scale);
@@ -700,10 +656,39 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
                 }
             }
         }
+        tree_barrier();
+        if (odd) {
+            // Values that are not finite, for the rows that see them: an infinity or a NaN of whatever weight is the result's.
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            for (int e = (int)threadIdx.x; e < T::kRows * a.dim; e += kTreeThreads) {
+                const int x = e / a.dim, dim = e - x * a.dim;
+                const TreeRow t = tree_row(a, w, d, h, (int64_t)block * T::kRows + x);
+                const Sight s = sight_of(a, d, t, row_from[x]);
+                float add = 0.f;
+                const uint32_t t_end = (uint32_t)min((int64_t)d.end, (int64_t)d.start + (int64_t)last * T::kTokens);
+#pragma nounroll
+                for (uint32_t tok = (uint32_t)d.start + (uint32_t)tile * T::kTokens; tok < t_end; ++tok) {
+                    if (!hidden(tok & ~(uint32_t)(T::kStaged - 1)) || !(s(d, a.words, tok) & 1)) continue;
+                    const uint32_t at_page = a.page.div(tok);
+                    const int32_t number = row[at_page];
+                    if ((uint32_t)number >= (uint32_t)a.pages) continue;
+                    const char *const v = vbase + number * a.v.page_bytes + (int64_t)(tok - at_page * a.page.d) * a.v.token_bytes + EB * dim;
+                    const uint32_t y = F8 ? *(const uint8_t *)v : *(const u16_any *)v;
+                    if (F8 ? (y & 0x7f) == 0x7f : (y & E::kExponent) == E::kExponent) add += F8 ? NAN : Elem<DT>::to_float((uint16_t)y);
+                }
+                if (t.there && add != 0.f) {
+                    if (whole) ((u16_any *)(a.out + t.head * a.out_head_bytes + (int64_t)(d.row0 + t.node) * a.out_row_bytes))[dim] = Elem<DT>::from_float(add);
+                    else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, add), shared.sums, shared.sum_at(part_slot, x, dim), 0, kTreeAux);
+                }
+            }
+            __syncthreads();
+            if (threadIdx.x == 0) odd = 0;
+        }
         if (!whole) {
             const int64_t first = at - tile;
-            TreeLeft u = {begun ? (int)group : (int)tree_scaled_up(first + 1, groups, total) - 1, 0, request, h, block};
-            u.parts = (int)tree_scaled_up(first + d.tiles, groups, total) - u.begins;
+            TreeLeft u = {begun ? group : (int)tree_ratio_up(first + 1, groups, total) - 1, 0, request, h, block};
+            u.parts = (int)tree_ratio_up(first + d.tiles, groups, total) - u.begins;
             if (w.left) {
                 if (begun && threadIdx.x == 0) w.left[group] = u;
             } else {
@@ -717,15 +702,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
             unit = 0;
             ++request;
         }
-        if (at < end) {
-            tree_barrier();
-            // (what the joining has put over the dimensions that no load fills)
-            if (T::kGroups > 1 && 16 * kPieces > row_bytes) {
-                for (int b = 0; b < (T::kAlone ? 1 : T::kBuffers); ++b)
-                    for (int x = 16 * loader; x < T::kBuffer; x += 16 * kLoaders) *(u32x4 *)(ours + b * T::kBuffer + x) = u32x4{0u, 0u, 0u, 0u};
-                if (!T::kAlone) tree_barrier();
-            }
-        }
+        tree_barrier();
     }
     if (w.left || unfinished == 0) return;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -737,6 +714,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
             if (joins[i]) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
     __syncthreads();
+#pragma nounroll
     for (int i = 0; i < unfinished; ++i)
         if (joins[i]) tree_join<DT, DC, WR>(a, w, left[i], 0, T::kRows, F8 ? a.v.scale[left[i].h] : 1.f);
 }
