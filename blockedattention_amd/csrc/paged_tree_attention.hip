@@ -48,7 +48,7 @@ int launch_paged_tree_attention(const PagedTreeAttentionArgs &a, int dtype, int 
     TreeWork w = tree_work(a.heads, a.group, a.dim, a.tokens, a.requests, a.width, a.page.d, a.window, workspace, nullptr);
     w.counters = counters;
     // Joining within the kernel saves the second launch, but one workgroup then reads all parts of a unit.
-    if (w.groups <= kTreeFewParts * std::max<int64_t>(1, a.tokens * a.group / (32 * waves)) * a.heads) w.left = nullptr;
+    if (waves == 1 && w.groups <= kTreeFewParts * std::max<int64_t>(1, a.tokens * a.group / (32 * waves)) * a.heads) w.left = nullptr;
     const uint64_t bits = (uint64_t)a.k.base | (uint64_t)a.v.base | (uint64_t)a.k.page_bytes | (uint64_t)a.v.page_bytes | (uint64_t)a.k.head_bytes |
                           (uint64_t)a.v.head_bytes | (uint64_t)a.k.token_bytes | (uint64_t)a.v.token_bytes;
     const bool any = bits % 16 != 0 || a.dim % (f8 ? 16 : 8) != 0;

@@ -21,7 +21,8 @@ typedef __attribute__((address_space(3))) s16x4 *LdsPiece;
 
 constexpr int kTreeWaves = 4;
 constexpr int kTreeThreads = 64 * kTreeWaves;
-constexpr int kTreeShare = 2;                // tiles of a workgroup at least, unless units are shorter
+constexpr int kTreeUnit = 3;                 // what a unit costs besides its tiles, in tiles: queries, first loads, joining, results
+constexpr int kTreeShare = 5;                // of both, what a workgroup has at least, unless units are shorter
 constexpr int kTreeWhole = 4;                // units of up to so many tiles are not split between workgroups
 constexpr int kTreeFewParts = 8;             // parts of a unit, on the average, up to which the kernel itself joins them
 
@@ -39,7 +40,6 @@ template <int DC, int WR> struct TreeTile {
     static constexpr int kStaged = kAlone ? kMine : kTokens;              // tokens that are loaded together
     static constexpr int kBuffer = kStaged * (kPitchK + kPitchV);
     static constexpr int kLds = (kAlone ? kTreeWaves : kBuffers) * kBuffer;
-    static constexpr int kPitchO = DC + 4;                                // floats between rows where wavefronts are joined
     static constexpr int kResident = DC == 64 ? 3 : DC == 128 ? 2 : 1;    // workgroups of a compute unit, by LDS and registers
 };
 
@@ -58,6 +58,18 @@ struct TreeWork {
     PageDiv group;                           // query heads of a key head
     int32_t groups, pitch;
 };
+
+struct TreeArgs {
+    PagedTreeAttentionArgs a;
+    TreeWork w;
+};
+// The kernel's arguments, fetched again.  Held in scalar registers from the start they, and what is derived from them, are twice what there is; the
+// compiler then moves whole groups of them to and from vector registers within the loop over tiles (ELSEWHERE us).
+__device__ __forceinline__ const TreeArgs &tree_args() {
+    auto p = (const __attribute__((address_space(4))) TreeArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const TreeArgs *)p;
+}
 
 // A request's draft.
 struct Draft {
@@ -156,47 +168,63 @@ __device__ __forceinline__ void tree_result(const PagedTreeAttentionArgs &a, con
     tree_store<DT>(a.out + t.head * a.out_head_bytes + (int64_t)(d.row0 + t.node) * a.out_row_bytes, dim0, a.dim, acc * f);
 }
 
-// Joins the parts of a unit for its rows [row0, row1), by a whole workgroup: DC / 4 threads a row.
+// Joins the parts of a unit for its rows [row0, row1), by a whole workgroup: DC / 4 threads a row, kDeep rows of a thread and four parts of
+// each on their way together (a load from where all dies meet takes some 2 us, however many there are).
 template <int DT, int DC, int WR>
 __device__ __forceinline__ void tree_join(const PagedTreeAttentionArgs &a, const TreeWork &w, const TreeLeft &u, int row0, int row1, float v_scale) {
     typedef TreeTile<DC, WR> T;
-    constexpr int kLanes = DC / 4, kAtOnce = kTreeThreads / kLanes, kAhead = 8;
+    constexpr int kLanes = DC / 4, kAtOnce = kTreeThreads / kLanes, kAhead = 4, kDeep = 4;
     const Draft d = draft_of<DC, WR, false>(a, u.request);
     const TreeShared<T::kRows> shared(w);
     const int dim0 = 4 * ((int)threadIdx.x % kLanes);
-    for (int x = row0 + (int)threadIdx.x / kLanes; x < row1; x += kAtOnce) {
-        const TreeRow t = tree_row(a, w, d, u.h, (int64_t)u.block * T::kRows + x);
-        if (!t.there || dim0 >= a.dim) continue;
-        float m = -INFINITY, l = 0.f;
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    const int rows = (int)min((int64_t)row1, (int64_t)d.rows * a.group - (int64_t)u.block * T::kRows);
+#pragma nounroll
+    for (int x0 = row0 + (int)threadIdx.x / kLanes; x0 < rows; x0 += kDeep * kAtOnce) {
+        float m[kDeep], l[kDeep];
+        f32x4 acc[kDeep];
+#pragma unroll
+        for (int z = 0; z < kDeep; ++z) {
+            m[z] = -INFINITY;
+            l[z] = 0.f;
+            acc[z] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+#pragma nounroll
         for (int p0 = 0; p0 < u.parts; p0 += kAhead) {
-            TreePart part[kAhead];
-            f32x4 sum[kAhead];
+            TreePart part[kDeep][kAhead];
+            f32x4 sum[kDeep][kAhead];
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
-                part[i] = {-INFINITY, 0.f};
-                sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (p0 + i < u.parts) {
-                    const int slot = 2 * (u.begins + p0 + i) + (p0 + i == 0 ? 1 : 0);
-                    part[i] = shared.part(slot, x);
-                    sum[i] = shared.sum(slot, x, dim0);
+                const int p = min(p0 + i, u.parts - 1), slot = 2 * (u.begins + p) + (p == 0 ? 1 : 0);
+#pragma unroll
+                for (int z = 0; z < kDeep; ++z) {
+                    const int x = min(x0 + z * kAtOnce, rows - 1);       // (what is there already once more, and not used)
+                    part[z][i] = shared.part(slot, x);
+                    sum[z][i] = shared.sum(slot, x, min(dim0, w.pitch - 4));
                 }
             }
-            float top = m;
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) top = fmaxf(top, part[i].m);
-            const float base = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f(m - base);
-            l *= old;
-            acc *= old;
-            m = top;
+            for (int z = 0; z < kDeep; ++z) {
+                float top = m[z];
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                const float f = __builtin_amdgcn_exp2f(part[i].m - base);
-                l += f * part[i].l;
-                acc += f * sum[i];
+                for (int i = 0; i < kAhead; ++i) {
+                    if (p0 + i >= u.parts) part[z][i] = {-INFINITY, 0.f};
+                    top = fmaxf(top, part[z][i].m);
+                }
+                const float base = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f(m[z] - base);
+                l[z] *= old;
+                acc[z] *= old;
+                m[z] = top;
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    const float f = __builtin_amdgcn_exp2f(part[z][i].m - base);
+                    l[z] += f * part[z][i].l;
+                    if (p0 + i < u.parts) acc[z] += f * sum[z][i];
+                }
             }
         }
-        tree_result<DT>(a, d, t, dim0, acc, l, v_scale);
+#pragma unroll
+        for (int z = 0; z < kDeep; ++z)
+            if (const int x = x0 + z * kAtOnce; x < rows) tree_result<DT>(a, d, tree_row(a, w, d, u.h, (int64_t)u.block * T::kRows + x), dim0, acc[z], l[z], v_scale);
     }
 }
 
@@ -308,7 +336,7 @@ __device__ __forceinline__ int window_from(const PagedTreeAttentionArgs &a, cons
 
 // DC: dimensions that the registers hold (64, 128, 256).  ANY: rows at any address.
 template <int DT, bool F8, int DC, int WR, bool ANY>
-__global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) paged_tree_attention_kernel(PagedTreeAttentionArgs a, TreeWork w) {
+__global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) paged_tree_attention_kernel(TreeArgs) {
     typedef TreeTile<DC, WR> T;
     typedef TreeElem<DT> E;
     constexpr int EB = F8 ? 1 : 2, kPieces = DC * EB / 16;   // bytes of an element, 16-byte pieces of a row
@@ -323,18 +351,22 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
         int64_t at;
     };
     __shared__ Place places[2];
-    __shared__ int64_t scan[2 * kTreeWaves];
+    __shared__ int64_t scan[2 * kTreeWaves], dealt[2];       // (dealt: tiles, workgroups that have some)
     __shared__ float wave_m[kTreeWaves][32], wave_l[kTreeWaves][32];
     __shared__ TreeLeft left[2];
     __shared__ int32_t joins[2], row_from[T::kRows], odd;    // odd: whether a part's hidden tiles have values that are not finite
-    int unfinished = 0;
+    __shared__ int64_t spots[kTreeWaves][2][64];             // where the tokens that a wavefront looks after lie, of keys and values
+    int unfinished = 0, group;
 
+    {
+    const PagedTreeAttentionArgs &a = tree_args().a;
+    const TreeWork &w = tree_args().w;
     // ---- the share: tiles of all units in the order of requests, key heads, blocks of rows.  Thread i adds up requests [i c, (i + 1) c).
     const int c = (a.requests + kTreeThreads - 1) / kTreeThreads, r0 = (int)threadIdx.x * c, r1 = min(a.requests, r0 + c);
     int64_t mine = 0, units = 0;
     for (int r = r0; r < r1; ++r) {
         const Draft d = draft_of<DC, WR, false>(a, r);
-        mine += (int64_t)a.heads * d.blocks * d.tiles;
+        mine += (int64_t)a.heads * d.blocks * (d.tiles + kTreeUnit);
         units += (int64_t)a.heads * d.blocks;
     }
     int64_t upto = wave_inclusive_scan(mine);
@@ -352,7 +384,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
     }
     total = uniform64(total);
     const int64_t groups = uniform64(min((int64_t)w.groups, max((total + kTreeShare - 1) / kTreeShare, units)));
-    const int group = (int)blockIdx.x;
+    group = (int)blockIdx.x;
     if (w.left && threadIdx.x == 0) w.left[group].parts = 0;
     // rows of no request: zeros
     {
@@ -367,25 +399,29 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
         }
     }
     if (group >= groups) return;
+    if (threadIdx.x == 0) { dealt[0] = total; dealt[1] = groups; }
 #pragma nounroll
     for (int k = 0; k < 2; ++k) {
         int64_t at = tree_ratio(group + k, total, groups);
         if (at >= total) {
-            if (threadIdx.x == 0) places[k] = {a.requests, 0, 0, total};
+            if (threadIdx.x == 0) places[k] = {a.requests, 0, 0, total + kTreeUnit};
         } else if (at < upto && at >= upto - mine) {
             int64_t before = upto - mine, all;
             int r = r0 - 1;
             Draft d;
             for (all = 0;; before += all) {
                 d = draft_of<DC, WR, false>(a, ++r);
-                all = (int64_t)a.heads * d.blocks * d.tiles;
+                all = (int64_t)a.heads * d.blocks * (d.tiles + kTreeUnit);
                 if (at < before + all) break;
             }
-            int unit = (int)tree_ratio(at - before, 1, d.tiles), tile = (int)((at - before) - (int64_t)unit * d.tiles);
+            // (a unit's own cost comes before its tiles: what begins within it begins with tile 0)
+            int unit = (int)tree_ratio(at - before, 1, d.tiles + kTreeUnit), tile = (int)((at - before) - (int64_t)unit * (d.tiles + kTreeUnit)) - kTreeUnit;
+            at += max(-tile, 0);
+            tile = max(tile, 0);
             if (d.tiles <= kTreeWhole && tile) {             // short units go where most of them lies
                 at -= tile;
                 if (2 * tile > d.tiles) {
-                    at += d.tiles;
+                    at += d.tiles + kTreeUnit;
                     if (++unit == a.heads * d.blocks) {
                         unit = 0;
                         ++r;
@@ -396,111 +432,302 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
             places[k] = {r, unit, tile, at};
         }
     }
+    }
     __syncthreads();
     const int64_t end = uniform64(places[1].at);
-    int64_t at = uniform64(places[0].at);
-    int request = uniform(places[0].request), unit = uniform(places[0].unit), tile = uniform(places[0].tile);
 
     char *const ours = lds + (T::kAlone ? wave * T::kBuffer : 0);
     const int loader = T::kAlone ? lane : (int)threadIdx.x, piece = loader % kPieces, line = loader / kPieces;
-    const int row_bytes = EB * a.dim;
-    const bool has_piece = 16 * piece < row_bytes;
+    // A unit's part that is this workgroup's: tiles [tile, last); `at`: place of the first one in the order of all.
+    struct Unit {
+        Draft d;
+        int64_t at;
+        int32_t request, unit, tile, last, h, block;
+    };
+    auto unit_of = [&](int request, int unit, int tile, int64_t at) {
+        const PagedTreeAttentionArgs &a = tree_args().a;
+        Unit u;
+        u.d = draft_of<DC, WR, true>(a, request);
+        while (u.d.blocks == 0) u.d = draft_of<DC, WR, true>(a, ++request);
+        u.request = request; u.unit = unit; u.tile = tile; u.at = at;
+        u.h = unit / u.d.blocks;
+        u.block = unit - u.h * u.d.blocks;
+        u.last = (int)min((int64_t)u.d.tiles, tile + (end - at));
+        return u;
+    };
+    auto after = [&](const Unit &u) {                        // the unit behind it, whose first tile lies at ...
+        const bool done = u.unit + 1 == tree_args().a.heads * u.d.blocks;
+        return unit_of(u.request + (done ? 1 : 0), done ? 0 : u.unit + 1, 0, u.at + (u.last - u.tile) + kTreeUnit);
+    };
 
-    while (at < end) {
-        // ---- a unit's part: tiles [tile, last)
-        Draft d = draft_of<DC, WR, true>(a, request);
-        while (d.blocks == 0) d = draft_of<DC, WR, true>(a, ++request);
-        const int h = unit / d.blocks, block = unit - h * d.blocks, last = (int)min((int64_t)d.tiles, tile + (end - at));
-        const int32_t *const row = a.table + request * a.table_stride;
-        const char *const kbase = a.k.base + h * a.k.head_bytes, *const vbase = a.v.base + h * a.v.head_bytes;
-        const TreeRow mine_row = tree_row(a, w, d, h, (int64_t)block * T::kRows + 32 * wr + l32);
-
-        // queries, by way of LDS: column l32 of the scores
-        for (int x = loader; x < (T::kAlone ? 32 : T::kRows) * (DC / 8); x += kLoaders) {
-            const int i = x / (DC / 8), d0 = 8 * (x % (DC / 8));
-            const TreeRow t = tree_row(a, w, d, h, (int64_t)block * T::kRows + i);
-            uint32_t y[4] = {0, 0, 0, 0};
-            if (t.there) load_part<4>(y, a.q + t.head * a.q_head_bytes + (int64_t)(d.row0 + t.node) * a.q_row_bytes + 2 * d0, 2 * (a.dim - d0));
-            *(u32x4 *)(ours + i * T::kPitchK + 2 * d0) = u32x4{y[0], y[1], y[2], y[3]};
-        }
-        static_assert((T::kAlone ? 32 : T::kRows) * T::kPitchK <= (T::kAlone ? T::kBuffer : T::kLds));
-        Sight sight = sight_of(a, d, mine_row, 0);
-        if (a.window) sight.from = window_from(a, d, sight);
-        if (wt == 0 && half == 0) row_from[32 * wr + l32] = sight.from;
-        // tiles from here on are seen by all rows as far as they lie before the draft
-        const int all_from = a.window ? max(d.before - a.window + min(d.end - d.before, a.window), 0) : 0;
-        auto hidden = [&](uint32_t t) { return t + T::kStaged > (uint32_t)d.before || t < (uint32_t)all_from; };        // staged tokens from t on: not all rows see all
-        if (!T::kAlone) tree_barrier();
-        u32x4 q[KS];
+    // ---- rows of keys and values.  Lane i looks after token i of what its wavefront or workgroup stages: it asks for the token's page number, two
+    // tiles ahead, and leaves the place for those that load it, a tile ahead.
+    const int mine_at = lane & (T::kStaged - 1);
+    auto first_of = [&](const Unit &u, int i) { return (uint32_t)u.d.start + (uint32_t)i * T::kTokens + (T::kAlone ? wave * T::kMine : 0); };
+    auto look_up = [&](const Unit &u, const int32_t *row, const PageDiv &page, int i) {
+        const uint32_t t = first_of(u, i) + (uint32_t)mine_at;
+        return i < u.last && t < (uint32_t)u.d.end ? row[page.div(t)] : -1;
+    };
+    auto row_of = [&](const Unit &u) {
+        const PagedTreeAttentionArgs &a = tree_args().a;
+        return (const int32_t *)uniform64((int64_t)(uintptr_t)(a.table + u.request * a.table_stride));
+    };
+    uint32_t kx[kPasses][4], vx[kPasses][4];
+    uint32_t missing = 0;                                    // bit p: the token of pass p is not there
+    auto load = [&](const Unit &u, int i, int32_t number) {
+        const PagedTreeAttentionArgs &a = tree_args().a;
+        const char *const kbase = a.k.base + u.h * a.k.head_bytes, *const vbase = a.v.base + u.h * a.v.head_bytes, *const readable = a.q;
+        const int row_bytes = EB * a.dim;
+        const uint32_t t = first_of(u, i) + (uint32_t)mine_at, in = t - a.page.div(t) * a.page.d;
+        const bool none = (uint32_t)number >= (uint32_t)a.pages, alike = a.k.page_bytes == a.v.page_bytes && a.k.token_bytes == a.v.token_bytes;
+        spots[wave][0][lane] = none ? -1 : (int64_t)number * a.k.page_bytes + (int64_t)in * a.k.token_bytes;
+        if (!alike) spots[wave][1][lane] = none ? -1 : (int64_t)number * a.v.page_bytes + (int64_t)in * a.v.token_bytes;
+        __builtin_amdgcn_wave_barrier();
+        int64_t ko[kPasses], vo[kPasses];
 #pragma unroll
-        for (int k = 0; k < KS; ++k) q[k] = *(const u32x4 *)(ours + (T::kAlone ? l32 : 32 * wr + l32) * T::kPitchK + 32 * k + 16 * half);
-        if (!T::kAlone) tree_barrier();
-
-        const float to_log2 = a.scale * kLog2e * (F8 ? a.k.scale[h] : 1.f);
-        f32x16 o[DB];
+        for (int p = 0; p < kPasses; ++p) vo[p] = ko[p] = spots[wave][0][p * kAtOnce + line];
+        if (!alike)
 #pragma unroll
-        for (int j = 0; j < DB; ++j)
+            for (int p = 0; p < kPasses; ++p) vo[p] = spots[wave][1][p * kAtOnce + line];
+        missing = 0;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[j][i] = 0.f;
-        float m = -INFINITY, l = 0.f;
-
-        // ---- tiles.  While one is worked on, the next one's rows are on their way, and the page numbers of the one behind it.
-        uint32_t kx[kPasses][4], vx[kPasses][4];
-        if (!has_piece)                                      // dimensions behind the rows' end
+        for (int p = 0; p < kPasses; ++p) missing |= ko[p] < 0 ? 1u << p : 0u;
+        if (16 * piece < row_bytes) {
+            const int b = ANY ? max(min(16 * piece, row_bytes - 16), 0) : 16 * piece;
+#pragma unroll
+            for (int p = 0; p < kPasses; ++p) {
+                const char *const kp = (ko[p] < 0 ? readable : kbase + ko[p]) + b, *const vp = (ko[p] < 0 ? readable : vbase + vo[p]) + b;
+                if (ANY && row_bytes < 16) {
+                    load_part<4>(kx[p], kp, row_bytes);
+                    load_part<4>(vx[p], vp, row_bytes);
+                } else {
+                    load_stream<4>(kx[p], kp);
+                    load_stream<4>(vx[p], vp);
+                }
+            }
+        } else {                                             // dimensions behind the rows' end
 #pragma unroll
             for (int p = 0; p < kPasses; ++p)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) kx[p][x] = vx[p][x] = 0;
-        uint32_t missing = 0;                                // bit p: the token of pass p is not there
-        auto first_of = [&](int i) { return (uint32_t)d.start + (uint32_t)i * T::kTokens + (T::kAlone ? wave * T::kMine : 0); };
-        // Lane i looks after token i of what its wavefront or workgroup stages.
-        const int mine_at = lane & (T::kStaged - 1);
-        auto look_up = [&](int i) {
-            const uint32_t t = first_of(i) + (uint32_t)mine_at;
-            return i < last && t < (uint32_t)d.end ? row[a.page.div(t)] : -1;
-        };
-        int32_t page = look_up(tile);
-        for (int i = tile - 1; i < last; ++i) {
-            char *const buf = ours + (T::kAlone ? 0 : (i & 1) * T::kBuffer);
-            if (i >= tile) {
-                // -- the tile's rows, which have arrived, into LDS, in 16 bits
-                if (ANY && 16 * piece + 16 > row_bytes && has_piece && row_bytes >= 16) {
-                    const int past = 16 * piece - (row_bytes - 16);
+        }
+    };
+    // Staged tokens from t on that not all rows see: those of the draft, and where the rows' windows begin.
+    auto hidden = [&](const Draft &d, int window, uint32_t t) {
+        const int all_from = window ? max(d.before - window + min(d.end - d.before, window), 0) : 0;
+        return t + T::kStaged > (uint32_t)d.before || t < (uint32_t)all_from;
+    };
+
+    Unit cur, next = unit_of(uniform(places[0].request), uniform(places[0].unit), uniform(places[0].tile), uniform64(places[0].at));
+    bool begun_any = false, more = next.at < end;
+    int32_t number = -1;
+    if (more) number = look_up(next, row_of(next), tree_args().a.page, next.tile);
+    f32x16 o[DB];
+    float m = -INFINITY, l = 0.f;
+    while (more || begun_any) {
+        // ---- the next unit's first tile and queries are on their way while this one is finished
+        constexpr int kQueries = T::kAlone ? 32 : T::kRows, kEach = kQueries * (DC / 8) / kLoaders;
+        static_assert(kQueries * T::kPitchK <= (T::kAlone ? T::kBuffer : T::kLds) && kQueries * (DC / 8) % kLoaders == 0);
+        u32x4 y[kEach];
+        if (more) {
+            const PagedTreeAttentionArgs &a = tree_args().a;
+            const TreeWork &w = tree_args().w;
+            load(next, next.tile, number);
 #pragma unroll
-                    for (int p = 0; p < kPasses; ++p) { tree_shift(kx[p], past); tree_shift(vx[p], past); }
+            for (int e = 0; e < kEach; ++e) {
+                const int x = loader + e * kLoaders, b = 16 * (x % (DC / 8));
+                const TreeRow t = tree_row(a, w, next.d, next.h, (int64_t)next.block * T::kRows + x / (DC / 8));
+                const char *const p = a.q + t.head * a.q_head_bytes + (int64_t)(next.d.row0 + t.node) * a.q_row_bytes;
+                uint32_t z[4] = {0, 0, 0, 0};
+                if (t.there && b < 2 * a.dim) {
+                    if (ANY && 2 * a.dim < 16) load_part<4>(z, p, 2 * a.dim);
+                    else load_stream<4>(z, p + min(b, 2 * a.dim - 16));
                 }
-                if (__any(missing)) {
-                    // Tokens that are not there, or on a page outside the cache: values of zero; keys of NaN, which is the result of a row that
-                    // sees them (zeros behind the row's end: the queries' zeros there would make NaN of those as well).
+                y[e] = u32x4{z[0], z[1], z[2], z[3]};
+            }
+        }
+        if (begun_any) {
+            // ---- the unit's end: join the wavefronts, give out the result or leave a part.  By way of LDS, so that whole rows are stored.
+            const PagedTreeAttentionArgs &a = tree_args().a;
+            const TreeWork &w = tree_args().w;
+            const Draft &d = cur.d;
+            const bool begun = cur.tile == 0, done = cur.last == d.tiles, whole = begun && done;
+            const int part_slot = 2 * group + (begun ? 1 : 0);
+            const float v_scale = F8 ? a.v.scale[cur.h] : 1.f;
+            const TreeShared<T::kRows> shared(w);
+            constexpr int kPart = T::kAlone ? T::kBuffer : T::kLds / kTreeWaves, kDims = DC < 128 ? DC : 128, kPitch = kDims + 4;       // (dimensions at a time)
+            static_assert(32 * kPitch * 4 <= kPart && kPart % 16 == 0);
+            float *const mineo = (float *)(lds + wave * kPart) + l32 * kPitch;
+            l = pair_sum(l);
+            if (half == 0) { wave_m[wave][l32] = m; wave_l[wave][l32] = l; }
+            if (!T::kAlone) tree_barrier();                  // (else a wavefront's part lies where its own tokens did)
 #pragma unroll
-                    for (int p = 0; p < kPasses; ++p)
+            for (int c = 0; c < DC / kDims; ++c) {
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const int bytes = ANY ? row_bytes - 16 * piece - 4 * x : 4;
-                            const uint32_t nan = (F8 ? 0x7f7f7f7fu : 0x7fff7fffu) & (bytes >= 4 ? 0xffffffffu : bytes <= 0 ? 0u : (1u << (8 * bytes)) - 1u);
-                            const bool none = missing >> p & 1;
-                            kx[p][x] = none && has_piece ? nan : kx[p][x];
-                            vx[p][x] = none ? 0u : vx[p][x];
+                for (int j = 0; j < kDims / 32; ++j)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        *(f32x4 *)(mineo + 32 * j + 8 * g + 4 * half) =
+                            f32x4{o[c * (kDims / 32) + j][4 * g], o[c * (kDims / 32) + j][4 * g + 1], o[c * (kDims / 32) + j][4 * g + 2], o[c * (kDims / 32) + j][4 * g + 3]};
+                if (T::kGroups > 1) tree_barrier();
+                else __builtin_amdgcn_wave_barrier();
+                // kGroups > 1: all threads have the rows of all; else each wavefront has its own
+                constexpr int kThreads = T::kGroups > 1 ? kTreeThreads : 64, kMany = (T::kGroups > 1 ? T::kRows : 32) * (kDims / 4);
+#pragma unroll 2
+                for (int e = T::kGroups > 1 ? (int)threadIdx.x : lane; e < kMany; e += kThreads) {
+                    const int x = e / (kDims / 4) + (T::kGroups > 1 ? 0 : 32 * wr), dim1 = 4 * (e % (kDims / 4)), dim0 = c * kDims + dim1;
+                    const TreeRow t = tree_row(a, w, d, cur.h, (int64_t)cur.block * T::kRows + x);
+                    float top = -INFINITY, sum = 0.f;
+                    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+                    if (T::kGroups == 1) {
+                        top = wave_m[wave][x % 32];
+                        sum = wave_l[wave][x % 32];
+                        acc = *(const f32x4 *)((const float *)(lds + wave * kPart) + (x % 32) * kPitch + dim1);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < T::kGroups; ++i) top = fmaxf(top, wave_m[i * WR + x / 32][x % 32]);
+                        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+                        for (int i = 0; i < T::kGroups; ++i) {
+                            const int v = i * WR + x / 32;
+                            const float f = __builtin_amdgcn_exp2f(wave_m[v][x % 32] - base);
+                            sum += f * wave_l[v][x % 32];
+                            acc += f * *(const f32x4 *)((const float *)(lds + v * kPart) + (x % 32) * kPitch + dim1);
                         }
+                    }
+                    if (t.there && dim0 < a.dim) {
+                        if (whole) {
+                            tree_result<DT>(a, d, t, dim0, acc, sum, v_scale);
+                        } else {
+                            shared.store(part_slot, x, dim0, acc);
+                            if (dim0 == 0) shared.store(part_slot, x, TreePart{top, sum});
+                        }
+                    }
                 }
-                if (hidden(first_of(i))) {
-                    // Values that are not finite where not every row sees every token: a probability of 0 times them would be NaN.  They take part
-                    // as zeros, and rows that see them get them at the unit's end.
-                    constexpr int kWidth = F8 ? 8 : 16;
-                    constexpr uint32_t kTop = F8 ? 0x7fu : E::kExponent, kAll = F8 ? 0xffu : 0xffffu;
-                    bool found = false;
-#pragma unroll
-                    for (int p = 0; p < kPasses; ++p)
-#pragma unroll
-                        for (int x = 0; x < 4; ++x)
-#pragma unroll
-                            for (int b = 0; b < 32; b += kWidth) {
-                                const bool hit = (vx[p][x] >> b & kTop) == kTop;
-                                found |= hit;
-                                vx[p][x] &= hit ? ~(kAll << b) : 0xffffffffu;
-                            }
-                    if (found && has_piece) odd = 1;
+                if (c + 1 < DC / kDims) {
+                    if (T::kGroups > 1) tree_barrier();
+                    else __builtin_amdgcn_wave_barrier();
                 }
+            }
+            tree_barrier();
+            if (odd) {
+                // Values that are not finite, for the rows that see them: an infinity or a NaN of whatever weight is the result's.
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+                const int32_t *const row = row_of(cur);
+                for (int e = (int)threadIdx.x; e < T::kRows * a.dim; e += kTreeThreads) {
+                    const int x = e / a.dim, dim = e - x * a.dim;
+                    const TreeRow t = tree_row(a, w, d, cur.h, (int64_t)cur.block * T::kRows + x);
+                    const Sight s = sight_of(a, d, t, row_from[x]);
+                    float add = 0.f;
+                    const uint32_t t_end = (uint32_t)min((int64_t)d.end, (int64_t)d.start + (int64_t)cur.last * T::kTokens);
+#pragma nounroll
+                    for (uint32_t tok = (uint32_t)d.start + (uint32_t)cur.tile * T::kTokens; tok < t_end; ++tok) {
+                        if (!hidden(d, a.window, tok & ~(uint32_t)(T::kStaged - 1)) || !(s(d, a.words, tok) & 1)) continue;
+                        const uint32_t at_page = a.page.div(tok);
+                        const int32_t in_page = row[at_page];
+                        if ((uint32_t)in_page >= (uint32_t)a.pages) continue;
+                        const char *const v = a.v.base + cur.h * a.v.head_bytes + in_page * a.v.page_bytes + (int64_t)(tok - at_page * a.page.d) * a.v.token_bytes + EB * dim;
+                        const uint32_t bits = F8 ? *(const uint8_t *)v : *(const u16_any *)v;
+                        if (F8 ? (bits & 0x7f) == 0x7f : (bits & E::kExponent) == E::kExponent) add += F8 ? NAN : Elem<DT>::to_float((uint16_t)bits);
+                    }
+                    if (t.there && add != 0.f) {
+                        if (whole) ((u16_any *)(a.out + t.head * a.out_head_bytes + (int64_t)(d.row0 + t.node) * a.out_row_bytes))[dim] = Elem<DT>::from_float(add);
+                        else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, add), shared.sums, shared.sum_at(part_slot, x, dim), 0, kTreeAux);
+                    }
+                }
+                __syncthreads();
+                if (threadIdx.x == 0) odd = 0;
+                __syncthreads();
+            }
+            if (!whole) {
+                const int64_t first = cur.at - cur.tile, total = uniform64(dealt[0]), groups = uniform64(dealt[1]);
+                TreeLeft u = {begun ? group : (int)tree_ratio_up(first + 1, groups, total) - 1, 0, cur.request, cur.h, cur.block};
+                u.parts = (int)tree_ratio_up(first + d.tiles, groups, total) - u.begins;
+                if (w.left) {
+                    if (begun && threadIdx.x == 0) w.left[group] = u;
+                } else {
+                    if (threadIdx.x == 0) left[unfinished] = u;
+                    ++unfinished;                            // (the first unit of the share at most, and its last)
+                }
+            }
+            if (!more) break;
+        }
+        // ---- queries by way of LDS: column l32 of the scores
+        cur = next;
+        begun_any = true;
+        const PagedTreeAttentionArgs &a = tree_args().a;
+        const Draft &d = cur.d;
+        u32x4 q[KS];
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const int x = loader + e * kLoaders, b = 16 * (x % (DC / 8));
+            uint32_t z[4] = {y[e][0], y[e][1], y[e][2], y[e][3]};
+            if (ANY && 2 * a.dim >= 16) tree_shift(z, max(b - (2 * a.dim - 16), 0));
+            *(u32x4 *)(ours + x / (DC / 8) * T::kPitchK + b) = u32x4{z[0], z[1], z[2], z[3]};
+        }
+        if (!T::kAlone) tree_barrier();
+#pragma unroll
+        for (int k = 0; k < KS; ++k) q[k] = *(const u32x4 *)(ours + (T::kAlone ? l32 : 32 * wr + l32) * T::kPitchK + 32 * k + 16 * half);
+        if (!T::kAlone) tree_barrier();
+        const int32_t *const row = row_of(cur);
+        Sight sight = sight_of(a, d, tree_row(a, tree_args().w, d, cur.h, (int64_t)cur.block * T::kRows + 32 * wr + l32), 0);
+        if (a.window) sight.from = window_from(a, d, sight);
+        if (wt == 0 && half == 0) row_from[32 * wr + l32] = sight.from;
+        const int window = uniform(a.window), words = uniform(a.words), row_bytes = uniform(EB * a.dim);
+        const PageDiv page_div = {(uint32_t)uniform((int)a.page.d), (uint32_t)uniform((int)a.page.mul), (uint32_t)uniform((int)a.page.shift)};
+        const bool has_piece = 16 * piece < row_bytes;
+        const float to_log2 = a.scale * kLog2e * (F8 ? a.k.scale[cur.h] : 1.f);
+#pragma unroll
+        for (int j = 0; j < DB; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[j][i] = 0.f;
+        m = -INFINITY; l = 0.f;
+        more = cur.at + (cur.last - cur.tile) + kTreeUnit < end;
+
+        number = look_up(cur, row, page_div, cur.tile + 1);
+        for (int i = cur.tile; i < cur.last; ++i) {
+            char *const buf = ours + (T::kAlone ? 0 : (i & 1) * T::kBuffer);
+            const bool some_hidden = hidden(d, window, first_of(cur, i));
+            // -- the tile's rows, which have arrived, into LDS, in 16 bits
+            if (ANY && 16 * piece + 16 > row_bytes && has_piece && row_bytes >= 16) {
+                const int past = 16 * piece - (row_bytes - 16);
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p) { tree_shift(kx[p], past); tree_shift(vx[p], past); }
+            }
+            if (__any(missing)) {
+                // Tokens that are not there, or on a page outside the cache: values of zero; keys of NaN, which is the result of a row that
+                // sees them (zeros behind the row's end: the queries' zeros there would make NaN of those as well).
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int bytes = ANY ? row_bytes - 16 * piece - 4 * x : 4;
+                        const uint32_t nan = (F8 ? 0x7f7f7f7fu : 0x7fff7fffu) & (bytes >= 4 ? 0xffffffffu : bytes <= 0 ? 0u : (1u << (8 * bytes)) - 1u);
+                        const bool none = missing >> p & 1;
+                        kx[p][x] = none && has_piece ? nan : kx[p][x];
+                        vx[p][x] = none ? 0u : vx[p][x];
+                    }
+            }
+            if (some_hidden) {
+                // Values that are not finite where not every row sees every token: a probability of 0 times them would be NaN.  They take part
+                // as zeros, and rows that see them get them at the unit's end.
+                constexpr int kWidth = F8 ? 8 : 16;
+                constexpr uint32_t kTop = F8 ? 0x7fu : E::kExponent, kAll = F8 ? 0xffu : 0xffffu;
+                bool found = false;
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+#pragma unroll
+                        for (int b = 0; b < 32; b += kWidth) {
+                            const bool hit = (vx[p][x] >> b & kTop) == kTop;
+                            found |= hit;
+                            vx[p][x] &= hit ? ~(kAll << b) : 0xffffffffu;
+                        }
+                if (found && has_piece) odd = 1;
+            }
+            {
                 char *const kt = buf + line * T::kPitchK + (F8 ? 32 : 16) * piece, *const vt = buf + T::kStaged * T::kPitchK + line * T::kPitchV + (F8 ? 32 : 16) * piece;
                 auto put = [&](char *to, const uint32_t (&x)[4]) {
                     if (F8) {
@@ -516,37 +743,17 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
                     put(vt + p * kAtOnce * T::kPitchV, vx[p]);
                 }
             }
-            if (i + 1 < last) {
-                // -- the next tile's rows, where their pages are; the lane that looks after a token hands its place to those that load it
-                const uint32_t t = first_of(i + 1) + (uint32_t)mine_at, in = t - a.page.div(t) * a.page.d;
-                const bool none = (uint32_t)page >= (uint32_t)a.pages;
-                const int64_t k_at = none ? -1 : (int64_t)page * a.k.page_bytes + (int64_t)in * a.k.token_bytes;
-                const int64_t v_at = none ? -1 : (int64_t)page * a.v.page_bytes + (int64_t)in * a.v.token_bytes;
-                missing = 0;
-#pragma unroll
-                for (int p = 0; p < kPasses; ++p) {
-                    const int64_t ko = shuffle64(k_at, p * kAtOnce + line), vo = shuffle64(v_at, p * kAtOnce + line);
-                    missing |= ko < 0 ? 1u << p : 0u;
-                    // (a.q: somewhere that can be read)
-                    const char *const kp = ko < 0 ? a.q : kbase + ko, *const vp = ko < 0 ? a.q : vbase + vo;
-                    if (has_piece) {
-                        if (ANY && row_bytes < 16) {
-                            load_part<4>(kx[p], kp, row_bytes);
-                            load_part<4>(vx[p], vp, row_bytes);
-                        } else {
-                            const int b = ANY ? min(16 * piece, row_bytes - 16) : 16 * piece;
-                            load_stream<4>(kx[p], kp + b);
-                            load_stream<4>(vx[p], vp + b);
-                        }
-                    }
-                }
-                page = look_up(i + 2);
+            if (i + 1 < cur.last) {
+                load(cur, i + 1, number);
+                number = look_up(cur, row, page_div, i + 2);
+            } else if (more) {
+                next = after(cur);
+                number = look_up(next, row_of(next), page_div, next.tile);
             }
-            if (i < tile) continue;
             if (!T::kAlone) tree_barrier();
 
             // -- scores of tokens t0 + 32 u + 8 (x / 4) + 4 half + x % 4
-            const uint32_t t0 = first_of(i) + (T::kAlone ? 0 : wt * T::kMine);
+            const uint32_t t0 = first_of(cur, i) + (T::kAlone ? 0 : wt * T::kMine);
             const char *const kt = buf + ((T::kAlone ? 0 : wt * T::kMine) + l32) * T::kPitchK + 16 * half;
             f32x16 s[SUBS];
 #pragma unroll
@@ -558,8 +765,8 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
             }
 #pragma unroll
             for (int u = 0; u < SUBS; ++u) s[u] *= to_log2;
-            if (hidden(first_of(i))) {
-                const uint64_t see = sight(d, a.words, t0) >> (4 * half);
+            if (some_hidden) {
+                const uint64_t see = sight(d, words, t0) >> (4 * half);
 #pragma unroll
                 for (int u = 0; u < SUBS; ++u)
 #pragma unroll
@@ -600,110 +807,9 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
                     o[j] = E::mfma(u32x4{lo[0], lo[1], hi[0], hi[1]}, p[k], o[j]);
                 }
         }
-        l = pair_sum(l);
-
-        // ---- the unit's end: join the wavefronts, give out the result or leave a part
-        const bool begun = tile == 0, done = last == d.tiles, whole = begun && done;
-        const int part_slot = 2 * group + (begun ? 1 : 0);
-        const float v_scale = F8 ? a.v.scale[h] : 1.f;
-        const TreeShared<T::kRows> shared(w);
-        if constexpr (T::kGroups == 1) {
-            if (mine_row.there) {
-#pragma unroll
-                for (int j = 0; j < DB; ++j)
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int dim0 = 32 * j + 8 * g + 4 * half;
-                        const f32x4 acc = {o[j][4 * g], o[j][4 * g + 1], o[j][4 * g + 2], o[j][4 * g + 3]};
-                        if (whole) tree_result<DT>(a, d, mine_row, dim0, acc, l, v_scale);
-                        else if (dim0 < a.dim) shared.store(part_slot, 32 * wr + l32, dim0, acc);
-                    }
-                if (!whole && half == 0) shared.store(part_slot, 32 * wr + l32, TreePart{m, l});
-            }
-        } else {
-            if (!T::kAlone) tree_barrier();                  // (else a wavefront's part lies where its own tokens did)
-            constexpr int kPart = T::kAlone ? T::kBuffer : 32 * T::kPitchO * 4;
-            static_assert(32 * T::kPitchO * 4 <= kPart && kTreeWaves * kPart <= T::kLds);
-            float *const mineo = (float *)(lds + wave * kPart) + l32 * T::kPitchO;
-            if (half == 0) { wave_m[wave][l32] = m; wave_l[wave][l32] = l; }
-#pragma unroll
-            for (int j = 0; j < DB; ++j)
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    *(f32x4 *)(mineo + 32 * j + 8 * g + 4 * half) = f32x4{o[j][4 * g], o[j][4 * g + 1], o[j][4 * g + 2], o[j][4 * g + 3]};
-            tree_barrier();
-            for (int e = (int)threadIdx.x; e < T::kRows * (DC / 4); e += kTreeThreads) {
-                const int x = e / (DC / 4), dim0 = 4 * (e % (DC / 4));
-                const TreeRow t = tree_row(a, w, d, h, (int64_t)block * T::kRows + x);
-                if (!t.there || dim0 >= a.dim) continue;
-                float top = -INFINITY, sum = 0.f;
-                f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int i = 0; i < T::kGroups; ++i) top = fmaxf(top, wave_m[i * WR + x / 32][x % 32]);
-                const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-                for (int i = 0; i < T::kGroups; ++i) {
-                    const int v = i * WR + x / 32;
-                    const float f = __builtin_amdgcn_exp2f(wave_m[v][x % 32] - base);
-                    sum += f * wave_l[v][x % 32];
-                    acc += f * *(const f32x4 *)((const float *)(lds + v * kPart) + (x % 32) * T::kPitchO + dim0);
-                }
-                if (whole) {
-                    tree_result<DT>(a, d, t, dim0, acc, sum, v_scale);
-                } else {
-                    shared.store(part_slot, x, dim0, acc);
-                    if (dim0 == 0) shared.store(part_slot, x, TreePart{top, sum});
-                }
-            }
-        }
-        tree_barrier();
-        if (odd) {
-            // Values that are not finite, for the rows that see them: an infinity or a NaN of whatever weight is the result's.
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            for (int e = (int)threadIdx.x; e < T::kRows * a.dim; e += kTreeThreads) {
-                const int x = e / a.dim, dim = e - x * a.dim;
-                const TreeRow t = tree_row(a, w, d, h, (int64_t)block * T::kRows + x);
-                const Sight s = sight_of(a, d, t, row_from[x]);
-                float add = 0.f;
-                const uint32_t t_end = (uint32_t)min((int64_t)d.end, (int64_t)d.start + (int64_t)last * T::kTokens);
-#pragma nounroll
-                for (uint32_t tok = (uint32_t)d.start + (uint32_t)tile * T::kTokens; tok < t_end; ++tok) {
-                    if (!hidden(tok & ~(uint32_t)(T::kStaged - 1)) || !(s(d, a.words, tok) & 1)) continue;
-                    const uint32_t at_page = a.page.div(tok);
-                    const int32_t number = row[at_page];
-                    if ((uint32_t)number >= (uint32_t)a.pages) continue;
-                    const char *const v = vbase + number * a.v.page_bytes + (int64_t)(tok - at_page * a.page.d) * a.v.token_bytes + EB * dim;
-                    const uint32_t y = F8 ? *(const uint8_t *)v : *(const u16_any *)v;
-                    if (F8 ? (y & 0x7f) == 0x7f : (y & E::kExponent) == E::kExponent) add += F8 ? NAN : Elem<DT>::to_float((uint16_t)y);
-                }
-                if (t.there && add != 0.f) {
-                    if (whole) ((u16_any *)(a.out + t.head * a.out_head_bytes + (int64_t)(d.row0 + t.node) * a.out_row_bytes))[dim] = Elem<DT>::from_float(add);
-                    else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, add), shared.sums, shared.sum_at(part_slot, x, dim), 0, kTreeAux);
-                }
-            }
-            __syncthreads();
-            if (threadIdx.x == 0) odd = 0;
-        }
-        if (!whole) {
-            const int64_t first = at - tile;
-            TreeLeft u = {begun ? group : (int)tree_ratio_up(first + 1, groups, total) - 1, 0, request, h, block};
-            u.parts = (int)tree_ratio_up(first + d.tiles, groups, total) - u.begins;
-            if (w.left) {
-                if (begun && threadIdx.x == 0) w.left[group] = u;
-            } else {
-                if (threadIdx.x == 0) left[unfinished] = u;
-                ++unfinished;                                // (the first unit of the share at most, and its last)
-            }
-        }
-        at += last - tile;
-        tile = 0;
-        if (++unit == a.heads * d.blocks) {
-            unit = 0;
-            ++request;
-        }
-        tree_barrier();
     }
+    const PagedTreeAttentionArgs &a = tree_args().a;
+    const TreeWork &w = tree_args().w;
     if (w.left || unfinished == 0) return;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -720,7 +826,9 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
 }
 
 // The joining as a kernel of its own: grid (workgroups of the other, blocks of rows).
-template <int DT, int DC, int WR> __global__ void __launch_bounds__(kTreeThreads) paged_tree_join_kernel(PagedTreeAttentionArgs a, TreeWork w, int rows) {
+template <int DT, int DC, int WR> __global__ void __launch_bounds__(kTreeThreads) paged_tree_join_kernel(TreeArgs args, int rows) {
+    const PagedTreeAttentionArgs &a = args.a;
+    const TreeWork &w = args.w;
     const TreeLeft u = w.left[blockIdx.x];
     const int row0 = (int)blockIdx.y * rows;
     if (u.parts) tree_join<DT, DC, WR>(a, w, u, row0, row0 + rows, a.v.scale ? a.v.scale[u.h] : 1.f);
@@ -736,10 +844,10 @@ template <int DT, bool F8, int DC, int WR, bool ANY> static int launch_tree_buil
     static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&paged_tree_attention_kernel<DT, F8, DC, WR, ANY>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds);
     if (attr != hipSuccess) return BA_ERR_LAUNCH;
-    paged_tree_attention_kernel<DT, F8, DC, WR, ANY><<<w.groups, kTreeThreads, T::kLds, stream>>>(a, w);
+    paged_tree_attention_kernel<DT, F8, DC, WR, ANY><<<w.groups, kTreeThreads, T::kLds, stream>>>(TreeArgs{a, w});
     if (w.left) {
-        constexpr int kRows = kTreeThreads / (DC / 4);
-        paged_tree_join_kernel<DT, DC, WR><<<dim3((unsigned)w.groups, T::kRows / kRows), kTreeThreads, 0, stream>>>(a, w, kRows);
+        constexpr int kRows = std::min(T::kRows, 4 * kTreeThreads / (DC / 4));      // (a round of its threads)
+        paged_tree_join_kernel<DT, DC, WR><<<dim3((unsigned)w.groups, T::kRows / kRows), kTreeThreads, 0, stream>>>(TreeArgs{a, w}, kRows);
     }
     return hipGetLastError() == hipSuccess ? BA_OK : BA_ERR_LAUNCH;
 }
