@@ -4,10 +4,10 @@
 
 namespace ba {
 
-extern template int launch_tree_types<0, false>(const PagedTreeAttentionArgs &a, const TreeWork &w, bool any, int waves, hipStream_t stream);
-extern template int launch_tree_types<1, false>(const PagedTreeAttentionArgs &a, const TreeWork &w, bool any, int waves, hipStream_t stream);
-extern template int launch_tree_types<0, true>(const PagedTreeAttentionArgs &a, const TreeWork &w, bool any, int waves, hipStream_t stream);
-extern template int launch_tree_types<1, true>(const PagedTreeAttentionArgs &a, const TreeWork &w, bool any, int waves, hipStream_t stream);
+extern template int launch_tree_types<0, false>(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int waves, hipStream_t stream);
+extern template int launch_tree_types<1, false>(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int waves, hipStream_t stream);
+extern template int launch_tree_types<0, true>(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int waves, hipStream_t stream);
+extern template int launch_tree_types<1, true>(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int waves, hipStream_t stream);
 
 static int resident_of(int dims) { return dims == 64 ? TreeTile<64, 4>::kResident : dims == 128 ? TreeTile<128, 4>::kResident : TreeTile<256, 4>::kResident; }
 
@@ -51,9 +51,9 @@ int launch_paged_tree_attention(const PagedTreeAttentionArgs &a, int dtype, int 
     if (waves == 1 && w.groups <= kTreeFewParts * std::max<int64_t>(1, a.tokens * a.group / (32 * waves)) * a.heads) w.left = nullptr;
     const uint64_t bits = (uint64_t)a.k.base | (uint64_t)a.v.base | (uint64_t)a.k.page_bytes | (uint64_t)a.v.page_bytes | (uint64_t)a.k.head_bytes |
                           (uint64_t)a.v.head_bytes | (uint64_t)a.k.token_bytes | (uint64_t)a.v.token_bytes;
-    const bool any = bits % 16 != 0 || a.dim % (f8 ? 16 : 8) != 0;
-    if (dtype == BA_F16) return f8 ? launch_tree_types<0, true>(a, w, any, waves, stream) : launch_tree_types<0, false>(a, w, any, waves, stream);
-    return f8 ? launch_tree_types<1, true>(a, w, any, waves, stream) : launch_tree_types<1, false>(a, w, any, waves, stream);
+    const TreeRows rows = a.dim * (f8 ? 1 : 2) < 16 ? kTreeShort : bits % 16 != 0 || a.dim % (f8 ? 16 : 8) != 0 ? kTreeAny : kTreePieces;
+    if (dtype == BA_F16) return f8 ? launch_tree_types<0, true>(a, w, rows, waves, stream) : launch_tree_types<0, false>(a, w, rows, waves, stream);
+    return f8 ? launch_tree_types<1, true>(a, w, rows, waves, stream) : launch_tree_types<1, false>(a, w, rows, waves, stream);
 }
 
 }  // namespace ba

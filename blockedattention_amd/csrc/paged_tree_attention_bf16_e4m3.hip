@@ -2,5 +2,5 @@
 #include "paged_tree_attention_kernel.hpp"
 
 namespace ba {
-template int launch_tree_types<1, true>(const PagedTreeAttentionArgs &a, const TreeWork &w, bool any, int waves, hipStream_t stream);
+template int launch_tree_types<1, true>(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int waves, hipStream_t stream);
 }  // namespace ba

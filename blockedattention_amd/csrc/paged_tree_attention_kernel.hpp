@@ -334,14 +334,18 @@ __device__ __forceinline__ int window_from(const PagedTreeAttentionArgs &a, cons
     }
 }
 
-// DC: dimensions that the registers hold (64, 128, 256).  ANY: rows at any address.
-template <int DT, bool F8, int DC, int WR, bool ANY>
+// What is known of the rows: whole 16-byte pieces at multiples of 16 bytes; at any address, of 16 bytes or more; shorter.
+enum TreeRows { kTreePieces, kTreeAny, kTreeShort };
+
+// DC: dimensions that the registers hold (64, 128, 256).
+template <int DT, bool F8, int DC, int WR, TreeRows ROWS>
 __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) paged_tree_attention_kernel(TreeArgs) {
     typedef TreeTile<DC, WR> T;
     typedef TreeElem<DT> E;
     constexpr int EB = F8 ? 1 : 2, kPieces = DC * EB / 16;   // bytes of an element, 16-byte pieces of a row
     constexpr int kLoaders = T::kAlone ? 64 : kTreeThreads, kAtOnce = kLoaders / kPieces, kPasses = T::kStaged / kAtOnce;
     constexpr int KS = DC / 16, DB = DC / 32, SUBS = T::kMine / 32;
+    constexpr bool ANY = ROWS != kTreePieces, SHORT = ROWS == kTreeShort;
     static_assert(kLoaders % kPieces == 0 && T::kStaged % kAtOnce == 0 && T::kStaged <= 64);
     const int lane = lane_id(), l32 = lane & 31, half = lane >> 5, wave = uniform((int)threadIdx.x >> 6), wr = wave % WR, wt = wave / WR;
 
@@ -472,45 +476,42 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
         const PagedTreeAttentionArgs &a = tree_args().a;
         return (const int32_t *)uniform64((int64_t)(uintptr_t)(a.table + u.request * a.table_stride));
     };
+    // The rows of the next tile: where they are, then one after the other.  A burst of all of them holds the wavefront up (eight loads 2400 cycles, of
+    // the 7900 that a pair of tiles takes), so within a unit they go between the matrix instructions.
     uint32_t kx[kPasses][4], vx[kPasses][4];
-    uint32_t missing = 0;                                    // bit p: the token of pass p is not there
-    auto load = [&](const Unit &u, int i, int32_t number) {
+    uint64_t missing = 0;                                    // bit i: the token that lane i looks after is not there
+    // (tokens that are not there, pieces behind the row's end: anything that can be read, for 16 bytes)
+    auto aim = [&](const Unit &u, int i, int32_t number) {
         const PagedTreeAttentionArgs &a = tree_args().a;
-        const char *const kbase = a.k.base + u.h * a.k.head_bytes, *const vbase = a.v.base + u.h * a.v.head_bytes, *const readable = a.q;
-        const int row_bytes = EB * a.dim;
         const uint32_t t = first_of(u, i) + (uint32_t)mine_at, in = t - a.page.div(t) * a.page.d;
-        const bool none = (uint32_t)number >= (uint32_t)a.pages, alike = a.k.page_bytes == a.v.page_bytes && a.k.token_bytes == a.v.token_bytes;
+        const bool none = (uint32_t)number >= (uint32_t)a.pages;
+        missing = __ballot(none);
         spots[wave][0][lane] = none ? -1 : (int64_t)number * a.k.page_bytes + (int64_t)in * a.k.token_bytes;
-        if (!alike) spots[wave][1][lane] = none ? -1 : (int64_t)number * a.v.page_bytes + (int64_t)in * a.v.token_bytes;
+        spots[wave][1][lane] = none ? -1 : (int64_t)number * a.v.page_bytes + (int64_t)in * a.v.token_bytes;
         __builtin_amdgcn_wave_barrier();
-        int64_t ko[kPasses], vo[kPasses];
+    };
+    auto aim_nowhere = [&]() {
+        spots[wave][0][lane] = spots[wave][1][lane] = -1;
+        __builtin_amdgcn_wave_barrier();
+    };
+    struct Bases {
+        const char *k, *v, *readable;
+        int row_bytes;
+    };
+    auto bases_of = [&](const Unit &u) {
+        const PagedTreeAttentionArgs &a = tree_args().a;
+        const int row_bytes = EB * a.dim, b = SHORT ? 0 : ANY ? min(16 * piece, row_bytes - 16) : 16 * piece;
+        return Bases{a.k.base + u.h * a.k.head_bytes + b, a.v.base + u.h * a.v.head_bytes + b, a.q, row_bytes};
+    };
+    auto fetch = [&](uint32_t (&x)[4], const Bases &from, int which, int p) {
+        const int64_t at = spots[wave][which][p * kAtOnce + line];
+        const char *const q = at >= 0 && 16 * piece < from.row_bytes ? (which ? from.v : from.k) + at : from.readable;
+        if (SHORT) load_part<4>(x, q, from.row_bytes);
+        else load_stream<4>(x, q);
+    };
+    auto fetch_all = [&](const Bases &from) {
 #pragma unroll
-        for (int p = 0; p < kPasses; ++p) vo[p] = ko[p] = spots[wave][0][p * kAtOnce + line];
-        if (!alike)
-#pragma unroll
-            for (int p = 0; p < kPasses; ++p) vo[p] = spots[wave][1][p * kAtOnce + line];
-        missing = 0;
-#pragma unroll
-        for (int p = 0; p < kPasses; ++p) missing |= ko[p] < 0 ? 1u << p : 0u;
-        if (16 * piece < row_bytes) {
-            const int b = ANY ? max(min(16 * piece, row_bytes - 16), 0) : 16 * piece;
-#pragma unroll
-            for (int p = 0; p < kPasses; ++p) {
-                const char *const kp = (ko[p] < 0 ? readable : kbase + ko[p]) + b, *const vp = (ko[p] < 0 ? readable : vbase + vo[p]) + b;
-                if (ANY && row_bytes < 16) {
-                    load_part<4>(kx[p], kp, row_bytes);
-                    load_part<4>(vx[p], vp, row_bytes);
-                } else {
-                    load_stream<4>(kx[p], kp);
-                    load_stream<4>(vx[p], vp);
-                }
-            }
-        } else {                                             // dimensions behind the rows' end
-#pragma unroll
-            for (int p = 0; p < kPasses; ++p)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) kx[p][x] = vx[p][x] = 0;
-        }
+        for (int p = 0; p < kPasses; ++p) { fetch(kx[p], from, 0, p); fetch(vx[p], from, 1, p); }
     };
     // Staged tokens from t on that not all rows see: those of the draft, and where the rows' windows begin.
     auto hidden = [&](const Draft &d, int window, uint32_t t) {
@@ -532,7 +533,8 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
         if (more) {
             const PagedTreeAttentionArgs &a = tree_args().a;
             const TreeWork &w = tree_args().w;
-            load(next, next.tile, number);
+            aim(next, next.tile, number);
+            fetch_all(bases_of(next));
 #pragma unroll
             for (int e = 0; e < kEach; ++e) {
                 const int x = loader + e * kLoaders, b = 16 * (x % (DC / 8));
@@ -685,17 +687,18 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
         m = -INFINITY; l = 0.f;
         more = cur.at + (cur.last - cur.tile) + kTreeUnit < end;
 
+        const Bases from = bases_of(cur);
         number = look_up(cur, row, page_div, cur.tile + 1);
         for (int i = cur.tile; i < cur.last; ++i) {
             char *const buf = ours + (T::kAlone ? 0 : (i & 1) * T::kBuffer);
             const bool some_hidden = hidden(d, window, first_of(cur, i));
             // -- the tile's rows, which have arrived, into LDS, in 16 bits
-            if (ANY && 16 * piece + 16 > row_bytes && has_piece && row_bytes >= 16) {
+            if (ANY && !SHORT && 16 * piece + 16 > row_bytes && has_piece) {
                 const int past = 16 * piece - (row_bytes - 16);
 #pragma unroll
                 for (int p = 0; p < kPasses; ++p) { tree_shift(kx[p], past); tree_shift(vx[p], past); }
             }
-            if (__any(missing)) {
+            if (missing) {
                 // Tokens that are not there, or on a page outside the cache: values of zero; keys of NaN, which is the result of a row that
                 // sees them (zeros behind the row's end: the queries' zeros there would make NaN of those as well).
 #pragma unroll
@@ -704,7 +707,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
                     for (int x = 0; x < 4; ++x) {
                         const int bytes = ANY ? row_bytes - 16 * piece - 4 * x : 4;
                         const uint32_t nan = (F8 ? 0x7f7f7f7fu : 0x7fff7fffu) & (bytes >= 4 ? 0xffffffffu : bytes <= 0 ? 0u : (1u << (8 * bytes)) - 1u);
-                        const bool none = missing >> p & 1;
+                        const bool none = missing >> (p * kAtOnce + line) & 1;
                         kx[p][x] = none && has_piece ? nan : kx[p][x];
                         vx[p][x] = none ? 0u : vx[p][x];
                     }
@@ -727,6 +730,15 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
                         }
                 if (found && has_piece) odd = 1;
             }
+            if (row_bytes < 16 * kPieces) {
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        kx[p][x] = has_piece ? kx[p][x] : 0u;
+                        vx[p][x] = has_piece ? vx[p][x] : 0u;
+                    }
+            }
             {
                 char *const kt = buf + line * T::kPitchK + (F8 ? 32 : 16) * piece, *const vt = buf + T::kStaged * T::kPitchK + line * T::kPitchV + (F8 ? 32 : 16) * piece;
                 auto put = [&](char *to, const uint32_t (&x)[4]) {
@@ -743,12 +755,17 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
                     put(vt + p * kAtOnce * T::kPitchV, vx[p]);
                 }
             }
-            if (i + 1 < cur.last) {
-                load(cur, i + 1, number);
+            const bool follows = i + 1 < cur.last;
+            if (follows) {
+                aim(cur, i + 1, number);
+                if (SHORT) fetch_all(from);
                 number = look_up(cur, row, page_div, i + 2);
-            } else if (more) {
-                next = after(cur);
-                number = look_up(next, row_of(next), page_div, next.tile);
+            } else {
+                aim_nowhere();
+                if (more) {
+                    next = after(cur);
+                    number = look_up(next, row_of(next), page_div, next.tile);
+                }
             }
             if (!T::kAlone) tree_barrier();
 
@@ -761,7 +778,11 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
 #pragma unroll
                 for (int x = 0; x < 16; ++x) s[u][x] = 0.f;
 #pragma unroll
-                for (int k = 0; k < KS; ++k) s[u] = E::mfma(*(const u32x4 *)(kt + 32 * u * T::kPitchK + 32 * k), q[k], s[u]);
+                for (int k = 0; k < KS; ++k) {
+                    s[u] = E::mfma(*(const u32x4 *)(kt + 32 * u * T::kPitchK + 32 * k), q[k], s[u]);
+                    constexpr int kEvery = SUBS * KS / kPasses;
+                    if (!SHORT && (u * KS + k + 1) % kEvery == 0) fetch(kx[(u * KS + k) / kEvery], from, 0, (u * KS + k) / kEvery);
+                }
             }
 #pragma unroll
             for (int u = 0; u < SUBS; ++u) s[u] *= to_log2;
@@ -805,6 +826,8 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeTile<DC, WR>::kResident)) p
                     const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPiece)(vt + 16 * k * T::kPitchV + 64 * j)));
                     const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPiece)(vt + (16 * k + 8) * T::kPitchV + 64 * j)));
                     o[j] = E::mfma(u32x4{lo[0], lo[1], hi[0], hi[1]}, p[k], o[j]);
+                    constexpr int kEvery = 2 * SUBS * DB / kPasses;
+                    if (!SHORT && (k * DB + j + 1) % kEvery == 0) fetch(vx[(k * DB + j) / kEvery], from, 1, (k * DB + j) / kEvery);
                 }
         }
     }
@@ -839,12 +862,12 @@ template <int DT, int DC, int WR> __global__ void __launch_bounds__(kTreeThreads
 static inline int tree_dims(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 static inline int tree_waves(int64_t tokens, int64_t requests, int64_t group) { return tokens * group <= 32 * std::max<int64_t>(1, requests) ? 1 : 4; }
 
-template <int DT, bool F8, int DC, int WR, bool ANY> static int launch_tree_build(const PagedTreeAttentionArgs &a, const TreeWork &w, hipStream_t stream) {
+template <int DT, bool F8, int DC, int WR, TreeRows ROWS> static int launch_tree_build(const PagedTreeAttentionArgs &a, const TreeWork &w, hipStream_t stream) {
     typedef TreeTile<DC, WR> T;
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&paged_tree_attention_kernel<DT, F8, DC, WR, ANY>),
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&paged_tree_attention_kernel<DT, F8, DC, WR, ROWS>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds);
     if (attr != hipSuccess) return BA_ERR_LAUNCH;
-    paged_tree_attention_kernel<DT, F8, DC, WR, ANY><<<w.groups, kTreeThreads, T::kLds, stream>>>(TreeArgs{a, w});
+    paged_tree_attention_kernel<DT, F8, DC, WR, ROWS><<<w.groups, kTreeThreads, T::kLds, stream>>>(TreeArgs{a, w});
     if (w.left) {
         constexpr int kRows = std::min(T::kRows, 4 * kTreeThreads / (DC / 4));      // (a round of its threads)
         paged_tree_join_kernel<DT, DC, WR><<<dim3((unsigned)w.groups, T::kRows / kRows), kTreeThreads, 0, stream>>>(TreeArgs{a, w}, kRows);
@@ -852,16 +875,19 @@ template <int DT, bool F8, int DC, int WR, bool ANY> static int launch_tree_buil
     return hipGetLastError() == hipSuccess ? BA_OK : BA_ERR_LAUNCH;
 }
 
-template <int DT, bool F8, int DC> static int launch_tree_dims(const PagedTreeAttentionArgs &a, const TreeWork &w, bool any, int waves, hipStream_t stream) {
-    if (waves == 1) return any ? launch_tree_build<DT, F8, DC, 1, true>(a, w, stream) : launch_tree_build<DT, F8, DC, 1, false>(a, w, stream);
-    return any ? launch_tree_build<DT, F8, DC, 4, true>(a, w, stream) : launch_tree_build<DT, F8, DC, 4, false>(a, w, stream);
+template <int DT, bool F8, int DC, int WR> static int launch_tree_rows(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, hipStream_t stream) {
+    if constexpr (DC == 64)
+        if (rows == kTreeShort) return launch_tree_build<DT, F8, DC, WR, kTreeShort>(a, w, stream);
+    return rows == kTreePieces ? launch_tree_build<DT, F8, DC, WR, kTreePieces>(a, w, stream) : launch_tree_build<DT, F8, DC, WR, kTreeAny>(a, w, stream);
 }
-
-template <int DT, bool F8> int launch_tree_types(const PagedTreeAttentionArgs &a, const TreeWork &w, bool any, int waves, hipStream_t stream) {
+template <int DT, bool F8, int DC> static int launch_tree_dims(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int waves, hipStream_t stream) {
+    return waves == 1 ? launch_tree_rows<DT, F8, DC, 1>(a, w, rows, stream) : launch_tree_rows<DT, F8, DC, 4>(a, w, rows, stream);
+}
+template <int DT, bool F8> int launch_tree_types(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int waves, hipStream_t stream) {
     switch (tree_dims(a.dim)) {
-        case 64: return launch_tree_dims<DT, F8, 64>(a, w, any, waves, stream);
-        case 128: return launch_tree_dims<DT, F8, 128>(a, w, any, waves, stream);
-        default: return launch_tree_dims<DT, F8, 256>(a, w, any, waves, stream);
+        case 64: return launch_tree_dims<DT, F8, 64>(a, w, rows, waves, stream);
+        case 128: return launch_tree_dims<DT, F8, 128>(a, w, rows, waves, stream);
+        default: return launch_tree_dims<DT, F8, 256>(a, w, rows, waves, stream);
     }
 }
 
