@@ -1,0 +1,558 @@
+// Attention of the drafted tokens of each request over a paged key-value cache: what its two kernels share (paged_tree_few.hpp,
+// paged_tree_wide.hpp).
+//
+// out[h][i] = sum_t softmax_t(scale q[h][i] . K[t]) V[t] over the tokens t that row i sees: those before the draft, of the draft
+// those with a bit in the row's mask, of these the last `window`.  A key takes part in one product for every row and query head that
+// shares it, n x group of them.
+//
+// Split.  A unit is a block of rows (nodes and the query heads that share a key head, heads fastest) of a request and key head.  Its tokens are
+// cut into tiles, and the tiles of all units, in the order of requests, key heads and blocks, are dealt out to the workgroups in equal
+// shares, with a constant for what a unit costs besides; sums and lengths are on the GPU only, so every workgroup adds them up itself.
+// A unit that lies in one share is done then; for others each workgroup leaves maxima, sums and fp32 accumulators in memory.
+// Where units have few parts, each counts itself in and the last one joins them all, in the order of the tokens whoever it is; else a
+// second kernel does.
+//
+// Tiles that not all rows see all of -- the draft's own, and where windows begin -- hide scores by the rows' bits.  Values there that are not
+// finite become zeros, since a probability of 0 times them would be NaN; rows that see them get them at the unit's end.
+#pragma once
+#include "paged_attention_kernel.hpp"
+
+namespace ba {
+
+constexpr int kTreeThreads = kPagedThreads, kTreeWaves = kPagedWaves;
+constexpr int kTreeUnit = 3;                 // what a unit costs besides its tiles, in tiles: queries, first loads, joining, results
+constexpr int kTreeShare = 5;                // of both, what a workgroup has at least, unless units are shorter
+constexpr int kTreeWhole = 4;                // units of up to so many tiles are not split between workgroups
+constexpr int kTreeFewParts = 8;             // parts of a unit, on the average, up to which the kernel itself joins them
+
+// A unit of which several workgroups did a part each: the one that has its first tile, how many they are (0: not split).
+struct TreeLeft {
+    int32_t begins, parts, request, h, block;
+};
+struct TreeWork {
+    int32_t *counters;                       // [groups]: how many have left their part of the unit begun by a workgroup; 0 between calls
+    TreeLeft *left;                          // not NULL: instead of counting, an entry a workgroup for the joining kernel
+    PagedPart *parts;                        // [2 * groups][rows of a unit]
+    float *sums;                             // [2 * groups][rows of a unit][pitch]
+    PageDiv group;                           // query heads of a key head
+    int32_t groups, pitch;
+};
+struct TreeArgs {
+    PagedTreeAttentionArgs a;
+    TreeWork w;
+};
+// The kernel's arguments, fetched again.  Held in scalar registers from the start they, and what is derived from them, are twice what there is; the
+// compiler then moves whole groups of them to and from vector registers within the loop over tiles (that loop's loads took 2300 cycles, not 700).
+__device__ __forceinline__ const TreeArgs &tree_args() {
+    auto p = (const __attribute__((address_space(4))) TreeArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const TreeArgs *)p;
+}
+// The same number, of which the compiler knows nothing: what is worked out from it for a unit's beginning and end is then worked out there, and not
+// kept in vector registers throughout the tiles.
+__device__ __forceinline__ int opaque(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// Tiles of a kernel, T:  kRows rows of a unit; kTokens tokens of a tile; kStaged of them are loaded together; kGroups wavefronts with the same rows;
+// kDims dimensions that are joined and stored at a time, rows kPitch floats apart, kPart bytes of LDS a wavefront; kResident workgroups a compute unit.
+
+// A request's draft.
+struct Draft {
+    int64_t node0;                           // number of the node of its first row
+    int32_t row0, rows;                      // rows of q and out
+    int32_t before, end;                     // tokens before the draft, tokens; as far as the table's row holds them
+    int32_t blocks, start, tiles;            // of kRows rows; first token of the first tile that may be seen, tiles
+};
+// UNIFORM: r is the same in all lanes (scalar loads).
+template <class T, bool UNIFORM> __device__ __forceinline__ Draft draft_of(const PagedTreeAttentionArgs &a, int r) {
+    typedef typename std::conditional<UNIFORM, ConstI64, const int64_t *>::type Numbers;
+    const Numbers accum = (Numbers)(uintptr_t)a.accum, lens = (Numbers)(uintptr_t)a.lens;
+    constexpr int64_t kFar = int64_t(1) << 40;               // sums and lengths beyond any array
+    const int64_t a0 = min(max(accum[r], -kFar), kFar), a1 = min(max(accum[r + 1], -kFar), kFar), length = min(max(lens[r], (int64_t)0), kFar);
+    const int64_t n = max(a1 - a0, (int64_t)0), room = (int64_t)a.width * a.page.d;
+    const int64_t first = min(max(a0, (int64_t)0), a.tokens), last = min(max(a1, first), a.tokens);
+    Draft d;
+    d.row0 = (int)first;
+    d.rows = (int)(last - first);
+    d.node0 = first - a0;
+    d.end = (int)min(length, room);
+    d.before = (int)min(max(length - n, (int64_t)0), (int64_t)d.end);
+    d.blocks = (int)(((int64_t)d.rows * a.group + T::kRows - 1) / T::kRows);
+    d.start = a.window && d.before > a.window ? (d.before - a.window) & ~(T::kTokens - 1) : 0;
+    d.tiles = d.end > d.start ? (int)((uint32_t)(d.end - 1 - d.start) / T::kTokens) + 1 : 1;
+    return d;
+}
+
+// x y / z, rounded down and up, for 0 <= x y < 2^62 and 0 < z: the quotient of fp64 numbers is off by one at most while it is below 2^51
+// (a division of 64-bit integers is ten times the code).
+__device__ __forceinline__ int64_t tree_ratio(int64_t x, int64_t y, int64_t z) {
+    const int64_t p = x * y;
+    int64_t q = (int64_t)((double)p / (double)z);
+    q -= q * z > p ? 1 : 0;
+    q += p - q * z >= z ? 1 : 0;
+    return q;
+}
+__device__ __forceinline__ int64_t tree_ratio_up(int64_t x, int64_t y, int64_t z) {
+    const int64_t q = tree_ratio(x, y, z);
+    return q + (q * z < x * y);
+}
+
+// Parts in memory, as in paged_attention_kernel.hpp.
+template <class T> __device__ __forceinline__ Shared tree_shared(const TreeWork &w) {
+    return {__builtin_amdgcn_make_buffer_rsrc(w.parts, 0, 2 * w.groups * T::kRows * (int)sizeof(PagedPart), kRsrcFlags),
+            __builtin_amdgcn_make_buffer_rsrc(w.sums, 0, 2 * w.groups * T::kRows * w.pitch * 4, kRsrcFlags), T::kRows, w.pitch};
+}
+
+// Row `x` of a request's rows and query heads of a key head: a row of q and out, and one of the heads.
+struct TreeRow {
+    int node, head;                          // number within the request's rows, query head
+    bool there;
+};
+__device__ __forceinline__ TreeRow tree_row(const PagedTreeAttentionArgs &a, const TreeWork &w, const Draft &d, int h, int64_t x) {
+    TreeRow t;
+    t.there = x < (int64_t)d.rows * a.group;
+    const uint32_t y = t.there ? (uint32_t)x : 0u;
+    t.node = (int)w.group.div(y);
+    t.head = h * a.group + (int)(y - (uint32_t)t.node * w.group.d);
+    return t;
+}
+__device__ __forceinline__ char *tree_out(const PagedTreeAttentionArgs &a, const Draft &d, const TreeRow &t) {
+    return a.out + t.head * a.out_head_bytes + (int64_t)(d.row0 + t.node) * a.out_row_bytes;
+}
+// What accumulators are multiplied with: 0 for rows that see nothing.
+__device__ __forceinline__ float tree_factor(float l, float v_scale) { return l == 0.f ? 0.f : v_scale / l; }
+
+// Joins the parts of a unit for its rows [row0, row1), by a whole workgroup: DC / 4 threads a row, kDeep rows of a thread and four parts of
+// each on their way together (a load from where all dies meet takes some 2 us, however many there are).
+template <int DT, int DC, class T>
+__device__ __forceinline__ void tree_join(const PagedTreeAttentionArgs &a, const TreeWork &w, const TreeLeft &u, int row0, int row1, float v_scale) {
+    constexpr int kLanes = DC / 4, kAtOnce = kTreeThreads / kLanes, kAhead = 4, kDeep = 4;
+    const Draft d = draft_of<T, false>(a, u.request);
+    const Shared shared = tree_shared<T>(w);
+    const int dim0 = 4 * ((int)threadIdx.x % kLanes);
+    const int rows = (int)min((int64_t)row1, (int64_t)d.rows * a.group - (int64_t)u.block * T::kRows);
+#pragma nounroll
+    for (int x0 = row0 + (int)threadIdx.x / kLanes; x0 < rows; x0 += kDeep * kAtOnce) {
+        float m[kDeep], l[kDeep];
+        f32x4 acc[kDeep];
+#pragma unroll
+        for (int z = 0; z < kDeep; ++z) {
+            m[z] = -INFINITY;
+            l[z] = 0.f;
+            acc[z] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+#pragma nounroll
+        for (int p0 = 0; p0 < u.parts; p0 += kAhead) {
+            PagedPart part[kDeep][kAhead];
+            f32x4 sum[kDeep][kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int p = min(p0 + i, u.parts - 1), slot = 2 * (u.begins + p) + (p == 0 ? 1 : 0);
+#pragma unroll
+                for (int z = 0; z < kDeep; ++z) {
+                    const int x = min(x0 + z * kAtOnce, rows - 1);       // (what is there already once more, and not used)
+                    part[z][i] = shared.part(slot, x);
+                    sum[z][i] = shared.sum(slot, x, min(dim0, w.pitch - 4));
+                }
+            }
+#pragma unroll
+            for (int z = 0; z < kDeep; ++z) {
+                float top = m[z];
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    if (p0 + i >= u.parts) part[z][i] = {-INFINITY, 0.f};
+                    top = fmaxf(top, part[z][i].m);
+                }
+                const float base = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f(m[z] - base);
+                l[z] *= old;
+                acc[z] *= old;
+                m[z] = top;
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    const float f = __builtin_amdgcn_exp2f(part[z][i].m - base);
+                    l[z] += f * part[z][i].l;
+                    if (p0 + i < u.parts) acc[z] += f * sum[z][i];
+                }
+            }
+        }
+#pragma unroll
+        for (int z = 0; z < kDeep; ++z)
+            if (const int x = x0 + z * kAtOnce; x < rows && dim0 < a.dim) {
+                if (l[z] == 0.f) acc[z] = f32x4{0.f, 0.f, 0.f, 0.f};
+                store_result<DT>(tree_out(a, d, tree_row(a, w, d, u.h, (int64_t)u.block * T::kRows + x)), dim0, a.dim, acc[z] * tree_factor(l[z], v_scale));
+            }
+    }
+}
+
+__device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
+
+// What a row sees of the tokens from a place on.
+struct Sight {
+    const int64_t *bits;                     // its row of the mask, or NULL
+    uint64_t word0;                          // the first word there
+    int counted, chain, from;                // nodes that have bits; without a mask nodes that it sees; first token of the window
+    bool there;
+    // bit i: token t0 + i
+    __device__ __forceinline__ uint64_t operator()(const Draft &d, int words, uint32_t t0) const {
+        if (!there || t0 >= (uint32_t)d.end) return 0;
+        const int j0 = (int)t0 - d.before, j = max(j0, 0);   // node of the first token; the first node
+        uint64_t x = low_bits(chain - j);
+        if (bits) {
+            x = 0;
+            if (j < counted) {
+                x = (j < 64 ? word0 : (uint64_t)bits[j >> 6]) >> (j & 63);
+                if ((j & 63) && (j >> 6) + 1 < words) x |= (uint64_t)bits[(j >> 6) + 1] << (64 - (j & 63));
+            }
+        }
+        const int before = j - j0;                           // tokens that lie before the draft
+        x = before >= 64 ? ~0ull : x << before | low_bits(before);
+        return x & low_bits(d.end - (int)t0) & ~low_bits(from - (int)t0);
+    }
+};
+__device__ __forceinline__ Sight sight_of(const PagedTreeAttentionArgs &a, const Draft &d, const TreeRow &t, int from) {
+    const int drafted = d.end - d.before;
+    Sight s;
+    s.bits = a.mask ? a.mask + (int64_t)(d.row0 + t.node) * a.mask_stride : nullptr;
+    s.word0 = a.mask ? (uint64_t)s.bits[0] : 0;
+    s.counted = a.mask ? (int)min((int64_t)drafted, 64 * (int64_t)a.words) : drafted;
+    s.chain = (int)min(d.node0 + t.node + 1, (int64_t)drafted);
+    s.from = from;
+    s.there = t.there;
+    return s;
+}
+// The first token that the window leaves of what a row sees.
+__device__ __forceinline__ int window_from(const PagedTreeAttentionArgs &a, const Draft &d, const Sight &s) {
+    int skip = s.chain - a.window, j = 0;                    // nodes that it sees no more
+    if (s.bits) {
+        skip = -a.window;
+        for (j = 0; j < s.counted; j += 64) skip += __builtin_popcountll((uint64_t)s.bits[j >> 6] & low_bits(s.counted - j));
+    }
+    if (skip <= 0) return max(d.before + skip, 0);
+    if (!s.bits) return d.before + skip;
+    for (j = 0;; j += 64) {
+        uint64_t x = (uint64_t)s.bits[j >> 6];
+        const int n = __builtin_popcountll(x);
+        if (n > skip) {
+            for (; skip > 0; --skip) x &= x - 1;
+            return d.before + j + __builtin_ctzll(x);
+        }
+        skip -= n;
+    }
+}
+// Staged tokens from t on that not all rows see: those of the draft, and where the rows' windows begin.
+template <class T> __device__ __forceinline__ bool hidden(const Draft &d, int window, uint32_t t) {
+    const int all_from = window ? max(d.before - window + min(d.end - d.before, window), 0) : 0;
+    return t + T::kStaged > (uint32_t)d.before || t < (uint32_t)all_from;
+}
+
+// A workgroup's LDS besides its tiles.
+template <class T> struct TreeLds {
+    struct Place {
+        int32_t request, unit, tile;
+        int64_t at;
+    };
+    Place places[2];
+    int64_t scan[2 * kTreeWaves], dealt[2];                  // (dealt: tiles, workgroups that have some)
+    int64_t spots[kTreeWaves][2][T::kStaged];                // where the tokens that a wavefront looks after lie, of keys and values
+    float m[kTreeWaves][32], l[kTreeWaves][32];
+    TreeLeft left[2];
+    int32_t joins[2], row_from[T::kRows], odd;               // odd: whether a part's hidden tiles have values that are not finite
+};
+
+// A unit's part that is a workgroup's: tiles [tile, last); `at`: place of the first one in the order of all.
+struct TreeUnit {
+    Draft d;
+    int64_t at;
+    int32_t request, unit, tile, last, h, block;
+};
+template <class T> __device__ __forceinline__ TreeUnit unit_of(int request, int unit, int tile, int64_t at, int64_t end) {
+    const PagedTreeAttentionArgs &a = tree_args().a;
+    TreeUnit u;
+    u.d = draft_of<T, true>(a, request);
+    while (u.d.blocks == 0) u.d = draft_of<T, true>(a, ++request);
+    u.request = request; u.unit = unit; u.tile = tile; u.at = at;
+    u.h = unit / u.d.blocks;
+    u.block = unit - u.h * u.d.blocks;
+    u.last = (int)min((int64_t)u.d.tiles, tile + (end - at));
+    return u;
+}
+// The unit behind it, if the share goes on.
+__device__ __forceinline__ int64_t tree_next(const TreeUnit &u) { return u.at + (u.last - u.tile) + kTreeUnit; }
+template <class T> __device__ __forceinline__ TreeUnit unit_after(const TreeUnit &u, int64_t end) {
+    const bool done = u.unit + 1 == tree_args().a.heads * u.d.blocks;
+    return unit_of<T>(u.request + (done ? 1 : 0), done ? 0 : u.unit + 1, 0, tree_next(u), end);
+}
+
+// The workgroup's share.  Thread i adds up requests [i c, (i + 1) c).  Rows of no request get their zeros here.  Returns where the share ends, or -1
+// if there is none.
+template <class T> __device__ __forceinline__ int64_t tree_deal(TreeLds<T> &sh, TreeUnit &first) {
+    const PagedTreeAttentionArgs &a = tree_args().a;
+    const TreeWork &w = tree_args().w;
+    const int group = (int)blockIdx.x, lane = lane_id(), wave = uniform((int)threadIdx.x >> 6);
+    const int c = (a.requests + kTreeThreads - 1) / kTreeThreads, r0 = (int)threadIdx.x * c, r1 = min(a.requests, r0 + c);
+    int64_t mine = 0, units = 0;
+    for (int r = r0; r < r1; ++r) {
+        const Draft d = draft_of<T, false>(a, r);
+        mine += (int64_t)a.heads * d.blocks * (d.tiles + kTreeUnit);
+        units += (int64_t)a.heads * d.blocks;
+    }
+    int64_t upto = wave_inclusive_scan(mine);
+    units = wave_inclusive_scan(units);
+    if (lane == 63) { sh.scan[wave] = upto; sh.scan[kTreeWaves + wave] = units; }
+    if (threadIdx.x == 0) sh.odd = 0;
+    __syncthreads();
+    int64_t total = 0;
+    units = 0;
+#pragma unroll
+    for (int i = 0; i < kTreeWaves; ++i) {
+        if (i < wave) upto += sh.scan[i];
+        total += sh.scan[i];
+        units += sh.scan[kTreeWaves + i];
+    }
+    total = uniform64(total);
+    const int64_t groups = uniform64(min((int64_t)w.groups, max((total + kTreeShare - 1) / kTreeShare, units)));
+    if (w.left && threadIdx.x == 0) w.left[group].parts = 0;
+    {
+        const int64_t head = a.requests ? min(max(a.accum[0], (int64_t)0), a.tokens) : a.tokens;
+        const int64_t tail = a.requests ? min(max(a.accum[a.requests], head), a.tokens) : a.tokens;
+        for (int64_t i = group; i < head + a.tokens - tail; i += gridDim.x) {
+            char *const out = a.out + (i < head ? i : tail + (i - head)) * a.out_row_bytes;
+            for (int x = (int)threadIdx.x; x < a.heads * a.group * a.dim; x += kTreeThreads) {
+                const int head_of = x / a.dim;
+                *(u16_any *)(out + head_of * a.out_head_bytes + 2 * (x - head_of * a.dim)) = 0;
+            }
+        }
+    }
+    if (group >= groups) return -1;
+    if (threadIdx.x == 0) { sh.dealt[0] = total; sh.dealt[1] = groups; }
+#pragma nounroll
+    for (int k = 0; k < 2; ++k) {
+        int64_t at = tree_ratio(group + k, total, groups);
+        if (at >= total) {
+            if (threadIdx.x == 0) sh.places[k] = {a.requests, 0, 0, total + kTreeUnit};
+        } else if (at < upto && at >= upto - mine) {
+            int64_t before = upto - mine, all;
+            int r = r0 - 1;
+            Draft d;
+            for (all = 0;; before += all) {
+                d = draft_of<T, false>(a, ++r);
+                all = (int64_t)a.heads * d.blocks * (d.tiles + kTreeUnit);
+                if (at < before + all) break;
+            }
+            // (a unit's own cost comes before its tiles: what begins within it begins with tile 0)
+            int unit = (int)tree_ratio(at - before, 1, d.tiles + kTreeUnit), tile = (int)((at - before) - (int64_t)unit * (d.tiles + kTreeUnit)) - kTreeUnit;
+            at += max(-tile, 0);
+            tile = max(tile, 0);
+            if (d.tiles <= kTreeWhole && tile) {             // short units go where most of them lies
+                at -= tile;
+                if (2 * tile > d.tiles) {
+                    at += d.tiles + kTreeUnit;
+                    if (++unit == a.heads * d.blocks) {
+                        unit = 0;
+                        ++r;
+                    }
+                }
+                tile = 0;
+            }
+            sh.places[k] = {r, unit, tile, at};
+        }
+    }
+    __syncthreads();
+    const int64_t end = uniform64(sh.places[1].at), at = uniform64(sh.places[0].at);
+    if (at >= end) return -1;
+    first = unit_of<T>(uniform(sh.places[0].request), uniform(sh.places[0].unit), uniform(sh.places[0].tile), at, end);
+    return end;
+}
+
+// ---- rows of keys and values.  Lane i of a wavefront looks after token i of those that are staged: it asks for the token's page number, two tiles ahead,
+// and leaves the token's place for the lanes that load it.
+typedef const __attribute__((address_space(1))) int32_t *TableRow;       // (loads through a generic pointer would wait for LDS too)
+__device__ __forceinline__ TableRow table_row(const TreeUnit &u) {
+    const PagedTreeAttentionArgs &a = tree_args().a;
+    return (TableRow)(uintptr_t)uniform64((int64_t)(uintptr_t)(a.table + u.request * a.table_stride));
+}
+struct TreeSteps {                           // of pages and tokens, each in registers of its own
+    int64_t k_page, v_page;
+    int k_token, v_token, pages;
+    PageDiv page;
+};
+__device__ __forceinline__ TreeSteps tree_steps() {
+    const PagedTreeAttentionArgs &a = tree_args().a;
+    return {uniform64(a.k.page_bytes), uniform64(a.v.page_bytes), uniform(a.k.token_bytes), uniform(a.v.token_bytes), uniform(a.pages),
+            {(uint32_t)uniform((int)a.page.d), (uint32_t)uniform((int)a.page.mul), (uint32_t)uniform((int)a.page.shift)}};
+}
+__device__ __forceinline__ int32_t look_up(const TreeUnit &u, TableRow row, const PageDiv &page, bool has, uint32_t t) {
+    return has && t < (uint32_t)u.d.end ? row[page.div(t)] : -1;
+}
+// Places of tokens t of page `number`, -1 for those that are not there or on a page outside the cache; the latter's bits.
+template <class T> __device__ __forceinline__ uint64_t tree_aim(int64_t (&spots)[2][T::kStaged], int i, const TreeSteps &by, uint32_t t, int32_t number) {
+    const uint32_t in = t - by.page.div(t) * by.page.d;
+    const bool none = (uint32_t)number >= (uint32_t)by.pages;
+    auto wide = [](uint32_t x, int64_t y) { return (int64_t)((uint64_t)x * (uint32_t)y + ((uint64_t)(x * (uint32_t)((uint64_t)y >> 32)) << 32)); };
+    spots[0][i] = none ? -1 : wide((uint32_t)number, by.k_page) + (int64_t)((uint64_t)in * (uint32_t)by.k_token);
+    spots[1][i] = none ? -1 : wide((uint32_t)number, by.v_page) + (int64_t)((uint64_t)in * (uint32_t)by.v_token);
+    __builtin_amdgcn_wave_barrier();
+    return __ballot(none);
+}
+
+// Takes values that are not finite out of N dwords; says whether there are any.
+template <int DT, bool F8> constexpr uint32_t kNotFinite = F8 ? 0x7fu : DT == 0 ? 0x7c00u : 0x7f80u;
+template <int DT, bool F8, int N> __device__ __forceinline__ bool take_out(uint32_t (&x)[N]) {
+    constexpr int kWidth = F8 ? 8 : 16;
+    constexpr uint32_t kAll = F8 ? 0xffu : 0xffffu;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int b = 0; b < 32; b += kWidth) {
+            const bool hit = (x[i] >> b & kNotFinite<DT, F8>) == kNotFinite<DT, F8>;
+            found |= hit;
+            x[i] &= hit ? ~(kAll << b) : 0xffffffffu;
+        }
+    return found;
+}
+
+// ---- the end of a unit, whose wavefronts have their maxima and sums in sh.m and sh.l.  Dimensions c .. c + kDims of the accumulators lie in LDS, rows
+// kPitch floats apart, kPart bytes a wavefront: they are joined, and given out or left as a part.  By way of LDS so that whole rows are stored.
+template <int DT, class T>
+__device__ __forceinline__ void tree_store(const TreeLds<T> &sh, const char *lds, const TreeUnit &u, int me, int c, float v_scale) {
+    const PagedTreeAttentionArgs &a = tree_args().a;
+    const TreeWork &w = tree_args().w;
+    const bool begun = u.tile == 0, whole = begun && u.last == u.d.tiles;
+    const int slot = 2 * (int)blockIdx.x + (begun ? 1 : 0), wave = uniform(me >> 6);
+    const Shared shared = tree_shared<T>(w);
+    // kGroups > 1: all threads have the rows of all; else each wavefront has its own 32
+    constexpr int kThreads = T::kGroups > 1 ? kTreeThreads : 64, kLanes = T::kDims / 4, kMany = (T::kGroups > 1 ? T::kRows : 32) * kLanes;
+    const int dim1 = 4 * (me % kLanes), dim0 = c + dim1;
+#pragma unroll 4
+    for (int e = T::kGroups > 1 ? me : me & 63; e < kMany; e += kThreads) {
+        const int y = e / kLanes, x = T::kGroups > 1 ? y : 32 * wave + y;
+        const TreeRow t = tree_row(a, w, u.d, u.h, (int64_t)u.block * T::kRows + x);
+        float top = -INFINITY, sum = 0.f;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        if (T::kGroups == 1) {
+            top = sh.m[wave][y];
+            sum = sh.l[wave][y];
+            acc = *(const f32x4 *)((const float *)(lds + wave * T::kPart) + y * T::kPitch + dim1);
+        } else {
+#pragma unroll
+            for (int i = 0; i < T::kGroups; ++i) top = fmaxf(top, sh.m[i][x]);
+            const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int i = 0; i < T::kGroups; ++i) {
+                const float f = __builtin_amdgcn_exp2f(sh.m[i][x] - base);
+                sum += f * sh.l[i][x];
+                acc += f * *(const f32x4 *)((const float *)(lds + i * T::kPart) + x * T::kPitch + dim1);
+            }
+        }
+        if (t.there && dim0 < a.dim) {
+            if (whole) {
+                if (sum == 0.f) acc = f32x4{0.f, 0.f, 0.f, 0.f};
+                store_result<DT>(tree_out(a, u.d, t), dim0, a.dim, acc * tree_factor(sum, v_scale));
+            } else {
+                shared.store(slot, x, dim0, acc);
+                if (dim0 == 0) shared.store(slot, x, PagedPart{top, sum});
+            }
+        }
+    }
+}
+// Values that are not finite, for the rows that see them (an infinity or a NaN of whatever weight is the result's), and what is said of a part.
+// A barrier comes before.
+template <int DT, bool F8, class T> __device__ __forceinline__ void tree_end(TreeLds<T> &sh, const TreeUnit &u, int me, int &unfinished) {
+    const PagedTreeAttentionArgs &a = tree_args().a;
+    const TreeWork &w = tree_args().w;
+    const Draft &d = u.d;
+    const bool begun = u.tile == 0, whole = begun && u.last == d.tiles;
+    const int group = (int)blockIdx.x, slot = 2 * group + (begun ? 1 : 0);
+    if (sh.odd) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        const TableRow row = table_row(u);
+        const Shared shared = tree_shared<T>(w);
+        const uint32_t t_end = (uint32_t)min((int64_t)d.end, (int64_t)d.start + (int64_t)u.last * T::kTokens);
+        for (int e = me; e < T::kRows * a.dim; e += kTreeThreads) {
+            const int x = e / a.dim, dim = e - x * a.dim;
+            const TreeRow t = tree_row(a, w, d, u.h, (int64_t)u.block * T::kRows + x);
+            const Sight s = sight_of(a, d, t, sh.row_from[x]);
+            float add = 0.f;
+#pragma nounroll
+            for (uint32_t tok = (uint32_t)d.start + (uint32_t)u.tile * T::kTokens; tok < t_end; ++tok) {
+                if (!hidden<T>(d, a.window, tok & ~(uint32_t)(T::kStaged - 1)) || !(s(d, a.words, tok) & 1)) continue;
+                const uint32_t at_page = a.page.div(tok);
+                const int32_t in_page = row[at_page];
+                if ((uint32_t)in_page >= (uint32_t)a.pages) continue;
+                const char *const v = a.v.base + u.h * a.v.head_bytes + in_page * a.v.page_bytes + (int64_t)(tok - at_page * a.page.d) * a.v.token_bytes + (F8 ? 1 : 2) * dim;
+                const uint32_t bits = F8 ? *(const uint8_t *)v : *(const u16_any *)v;
+                if ((bits & kNotFinite<DT, F8>) == kNotFinite<DT, F8>) add += F8 ? NAN : Elem<DT>::to_float((uint16_t)bits);
+            }
+            if (t.there && add != 0.f) {
+                if (whole) ((u16_any *)tree_out(a, d, t))[dim] = Elem<DT>::from_float(add);
+                else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, add), shared.sums, shared.sum_at(slot, x, dim), 0, kSharedAux);
+            }
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) sh.odd = 0;
+        __syncthreads();
+    }
+    if (!whole) {
+        const int64_t first = u.at - u.tile, total = uniform64(sh.dealt[0]), groups = uniform64(sh.dealt[1]);
+        TreeLeft left = {begun ? group : (int)tree_ratio_up(first + 1, groups, total) - 1, 0, u.request, u.h, u.block};
+        left.parts = (int)tree_ratio_up(first + d.tiles, groups, total) - left.begins;
+        if (w.left) {
+            if (begun && threadIdx.x == 0) w.left[group] = left;
+        } else {
+            if (threadIdx.x == 0) sh.left[unfinished] = left;
+            ++unfinished;                                    // (the first unit of the share at most, and its last)
+        }
+    }
+}
+// The end of a workgroup: the last one that has left its part of a unit joins them.
+template <int DT, bool F8, int DC, class T> __device__ __forceinline__ void tree_count_in(TreeLds<T> &sh, int unfinished) {
+    const PagedTreeAttentionArgs &a = tree_args().a;
+    const TreeWork &w = tree_args().w;
+    if (w.left || unfinished == 0) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0)
+        for (int i = 0; i < unfinished; ++i) {
+            int32_t *const counter = w.counters + sh.left[i].begins;
+            sh.joins[i] = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == sh.left[i].parts - 1;
+            if (sh.joins[i]) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    __syncthreads();
+#pragma nounroll
+    for (int i = 0; i < unfinished; ++i)
+        if (sh.joins[i]) tree_join<DT, DC, T>(a, w, sh.left[i], 0, T::kRows, F8 ? a.v.scale[sh.left[i].h] : 1.f);
+}
+
+// The joining as a kernel of its own: grid (workgroups of the other, blocks of rows).
+template <int DT, int DC, class T> __global__ void __launch_bounds__(kTreeThreads) paged_tree_join_kernel(TreeArgs args, int rows) {
+    const TreeLeft u = args.w.left[blockIdx.x];
+    const int row0 = (int)blockIdx.y * rows;
+    if (u.parts) tree_join<DT, DC, T>(args.a, args.w, u, row0, row0 + rows, args.a.v.scale ? args.a.v.scale[u.h] : 1.f);
+}
+
+// What is known of the rows: whole 16-byte pieces at multiples of 16 bytes; at any address, of 16 bytes or more; shorter.
+enum TreeRows { kTreePieces, kTreeAny, kTreeShort };
+
+// ------------------------------------------------------------------ host
+template <int DT, int DC, class T, typename K> int tree_launch(K kernel, const PagedTreeAttentionArgs &a, const TreeWork &w, hipStream_t stream) {
+    kernel<<<w.groups, kTreeThreads, T::kLds, stream>>>(TreeArgs{a, w});
+    if (w.left) {
+        constexpr int kRows = std::min(T::kRows, 4 * kTreeThreads / (DC / 4));       // (a round of its threads)
+        paged_tree_join_kernel<DT, DC, T><<<dim3((unsigned)w.groups, T::kRows / kRows), kTreeThreads, 0, stream>>>(TreeArgs{a, w}, kRows);
+    }
+    return hipGetLastError() == hipSuccess ? BA_OK : BA_ERR_LAUNCH;
+}
+
+// Which kernel takes a call, by the rows that a request and key head have on the average: up to 16 or 32 of one set or two of columns, or 128.
+static inline int tree_rows(int64_t tokens, int64_t requests, int64_t group) {
+    const int64_t rows = tokens * group, many = std::max<int64_t>(1, requests);
+    return rows <= 16 * many ? 16 : rows <= 32 * many ? 32 : 128;
+}
+template <int DT, bool F8> int launch_tree_few(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int sets, hipStream_t stream);
+template <int DT, bool F8> int launch_tree_wide(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, hipStream_t stream);
+
+}  // namespace ba

@@ -1,0 +1,6 @@
+// Attention of drafted tokens, few rows: fp16 queries and cache.
+#include "paged_tree_few.hpp"
+
+namespace ba {
+template int launch_tree_few<0, false>(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int sets, hipStream_t stream);
+}  // namespace ba

@@ -1,0 +1,348 @@
+// Attention of drafted tokens for many rows a key head (more than 32 on the average).
+//
+// A unit is 128 rows, 32 a wavefront.  All four wavefronts take the same tile of 64 tokens (32 where there are more than 128 dimensions), which they
+// bring into LDS together, in 16 bits, by way of registers; two tiles lie there in turn.
+//   Scores, S[token][row] = K Q^T on the 32 x 32 x 16 matrix instruction, so that a lane has sixteen tokens of one row: maxima and sums cost one
+//   exchange between the halves, and the probabilities are, packed to 16 bits, the second product's operand as they are, if that runs over the
+//   tokens in the order in which the lanes have them.
+//   Values, O[d][row] = V^T P: the transposing LDS read gives four tokens of a dimension.
+// A row's maximum is only moved when a larger one comes by more than 2^7, so accumulators are scaled seldom.  A probability is rounded to 16 bits once,
+// to the nearest: an error of half a step in each, independent of the others, so that the result's own rounding is the larger half of
+// the whole error; two terms as in the kernel for few rows would cost half as much again of a kernel that is bound by its products.
+#pragma once
+#include "paged_tree_attention.hpp"
+
+namespace ba {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char *LdsBytes;
+typedef __attribute__((address_space(3))) s16x4 *LdsPiece;
+
+template <int DC_> struct TreeWide {
+    static constexpr int DC = DC_, kRows = 128, kGroups = 1;
+    static constexpr int kTokens = DC < 256 ? 64 : 32, kStaged = kTokens;
+    // Bytes between rows in LDS: keys 16 more than whole lines of banks, so that sixteen rows' pieces lie side by side; values 64 more, so
+    // that four rows' 64 bytes do.
+    static constexpr int kPitchK = 2 * DC + 16, kPitchV = 2 * DC + 64, kBuffer = kTokens * (kPitchK + kPitchV), kLds = 2 * kBuffer;
+    static constexpr int kDims = DC < 128 ? DC : 128, kPitch = kDims + 4, kPart = kLds / kTreeWaves;
+    static constexpr int kResident = DC == 64 ? 3 : DC == 128 ? 2 : 1;    // by LDS and registers
+    static_assert(32 * kPitch * 4 <= kPart && kPart % 16 == 0 && kRows * kPitchK <= kLds);
+};
+
+template <int DT> __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (DT == 0) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Probabilities are lifted by a power of two, so that small ones stay apart from zero in fp16.  A maximum that is kept though a
+// larger one has come (by up to 2^7) leaves them below 2^13, and with scores so large that neighbouring fp32 numbers lie 2, 4 or 8 apart,
+// where the difference rounds, below 2^15.
+template <int DT> constexpr float kTreeLift = DT == 0 ? 6.f : 0.f;
+constexpr float kTreeLag = 7.f;
+constexpr int kMatrix = 0x8, kDsRead = 0x100;                // kinds of instructions, for the scheduler
+
+// Greatest and sum over a lane and its partner, 32 lanes on.
+__device__ __forceinline__ float pair_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ __forceinline__ float pair_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+
+// DC: dimensions that the registers hold (64, 128, 256).
+template <int DT, bool F8, int DC, TreeRows ROWS>
+__global__ void __launch_bounds__(kTreeThreads, TreeWide<DC>::kResident) paged_tree_wide_kernel(TreeArgs) {
+    typedef TreeWide<DC> T;
+    constexpr bool ANY = ROWS != kTreePieces, SHORT = ROWS == kTreeShort;
+    constexpr int EB = F8 ? 1 : 2, kPieces = DC * EB / 16;   // bytes of an element, 16-byte pieces of a row
+    constexpr int kAtOnce = kTreeThreads / kPieces, kPasses = T::kTokens / kAtOnce;      // rows of a load, loads of a tile
+    constexpr int KS = DC / 16, DB = DC / 32, SUBS = T::kTokens / 32;
+    static_assert(kTreeThreads % kPieces == 0 && T::kTokens % kAtOnce == 0);
+    const int lane = lane_id(), l32 = lane & 31, half = lane >> 5, wave = uniform((int)threadIdx.x >> 6);
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ TreeLds<T> sh;
+    int unfinished = 0;
+    TreeUnit cur, next;
+    const int64_t end = tree_deal<T>(sh, next);
+    if (end < 0) return;
+
+    const int piece = (int)threadIdx.x % kPieces, line = (int)threadIdx.x / kPieces, mine_at = lane & (T::kTokens - 1);
+    // The rows of the next tile: where they are, then one after the other.  A burst of all of them holds the wavefront up (eight loads 2400 cycles, of
+    // the 7900 that a pair of tiles took), so within a unit they go between the matrix instructions.
+    uint32_t kx[kPasses][4], vx[kPasses][4];
+    uint64_t missing = 0;                                    // bit i: token i of the tile is not there
+    auto first_of = [&](const TreeUnit &u, int i) { return (uint32_t)u.d.start + (uint32_t)i * T::kTokens; };
+    struct Bases {
+        const char *k, *v, *readable;
+        int row_bytes;
+    };
+    auto bases_of = [&](const TreeUnit &u) {
+        const PagedTreeAttentionArgs &a = tree_args().a;
+        const int row_bytes = EB * a.dim, b = SHORT ? 0 : ANY ? min(16 * piece, row_bytes - 16) : 16 * piece;
+        return Bases{a.k.base + u.h * a.k.head_bytes + b, a.v.base + u.h * a.v.head_bytes + b, a.q, row_bytes};
+    };
+    // (tokens that are not there, pieces behind the row's end: anything that can be read, for 16 bytes)
+    auto fetch = [&](uint32_t (&x)[4], const Bases &from, int which, int p) {
+        const int64_t at = sh.spots[wave][which][p * kAtOnce + line];
+        const char *const q = at >= 0 && 16 * piece < from.row_bytes ? (which ? from.v : from.k) + at : from.readable;
+        if (SHORT) load_part<4>(x, q, from.row_bytes);
+        else load_stream<4>(x, q);
+    };
+    auto fetch_all = [&](const Bases &from) {
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) { fetch(kx[p], from, 0, p); fetch(vx[p], from, 1, p); }
+    };
+
+    bool any = false, more = true;
+    int32_t number = look_up(next, table_row(next), tree_args().a.page, true, first_of(next, next.tile) + mine_at);
+    f32x16 o[DB];
+    float m = -INFINITY, l = 0.f;
+    for (;;) {
+        // ---- the next unit's first tile and queries are on their way while this one is finished
+        constexpr int kEach = T::kRows * (DC / 8) / kTreeThreads;
+        u32x4 y[kEach];
+        if (more) {
+            const PagedTreeAttentionArgs &a = tree_args().a;
+            const TreeWork &w = tree_args().w;
+            missing = tree_aim<T>(sh.spots[wave], mine_at, tree_steps(), first_of(next, next.tile) + mine_at, number);
+            fetch_all(bases_of(next));
+            const int me = opaque((int)threadIdx.x);
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                const int x = me + e * kTreeThreads, b = 16 * (x % (DC / 8));
+                const TreeRow t = tree_row(a, w, next.d, next.h, (int64_t)next.block * T::kRows + x / (DC / 8));
+                const char *const p = a.q + t.head * a.q_head_bytes + (int64_t)(next.d.row0 + t.node) * a.q_row_bytes;
+                uint32_t z[4] = {0, 0, 0, 0};
+                if (t.there && b < 2 * a.dim) {
+                    if (ANY && 2 * a.dim < 16) load_part<4>(z, p, 2 * a.dim);
+                    else load_stream<4>(z, p + min(b, 2 * a.dim - 16));
+                }
+                y[e] = u32x4{z[0], z[1], z[2], z[3]};
+            }
+        }
+        if (any) {
+            const int me = opaque((int)threadIdx.x), my32 = me & 31;
+            float *const mineo = (float *)(lds + wave * T::kPart) + my32 * T::kPitch + 4 * (me >> 5 & 1);
+            const float v_scale = F8 ? tree_args().a.v.scale[cur.h] : 1.f;
+            l = pair_sum(l);
+            if ((me & 32) == 0) { sh.m[wave][my32] = m; sh.l[wave][my32] = l; }
+            lds_barrier();
+#pragma unroll
+            for (int c = 0; c < DC; c += T::kDims) {
+#pragma unroll
+                for (int j = 0; j < T::kDims / 32; ++j)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const f32x16 &x = o[c / 32 + j];
+                        *(f32x4 *)(mineo + 32 * j + 8 * g) = f32x4{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
+                    }
+                __builtin_amdgcn_wave_barrier();
+                tree_store<DT, T>(sh, lds, cur, me, c, v_scale);
+                __builtin_amdgcn_wave_barrier();
+            }
+            lds_barrier();
+            tree_end<DT, F8, T>(sh, cur, me, unfinished);
+            if (!more) break;
+        }
+        // ---- queries by way of LDS: column l32 of the scores
+        cur = next;
+        any = true;
+        const PagedTreeAttentionArgs &a = tree_args().a;
+        const Draft &d = cur.d;
+        u32x4 q[KS];
+        const int me = opaque((int)threadIdx.x);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const int x = me + e * kTreeThreads, b = 16 * (x % (DC / 8));
+            uint32_t z[4] = {y[e][0], y[e][1], y[e][2], y[e][3]};
+            if (ANY && 2 * a.dim >= 16) shift_down<4>(z, max(b - (2 * a.dim - 16), 0));
+            *(u32x4 *)(lds + x / (DC / 8) * T::kPitchK + b) = u32x4{z[0], z[1], z[2], z[3]};
+        }
+        lds_barrier();
+#pragma unroll
+        for (int k = 0; k < KS; ++k) q[k] = *(const u32x4 *)(lds + (32 * wave + (me & 31)) * T::kPitchK + 32 * k + 16 * (me >> 5 & 1));
+        lds_barrier();
+        const TableRow row = table_row(cur);
+        Sight sight = sight_of(a, d, tree_row(a, tree_args().w, d, cur.h, (int64_t)cur.block * T::kRows + 32 * wave + (me & 31)), 0);
+        if (a.window) sight.from = window_from(a, d, sight);
+        if ((me & 32) == 0) sh.row_from[32 * wave + (me & 31)] = sight.from;
+        const int window = uniform(a.window), words = uniform(a.words), row_bytes = uniform(EB * a.dim);
+        const TreeSteps by = tree_steps();
+        const Bases from = bases_of(cur);
+        const bool has_piece = 16 * piece < row_bytes;
+        const float to_log2 = a.scale * kLog2e * (F8 ? a.k.scale[cur.h] : 1.f);
+#pragma unroll
+        for (int j = 0; j < DB; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[j][i] = 0.f;
+        m = -INFINITY; l = 0.f;
+        more = tree_next(cur) < end;
+
+        number = look_up(cur, row, by.page, cur.tile + 1 < cur.last, first_of(cur, cur.tile + 1) + mine_at);
+        for (int i = cur.tile; i < cur.last; ++i) {
+            char *const buf = lds + (i & 1) * T::kBuffer;
+            const bool some_hidden = hidden<T>(d, window, first_of(cur, i));
+            // -- the tile's rows, which have arrived, into LDS, in 16 bits
+            if (ANY && !SHORT && 16 * piece + 16 > row_bytes && has_piece) {
+                const int past = 16 * piece - (row_bytes - 16);
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p) { shift_down<4>(kx[p], past); shift_down<4>(vx[p], past); }
+            }
+            if (missing) {
+                // Tokens that are not there, or on a page outside the cache: values of zero; keys of NaN, which is the result of a row that
+                // sees them (zeros behind the row's end: the queries' zeros there would make NaN of those as well).
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int bytes = ANY ? row_bytes - 16 * piece - 4 * x : 4;
+                        const uint32_t nan = (F8 ? 0x7f7f7f7fu : 0x7fff7fffu) & (bytes >= 4 ? 0xffffffffu : bytes <= 0 ? 0u : (1u << (8 * bytes)) - 1u);
+                        const bool none = missing >> (p * kAtOnce + line) & 1;
+                        kx[p][x] = none ? nan : kx[p][x];
+                        vx[p][x] = none ? 0u : vx[p][x];
+                    }
+            }
+            if (row_bytes < 16 * kPieces) {
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        kx[p][x] = has_piece ? kx[p][x] : 0u;
+                        vx[p][x] = has_piece ? vx[p][x] : 0u;
+                    }
+            }
+            if (some_hidden) {
+                bool found = false;
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p) found |= take_out<DT, F8>(vx[p]);
+                if (found) sh.odd = 1;
+            }
+            {
+                char *const kt = buf + line * T::kPitchK + (F8 ? 32 : 16) * piece, *const vt = buf + T::kTokens * T::kPitchK + line * T::kPitchV + (F8 ? 32 : 16) * piece;
+                auto put = [&](char *to, const uint32_t (&x)[4]) {
+                    if (F8) {
+                        *(u32x4 *)to = u32x4{widen<DT, false>(x[0]), widen<DT, true>(x[0]), widen<DT, false>(x[1]), widen<DT, true>(x[1])};
+                        *(u32x4 *)(to + 16) = u32x4{widen<DT, false>(x[2]), widen<DT, true>(x[2]), widen<DT, false>(x[3]), widen<DT, true>(x[3])};
+                    } else {
+                        *(u32x4 *)to = u32x4{x[0], x[1], x[2], x[3]};
+                    }
+                };
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p) {
+                    put(kt + p * kAtOnce * T::kPitchK, kx[p]);
+                    put(vt + p * kAtOnce * T::kPitchV, vx[p]);
+                }
+            }
+            if (i + 1 < cur.last) {
+                missing = tree_aim<T>(sh.spots[wave], mine_at, by, first_of(cur, i + 1) + mine_at, number);
+                if (SHORT) fetch_all(from);
+                number = look_up(cur, row, by.page, i + 2 < cur.last, first_of(cur, i + 2) + mine_at);
+            } else {
+                sh.spots[wave][0][mine_at] = sh.spots[wave][1][mine_at] = -1;
+                __builtin_amdgcn_wave_barrier();
+                if (more) {
+                    next = unit_after<T>(cur, end);
+                    number = look_up(next, table_row(next), by.page, true, first_of(next, next.tile) + mine_at);
+                }
+            }
+            lds_barrier();
+
+            // -- scores of tokens t0 + 32 u + 8 (x / 4) + 4 half + x % 4
+            const uint32_t t0 = first_of(cur, i);
+            const char *const kt = buf + l32 * T::kPitchK + 16 * half;
+            f32x16 s[SUBS];
+#pragma unroll
+            for (int u = 0; u < SUBS; ++u) {
+#pragma unroll
+                for (int x = 0; x < 16; ++x) s[u][x] = 0.f;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    s[u] = mfma32<DT>(*(const u32x4 *)(kt + 32 * u * T::kPitchK + 32 * k), q[k], s[u]);
+                    constexpr int kEvery = SUBS * KS / kPasses;
+                    if (!SHORT && (u * KS + k + 1) % kEvery == 0) fetch(kx[(u * KS + k) / kEvery], from, 0, (u * KS + k) / kEvery);
+                }
+            }
+            // (four operands on their way from LDS ahead of the products)
+            __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
+#pragma unroll
+            for (int n = 0; n < SUBS * KS; ++n) {
+                __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+            }
+#pragma unroll
+            for (int u = 0; u < SUBS; ++u) s[u] *= to_log2;
+            if (some_hidden) {
+                const uint64_t see = sight(d, words, t0) >> (4 * half);
+#pragma unroll
+                for (int u = 0; u < SUBS; ++u)
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) s[u][x] = (uint32_t)(see >> (32 * u)) >> (8 * (x / 4) + x % 4) & 1 ? s[u][x] : -INFINITY;
+            }
+            float top = m;
+#pragma unroll
+            for (int u = 0; u < SUBS; ++u)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) top = fmaxf(top, s[u][x]);
+            top = pair_max(top);
+            if (__any(top > m + kTreeLag)) {                 // (also the first that is seen: m is -inf)
+                const float shrink = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
+                l *= shrink;
+#pragma unroll
+                for (int j = 0; j < DB; ++j) o[j] *= shrink;
+                m = top;
+            }
+            const float base = (m == -INFINITY ? 0.f : m) - kTreeLift<DT>;
+            u32x4 p[2 * SUBS];
+#pragma unroll
+            for (int u = 0; u < SUBS; ++u)
+#pragma unroll
+                for (int x = 0; x < 16; x += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(s[u][x] - base), p1 = __builtin_amdgcn_exp2f(s[u][x + 1] - base);
+                    l += p0 + p1;
+                    p[2 * u + x / 8][x % 8 / 2] = Elem<DT>::pack2(p0, p1);
+                }
+            // -- values: lane (dimension 32 j + l32, half) has tokens 16 k + 4 half + 0 .. 3 and 8 behind those
+            const LdsBytes vt = (LdsBytes)(buf + T::kTokens * T::kPitchK) + (4 * half + (lane & 15) / 4) * T::kPitchV + 32 * (lane >> 4 & 1) + 8 * (lane & 3);
+#pragma unroll
+            for (int k = 0; k < 2 * SUBS; ++k)
+#pragma unroll
+                for (int j = 0; j < DB; ++j) {
+                    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPiece)(vt + 16 * k * T::kPitchV + 64 * j)));
+                    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPiece)(vt + (16 * k + 8) * T::kPitchV + 64 * j)));
+                    o[j] = mfma32<DT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, p[k], o[j]);
+                    constexpr int kEvery = 2 * SUBS * DB / kPasses;
+                    if (!SHORT && (k * DB + j + 1) % kEvery == 0) fetch(vx[(k * DB + j) / kEvery], from, 1, (k * DB + j) / kEvery);
+                }
+            __builtin_amdgcn_sched_group_barrier(kDsRead, 8, 1);
+#pragma unroll
+            for (int n = 0; n < 2 * SUBS * DB; ++n) {
+                __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 1);
+                __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 1);
+            }
+        }
+    }
+    tree_count_in<DT, F8, DC, T>(sh, unfinished);
+}
+
+// ------------------------------------------------------------------ host
+template <int DT, bool F8, int DC, TreeRows ROWS> static int launch_wide_rows(const PagedTreeAttentionArgs &a, const TreeWork &w, hipStream_t stream) {
+    typedef TreeWide<DC> T;
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&paged_tree_wide_kernel<DT, F8, DC, ROWS>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds);
+    if (attr != hipSuccess) return BA_ERR_LAUNCH;
+    return tree_launch<DT, DC, T>(paged_tree_wide_kernel<DT, F8, DC, ROWS>, a, w, stream);
+}
+template <int DT, bool F8> int launch_tree_wide(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, hipStream_t stream) {
+    switch (dim_class(a.dim)) {
+        case 64:
+            if (rows == kTreeShort) return launch_wide_rows<DT, F8, 64, kTreeShort>(a, w, stream);
+            return rows == kTreePieces ? launch_wide_rows<DT, F8, 64, kTreePieces>(a, w, stream) : launch_wide_rows<DT, F8, 64, kTreeAny>(a, w, stream);
+        case 128: return rows == kTreePieces ? launch_wide_rows<DT, F8, 128, kTreePieces>(a, w, stream) : launch_wide_rows<DT, F8, 128, kTreeAny>(a, w, stream);
+        default: return rows == kTreePieces ? launch_wide_rows<DT, F8, 256, kTreePieces>(a, w, stream) : launch_wide_rows<DT, F8, 256, kTreeAny>(a, w, stream);
+    }
+}
+
+}  // namespace ba

@@ -1,0 +1,6 @@
+// Attention of drafted tokens, many rows: bf16 queries, 8-bit cache.
+#include "paged_tree_wide.hpp"
+
+namespace ba {
+template int launch_tree_wide<1, true>(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, hipStream_t stream);
+}  // namespace ba
