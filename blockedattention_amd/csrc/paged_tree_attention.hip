@@ -6,22 +6,22 @@ namespace ba {
 
 #define BA_TREE(DT, F8) \
     extern template int launch_tree_few<DT, F8>(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int sets, hipStream_t stream); \
-    extern template int launch_tree_wide<DT, F8>(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, hipStream_t stream);
+    extern template int launch_tree_wide<DT, F8>(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int waves, hipStream_t stream);
 BA_TREE(0, false)
 BA_TREE(1, false)
 BA_TREE(0, true)
 BA_TREE(1, true)
 
 template <int DC> static int resident_of(int rows) {
-    return rows == 128 ? TreeWide<DC>::kResident : rows == 32 ? TreeFew<DC, 2>::kResident : TreeFew<DC, 1>::kResident;
+    return rows == 128 ? TreeWide<DC, 4>::kResident : rows == 64 ? TreeWide<64, 2>::kResident : rows == 32 ? TreeFew<DC, 2>::kResident : TreeFew<DC, 1>::kResident;
 }
 
 // Workgroups: as many as are resident, or fewer where the longest possible requests would not give each its least share.
 static TreeWork tree_work(int64_t heads, int64_t group, int64_t dim, int64_t tokens, int64_t requests, int64_t width, int64_t page,
                           int64_t window, void *workspace, size_t *bytes) {
     TreeWork w{};
-    const int rows = tree_rows(tokens, requests, group), dims = dim_class(dim);
-    const int64_t tile = rows == 128 ? (dims == 256 ? 32 : 64) : 32 * kTreeWaves;
+    const int rows = tree_rows(tokens, requests, group, dim), dims = dim_class(dim);
+    const int64_t tile = rows < 64 ? 32 * kTreeWaves : rows == 128 && dims == 256 ? 32 : 64;
     const int64_t resident = (int64_t)device_cu_count() * (dims == 64 ? resident_of<64>(rows) : dims == 128 ? resident_of<128>(rows) : resident_of<256>(rows));
     const double units = (double)heads * (tokens * group / rows + requests);
     const double longest = window > 0 ? std::min((double)width * page, (double)window + tokens + tile) : (double)width * page;
@@ -49,19 +49,19 @@ size_t paged_tree_attention_workspace(int64_t heads, int64_t group, int64_t dim,
 
 int launch_paged_tree_attention(const PagedTreeAttentionArgs &a, int dtype, int cache_dtype, int32_t *counters, void *workspace, hipStream_t stream) {
     const bool f8 = cache_dtype == BA_F8_E4M3;
-    const int unit = tree_rows(a.tokens, a.requests, a.group);
+    const int unit = tree_rows(a.tokens, a.requests, a.group, a.dim);
     const uint64_t bits = (uint64_t)a.k.base | (uint64_t)a.v.base | (uint64_t)a.k.page_bytes | (uint64_t)a.v.page_bytes | (uint64_t)a.k.head_bytes |
                           (uint64_t)a.v.head_bytes | (uint64_t)a.k.token_bytes | (uint64_t)a.v.token_bytes;
     const TreeRows rows = a.dim * (f8 ? 1 : 2) < 16 ? kTreeShort : bits % 16 != 0 || a.dim % (f8 ? 16 : 8) != 0 ? kTreeAny : kTreePieces;
     TreeWork w = tree_work(a.heads, a.group, a.dim, a.tokens, a.requests, a.width, a.page.d, a.window, workspace, nullptr);
     w.counters = counters;
     // Joining within the kernel saves the second launch, but one workgroup then reads all parts of a unit.
-    if (unit < 128 && w.groups <= kTreeFewParts * std::max<int64_t>(1, a.tokens * a.group / unit) * a.heads) w.left = nullptr;
+    if (unit < 64 && w.groups <= kTreeFewParts * std::max<int64_t>(1, a.tokens * a.group / unit) * a.heads) w.left = nullptr;
     if (dtype == BA_F16) {
-        if (unit == 128) return f8 ? launch_tree_wide<0, true>(a, w, rows, stream) : launch_tree_wide<0, false>(a, w, rows, stream);
+        if (unit >= 64) return f8 ? launch_tree_wide<0, true>(a, w, rows, unit / 32, stream) : launch_tree_wide<0, false>(a, w, rows, unit / 32, stream);
         return f8 ? launch_tree_few<0, true>(a, w, rows, unit / 16, stream) : launch_tree_few<0, false>(a, w, rows, unit / 16, stream);
     }
-    if (unit == 128) return f8 ? launch_tree_wide<1, true>(a, w, rows, stream) : launch_tree_wide<1, false>(a, w, rows, stream);
+    if (unit >= 64) return f8 ? launch_tree_wide<1, true>(a, w, rows, unit / 32, stream) : launch_tree_wide<1, false>(a, w, rows, unit / 32, stream);
     return f8 ? launch_tree_few<1, true>(a, w, rows, unit / 16, stream) : launch_tree_few<1, false>(a, w, rows, unit / 16, stream);
 }
 

@@ -256,7 +256,7 @@ template <class T> struct TreeLds {
     Place places[2];
     int64_t scan[2 * kTreeWaves], dealt[2];                  // (dealt: tiles, workgroups that have some)
     int64_t spots[kTreeWaves][2][T::kStaged];                // where the tokens that a wavefront looks after lie, of keys and values
-    float m[kTreeWaves][32], l[kTreeWaves][32];
+    float m[kTreeWaves][T::kWaveRows], l[kTreeWaves][T::kWaveRows];
     TreeLeft left[2];
     int32_t joins[2], row_from[T::kRows], odd;               // odd: whether a part's hidden tiles have values that are not finite
 };
@@ -547,12 +547,14 @@ template <int DT, int DC, class T, typename K> int tree_launch(K kernel, const P
     return hipGetLastError() == hipSuccess ? BA_OK : BA_ERR_LAUNCH;
 }
 
-// Which kernel takes a call, by the rows that a request and key head have on the average: up to 16 or 32 of one set or two of columns, or 128.
-static inline int tree_rows(int64_t tokens, int64_t requests, int64_t group) {
+// Rows of a unit, and with them the kernel, by the rows that a request and key head have on the average (64 requests of 4000 tokens, 8 key heads
+// of 128: 16 rows 167 us, with units of 128 211; 32 rows 181 and 213; 64 rows of 128 dimensions 228 with units of 64 and 218 with 128, of
+// 64 dimensions 137 and 161).
+static inline int tree_rows(int64_t tokens, int64_t requests, int64_t group, int64_t dim) {
     const int64_t rows = tokens * group, many = std::max<int64_t>(1, requests);
-    return rows <= 16 * many ? 16 : rows <= 32 * many ? 32 : 128;
+    return rows <= 16 * many ? 16 : rows <= 32 * many ? 32 : rows <= 64 * many && dim <= 64 ? 64 : 128;
 }
 template <int DT, bool F8> int launch_tree_few(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int sets, hipStream_t stream);
-template <int DT, bool F8> int launch_tree_wide(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, hipStream_t stream);
+template <int DT, bool F8> int launch_tree_wide(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int waves, hipStream_t stream);
 
 }  // namespace ba

@@ -11,10 +11,12 @@
 namespace ba {
 
 template <int DC_, int SETS> struct TreeFew {
-    static constexpr int DC = DC_, kRows = 16 * SETS, kGroups = kTreeWaves;
+    static constexpr int DC = DC_, kRows = 16 * SETS, kGroups = kTreeWaves, kWaveRows = kRows;
     static constexpr int kTokens = 32 * kTreeWaves, kStaged = 32;
     static constexpr int kDims = DC < 128 ? DC : 128, kPitch = kDims + 4, kPart = kRows * kPitch * 4, kLds = kTreeWaves * kPart;
-    static constexpr int kResident = DC == 64 ? (SETS == 2 ? 2 : 3) : DC == 128 ? 2 : 1;      // workgroups of a compute unit, by registers
+    // Workgroups of a compute unit, by registers (128 dimensions: two sets with two workgroups, and registers in memory, 233 us for 64 requests of
+    // 4000 tokens and 32 rows a key head, with one 181; one set with three 579 for 500 of 1000, with two 384).
+    static constexpr int kResident = DC == 64 ? (SETS == 2 ? 2 : 3) : DC == 128 && SETS == 1 ? 2 : 1;
 };
 
 // DC: dimensions that the registers hold (64, 128, 256).
@@ -311,19 +313,20 @@ template <int DT, bool F8, int DC, int SETS, TreeRows ROWS> static int launch_fe
     }
     return tree_launch<DT, DC, T>(paged_tree_few_kernel<DT, F8, DC, SETS, ROWS>, a, w, stream);
 }
-template <int DT, bool F8, int SETS> static int launch_few_sets(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, hipStream_t stream) {
-    switch (dim_class(a.dim)) {
-        case 64:
-            if (rows == kTreeShort) return launch_few_rows<DT, F8, 64, SETS, kTreeShort>(a, w, stream);
-            return rows == kTreePieces ? launch_few_rows<DT, F8, 64, SETS, kTreePieces>(a, w, stream) : launch_few_rows<DT, F8, 64, SETS, kTreeAny>(a, w, stream);
-        case 128:
-            return rows == kTreePieces ? launch_few_rows<DT, F8, 128, SETS, kTreePieces>(a, w, stream) : launch_few_rows<DT, F8, 128, SETS, kTreeAny>(a, w, stream);
-        default:
-            return rows == kTreePieces ? launch_few_rows<DT, F8, 256, SETS, kTreePieces>(a, w, stream) : launch_few_rows<DT, F8, 256, SETS, kTreeAny>(a, w, stream);
-    }
+template <int DT, bool F8, int DC, int SETS> static int launch_few_dims(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, hipStream_t stream) {
+    if constexpr (DC == 64)
+        if (rows == kTreeShort) return launch_few_rows<DT, F8, 64, SETS, kTreeShort>(a, w, stream);
+    return rows == kTreePieces ? launch_few_rows<DT, F8, DC, SETS, kTreePieces>(a, w, stream) : launch_few_rows<DT, F8, DC, SETS, kTreeAny>(a, w, stream);
+}
+template <int DT, bool F8, int DC> static int launch_few_sets(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int sets, hipStream_t stream) {
+    return sets == 2 ? launch_few_dims<DT, F8, DC, 2>(a, w, rows, stream) : launch_few_dims<DT, F8, DC, 1>(a, w, rows, stream);
 }
 template <int DT, bool F8> int launch_tree_few(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int sets, hipStream_t stream) {
-    return sets == 2 ? launch_few_sets<DT, F8, 2>(a, w, rows, stream) : launch_few_sets<DT, F8, 1>(a, w, rows, stream);
+    switch (dim_class(a.dim)) {
+        case 64: return launch_few_sets<DT, F8, 64>(a, w, rows, sets, stream);
+        case 128: return launch_few_sets<DT, F8, 128>(a, w, rows, sets, stream);
+        default: return launch_few_sets<DT, F8, 256>(a, w, rows, sets, stream);
+    }
 }
 
 }  // namespace ba

@@ -1,7 +1,7 @@
 // Attention of drafted tokens for many rows a key head (more than 32 on the average).
 //
-// A unit is 128 rows, 32 a wavefront.  All four wavefronts take the same tile of 64 tokens (32 where there are more than 128 dimensions), which they
-// bring into LDS together, in 16 bits, by way of registers; two tiles lie there in turn.
+// A unit is 128 rows, 32 a wavefront, or (64 dimensions) 64, of which two wavefronts have the same and half of the tile's tokens each.  All four wavefronts bring a tile
+// of 64 tokens (32 for 128 rows of more than 128 dimensions) into LDS together, in 16 bits, by way of registers; two tiles lie there in turn.
 //   Scores, S[token][row] = K Q^T on the 32 x 32 x 16 matrix instruction, so that a lane has sixteen tokens of one row: maxima and sums cost one
 //   exchange between the halves, and the probabilities are, packed to 16 bits, the second product's operand as they are, if that runs over the
 //   tokens in the order in which the lanes have them.
@@ -19,15 +19,16 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char *LdsBytes;
 typedef __attribute__((address_space(3))) s16x4 *LdsPiece;
 
-template <int DC_> struct TreeWide {
-    static constexpr int DC = DC_, kRows = 128, kGroups = 1;
-    static constexpr int kTokens = DC < 256 ? 64 : 32, kStaged = kTokens;
+// WR: wavefronts side by side over the rows, 2 or 4.
+template <int DC_, int WR> struct TreeWide {
+    static constexpr int DC = DC_, kRows = 32 * WR, kGroups = kTreeWaves / WR, kWaveRows = kGroups > 1 ? kRows : 32;
+    static constexpr int kTokens = DC < 256 ? 64 : 32, kStaged = kTokens, kMine = kTokens / kGroups;      // kMine: of a wavefront
     // Bytes between rows in LDS: keys 16 more than whole lines of banks, so that sixteen rows' pieces lie side by side; values 64 more, so
     // that four rows' 64 bytes do.
     static constexpr int kPitchK = 2 * DC + 16, kPitchV = 2 * DC + 64, kBuffer = kTokens * (kPitchK + kPitchV), kLds = 2 * kBuffer;
-    static constexpr int kDims = DC < 128 ? DC : 128, kPitch = kDims + 4, kPart = kLds / kTreeWaves;
+    static constexpr int kDims = DC < 128 ? DC : 128, kPitch = kDims + 4, kPart = kWaveRows * kPitch * 4;
     static constexpr int kResident = DC == 64 ? 3 : DC == 128 ? 2 : 1;    // by LDS and registers
-    static_assert(32 * kPitch * 4 <= kPart && kPart % 16 == 0 && kRows * kPitchK <= kLds);
+    static_assert((kGroups > 1 ? kGroups : kTreeWaves) * kPart <= kLds && kRows * kPitchK <= kLds);
 };
 
 template <int DT> __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
@@ -53,15 +54,15 @@ __device__ __forceinline__ float pair_sum(float v) {
 }
 
 // DC: dimensions that the registers hold (64, 128, 256).
-template <int DT, bool F8, int DC, TreeRows ROWS>
-__global__ void __launch_bounds__(kTreeThreads, TreeWide<DC>::kResident) paged_tree_wide_kernel(TreeArgs) {
-    typedef TreeWide<DC> T;
+template <int DT, bool F8, int DC, int WR, TreeRows ROWS>
+__global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) paged_tree_wide_kernel(TreeArgs) {
+    typedef TreeWide<DC, WR> T;
     constexpr bool ANY = ROWS != kTreePieces, SHORT = ROWS == kTreeShort;
     constexpr int EB = F8 ? 1 : 2, kPieces = DC * EB / 16;   // bytes of an element, 16-byte pieces of a row
     constexpr int kAtOnce = kTreeThreads / kPieces, kPasses = T::kTokens / kAtOnce;      // rows of a load, loads of a tile
-    constexpr int KS = DC / 16, DB = DC / 32, SUBS = T::kTokens / 32;
+    constexpr int KS = DC / 16, DB = DC / 32, SUBS = T::kMine / 32;
     static_assert(kTreeThreads % kPieces == 0 && T::kTokens % kAtOnce == 0);
-    const int lane = lane_id(), l32 = lane & 31, half = lane >> 5, wave = uniform((int)threadIdx.x >> 6);
+    const int lane = lane_id(), l32 = lane & 31, half = lane >> 5, wave = uniform((int)threadIdx.x >> 6), wr = wave % WR, wt = wave / WR;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ TreeLds<T> sh;
     int unfinished = 0;
@@ -125,10 +126,12 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<DC>::kResident) paged_t
         }
         if (any) {
             const int me = opaque((int)threadIdx.x), my32 = me & 31;
-            float *const mineo = (float *)(lds + wave * T::kPart) + my32 * T::kPitch + 4 * (me >> 5 & 1);
+            // (kGroups > 1: the rows of all wavefronts with the same tokens are one part)
+            const int part = T::kGroups > 1 ? wt : wave, mine = T::kGroups > 1 ? 32 * wr + my32 : my32;
+            float *const mineo = (float *)(lds + part * T::kPart) + mine * T::kPitch + 4 * (me >> 5 & 1);
             const float v_scale = F8 ? tree_args().a.v.scale[cur.h] : 1.f;
             l = pair_sum(l);
-            if ((me & 32) == 0) { sh.m[wave][my32] = m; sh.l[wave][my32] = l; }
+            if ((me & 32) == 0) { sh.m[part][mine] = m; sh.l[part][mine] = l; }
             lds_barrier();
 #pragma unroll
             for (int c = 0; c < DC; c += T::kDims) {
@@ -139,9 +142,11 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<DC>::kResident) paged_t
                         const f32x16 &x = o[c / 32 + j];
                         *(f32x4 *)(mineo + 32 * j + 8 * g) = f32x4{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
                     }
-                __builtin_amdgcn_wave_barrier();
+                if (T::kGroups > 1) lds_barrier();
+                else __builtin_amdgcn_wave_barrier();
                 tree_store<DT, T>(sh, lds, cur, me, c, v_scale);
-                __builtin_amdgcn_wave_barrier();
+                if (T::kGroups > 1 && c + T::kDims < DC) lds_barrier();
+                else __builtin_amdgcn_wave_barrier();
             }
             lds_barrier();
             tree_end<DT, F8, T>(sh, cur, me, unfinished);
@@ -163,12 +168,12 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<DC>::kResident) paged_t
         }
         lds_barrier();
 #pragma unroll
-        for (int k = 0; k < KS; ++k) q[k] = *(const u32x4 *)(lds + (32 * wave + (me & 31)) * T::kPitchK + 32 * k + 16 * (me >> 5 & 1));
+        for (int k = 0; k < KS; ++k) q[k] = *(const u32x4 *)(lds + (32 * wr + (me & 31)) * T::kPitchK + 32 * k + 16 * (me >> 5 & 1));
         lds_barrier();
         const TableRow row = table_row(cur);
-        Sight sight = sight_of(a, d, tree_row(a, tree_args().w, d, cur.h, (int64_t)cur.block * T::kRows + 32 * wave + (me & 31)), 0);
+        Sight sight = sight_of(a, d, tree_row(a, tree_args().w, d, cur.h, (int64_t)cur.block * T::kRows + 32 * wr + (me & 31)), 0);
         if (a.window) sight.from = window_from(a, d, sight);
-        if ((me & 32) == 0) sh.row_from[32 * wave + (me & 31)] = sight.from;
+        if (wt == 0 && (me & 32) == 0) sh.row_from[32 * wr + (me & 31)] = sight.from;
         const int window = uniform(a.window), words = uniform(a.words), row_bytes = uniform(EB * a.dim);
         const TreeSteps by = tree_steps();
         const Bases from = bases_of(cur);
@@ -251,8 +256,8 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<DC>::kResident) paged_t
             lds_barrier();
 
             // -- scores of tokens t0 + 32 u + 8 (x / 4) + 4 half + x % 4
-            const uint32_t t0 = first_of(cur, i);
-            const char *const kt = buf + l32 * T::kPitchK + 16 * half;
+            const uint32_t t0 = first_of(cur, i) + wt * T::kMine;
+            const char *const kt = buf + (wt * T::kMine + l32) * T::kPitchK + 16 * half;
             f32x16 s[SUBS];
 #pragma unroll
             for (int u = 0; u < SUBS; ++u) {
@@ -305,7 +310,7 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<DC>::kResident) paged_t
                     p[2 * u + x / 8][x % 8 / 2] = Elem<DT>::pack2(p0, p1);
                 }
             // -- values: lane (dimension 32 j + l32, half) has tokens 16 k + 4 half + 0 .. 3 and 8 behind those
-            const LdsBytes vt = (LdsBytes)(buf + T::kTokens * T::kPitchK) + (4 * half + (lane & 15) / 4) * T::kPitchV + 32 * (lane >> 4 & 1) + 8 * (lane & 3);
+            const LdsBytes vt = (LdsBytes)(buf + T::kTokens * T::kPitchK) + (wt * T::kMine + 4 * half + (lane & 15) / 4) * T::kPitchV + 32 * (lane >> 4 & 1) + 8 * (lane & 3);
 #pragma unroll
             for (int k = 0; k < 2 * SUBS; ++k)
 #pragma unroll
@@ -328,20 +333,28 @@ __global__ void __launch_bounds__(kTreeThreads, TreeWide<DC>::kResident) paged_t
 }
 
 // ------------------------------------------------------------------ host
-template <int DT, bool F8, int DC, TreeRows ROWS> static int launch_wide_rows(const PagedTreeAttentionArgs &a, const TreeWork &w, hipStream_t stream) {
-    typedef TreeWide<DC> T;
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&paged_tree_wide_kernel<DT, F8, DC, ROWS>),
+template <int DT, bool F8, int DC, int WR, TreeRows ROWS> static int launch_wide_rows(const PagedTreeAttentionArgs &a, const TreeWork &w, hipStream_t stream) {
+    typedef TreeWide<DC, WR> T;
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(&paged_tree_wide_kernel<DT, F8, DC, WR, ROWS>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds);
     if (attr != hipSuccess) return BA_ERR_LAUNCH;
-    return tree_launch<DT, DC, T>(paged_tree_wide_kernel<DT, F8, DC, ROWS>, a, w, stream);
+    return tree_launch<DT, DC, T>(paged_tree_wide_kernel<DT, F8, DC, WR, ROWS>, a, w, stream);
 }
-template <int DT, bool F8> int launch_tree_wide(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, hipStream_t stream) {
+template <int DT, bool F8, int DC, int WR> static int launch_wide_waves(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, hipStream_t stream) {
+    if constexpr (DC == 64)
+        if (rows == kTreeShort) return launch_wide_rows<DT, F8, DC, WR, kTreeShort>(a, w, stream);
+    return rows == kTreePieces ? launch_wide_rows<DT, F8, DC, WR, kTreePieces>(a, w, stream) : launch_wide_rows<DT, F8, DC, WR, kTreeAny>(a, w, stream);
+}
+template <int DT, bool F8, int DC> static int launch_wide_dims(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int waves, hipStream_t stream) {
+    if constexpr (DC == 64)
+        if (waves == 2) return launch_wide_waves<DT, F8, DC, 2>(a, w, rows, stream);
+    return launch_wide_waves<DT, F8, DC, 4>(a, w, rows, stream);
+}
+template <int DT, bool F8> int launch_tree_wide(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int waves, hipStream_t stream) {
     switch (dim_class(a.dim)) {
-        case 64:
-            if (rows == kTreeShort) return launch_wide_rows<DT, F8, 64, kTreeShort>(a, w, stream);
-            return rows == kTreePieces ? launch_wide_rows<DT, F8, 64, kTreePieces>(a, w, stream) : launch_wide_rows<DT, F8, 64, kTreeAny>(a, w, stream);
-        case 128: return rows == kTreePieces ? launch_wide_rows<DT, F8, 128, kTreePieces>(a, w, stream) : launch_wide_rows<DT, F8, 128, kTreeAny>(a, w, stream);
-        default: return rows == kTreePieces ? launch_wide_rows<DT, F8, 256, kTreePieces>(a, w, stream) : launch_wide_rows<DT, F8, 256, kTreeAny>(a, w, stream);
+        case 64: return launch_wide_dims<DT, F8, 64>(a, w, rows, waves, stream);
+        case 128: return launch_wide_dims<DT, F8, 128>(a, w, rows, waves, stream);
+        default: return launch_wide_dims<DT, F8, 256>(a, w, rows, waves, stream);
     }
 }
 

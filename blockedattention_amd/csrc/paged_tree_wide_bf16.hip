@@ -2,5 +2,5 @@
 #include "paged_tree_wide.hpp"
 
 namespace ba {
-template int launch_tree_wide<1, false>(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, hipStream_t stream);
+template int launch_tree_wide<1, false>(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int waves, hipStream_t stream);
 }  // namespace ba
