@@ -252,6 +252,7 @@ template <class T> struct TreeLds {
     struct Place {
         int32_t request, unit, tile;
         int64_t at;
+        Draft d;
     };
     Place places[2];
     int64_t scan[2 * kTreeWaves], dealt[2];                  // (dealt: tiles, workgroups that have some)
@@ -267,12 +268,9 @@ struct TreeUnit {
     int64_t at;
     int32_t request, unit, tile, last, h, block;
 };
-template <class T> __device__ __forceinline__ TreeUnit unit_of(int request, int unit, int tile, int64_t at, int64_t end) {
-    const PagedTreeAttentionArgs &a = tree_args().a;
+__device__ __forceinline__ TreeUnit unit_of(const Draft &d, int request, int unit, int tile, int64_t at, int64_t end) {
     TreeUnit u;
-    u.d = draft_of<T, true>(a, request);
-    while (u.d.blocks == 0) u.d = draft_of<T, true>(a, ++request);
-    u.request = request; u.unit = unit; u.tile = tile; u.at = at;
+    u.d = d; u.request = request; u.unit = unit; u.tile = tile; u.at = at;
     u.h = unit / u.d.blocks;
     u.block = unit - u.h * u.d.blocks;
     u.last = (int)min((int64_t)u.d.tiles, tile + (end - at));
@@ -281,8 +279,12 @@ template <class T> __device__ __forceinline__ TreeUnit unit_of(int request, int 
 // The unit behind it, if the share goes on.
 __device__ __forceinline__ int64_t tree_next(const TreeUnit &u) { return u.at + (u.last - u.tile) + kTreeUnit; }
 template <class T> __device__ __forceinline__ TreeUnit unit_after(const TreeUnit &u, int64_t end) {
-    const bool done = u.unit + 1 == tree_args().a.heads * u.d.blocks;
-    return unit_of<T>(u.request + (done ? 1 : 0), done ? 0 : u.unit + 1, 0, tree_next(u), end);
+    const PagedTreeAttentionArgs &a = tree_args().a;
+    if (u.unit + 1 < a.heads * u.d.blocks) return unit_of(u.d, u.request, u.unit + 1, 0, tree_next(u), end);
+    int request = u.request + 1;
+    Draft d = draft_of<T, true>(a, request);
+    while (d.blocks == 0) d = draft_of<T, true>(a, ++request);
+    return unit_of(d, request, 0, 0, tree_next(u), end);
 }
 
 // The workgroup's share.  Thread i adds up requests [i c, (i + 1) c).  Rows of no request get their zeros here.  Returns where the share ends, or -1
@@ -292,9 +294,13 @@ template <class T> __device__ __forceinline__ int64_t tree_deal(TreeLds<T> &sh, 
     const TreeWork &w = tree_args().w;
     const int group = (int)blockIdx.x, lane = lane_id(), wave = uniform((int)threadIdx.x >> 6);
     const int c = (a.requests + kTreeThreads - 1) / kTreeThreads, r0 = (int)threadIdx.x * c, r1 = min(a.requests, r0 + c);
+    const int64_t head = a.requests ? min(max(a.accum[0], (int64_t)0), a.tokens) : a.tokens;         // rows of no request: before, from `tail` on
+    const int64_t tail = a.requests ? min(max(a.accum[a.requests], head), a.tokens) : a.tokens;
     int64_t mine = 0, units = 0;
+    Draft front = {};
     for (int r = r0; r < r1; ++r) {
         const Draft d = draft_of<T, false>(a, r);
+        if (r == r0) front = d;
         mine += (int64_t)a.heads * d.blocks * (d.tiles + kTreeUnit);
         units += (int64_t)a.heads * d.blocks;
     }
@@ -314,15 +320,11 @@ template <class T> __device__ __forceinline__ int64_t tree_deal(TreeLds<T> &sh, 
     total = uniform64(total);
     const int64_t groups = uniform64(min((int64_t)w.groups, max((total + kTreeShare - 1) / kTreeShare, units)));
     if (w.left && threadIdx.x == 0) w.left[group].parts = 0;
-    {
-        const int64_t head = a.requests ? min(max(a.accum[0], (int64_t)0), a.tokens) : a.tokens;
-        const int64_t tail = a.requests ? min(max(a.accum[a.requests], head), a.tokens) : a.tokens;
-        for (int64_t i = group; i < head + a.tokens - tail; i += gridDim.x) {
-            char *const out = a.out + (i < head ? i : tail + (i - head)) * a.out_row_bytes;
-            for (int x = (int)threadIdx.x; x < a.heads * a.group * a.dim; x += kTreeThreads) {
-                const int head_of = x / a.dim;
-                *(u16_any *)(out + head_of * a.out_head_bytes + 2 * (x - head_of * a.dim)) = 0;
-            }
+    for (int64_t i = group; i < head + a.tokens - tail; i += gridDim.x) {
+        char *const out = a.out + (i < head ? i : tail + (i - head)) * a.out_row_bytes;
+        for (int x = (int)threadIdx.x; x < a.heads * a.group * a.dim; x += kTreeThreads) {
+            const int head_of = x / a.dim;
+            *(u16_any *)(out + head_of * a.out_head_bytes + 2 * (x - head_of * a.dim)) = 0;
         }
     }
     if (group >= groups) return -1;
@@ -331,16 +333,12 @@ template <class T> __device__ __forceinline__ int64_t tree_deal(TreeLds<T> &sh, 
     for (int k = 0; k < 2; ++k) {
         int64_t at = tree_ratio(group + k, total, groups);
         if (at >= total) {
-            if (threadIdx.x == 0) sh.places[k] = {a.requests, 0, 0, total + kTreeUnit};
+            if (threadIdx.x == 0) sh.places[k] = {a.requests, 0, 0, total + kTreeUnit, front};
         } else if (at < upto && at >= upto - mine) {
-            int64_t before = upto - mine, all;
-            int r = r0 - 1;
-            Draft d;
-            for (all = 0;; before += all) {
-                d = draft_of<T, false>(a, ++r);
-                all = (int64_t)a.heads * d.blocks * (d.tiles + kTreeUnit);
-                if (at < before + all) break;
-            }
+            int64_t before = upto - mine;
+            int r = r0;
+            Draft d = front;
+            for (int64_t all; all = (int64_t)a.heads * d.blocks * (d.tiles + kTreeUnit), at >= before + all; before += all) d = draft_of<T, false>(a, ++r);
             // (a unit's own cost comes before its tiles: what begins within it begins with tile 0)
             int unit = (int)tree_ratio(at - before, 1, d.tiles + kTreeUnit), tile = (int)((at - before) - (int64_t)unit * (d.tiles + kTreeUnit)) - kTreeUnit;
             at += max(-tile, 0);
@@ -351,18 +349,22 @@ template <class T> __device__ __forceinline__ int64_t tree_deal(TreeLds<T> &sh, 
                     at += d.tiles + kTreeUnit;
                     if (++unit == a.heads * d.blocks) {
                         unit = 0;
-                        ++r;
+                        do {
+                            if (++r < a.requests) d = draft_of<T, false>(a, r);
+                        } while (r < a.requests && d.blocks == 0);
                     }
                 }
                 tile = 0;
             }
-            sh.places[k] = {r, unit, tile, at};
+            sh.places[k] = {r, unit, tile, at, d};
         }
     }
     __syncthreads();
     const int64_t end = uniform64(sh.places[1].at), at = uniform64(sh.places[0].at);
     if (at >= end) return -1;
-    first = unit_of<T>(uniform(sh.places[0].request), uniform(sh.places[0].unit), uniform(sh.places[0].tile), at, end);
+    const Draft &d = sh.places[0].d;
+    first = unit_of({uniform64(d.node0), uniform(d.row0), uniform(d.rows), uniform(d.before), uniform(d.end), uniform(d.blocks), uniform(d.start), uniform(d.tiles)},
+                    uniform(sh.places[0].request), uniform(sh.places[0].unit), uniform(sh.places[0].tile), at, end);
     return end;
 }
 
@@ -386,32 +388,41 @@ __device__ __forceinline__ TreeSteps tree_steps() {
 __device__ __forceinline__ int32_t look_up(const TreeUnit &u, TableRow row, const PageDiv &page, bool has, uint32_t t) {
     return has && t < (uint32_t)u.d.end ? row[page.div(t)] : -1;
 }
-// Places of tokens t of page `number`, -1 for those that are not there or on a page outside the cache; the latter's bits.
-template <class T> __device__ __forceinline__ uint64_t tree_aim(int64_t (&spots)[2][T::kStaged], int i, const TreeSteps &by, uint32_t t, int32_t number) {
+// Places of tokens t of page `number`, -1 for those that are not there or on a page outside the cache; all their bits, and of the latter alone.
+struct Missing {
+    uint64_t any, bad;
+};
+template <class T>
+__device__ __forceinline__ Missing tree_aim(int64_t (&spots)[2][T::kStaged], int i, const TreeSteps &by, const TreeUnit &u, uint32_t t, int32_t number) {
     const uint32_t in = t - by.page.div(t) * by.page.d;
     const bool none = (uint32_t)number >= (uint32_t)by.pages;
     auto wide = [](uint32_t x, int64_t y) { return (int64_t)((uint64_t)x * (uint32_t)y + ((uint64_t)(x * (uint32_t)((uint64_t)y >> 32)) << 32)); };
     spots[0][i] = none ? -1 : wide((uint32_t)number, by.k_page) + (int64_t)((uint64_t)in * (uint32_t)by.k_token);
     spots[1][i] = none ? -1 : wide((uint32_t)number, by.v_page) + (int64_t)((uint64_t)in * (uint32_t)by.v_token);
     __builtin_amdgcn_wave_barrier();
-    return __ballot(none);
+    return {__ballot(none), __ballot(none && t < (uint32_t)u.d.end)};
 }
 
-// Takes values that are not finite out of N dwords; says whether there are any.
+// Values that are not finite: `mark` is not 0 behind every dword that has one or more (its halves, for 16 bits, are above the type's exponent).
 template <int DT, bool F8> constexpr uint32_t kNotFinite = F8 ? 0x7fu : DT == 0 ? 0x7c00u : 0x7f80u;
-template <int DT, bool F8, int N> __device__ __forceinline__ bool take_out(uint32_t (&x)[N]) {
+template <int DT, bool F8, int N> __device__ __forceinline__ void watch(uint32_t &mark, const uint32_t (&x)[N]) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (F8) mark |= ((x[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+        else mark = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, mark), __builtin_bit_cast(u16x2, x[i] & 0x7fff7fffu)));
+    }
+}
+template <int DT, bool F8> __device__ __forceinline__ bool seen_odd(uint32_t mark) {
+    return F8 ? mark != 0 : (mark & 0xffffu) >= kNotFinite<DT, F8> || mark >> 16 >= kNotFinite<DT, F8>;
+}
+template <int DT, bool F8, int N> __device__ __forceinline__ void take_out(uint32_t (&x)[N]) {
     constexpr int kWidth = F8 ? 8 : 16;
     constexpr uint32_t kAll = F8 ? 0xffu : 0xffffu;
-    bool found = false;
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int b = 0; b < 32; b += kWidth) {
-            const bool hit = (x[i] >> b & kNotFinite<DT, F8>) == kNotFinite<DT, F8>;
-            found |= hit;
-            x[i] &= hit ? ~(kAll << b) : 0xffffffffu;
-        }
-    return found;
+        for (int b = 0; b < 32; b += kWidth) x[i] &= (x[i] >> b & kNotFinite<DT, F8>) == kNotFinite<DT, F8> ? ~(kAll << b) : 0xffffffffu;
 }
 
 // ---- the end of a unit, whose wavefronts have their maxima and sums in sh.m and sh.l.  Dimensions c .. c + kDims of the accumulators lie in LDS, rows

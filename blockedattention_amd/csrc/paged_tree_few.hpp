@@ -39,7 +39,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeFew<DC, SETS>::kResident)) 
 
     const int mine_at = lane & 31;
     uint32_t kx[2][KL][4], vx[8][L][N];
-    uint32_t missing = 0;                                    // bit i: token i of the wavefront's tile is not there
+    Missing missing = {};                                    // of the wavefront's tile
     u32x4 q[SETS][QK];
     auto first_of = [&](const TreeUnit &u, int i) { return (uint32_t)u.d.start + (uint32_t)i * T::kTokens + 32 * wave; };
     struct Bases {
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeFew<DC, SETS>::kResident)) 
         // ---- the next unit's first tile and queries are on their way while this one is finished
         if (more) {
             const PagedTreeAttentionArgs &a = tree_args().a;
-            missing = (uint32_t)tree_aim<T>(sh.spots[wave], mine_at, tree_steps(), first_of(next, next.tile) + mine_at, number);
+            missing = tree_aim<T>(sh.spots[wave], mine_at, tree_steps(), next, first_of(next, next.tile) + mine_at, number);
             const Bases from = bases_of(next);
             load_keys(from);
             load_values(from);
@@ -192,33 +192,42 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeFew<DC, SETS>::kResident)) 
             const bool some_hidden = hidden<T>(d, window, t0), follows = i + 1 < cur.last;
             settle_keys(row_bytes);
             settle_values(row_bytes);
-            if (missing) {
-                // Tokens that are not there, or on a page outside the cache: values of zero; keys of NaN, which is the result of a row that
-                // sees them (zeros behind the row's end: the queries' zeros there would make NaN of those as well).
+            // Tokens that are not there: values of zero.  On a page outside the cache: keys of NaN as well, which is the result of a row that sees them
+            // (zeros behind the row's end: the queries' zeros there would make NaN of those too).
+            if (missing.any) {
 #pragma unroll
-                for (int y = 0; y < 2; ++y)
-#pragma unroll
-                    for (int k = 0; k < KL; ++k)
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const int bytes = row_bytes - 64 * k - 16 * g - 4 * x;
-                            const uint32_t nan = (F8 ? 0x7f7f7f7fu : 0x7fff7fffu) & (bytes >= 4 ? 0xffffffffu : bytes <= 0 ? 0u : (1u << (8 * bytes)) - 1u);
-                            kx[y][k][x] = missing >> (16 * y + l16) & 1 ? nan : kx[y][k][x];
-                        }
-#pragma unroll
-                for (int y = 0; y < 8; ++y)
+                for (int y = 0; y < 8; ++y) {
+                    const bool none = (uint32_t)missing.any >> (16 * (y / 4) + 4 * g + y % 4) & 1;
 #pragma unroll
                     for (int k = 0; k < L; ++k)
 #pragma unroll
-                        for (int x = 0; x < N; ++x) vx[y][k][x] = missing >> (16 * (y / 4) + 4 * g + y % 4) & 1 ? 0u : vx[y][k][x];
+                        for (int x = 0; x < N; ++x) vx[y][k][x] = none ? 0u : vx[y][k][x];
+                }
+                if (missing.bad)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y)
+#pragma unroll
+                        for (int k = 0; k < KL; ++k)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                const int bytes = row_bytes - 64 * k - 16 * g - 4 * x;
+                                const uint32_t nan = (F8 ? 0x7f7f7f7fu : 0x7fff7fffu) & (bytes >= 4 ? 0xffffffffu : bytes <= 0 ? 0u : (1u << (8 * bytes)) - 1u);
+                                kx[y][k][x] = (uint32_t)missing.bad >> (16 * y + l16) & 1 ? nan : kx[y][k][x];
+                            }
             }
             if (some_hidden) {
-                bool found = false;
+                uint32_t mark = 0;
 #pragma unroll
                 for (int y = 0; y < 8; ++y)
 #pragma unroll
-                    for (int k = 0; k < L; ++k) found |= take_out<DT, F8>(vx[y][k]);
-                if (found) sh.odd = 1;
+                    for (int k = 0; k < L; ++k) watch<DT, F8>(mark, vx[y][k]);
+                if (__any(seen_odd<DT, F8>(mark))) {
+#pragma unroll
+                    for (int y = 0; y < 8; ++y)
+#pragma unroll
+                        for (int k = 0; k < L; ++k) take_out<DT, F8>(vx[y][k]);
+                    sh.odd = 1;
+                }
             }
             // -- scores of tokens t0 + 16 y + 4 g + j
             f32x4 sc[SETS][2];
@@ -233,7 +242,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeFew<DC, SETS>::kResident)) 
                 }
             // the next tile's keys are asked for as soon as the scores have used this one's, its values behind the second product
             if (follows) {
-                missing = (uint32_t)tree_aim<T>(sh.spots[wave], mine_at, by, first_of(cur, i + 1) + mine_at, number);
+                missing = tree_aim<T>(sh.spots[wave], mine_at, by, cur, first_of(cur, i + 1) + mine_at, number);
                 load_keys(from);
                 number = look_up(cur, row, by.page, i + 2 < cur.last, first_of(cur, i + 2) + mine_at);
             } else if (more) {

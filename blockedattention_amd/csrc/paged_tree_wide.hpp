@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
     // The rows of the next tile: where they are, then one after the other.  A burst of all of them holds the wavefront up (eight loads 2400 cycles, of
     // the 7900 that a pair of tiles took), so within a unit they go between the matrix instructions.
     uint32_t kx[kPasses][4], vx[kPasses][4];
-    uint64_t missing = 0;                                    // bit i: token i of the tile is not there
+    Missing missing = {};                                    // of the tile
     auto first_of = [&](const TreeUnit &u, int i) { return (uint32_t)u.d.start + (uint32_t)i * T::kTokens; };
     struct Bases {
         const char *k, *v, *readable;
@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
         if (more) {
             const PagedTreeAttentionArgs &a = tree_args().a;
             const TreeWork &w = tree_args().w;
-            missing = tree_aim<T>(sh.spots[wave], mine_at, tree_steps(), first_of(next, next.tile) + mine_at, number);
+            missing = tree_aim<T>(sh.spots[wave], mine_at, tree_steps(), next, first_of(next, next.tile) + mine_at, number);
             fetch_all(bases_of(next));
             const int me = opaque((int)threadIdx.x);
 #pragma unroll
@@ -196,19 +196,24 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
 #pragma unroll
                 for (int p = 0; p < kPasses; ++p) { shift_down<4>(kx[p], past); shift_down<4>(vx[p], past); }
             }
-            if (missing) {
-                // Tokens that are not there, or on a page outside the cache: values of zero; keys of NaN, which is the result of a row that
-                // sees them (zeros behind the row's end: the queries' zeros there would make NaN of those as well).
+            // Tokens that are not there: values of zero.  On a page outside the cache: keys of NaN as well, which is the result of a row that sees them
+            // (zeros behind the row's end: the queries' zeros there would make NaN of those too).
+            if (missing.any) {
 #pragma unroll
-                for (int p = 0; p < kPasses; ++p)
+                for (int p = 0; p < kPasses; ++p) {
+                    const bool none = missing.any >> (p * kAtOnce + line) & 1;
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const int bytes = ANY ? row_bytes - 16 * piece - 4 * x : 4;
-                        const uint32_t nan = (F8 ? 0x7f7f7f7fu : 0x7fff7fffu) & (bytes >= 4 ? 0xffffffffu : bytes <= 0 ? 0u : (1u << (8 * bytes)) - 1u);
-                        const bool none = missing >> (p * kAtOnce + line) & 1;
-                        kx[p][x] = none ? nan : kx[p][x];
-                        vx[p][x] = none ? 0u : vx[p][x];
-                    }
+                    for (int x = 0; x < 4; ++x) vx[p][x] = none ? 0u : vx[p][x];
+                }
+                if (missing.bad)
+#pragma unroll
+                    for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const int bytes = ANY ? row_bytes - 16 * piece - 4 * x : 4;
+                            const uint32_t nan = (F8 ? 0x7f7f7f7fu : 0x7fff7fffu) & (bytes >= 4 ? 0xffffffffu : bytes <= 0 ? 0u : (1u << (8 * bytes)) - 1u);
+                            kx[p][x] = missing.bad >> (p * kAtOnce + line) & 1 ? nan : kx[p][x];
+                        }
             }
             if (row_bytes < 16 * kPieces) {
 #pragma unroll
@@ -220,10 +225,14 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
                     }
             }
             if (some_hidden) {
-                bool found = false;
+                uint32_t mark = 0;
 #pragma unroll
-                for (int p = 0; p < kPasses; ++p) found |= take_out<DT, F8>(vx[p]);
-                if (found) sh.odd = 1;
+                for (int p = 0; p < kPasses; ++p) watch<DT, F8>(mark, vx[p]);
+                if (__any(seen_odd<DT, F8>(mark))) {
+#pragma unroll
+                    for (int p = 0; p < kPasses; ++p) take_out<DT, F8>(vx[p]);
+                    sh.odd = 1;
+                }
             }
             {
                 char *const kt = buf + line * T::kPitchK + (F8 ? 32 : 16) * piece, *const vt = buf + T::kTokens * T::kPitchK + line * T::kPitchV + (F8 ? 32 : 16) * piece;
@@ -242,7 +251,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
                 }
             }
             if (i + 1 < cur.last) {
-                missing = tree_aim<T>(sh.spots[wave], mine_at, by, first_of(cur, i + 1) + mine_at, number);
+                missing = tree_aim<T>(sh.spots[wave], mine_at, by, cur, first_of(cur, i + 1) + mine_at, number);
                 if (SHORT) fetch_all(from);
                 number = look_up(cur, row, by.page, i + 2 < cur.last, first_of(cur, i + 2) + mine_at);
             } else {
