@@ -238,7 +238,8 @@ __attribute__((visibility("default"))) int ba_paged_fork(const int32_t *table, i
         return BA_ERR_UNSUPPORTED;
     if (!workspace || workspace_bytes < ba_paged_fork_workspace(requests, pages) || ((uintptr_t)workspace & 255)) return BA_ERR_WORKSPACE;
     const PagedForkArgs a{table, shares, free_pages, table_out, shares_out, source, target, state_in, lens, origin, lens_out, state_out,
-                          table_stride, table_out_stride, pool, (int32_t)requests, (int32_t)width, (int32_t)pages, PageDiv::of((uint32_t)page)};
+                          table_stride, table_out_stride, pool, (int32_t)requests, (int32_t)width, (int32_t)pages, PageDiv::of((uint32_t)page),
+                          PageDiv::of((uint32_t)std::max<int64_t>(1, width))};
     return launch_paged_fork(a, workspace, (hipStream_t)stream);
 }
 

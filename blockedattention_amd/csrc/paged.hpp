@@ -117,7 +117,7 @@ struct PagedForkArgs {
     int64_t *lens_out, *state_out;
     int64_t table_stride, table_out_stride, pool;
     int32_t requests, width, pages;
-    PageDiv page;
+    PageDiv page, columns;              // columns: by the width
 };
 
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));

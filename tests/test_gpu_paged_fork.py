@@ -155,8 +155,9 @@ def refused(dev, table, free, state, shares, lens, origin, page, verdict):
     assert all(torch.equal(a, b) for a, b in zip(before, (table, free, state, shares, lens)))
 
 
-def test_refusals_change_nothing(dev):
-    w = Rows(4, 5, 40, 4)
+@pytest.mark.parametrize("pages", [40, 20000])                # one workgroup does all of it, or three launches
+def test_refusals_change_nothing(dev, pages):
+    w = Rows(4, 5, pages, 4)
     w.grow([9, 4, 0, 18])
     w.free = w.free[:2]
     fresh = lambda **change: [change.get(n, t) for n, t in zip(("table", "free", "state", "shares", "lens"), w.tensors(dev))]  # noqa: E731
@@ -169,9 +170,9 @@ def test_refusals_change_nothing(dev):
     refused(dev, *fresh(lens=torch.tensor([9, 4, 21, 18], device=dev)), [0, 1, 2, 3], 4, 4)
     refused(dev, *fresh(lens=torch.tensor([9, 4, 21, 18], device=dev)), [0, 1, 2, 9], 4, 36)
     refused(dev, *fresh(state=torch.tensor([-1, 0], device=dev)), [0, 1, 2, 3], 4, 16)
-    refused(dev, *fresh(state=torch.tensor([41, 0], device=dev)), [0, 1, 2, 3], 4, 16)
+    refused(dev, *fresh(state=torch.tensor([pages + 1, 0], device=dev)), [0, 1, 2, 3], 4, 16)
     refused(dev, *fresh(state=torch.tensor([2, 8], device=dev)), [0, 1, 2, 3], 4, 8)
-    for page in (-1, 40, -(1 << 31), (1 << 31) - 1):
+    for page in (-1, pages, -(1 << 31), (1 << 31) - 1):
         bad = table.clone()
         bad[3, 1] = page
         refused(dev, *fresh(table=bad), [0, 1, 2, -1], 4, 64)
@@ -180,8 +181,9 @@ def test_refusals_change_nothing(dev):
     refused(dev, *fresh(table=bad), [0, 1, 2, -1], 4, 64)
 
 
-def test_too_few_pages(dev):
-    w = Rows(5, 5, 40, 4)
+@pytest.mark.parametrize("pages", [40, 20000])
+def test_too_few_pages(dev, pages):
+    w = Rows(5, 5, pages, 4)
     w.grow([9, 4, 0, 0, 0])
     for n, verdict in ((3, 0), (2, 1), (0, 1)):
         table, free, state, shares, lens = w.tensors(dev)
@@ -206,8 +208,9 @@ def test_empty_tables(dev):
     assert got[1].tolist() == [0, 0, 0] and got[2].tolist() == [0, 0]
 
 
-def test_in_a_graph_and_on_another_stream(dev):
-    w = Rows(40, 20, 2000, 8, seed=4)
+@pytest.mark.parametrize("pages", [2000, 20000])
+def test_in_a_graph_and_on_another_stream(dev, pages):
+    w = Rows(40, 20, pages, 8, seed=4)
     w.grow(torch.randint(0, 150, (40,), generator=w.g).tolist())
     table, free, state, shares, lens = w.tensors(dev)
     origin = torch.arange(40, device=dev)
