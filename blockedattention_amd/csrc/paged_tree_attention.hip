@@ -25,7 +25,7 @@ static TreeWork tree_work(int64_t heads, int64_t group, int64_t dim, int64_t tok
     const int64_t resident = (int64_t)device_cu_count() * (dims == 64 ? resident_of<64>(rows) : dims == 128 ? resident_of<128>(rows) : resident_of<256>(rows));
     const double units = (double)heads * (tokens * group / rows + requests);
     const double longest = window > 0 ? std::min((double)width * page, (double)window + tokens + tile) : (double)width * page;
-    const double most = std::max(units, units * (longest / tile + 1 + kTreeUnit) / kTreeShare + 1);
+    const double most = units * (longest / tile + 1 + kTreeUnit) / kTreeShare + 1;
     w.groups = (int32_t)std::max<int64_t>(1, std::min<int64_t>(BA_PAGED_COUNTERS, (int64_t)std::min<double>((double)resident, most)));
     w.pitch = (int32_t)((dim + 3) & ~int64_t(3));
     w.group = PageDiv::of((uint32_t)group);

@@ -21,7 +21,7 @@ namespace ba {
 
 constexpr int kTreeThreads = kPagedThreads, kTreeWaves = kPagedWaves;
 constexpr int kTreeUnit = 3;                 // what a unit costs besides its tiles, in tiles: queries, first loads, joining, results
-constexpr int kTreeShare = 5;                // of both, what a workgroup has at least, unless units are shorter
+constexpr int kTreeShare = kTreeUnit + 1;    // of both, what a workgroup has at least: a unit of one tile
 constexpr int kTreeWhole = 4;                // units of up to so many tiles are not split between workgroups
 constexpr int kTreeFewParts = 8;             // parts of a unit, on the average, up to which the kernel itself joins them
 
@@ -121,8 +121,8 @@ __device__ __forceinline__ TreeRow tree_row(const PagedTreeAttentionArgs &a, con
 __device__ __forceinline__ char *tree_out(const PagedTreeAttentionArgs &a, const Draft &d, const TreeRow &t) {
     return a.out + t.head * a.out_head_bytes + (int64_t)(d.row0 + t.node) * a.out_row_bytes;
 }
-// What accumulators are multiplied with: 0 for rows that see nothing.
-__device__ __forceinline__ float tree_factor(float l, float v_scale) { return l == 0.f ? 0.f : v_scale / l; }
+// What accumulators are multiplied with: 0 for rows that see nothing.  (The reciprocal is off by 2^-23 at most, of results of 16 bits.)
+__device__ __forceinline__ float tree_factor(float l, float v_scale) { return l == 0.f ? 0.f : v_scale * __builtin_amdgcn_rcpf(l); }
 
 // Joins the parts of a unit for its rows [row0, row1), by a whole workgroup: DC / 4 threads a row, kDeep rows of a thread and four parts of
 // each on their way together (a load from where all dies meet takes some 2 us, however many there are).
@@ -255,7 +255,7 @@ template <class T> struct TreeLds {
         Draft d;
     };
     Place places[2];
-    int64_t scan[2 * kTreeWaves], dealt[2];                  // (dealt: tiles, workgroups that have some)
+    int64_t scan[kTreeWaves], dealt[2];                      // (dealt: tiles, workgroups that have some)
     int64_t spots[kTreeWaves][2][T::kStaged];                // where the tokens that a wavefront looks after lie, of keys and values
     float m[kTreeWaves][T::kWaveRows], l[kTreeWaves][T::kWaveRows];
     TreeLeft left[2];
@@ -287,38 +287,36 @@ template <class T> __device__ __forceinline__ TreeUnit unit_after(const TreeUnit
     return unit_of(d, request, 0, 0, tree_next(u), end);
 }
 
-// The workgroup's share.  Thread i adds up requests [i c, (i + 1) c).  Rows of no request get their zeros here.  Returns where the share ends, or -1
+// The workgroup's share.  The first half of the threads finds where it begins, the other where it ends: thread i of each adds up requests
+// [i c, (i + 1) c).  Rows of no request get their zeros here.  Returns where the share ends, or -1
 // if there is none.
 template <class T> __device__ __forceinline__ int64_t tree_deal(TreeLds<T> &sh, TreeUnit &first) {
     const PagedTreeAttentionArgs &a = tree_args().a;
     const TreeWork &w = tree_args().w;
     const int group = (int)blockIdx.x, lane = lane_id(), wave = uniform((int)threadIdx.x >> 6);
-    const int c = (a.requests + kTreeThreads - 1) / kTreeThreads, r0 = (int)threadIdx.x * c, r1 = min(a.requests, r0 + c);
+    constexpr int kHalf = kTreeThreads / 2, kHalfWaves = kTreeWaves / 2;
+    const int k = wave / kHalfWaves, me = (int)threadIdx.x % kHalf, c = (a.requests + kHalf - 1) / kHalf, r0 = me * c, r1 = min(a.requests, r0 + c);
     const int64_t head = a.requests ? min(max(a.accum[0], (int64_t)0), a.tokens) : a.tokens;         // rows of no request: before, from `tail` on
     const int64_t tail = a.requests ? min(max(a.accum[a.requests], head), a.tokens) : a.tokens;
-    int64_t mine = 0, units = 0;
+    int64_t mine = 0;
     Draft front = {};
     for (int r = r0; r < r1; ++r) {
         const Draft d = draft_of<T, false>(a, r);
         if (r == r0) front = d;
         mine += (int64_t)a.heads * d.blocks * (d.tiles + kTreeUnit);
-        units += (int64_t)a.heads * d.blocks;
     }
     int64_t upto = wave_inclusive_scan(mine);
-    units = wave_inclusive_scan(units);
-    if (lane == 63) { sh.scan[wave] = upto; sh.scan[kTreeWaves + wave] = units; }
+    if (lane == 63) sh.scan[wave] = upto;
     if (threadIdx.x == 0) sh.odd = 0;
     __syncthreads();
     int64_t total = 0;
-    units = 0;
 #pragma unroll
-    for (int i = 0; i < kTreeWaves; ++i) {
-        if (i < wave) upto += sh.scan[i];
+    for (int i = 0; i < kHalfWaves; ++i) {
+        if (i < wave % kHalfWaves) upto += sh.scan[i];
         total += sh.scan[i];
-        units += sh.scan[kTreeWaves + i];
     }
     total = uniform64(total);
-    const int64_t groups = uniform64(min((int64_t)w.groups, max((total + kTreeShare - 1) / kTreeShare, units)));
+    const int64_t groups = uniform64(min((int64_t)w.groups, (total + kTreeShare - 1) / kTreeShare));
     if (w.left && threadIdx.x == 0) w.left[group].parts = 0;
     for (int64_t i = group; i < head + a.tokens - tail; i += gridDim.x) {
         char *const out = a.out + (i < head ? i : tail + (i - head)) * a.out_row_bytes;
@@ -329,38 +327,36 @@ template <class T> __device__ __forceinline__ int64_t tree_deal(TreeLds<T> &sh, 
     }
     if (group >= groups) return -1;
     if (threadIdx.x == 0) { sh.dealt[0] = total; sh.dealt[1] = groups; }
-#pragma nounroll
-    for (int k = 0; k < 2; ++k) {
-        int64_t at = tree_ratio(group + k, total, groups);
-        if (at >= total) {
-            if (threadIdx.x == 0) sh.places[k] = {a.requests, 0, 0, total + kTreeUnit, front};
-        } else if (at < upto && at >= upto - mine) {
-            int64_t before = upto - mine;
-            int r = r0;
-            Draft d = front;
-            for (int64_t all; all = (int64_t)a.heads * d.blocks * (d.tiles + kTreeUnit), at >= before + all; before += all) d = draft_of<T, false>(a, ++r);
-            // (a unit's own cost comes before its tiles: what begins within it begins with tile 0)
-            int unit = (int)tree_ratio(at - before, 1, d.tiles + kTreeUnit), tile = (int)((at - before) - (int64_t)unit * (d.tiles + kTreeUnit)) - kTreeUnit;
-            at += max(-tile, 0);
-            tile = max(tile, 0);
-            if (d.tiles <= kTreeWhole && tile) {             // short units go where most of them lies
-                at -= tile;
-                if (2 * tile > d.tiles) {
-                    at += d.tiles + kTreeUnit;
-                    if (++unit == a.heads * d.blocks) {
-                        unit = 0;
-                        do {
-                            if (++r < a.requests) d = draft_of<T, false>(a, r);
-                        } while (r < a.requests && d.blocks == 0);
-                    }
+    int64_t at = tree_ratio(group + k, total, groups);
+    if (at >= total) {
+        if (me == 0) sh.places[k] = {a.requests, 0, 0, total + kTreeUnit, front};
+    } else if (at < upto && at >= upto - mine) {
+        int64_t before = upto - mine;
+        int r = r0;
+        Draft d = front;
+        for (int64_t all; all = (int64_t)a.heads * d.blocks * (d.tiles + kTreeUnit), at >= before + all; before += all) d = draft_of<T, false>(a, ++r);
+        // (a unit's own cost comes before its tiles: what begins within it begins with tile 0)
+        int unit = (int)tree_ratio(at - before, 1, d.tiles + kTreeUnit), tile = (int)((at - before) - (int64_t)unit * (d.tiles + kTreeUnit)) - kTreeUnit;
+        at += max(-tile, 0);
+        tile = max(tile, 0);
+        if (d.tiles <= kTreeWhole && tile) {             // short units go where most of them lies
+            at -= tile;
+            if (2 * tile > d.tiles) {
+                at += d.tiles + kTreeUnit;
+                if (++unit == a.heads * d.blocks) {
+                    unit = 0;
+                    do {
+                        if (++r < a.requests) d = draft_of<T, false>(a, r);
+                    } while (r < a.requests && d.blocks == 0);
                 }
-                tile = 0;
             }
-            sh.places[k] = {r, unit, tile, at, d};
+            tile = 0;
         }
+        sh.places[k] = {r, unit, tile, at, d};
     }
     __syncthreads();
-    const int64_t end = uniform64(sh.places[1].at), at = uniform64(sh.places[0].at);
+    const int64_t end = uniform64(sh.places[1].at);
+    at = uniform64(sh.places[0].at);
     if (at >= end) return -1;
     const Draft &d = sh.places[0].d;
     first = unit_of({uniform64(d.node0), uniform(d.row0), uniform(d.rows), uniform(d.before), uniform(d.end), uniform(d.blocks), uniform(d.start), uniform(d.tiles)},
