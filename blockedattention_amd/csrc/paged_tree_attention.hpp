@@ -24,6 +24,7 @@ constexpr int kTreeUnit = 3;                 // what a unit costs besides its ti
 constexpr int kTreeShare = kTreeUnit + 1;    // of both, what a workgroup has at least: a unit of one tile
 constexpr int kTreeWhole = 4;                // units of up to so many tiles are not split between workgroups
 constexpr int kTreeFewParts = 8;             // parts of a unit, on the average, up to which the kernel itself joins them
+constexpr int kTreeJoinAhead = 8;            // parts on their way together in that kernel
 
 // A unit of which several workgroups did a part each: the one that has its first tile, how many they are (0: not split).
 struct TreeLeft {
@@ -124,11 +125,11 @@ __device__ __forceinline__ char *tree_out(const PagedTreeAttentionArgs &a, const
 // What accumulators are multiplied with: 0 for rows that see nothing.  (The reciprocal is off by 2^-23 at most, of results of 16 bits.)
 __device__ __forceinline__ float tree_factor(float l, float v_scale) { return l == 0.f ? 0.f : v_scale * __builtin_amdgcn_rcpf(l); }
 
-// Joins the parts of a unit for its rows [row0, row1), by a whole workgroup: DC / 4 threads a row, kDeep rows of a thread and four parts of
+// Joins the parts of a unit for its rows [row0, row1), by a whole workgroup: DC / 4 threads a row, kDeep rows of a thread and kAhead parts of
 // each on their way together (a load from where all dies meet takes some 2 us, however many there are).
-template <int DT, int DC, class T>
+template <int DT, int DC, class T, int kDeep, int kAhead>
 __device__ __forceinline__ void tree_join(const PagedTreeAttentionArgs &a, const TreeWork &w, const TreeLeft &u, int row0, int row1, float v_scale) {
-    constexpr int kLanes = DC / 4, kAtOnce = kTreeThreads / kLanes, kAhead = 4, kDeep = 4;
+    constexpr int kLanes = DC / 4, kAtOnce = kTreeThreads / kLanes;
     const Draft d = draft_of<T, false>(a, u.request);
     const Shared shared = tree_shared<T>(w);
     const int dim0 = 4 * ((int)threadIdx.x % kLanes);
@@ -149,22 +150,23 @@ __device__ __forceinline__ void tree_join(const PagedTreeAttentionArgs &a, const
             f32x4 sum[kDeep][kAhead];
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
-                const int p = min(p0 + i, u.parts - 1), slot = 2 * (u.begins + p) + (p == 0 ? 1 : 0);
+                const int p = p0 + i, slot = 2 * (u.begins + p) + (p == 0 ? 1 : 0);
 #pragma unroll
                 for (int z = 0; z < kDeep; ++z) {
-                    const int x = min(x0 + z * kAtOnce, rows - 1);       // (what is there already once more, and not used)
-                    part[z][i] = shared.part(slot, x);
-                    sum[z][i] = shared.sum(slot, x, min(dim0, w.pitch - 4));
+                    part[z][i] = {-INFINITY, 0.f};
+                    sum[z][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    if (p < u.parts) {
+                        const int x = min(x0 + z * kAtOnce, rows - 1);   // (what is there already once more, and not used)
+                        part[z][i] = shared.part(slot, x);
+                        sum[z][i] = shared.sum(slot, x, min(dim0, w.pitch - 4));
+                    }
                 }
             }
 #pragma unroll
             for (int z = 0; z < kDeep; ++z) {
                 float top = m[z];
 #pragma unroll
-                for (int i = 0; i < kAhead; ++i) {
-                    if (p0 + i >= u.parts) part[z][i] = {-INFINITY, 0.f};
-                    top = fmaxf(top, part[z][i].m);
-                }
+                for (int i = 0; i < kAhead; ++i) top = fmaxf(top, part[z][i].m);
                 const float base = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f(m[z] - base);
                 l[z] *= old;
                 acc[z] *= old;
@@ -173,7 +175,7 @@ __device__ __forceinline__ void tree_join(const PagedTreeAttentionArgs &a, const
                 for (int i = 0; i < kAhead; ++i) {
                     const float f = __builtin_amdgcn_exp2f(part[z][i].m - base);
                     l[z] += f * part[z][i].l;
-                    if (p0 + i < u.parts) acc[z] += f * sum[z][i];
+                    acc[z] += f * sum[z][i];
                 }
             }
         }
@@ -531,14 +533,15 @@ template <int DT, bool F8, int DC, class T> __device__ __forceinline__ void tree
     __syncthreads();
 #pragma nounroll
     for (int i = 0; i < unfinished; ++i)
-        if (sh.joins[i]) tree_join<DT, DC, T>(a, w, sh.left[i], 0, T::kRows, F8 ? a.v.scale[sh.left[i].h] : 1.f);
+        if (sh.joins[i]) tree_join<DT, DC, T, 4, 4>(a, w, sh.left[i], 0, T::kRows, F8 ? a.v.scale[sh.left[i].h] : 1.f);
 }
 
-// The joining as a kernel of its own: grid (workgroups of the other, blocks of rows).
+// The joining as a kernel of its own: grid (workgroups of the other, blocks of rows), one row a thread, so that many workgroups share
+// the loads (32 parts of 32 rows 9 us; with four rows a thread 19).
 template <int DT, int DC, class T> __global__ void __launch_bounds__(kTreeThreads) paged_tree_join_kernel(TreeArgs args, int rows) {
     const TreeLeft u = args.w.left[blockIdx.x];
     const int row0 = (int)blockIdx.y * rows;
-    if (u.parts) tree_join<DT, DC, T>(args.a, args.w, u, row0, row0 + rows, args.a.v.scale ? args.a.v.scale[u.h] : 1.f);
+    if (u.parts) tree_join<DT, DC, T, 1, kTreeJoinAhead>(args.a, args.w, u, row0, row0 + rows, args.a.v.scale ? args.a.v.scale[u.h] : 1.f);
 }
 
 // What is known of the rows: whole 16-byte pieces at multiples of 16 bytes; at any address, of 16 bytes or more; shorter.
@@ -548,7 +551,7 @@ enum TreeRows { kTreePieces, kTreeAny, kTreeShort };
 template <int DT, int DC, class T, typename K> int tree_launch(K kernel, const PagedTreeAttentionArgs &a, const TreeWork &w, hipStream_t stream) {
     kernel<<<w.groups, kTreeThreads, T::kLds, stream>>>(TreeArgs{a, w});
     if (w.left) {
-        constexpr int kRows = std::min(T::kRows, 4 * kTreeThreads / (DC / 4));       // (a round of its threads)
+        constexpr int kRows = std::min(T::kRows, kTreeThreads / (DC / 4));           // (a round of its threads)
         paged_tree_join_kernel<DT, DC, T><<<dim3((unsigned)w.groups, T::kRows / kRows), kTreeThreads, 0, stream>>>(TreeArgs{a, w}, kRows);
     }
     return hipGetLastError() == hipSuccess ? BA_OK : BA_ERR_LAUNCH;

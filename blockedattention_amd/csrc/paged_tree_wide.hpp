@@ -37,8 +37,7 @@ template <int DT> __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32
 }
 
 // Probabilities are lifted by a power of two, so that small ones stay apart from zero in fp16.  A maximum that is kept though a
-// larger one has come (by up to 2^7) leaves them below 2^13, and with scores so large that neighbouring fp32 numbers lie 2, 4 or 8 apart,
-// where the difference rounds, below 2^15.
+// larger one has come (by up to 2^7) leaves them below 2^13.
 template <int DT> constexpr float kTreeLift = DT == 0 ? 6.f : 0.f;
 constexpr float kTreeLag = 7.f;
 constexpr int kMatrix = 0x8, kDsRead = 0x100;                // kinds of instructions, for the scheduler
@@ -51,6 +50,14 @@ __device__ __forceinline__ float pair_max(float v) {
 __device__ __forceinline__ float pair_sum(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
     return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+
+// A sum and both halves of a dword: of probabilities as they are after rounding, which the values are weighed with.
+template <int DT> __device__ __forceinline__ float add_both(uint32_t x, float sum) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    if constexpr (DT == 0) return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, x), __builtin_bit_cast(f16x2, 0x3c003c00u), sum, false);
+    else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x), __builtin_bit_cast(bf16x2, 0x3f803f80u), sum, false);
 }
 
 // DC: dimensions that the registers hold (64, 128, 256).
@@ -100,7 +107,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
     bool any = false, more = true;
     int32_t number = look_up(next, table_row(next), tree_args().a.page, true, first_of(next, next.tile) + mine_at);
     f32x16 o[DB];
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, base = kTreeLift<DT>;      // base: what is added to scores in the exponent
     for (;;) {
         // ---- the next unit's first tile and queries are on their way while this one is finished
         constexpr int kEach = T::kRows * (DC / 8) / kTreeThreads;
@@ -131,7 +138,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
             float *const mineo = (float *)(lds + part * T::kPart) + mine * T::kPitch + 4 * (me >> 5 & 1);
             const float v_scale = F8 ? tree_args().a.v.scale[cur.h] : 1.f;
             l = pair_sum(l);
-            if ((me & 32) == 0) { sh.m[part][mine] = m; sh.l[part][mine] = l; }
+            if ((me & 32) == 0) { sh.m[part][mine] = m == -INFINITY ? m : -base; sh.l[part][mine] = l; }
             lds_barrier();
 #pragma unroll
             for (int c = 0; c < DC; c += T::kDims) {
@@ -158,12 +165,17 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
         const PagedTreeAttentionArgs &a = tree_args().a;
         const Draft &d = cur.d;
         u32x4 q[KS];
+        // scores are scaled within the exponent, by a factor above 0: the sign goes to the queries, and 0 becomes next to nothing
+        const float scale = a.scale * kLog2e * (F8 ? a.k.scale[cur.h] : 1.f), to_log2 = fmaxf(fabsf(scale), 1e-37f), lag = kTreeLag / to_log2;
+        const uint32_t turn = scale < 0.f ? 0x80008000u : 0u;
         const int me = opaque((int)threadIdx.x);
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
             const int x = me + e * kTreeThreads, b = 16 * (x % (DC / 8));
             uint32_t z[4] = {y[e][0], y[e][1], y[e][2], y[e][3]};
             if (ANY && 2 * a.dim >= 16) shift_down<4>(z, max(b - (2 * a.dim - 16), 0));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[i] ^= turn;
             *(u32x4 *)(lds + x / (DC / 8) * T::kPitchK + b) = u32x4{z[0], z[1], z[2], z[3]};
         }
         lds_barrier();
@@ -178,12 +190,11 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
         const TreeSteps by = tree_steps();
         const Bases from = bases_of(cur);
         const bool has_piece = 16 * piece < row_bytes;
-        const float to_log2 = a.scale * kLog2e * (F8 ? a.k.scale[cur.h] : 1.f);
 #pragma unroll
         for (int j = 0; j < DB; ++j)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[j][i] = 0.f;
-        m = -INFINITY; l = 0.f;
+        m = -INFINITY; l = 0.f; base = kTreeLift<DT>;
         more = tree_next(cur) < end;
 
         number = look_up(cur, row, by.page, cur.tile + 1 < cur.last, first_of(cur, cur.tile + 1) + mine_at);
@@ -286,8 +297,6 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
                 __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
             }
-#pragma unroll
-            for (int u = 0; u < SUBS; ++u) s[u] *= to_log2;
             if (some_hidden) {
                 const uint64_t see = sight(d, words, t0) >> (4 * half);
 #pragma unroll
@@ -301,22 +310,30 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
 #pragma unroll
                 for (int x = 0; x < 16; ++x) top = fmaxf(top, s[u][x]);
             top = pair_max(top);
-            if (__any(top > m + kTreeLag)) {                 // (also the first that is seen: m is -inf)
-                const float shrink = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
+            if (__any(top - m > lag)) {                      // (also the first that is seen: m is -inf)
+                const float to = kTreeLift<DT> - (top == -INFINITY ? 0.f : top * to_log2);
+                const float shrink = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(to - base);
                 l *= shrink;
 #pragma unroll
                 for (int j = 0; j < DB; ++j) o[j] *= shrink;
                 m = top;
+                base = to;
             }
-            const float base = (m == -INFINITY ? 0.f : m) - kTreeLift<DT>;
+            // Scores so large that `base` is rounded by more than 2^-8: the maximum is taken off before.
+            float add = base;
+            if (__any(fabsf(base) > 0x1p16f)) {
+#pragma unroll
+                for (int u = 0; u < SUBS; ++u) s[u] -= m == -INFINITY ? 0.f : m;
+                add = kTreeLift<DT>;
+            }
             u32x4 p[2 * SUBS];
 #pragma unroll
             for (int u = 0; u < SUBS; ++u)
 #pragma unroll
                 for (int x = 0; x < 16; x += 2) {
-                    const float p0 = __builtin_amdgcn_exp2f(s[u][x] - base), p1 = __builtin_amdgcn_exp2f(s[u][x + 1] - base);
-                    l += p0 + p1;
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][x], to_log2, add)), p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][x + 1], to_log2, add));
                     p[2 * u + x / 8][x % 8 / 2] = Elem<DT>::pack2(p0, p1);
+                    l = add_both<DT>(p[2 * u + x / 8][x % 8 / 2], l);
                 }
             // -- values: lane (dimension 32 j + l32, half) has tokens 16 k + 4 half + 0 .. 3 and 8 behind those
             const LdsBytes vt = (LdsBytes)(buf + T::kTokens * T::kPitchK) + (wt * T::kMine + 4 * half + (lane & 15) / 4) * T::kPitchV + 32 * (lane >> 4 & 1) + 8 * (lane & 3);

@@ -446,3 +446,44 @@ def test_counters_are_zero_after_every_call(dev):
             assert (counters == 0).all()
         ref, bound = b.expect(0.125)
         assert ((out.double().cpu() - ref).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, -0.0, 1e-39])
+@pytest.mark.parametrize("nodes", [5, 12, 40])
+def test_scales_of_either_sign_and_none(dev, scale, nodes):
+    for dtype, dim, fp8 in ((torch.float16, 64, False), (torch.bfloat16, 128, True), (torch.float16, 84, False), (torch.bfloat16, 7, False)):
+        Drafts([0, 100, 30], [nodes, nodes, 1], 2, 2, dim, 16, dtype, fp8, seed=nodes).check(dev, scale)
+
+
+def test_scores_far_from_zero_for_many_rows(dev):
+    for dtype in (torch.float16, torch.bfloat16):
+        b = Drafts([300], [40], 1, 4, 64, 16, dtype, spread=30.0, seed=3)
+        for scale in (2.0 ** 12, 2.0 ** 19, -2.0 ** 16):
+            got = b.run(dev, scale).double().cpu()
+            k, v = b.values(b.k, None, 0, 340), b.values(b.v, None, 0, 340)
+            q = b.q.double().reshape(1, 4, 40, 64)
+            s = torch.where(b.seen(0, 0), torch.matmul(q, k[:, None].transpose(2, 3)) * scale, -torch.inf)
+            want = v[0][s.argmax(-1)].reshape(4, 40, 64)
+            lead = s.topk(2, -1).values
+            clear = (lead[..., 0] - lead[..., 1] > 2.0 ** -18 * lead[..., 0].abs() + 40).reshape(4, 40)
+            assert clear.sum() >= 100 and got.isfinite().all()
+            assert ((got - want).abs() <= U[dtype] * 2 * want.abs() + 1e-6)[clear].all()
+
+
+@pytest.mark.parametrize("nodes", [3, 8, 40])
+def test_many_small_probabilities(dev, nodes):
+    """60000 tokens of 2^-21 beside one of 1, which have to count in the sum as they do in the result.
+
+    Bound: 2^-10 for a probability as a denormal number of fp16 (2^-15 in steps of 2^-24 after lifting, half a step), 2^-11 for the result, and 2000
+    additions in fp32, a step each, twice."""
+    b = Drafts([60000], [nodes], 1, 4, 16, 64, torch.float16)
+    b.k[torch.isfinite(b.k)] = 0.0
+    b.v[torch.isfinite(b.v)] = 1.0
+    b.k[int(b.table[0, 0]), 0, 0, 0] = 21.0
+    b.v[int(b.table[0, 0]), 0, 0] = 0.0
+    b.q.zero_()
+    b.q[..., 0] = 1.0
+    got = b.run(dev, 0.6931471805599453).double().cpu()
+    n = 60000 - 1 + b.seen(0, 0)[:, 60000:].sum(-1).double()
+    want = (n * 2.0 ** -21 / (1 + n * 2.0 ** -21))[None, :, None]
+    assert ((got - want).abs() <= (2.0 ** -10 + 2.0 ** -11 + 4000 * 2.0 ** -24) * want).all()
