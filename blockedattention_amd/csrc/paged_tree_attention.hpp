@@ -386,17 +386,31 @@ __device__ __forceinline__ TreeSteps tree_steps() {
 __device__ __forceinline__ int32_t look_up(const TreeUnit &u, TableRow row, const PageDiv &page, bool has, uint32_t t) {
     return has && t < (uint32_t)u.d.end ? row[page.div(t)] : -1;
 }
-// Places of tokens t of page `number`, -1 for those that are not there or on a page outside the cache; all their bits, and of the latter alone.
+// Where a unit's rows lie.  The place of a token that is not there is that of the first bytes of the queries, which are as long as a row: whatever
+// is read is there, without a comparison at every load.
+struct TreeBases {
+    const char *k, *v;
+    int64_t k_none, v_none;
+    int row_bytes;
+};
+template <int EB> __device__ __forceinline__ TreeBases tree_bases(const TreeUnit &u) {
+    const PagedTreeAttentionArgs &a = tree_args().a;
+    TreeBases b = {a.k.base + u.h * a.k.head_bytes, a.v.base + u.h * a.v.head_bytes, 0, 0, uniform(EB * a.dim)};
+    b.k_none = uniform64((int64_t)((uintptr_t)a.q - (uintptr_t)b.k));
+    b.v_none = uniform64((int64_t)((uintptr_t)a.q - (uintptr_t)b.v));
+    return b;
+}
+// Places of tokens t of page `number`; the bits of those that are not there or on a page outside the cache, and of the latter alone.
 struct Missing {
     uint64_t any, bad;
 };
 template <class T>
-__device__ __forceinline__ Missing tree_aim(int64_t (&spots)[2][T::kStaged], int i, const TreeSteps &by, const TreeUnit &u, uint32_t t, int32_t number) {
+__device__ __forceinline__ Missing tree_aim(int64_t (&spots)[2][T::kStaged], int i, const TreeSteps &by, const TreeBases &from, const TreeUnit &u, uint32_t t, int32_t number) {
     const uint32_t in = t - by.page.div(t) * by.page.d;
     const bool none = (uint32_t)number >= (uint32_t)by.pages;
     auto wide = [](uint32_t x, int64_t y) { return (int64_t)((uint64_t)x * (uint32_t)y + ((uint64_t)(x * (uint32_t)((uint64_t)y >> 32)) << 32)); };
-    spots[0][i] = none ? -1 : wide((uint32_t)number, by.k_page) + (int64_t)((uint64_t)in * (uint32_t)by.k_token);
-    spots[1][i] = none ? -1 : wide((uint32_t)number, by.v_page) + (int64_t)((uint64_t)in * (uint32_t)by.v_token);
+    spots[0][i] = none ? from.k_none : wide((uint32_t)number, by.k_page) + (int64_t)((uint64_t)in * (uint32_t)by.k_token);
+    spots[1][i] = none ? from.v_none : wide((uint32_t)number, by.v_page) + (int64_t)((uint64_t)in * (uint32_t)by.v_token);
     __builtin_amdgcn_wave_barrier();
     return {__ballot(none), __ballot(none && t < (uint32_t)u.d.end)};
 }

@@ -42,21 +42,12 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeFew<DC, SETS>::kResident)) 
     Missing missing = {};                                    // of the wavefront's tile
     u32x4 q[SETS][QK];
     auto first_of = [&](const TreeUnit &u, int i) { return (uint32_t)u.d.start + (uint32_t)i * T::kTokens + 32 * wave; };
-    struct Bases {
-        const char *k, *v, *readable;
-        int row_bytes;
-    };
-    auto bases_of = [&](const TreeUnit &u) {
-        const PagedTreeAttentionArgs &a = tree_args().a;
-        return Bases{a.k.base + u.h * a.k.head_bytes, a.v.base + u.h * a.v.head_bytes, a.q, uniform(EB * a.dim)};
-    };
     // The rows of a tile: a lane has 16-byte pieces of tokens l16 and 16 + l16 of the keys, E dimensions at a time of tokens 16 i + 4 g + j of the values.
-    // (Tokens that are not there: the first bytes of the queries, which are as long as a row.  Pieces behind a row's end: the row's last bytes.)
-    auto load_keys = [&](const Bases &from) {
+    // (Pieces behind a row's end: the row's last bytes.)
+    auto load_keys = [&](const TreeBases &from) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int64_t at = sh.spots[wave][0][16 * i + l16];
-            const char *const p = at >= 0 ? from.k + at : from.readable;
+            const char *const p = from.k + sh.spots[wave][0][16 * i + l16];
 #pragma unroll
             for (int k = 0; k < KL; ++k) {
                 const int b = 64 * k + 16 * g;
@@ -65,11 +56,10 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeFew<DC, SETS>::kResident)) 
             }
         }
     };
-    auto load_values = [&](const Bases &from) {
+    auto load_values = [&](const TreeBases &from) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int64_t at = sh.spots[wave][1][16 * (i / 4) + 4 * g + i % 4];
-            const char *const p = at >= 0 ? from.v + at : from.readable;
+            const char *const p = from.v + sh.spots[wave][1][16 * (i / 4) + 4 * g + i % 4];
 #pragma unroll
             for (int k = 0; k < L; ++k) {
                 const int b = EB * E * (16 * k + l16);
@@ -111,8 +101,8 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeFew<DC, SETS>::kResident)) 
         // ---- the next unit's first tile and queries are on their way while this one is finished
         if (more) {
             const PagedTreeAttentionArgs &a = tree_args().a;
-            missing = tree_aim<T>(sh.spots[wave], mine_at, tree_steps(), next, first_of(next, next.tile) + mine_at, number);
-            const Bases from = bases_of(next);
+            const TreeBases from = tree_bases<EB>(next);
+            missing = tree_aim<T>(sh.spots[wave], mine_at, tree_steps(), from, next, first_of(next, next.tile) + mine_at, number);
             load_keys(from);
             load_values(from);
             const int me = opaque(lane);
@@ -177,7 +167,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeFew<DC, SETS>::kResident)) 
         }
         const int window = uniform(a.window), words = uniform(a.words), row_bytes = uniform(EB * a.dim);
         const TreeSteps by = tree_steps();
-        const Bases from = bases_of(cur);
+        const TreeBases from = tree_bases<EB>(cur);
         const float to_log2 = a.scale * kLog2e * (F8 ? a.k.scale[cur.h] : 1.f);
 #pragma unroll
         for (int z = 0; z < SETS; ++z) {
@@ -242,7 +232,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeFew<DC, SETS>::kResident)) 
                 }
             // the next tile's keys are asked for as soon as the scores have used this one's, its values behind the second product
             if (follows) {
-                missing = tree_aim<T>(sh.spots[wave], mine_at, by, cur, first_of(cur, i + 1) + mine_at, number);
+                missing = tree_aim<T>(sh.spots[wave], mine_at, by, from, cur, first_of(cur, i + 1) + mine_at, number);
                 load_keys(from);
                 number = look_up(cur, row, by.page, i + 2 < cur.last, first_of(cur, i + 2) + mine_at);
             } else if (more) {

@@ -83,23 +83,14 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
     uint32_t kx[kPasses][4], vx[kPasses][4];
     Missing missing = {};                                    // of the tile
     auto first_of = [&](const TreeUnit &u, int i) { return (uint32_t)u.d.start + (uint32_t)i * T::kTokens; };
-    struct Bases {
-        const char *k, *v, *readable;
-        int row_bytes;
-    };
-    auto bases_of = [&](const TreeUnit &u) {
-        const PagedTreeAttentionArgs &a = tree_args().a;
-        const int row_bytes = EB * a.dim, b = SHORT ? 0 : ANY ? min(16 * piece, row_bytes - 16) : 16 * piece;
-        return Bases{a.k.base + u.h * a.k.head_bytes + b, a.v.base + u.h * a.v.head_bytes + b, a.q, row_bytes};
-    };
-    // (tokens that are not there, pieces behind the row's end: anything that can be read, for 16 bytes)
-    auto fetch = [&](uint32_t (&x)[4], const Bases &from, int which, int p) {
-        const int64_t at = sh.spots[wave][which][p * kAtOnce + line];
-        const char *const q = at >= 0 && 16 * piece < from.row_bytes ? (which ? from.v : from.k) + at : from.readable;
+    // (pieces behind the row's end: its last bytes)
+    auto fetch = [&](uint32_t (&x)[4], const TreeBases &from, int which, int p) {
+        const int b = SHORT ? 0 : min(16 * piece, from.row_bytes - 16);
+        const char *const q = (which ? from.v : from.k) + b + sh.spots[wave][which][p * kAtOnce + line];
         if (SHORT) load_part<4>(x, q, from.row_bytes);
         else load_stream<4>(x, q);
     };
-    auto fetch_all = [&](const Bases &from) {
+    auto fetch_all = [&](const TreeBases &from) {
 #pragma unroll
         for (int p = 0; p < kPasses; ++p) { fetch(kx[p], from, 0, p); fetch(vx[p], from, 1, p); }
     };
@@ -115,8 +106,9 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
         if (more) {
             const PagedTreeAttentionArgs &a = tree_args().a;
             const TreeWork &w = tree_args().w;
-            missing = tree_aim<T>(sh.spots[wave], mine_at, tree_steps(), next, first_of(next, next.tile) + mine_at, number);
-            fetch_all(bases_of(next));
+            const TreeBases from = tree_bases<EB>(next);
+            missing = tree_aim<T>(sh.spots[wave], mine_at, tree_steps(), from, next, first_of(next, next.tile) + mine_at, number);
+            fetch_all(from);
             const int me = opaque((int)threadIdx.x);
 #pragma unroll
             for (int e = 0; e < kEach; ++e) {
@@ -188,7 +180,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
         if (wt == 0 && (me & 32) == 0) sh.row_from[32 * wr + (me & 31)] = sight.from;
         const int window = uniform(a.window), words = uniform(a.words), row_bytes = uniform(EB * a.dim);
         const TreeSteps by = tree_steps();
-        const Bases from = bases_of(cur);
+        const TreeBases from = tree_bases<EB>(cur);
         const bool has_piece = 16 * piece < row_bytes;
 #pragma unroll
         for (int j = 0; j < DB; ++j)
@@ -262,11 +254,12 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
                 }
             }
             if (i + 1 < cur.last) {
-                missing = tree_aim<T>(sh.spots[wave], mine_at, by, cur, first_of(cur, i + 1) + mine_at, number);
+                missing = tree_aim<T>(sh.spots[wave], mine_at, by, from, cur, first_of(cur, i + 1) + mine_at, number);
                 if (SHORT) fetch_all(from);
                 number = look_up(cur, row, by.page, i + 2 < cur.last, first_of(cur, i + 2) + mine_at);
             } else {
-                sh.spots[wave][0][mine_at] = sh.spots[wave][1][mine_at] = -1;
+                sh.spots[wave][0][mine_at] = from.k_none;
+                sh.spots[wave][1][mine_at] = from.v_none;
                 __builtin_amdgcn_wave_barrier();
                 if (more) {
                     next = unit_after<T>(cur, end);
