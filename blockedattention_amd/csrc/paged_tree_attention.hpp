@@ -8,7 +8,7 @@
 // Split.  A unit is a block of rows (nodes and the query heads that share a key head, heads fastest) of a request and key head.  Its tokens are
 // cut into tiles, and the tiles of all units, in the order of requests, key heads and blocks, are dealt out to the workgroups in equal
 // shares, with a constant for what a unit costs besides; sums and lengths are on the GPU only, so every workgroup adds them up itself.
-// A unit that lies in one share is done then; for others each workgroup leaves maxima, sums and fp32 accumulators in memory.
+// (Where there are about as many units as workgroups, each gets a unit.)  A unit that lies in one share is done then; for others each workgroup leaves maxima, sums and fp32 accumulators in memory.
 // Where units have few parts, each counts itself in and the last one joins them all, in the order of the tokens whoever it is; else a
 // second kernel does.
 //
@@ -22,6 +22,10 @@ namespace ba {
 constexpr int kTreeThreads = kPagedThreads, kTreeWaves = kPagedWaves;
 constexpr int kTreeUnit = 3;                 // what a unit costs besides its tiles, in tiles: queries, first loads, joining, results
 constexpr int kTreeShare = kTreeUnit + 1;    // of both, what a workgroup has at least: a unit of one tile
+// Where each unit can have a workgroup, it gets one, unless the longest has more than so many tiles above an equal share.  (60 requests of 1000 tokens,
+// 8 key heads, 480 units of 15 tiles for 512 workgroups: 82 us, 102 when split evenly.  28 requests of up to 1000, 12 key heads: 38.7 split, 43.4 whole;
+// there it is 4 tiles above a share of 7.)
+constexpr int kTreeSplit = 4;
 constexpr int kTreeWhole = 4;                // units of up to so many tiles are not split between workgroups
 constexpr int kTreeFewParts = 8;             // parts of a unit, on the average, up to which the kernel itself joins them
 constexpr int kTreeJoinAhead = 8;            // parts on their way together in that kernel
@@ -258,6 +262,7 @@ template <class T> struct TreeLds {
     };
     Place places[2];
     int64_t scan[kTreeWaves], dealt[2];                      // (dealt: tiles, workgroups that have some)
+    int32_t units[kTreeWaves], longest[kTreeWaves];
     int64_t spots[kTreeWaves][2][T::kStaged];                // where the tokens that a wavefront looks after lie, of keys and values
     float m[kTreeWaves][T::kWaveRows], l[kTreeWaves][T::kWaveRows];
     TreeLeft left[2];
@@ -301,24 +306,34 @@ template <class T> __device__ __forceinline__ int64_t tree_deal(TreeLds<T> &sh, 
     const int64_t head = a.requests ? min(max(a.accum[0], (int64_t)0), a.tokens) : a.tokens;         // rows of no request: before, from `tail` on
     const int64_t tail = a.requests ? min(max(a.accum[a.requests], head), a.tokens) : a.tokens;
     int64_t mine = 0;
+    int units = 0, longest = 0;                              // (as far as there are workgroups; tiles)
     Draft front = {};
     for (int r = r0; r < r1; ++r) {
         const Draft d = draft_of<T, false>(a, r);
         if (r == r0) front = d;
         mine += (int64_t)a.heads * d.blocks * (d.tiles + kTreeUnit);
+        units = (int)min(units + (int64_t)a.heads * d.blocks, (int64_t)BA_PAGED_COUNTERS + 1);
+        longest = d.blocks ? max(longest, d.tiles) : longest;
     }
     int64_t upto = wave_inclusive_scan(mine);
-    if (lane == 63) sh.scan[wave] = upto;
+    int units_upto = wave_inclusive_scan(units);
+    longest = wave_max_nonneg(longest);
+    if (lane == 63) { sh.scan[wave] = upto; sh.units[wave] = units_upto; sh.longest[wave] = longest; }
     if (threadIdx.x == 0) sh.odd = 0;
     __syncthreads();
     int64_t total = 0;
+    int all_units = 0;
 #pragma unroll
     for (int i = 0; i < kHalfWaves; ++i) {
-        if (i < wave % kHalfWaves) upto += sh.scan[i];
+        if (i < wave % kHalfWaves) { upto += sh.scan[i]; units_upto += sh.units[i]; }
         total += sh.scan[i];
+        all_units += sh.units[i];
+        longest = max(longest, sh.longest[i]);
     }
     total = uniform64(total);
-    const int64_t groups = uniform64(min((int64_t)w.groups, (total + kTreeShare - 1) / kTreeShare));
+    int64_t groups = uniform64(min((int64_t)w.groups, (total + kTreeShare - 1) / kTreeShare));
+    const bool whole = uniform(all_units) <= groups && (uniform(longest) + kTreeUnit - kTreeSplit) * groups <= total;
+    if (whole) groups = uniform(all_units);
     if (w.left && threadIdx.x == 0) w.left[group].parts = 0;
     for (int64_t i = group; i < head + a.tokens - tail; i += gridDim.x) {
         char *const out = a.out + (i < head ? i : tail + (i - head)) * a.out_row_bytes;
@@ -329,14 +344,19 @@ template <class T> __device__ __forceinline__ int64_t tree_deal(TreeLds<T> &sh, 
     }
     if (group >= groups) return -1;
     if (threadIdx.x == 0) { sh.dealt[0] = total; sh.dealt[1] = groups; }
-    int64_t at = tree_ratio(group + k, total, groups);
-    if (at >= total) {
+    const int number = group + k;
+    int64_t at = whole ? 0 : tree_ratio(number, total, groups);
+    if (number >= groups) {
         if (me == 0) sh.places[k] = {a.requests, 0, 0, total + kTreeUnit, front};
-    } else if (at < upto && at >= upto - mine) {
+    } else if (whole ? number < units_upto && number >= units_upto - units : at < upto && at >= upto - mine) {
         int64_t before = upto - mine;
-        int r = r0;
+        int r = r0, passed = units_upto - units;
         Draft d = front;
-        for (int64_t all; all = (int64_t)a.heads * d.blocks * (d.tiles + kTreeUnit), at >= before + all; before += all) d = draft_of<T, false>(a, ++r);
+        for (int64_t all; all = (int64_t)a.heads * d.blocks * (d.tiles + kTreeUnit), whole ? number >= passed + a.heads * d.blocks : at >= before + all; before += all) {
+            passed += a.heads * d.blocks;
+            d = draft_of<T, false>(a, ++r);
+        }
+        if (whole) at = before + (int64_t)(number - passed) * (d.tiles + kTreeUnit);
         // (a unit's own cost comes before its tiles: what begins within it begins with tile 0)
         int unit = (int)tree_ratio(at - before, 1, d.tiles + kTreeUnit), tile = (int)((at - before) - (int64_t)unit * (d.tiles + kTreeUnit)) - kTreeUnit;
         at += max(-tile, 0);
