@@ -156,7 +156,7 @@ __attribute__((visibility("default"))) size_t ba_paged_tree_attention_workspace(
                                                                                 int64_t requests, int64_t width) {
     ba_paged_cache plain;
     if (check_cache(cache, &plain) != BA_OK || heads < 1 || heads % cache->heads || tokens < 1 || requests < 0 || width < 0) return 0;
-    return paged_tree_attention_workspace(cache->heads, heads / cache->heads, cache->dim, cache->dtype, tokens, requests, width, cache->page);
+    return paged_tree_attention_workspace(cache->heads, heads / cache->heads, cache->dim, tokens, requests, width, cache->page);
 }
 
 __attribute__((visibility("default"))) int ba_paged_tree_attention(const ba_paged_cache *cache, int dtype, const void *q, int64_t q_head_stride,

@@ -164,8 +164,7 @@ int launch_paged_append(const PagedAppendArgs &args, int dtype, int cache_dtype,
 size_t paged_attention_workspace(int64_t cache_heads, int64_t group, int64_t dim, int cache_dtype, int64_t requests, int64_t width, int64_t page);
 int launch_paged_attention(const PagedAttentionArgs &args, int dtype, int cache_dtype, int32_t *counters, void *workspace, hipStream_t stream);
 int launch_paged_tree(const PagedTreeArgs &args, hipStream_t stream);
-size_t paged_tree_attention_workspace(int64_t cache_heads, int64_t group, int64_t dim, int cache_dtype, int64_t tokens, int64_t requests,
-                                      int64_t width, int64_t page);
+size_t paged_tree_attention_workspace(int64_t cache_heads, int64_t group, int64_t dim, int64_t tokens, int64_t requests, int64_t width, int64_t page);
 int launch_paged_tree_attention(const PagedTreeAttentionArgs &args, int dtype, int cache_dtype, int32_t *counters, void *workspace, hipStream_t stream);
 int launch_paged_keep(PagedKeepArgs args, hipStream_t stream);
 int launch_paged_copy(PagedCopyArgs args, const PagedArray (&arrays)[2], int64_t heads, int64_t page, int64_t row_bytes, hipStream_t stream);

@@ -570,11 +570,14 @@ template <int DT, bool F8, int DC, class T> __device__ __forceinline__ void tree
         if (sh.joins[i]) tree_join<DT, DC, T, 4, 4>(a, w, sh.left[i], 0, T::kRows, F8 ? a.v.scale[sh.left[i].h] : 1.f);
 }
 
-// The joining as a kernel of its own: grid (workgroups of the other, blocks of rows), one row a thread, so that many workgroups share
-// the loads (32 parts of 32 rows 9 us; with four rows a thread 19).
+// The joining as a kernel of its own: grid (blocks of rows, workgroups of the other), one row a thread, so that many workgroups share
+// the loads (32 parts of 32 rows 9 us; with four rows a thread 19).  Units often begin with every 32nd workgroup or so, which would all be on one XCD,
+// dies taking workgroups in turn (16 units of 32 parts of 128 rows 65 us): the number's low bits are mixed with those above.
 template <int DT, int DC, class T> __global__ void __launch_bounds__(kTreeThreads) paged_tree_join_kernel(TreeArgs args, int rows) {
-    const TreeLeft u = args.w.left[blockIdx.x];
-    const int row0 = (int)blockIdx.y * rows;
+    const int group = (int)blockIdx.y ^ ((int)(blockIdx.y >> 3) & 7) ^ ((int)(blockIdx.y >> 6) & 7);
+    if (group >= args.w.groups) return;
+    const TreeLeft u = args.w.left[group];
+    const int row0 = (int)blockIdx.x * rows;
     if (u.parts) tree_join<DT, DC, T, 1, kTreeJoinAhead>(args.a, args.w, u, row0, row0 + rows, args.a.v.scale ? args.a.v.scale[u.h] : 1.f);
 }
 
@@ -586,17 +589,26 @@ template <int DT, int DC, class T, typename K> int tree_launch(K kernel, const P
     kernel<<<w.groups, kTreeThreads, T::kLds, stream>>>(TreeArgs{a, w});
     if (w.left) {
         constexpr int kRows = std::min(T::kRows, kTreeThreads / (DC / 4));           // (a round of its threads)
-        paged_tree_join_kernel<DT, DC, T><<<dim3((unsigned)w.groups, T::kRows / kRows), kTreeThreads, 0, stream>>>(TreeArgs{a, w}, kRows);
+        paged_tree_join_kernel<DT, DC, T><<<dim3(T::kRows / kRows, (unsigned)(w.groups + 7) / 8 * 8), kTreeThreads, 0, stream>>>(TreeArgs{a, w}, kRows);
     }
     return hipGetLastError() == hipSuccess ? BA_OK : BA_ERR_LAUNCH;
 }
 
-// Rows of a unit, and with them the kernel, by the rows that a request and key head have on the average (64 requests of 4000 tokens, 8 key heads
-// of 128: 16 rows 167 us, with units of 128 211; 32 rows 181 and 213; 64 rows of 128 dimensions 228 with units of 64 and 218 with 128, of
-// 64 dimensions 137 and 161).
-static inline int tree_rows(int64_t tokens, int64_t requests, int64_t group, int64_t dim) {
+// Rows of a unit, and with them the kernel, by the rows that a request and key head have on the average: a unit's time hardly depends on how many of its
+// rows are there (64 requests of 4000 tokens, 8 key heads of 128: 16 rows 164 us, with units of 128 211; 32 rows 177 and 213; 64 rows of 128
+// dimensions 228 with units of 64 and 215 with 128, of 64 dimensions 137 and 161).
+// Small units also where requests are brief and their small units no more than there are compute units, which then share the rows (4 requests of 100
+// tokens, 128 rows: 15.9 us, with units of 128 23; 8 of 1000 35 and 39; but 24 of 200 35 and 28, 2 of 20000 104 and 68); a few of the smallest for 32
+// rows (500 tokens 14.8 us, with units of 32 17.7; 4 requests of 1000 21.0 and 22.4).
+// More than 128 dimensions have units of 16 or 128 rows, for want of registers (32 rows, 60 tokens: 43 us and 50; 4000 tokens 324 and 265).
+constexpr int64_t kTreeBrief = 2048;
+static inline int tree_rows(int64_t heads, int64_t tokens, int64_t requests, int64_t group, int64_t dim, int64_t longest) {
     const int64_t rows = tokens * group, many = std::max<int64_t>(1, requests);
-    return rows <= 16 * many ? 16 : rows <= 32 * many ? 32 : rows <= 64 * many && dim <= 64 ? 64 : 128;
+    const bool brief = longest <= kTreeBrief;
+    if (dim > 128) return rows <= (brief ? 32 : 24) * many ? 16 : 128;
+    if (rows <= 16 * many || (brief && rows <= 32 * many && heads * rows <= 16 * 64)) return 16;
+    if (rows <= 32 * many || (brief && heads * rows <= 32 * (int64_t)device_cu_count())) return 32;
+    return rows <= 64 * many && dim <= 64 ? 64 : 128;
 }
 template <int DT, bool F8> int launch_tree_few(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int sets, hipStream_t stream);
 template <int DT, bool F8> int launch_tree_wide(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int waves, hipStream_t stream);

@@ -1,4 +1,4 @@
-// Attention of drafted tokens for few rows a key head (up to 32 on the average).
+// Attention of drafted tokens for few rows a key head (units of 16 or 32; tree_rows).
 //
 // Every key and value is read once, so memory traffic is the floor, as for one query per request (paged_attention_kernel.hpp), and the tile is worked
 // on in the same way: nothing of the cache passes through LDS, the four wavefronts take 32 tokens each, scores are K Q^T on the
@@ -19,7 +19,7 @@ template <int DC_, int SETS> struct TreeFew {
     static constexpr int kResident = DC == 64 ? (SETS == 2 ? 2 : 3) : DC == 128 && SETS == 1 ? 2 : 1;
 };
 
-// DC: dimensions that the registers hold (64, 128, 256).
+// DC: dimensions that the registers hold (64, 128, 256: with one set).
 template <int DT, bool F8, int DC, int SETS, TreeRows ROWS>
 __global__ void __launch_bounds__(kTreeThreads, (TreeFew<DC, SETS>::kResident)) paged_tree_few_kernel(TreeArgs) {
     typedef TreeFew<DC, SETS> T;
@@ -318,7 +318,9 @@ template <int DT, bool F8, int DC, int SETS> static int launch_few_dims(const Pa
     return rows == kTreePieces ? launch_few_rows<DT, F8, DC, SETS, kTreePieces>(a, w, stream) : launch_few_rows<DT, F8, DC, SETS, kTreeAny>(a, w, stream);
 }
 template <int DT, bool F8, int DC> static int launch_few_sets(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int sets, hipStream_t stream) {
-    return sets == 2 ? launch_few_dims<DT, F8, DC, 2>(a, w, rows, stream) : launch_few_dims<DT, F8, DC, 1>(a, w, rows, stream);
+    if constexpr (DC <= 128)
+        if (sets == 2) return launch_few_dims<DT, F8, DC, 2>(a, w, rows, stream);
+    return launch_few_dims<DT, F8, DC, 1>(a, w, rows, stream);
 }
 template <int DT, bool F8> int launch_tree_few(const PagedTreeAttentionArgs &a, const TreeWork &w, TreeRows rows, int sets, hipStream_t stream) {
     switch (dim_class(a.dim)) {

@@ -1,4 +1,4 @@
-// Attention of drafted tokens for many rows a key head (more than 32 on the average).
+// Attention of drafted tokens for many rows a key head (units of 64 or 128; tree_rows).
 //
 // A unit is 128 rows, 32 a wavefront, or (64 dimensions) 64, of which two wavefronts have the same and half of the tile's tokens each.  All four wavefronts bring a tile
 // of 64 tokens (32 for 128 rows of more than 128 dimensions) into LDS together, in 16 bits, by way of registers; two tiles lie there in turn.

@@ -26,6 +26,8 @@ class Drafts:
     rows none).  pad rows belong to no request.
     """
 
+    room = 0                                                  # tokens that a row of the table has room for at least
+
     def __init__(self, base, nodes, heads, group, dim, page, dtype=torch.float16, fp8=False, mask="tree", order="heads", seed=0, spread=2.0,
                  pad=0, front=0, extra=2, words=None):
         g = torch.Generator().manual_seed(seed)
@@ -33,7 +35,7 @@ class Drafts:
         lens = [b + n for b, n in zip(base, nodes)]
         self.lens = lens
         need = [-(-n // page) for n in lens]
-        pages, width = sum(need) + extra, max(need + [1]) + 1
+        pages, width = sum(need) + extra, max(max(need + [1]) + 1, -(-self.room // page))
         self.table = torch.full((len(lens), width), -1, dtype=torch.int32)
         numbers, at = torch.randperm(pages, generator=g, dtype=torch.int32), 0
         shape = (pages, heads, page, dim) if order == "heads" else (pages, page, heads, dim)
@@ -487,3 +489,77 @@ def test_many_small_probabilities(dev, nodes):
     n = 60000 - 1 + b.seen(0, 0)[:, 60000:].sum(-1).double()
     want = (n * 2.0 ** -21 / (1 + n * 2.0 ** -21))[None, :, None]
     assert ((got - want).abs() <= (2.0 ** -10 + 2.0 ** -11 + 4000 * 2.0 ** -24) * want).all()
+
+
+@pytest.fixture
+def roomy(monkeypatch):
+    """Tables of long rows: calls with many rows then have units of 64 or 128 of them, however few the tokens are."""
+    monkeypatch.setattr(Drafts, "room", 4096)
+
+
+@pytest.mark.parametrize("dtype,fp8", [(torch.float16, False), (torch.bfloat16, False), (torch.float16, True), (torch.bfloat16, True)])
+@pytest.mark.parametrize("mask", ["tree", "chain", "any"])
+@pytest.mark.parametrize("dim,page,order", [(128, 16, "heads"), (64, 16, "tokens"), (80, 24, "heads"), (100, 7, "tokens"), (256, 32, "heads")])
+def test_many_rows(dev, roomy, dtype, fp8, mask, dim, page, order):
+    Drafts([0, 1, 33, 200, 5, 64], [3, 40, 80, 30, 0, 8], 2, 4, dim, page, dtype, fp8, mask, order, pad=3, front=2).check(dev)
+    if dim <= 64:
+        Drafts([0, 1, 33, 200, 5, 64], [3, 20, 17, 30, 0, 8], 2, 4, dim, page, dtype, fp8, mask, order, pad=3, front=2).check(dev)
+
+
+@pytest.mark.parametrize("dim", [1, 2, 3, 4, 7, 8, 9, 15, 16, 24, 31, 32, 33, 40, 48, 63, 65, 72, 96, 104, 127, 129, 136, 160, 192, 200, 224, 250, 255])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_many_rows_of_every_kind_of_dimension(dev, roomy, dim, fp8):
+    Drafts([50, 0, 130], [30, 15, 60], 2, 2, dim, 16, torch.float16, fp8, seed=dim).check(dev, 0.7 * dim ** -0.5, flat=dim % 2 == 0)
+    if dim <= 64:
+        Drafts([50, 0, 130], [30, 15, 20], 2, 2, dim, 16, torch.float16, fp8, seed=dim).check(dev, 0.7 * dim ** -0.5)
+
+
+@pytest.mark.parametrize("window", [1, 33, 64, 199, 1000])
+@pytest.mark.parametrize("mask", ["tree", "chain", "any"])
+def test_windows_of_many_rows(dev, window, mask):
+    Drafts([0, 10, 200, 301], [70, 7, 20, 130], 4, 16, 64, 16, torch.bfloat16, mask=mask, seed=window).check(dev, window=window)
+
+
+@pytest.mark.parametrize("page", [1, 3, 17, 64, 100, 1000])
+def test_pages_of_many_rows(dev, roomy, page):
+    Drafts([0, 10, 63, 64, 300], [25, 17, 42, 40, 29], 2, 3, 64, page, torch.float16, seed=page).check(dev)
+
+
+def test_unusual_values_in_long_tables(dev, roomy):
+    """Many rows over values that are not finite, rows that see nothing, scales of either sign."""
+    test_rows_that_see_nothing(dev)
+    for value in ("nan", "inf", "-inf"):
+        test_what_a_row_does_not_see_has_no_influence(dev, value, False)
+    test_what_a_row_does_not_see_has_no_influence(dev, "nan", True)
+    test_scores_far_from_zero_for_many_rows(dev)
+    for scale in (-0.3, 0.0, 1e-39):
+        test_scales_of_either_sign_and_none(dev, scale, 40)
+    for words in (1, 2, 5):
+        test_masks_narrower_and_wider_than_the_draft(dev, words)
+
+
+@pytest.mark.parametrize("dim,fp8", [(64, False), (128, True), (256, False), (100, False)])
+def test_infinite_values_that_many_rows_see(dev, roomy, dim, fp8):
+    b = Drafts([5, 33], [60, 3], 1, 4, dim, 16, torch.float16, fp8, mask="any", seed=2)
+    v = torch.zeros((1, 1, dim), dtype=torch.float16)
+    v[..., 7], v[..., 20] = torch.nan if fp8 else torch.inf, torch.nan
+    b.put(b.v, 0, 5 + 11, v.to(FP8) if fp8 else v)
+    got = b.run(dev, 0.125).double().cpu()
+    for i in range(60):
+        x, row = bool(b.sees[0][i, 11]), got[:, i]
+        assert (row[:, 7].isnan() if fp8 else row[:, 7] == torch.inf).all() if x else row[:, 7].isfinite().all()
+        assert row[:, 20].isnan().all() if x else row[:, 20].isfinite().all()
+        assert row[:, 30:].isfinite().all()
+
+
+@pytest.mark.parametrize("dim,fp8", [(64, False), (128, True), (256, False), (100, False), (7, False)])
+def test_page_numbers_outside_the_cache_for_many_rows(dev, roomy, dim, fp8):
+    b = Drafts([40, 40, 40], [40, 40, 40], 1, 2, dim, 16, torch.float16, fp8, mask="chain")
+    ref, bound = b.expect(0.125)
+    for bad in (-1, b.k.shape[0], (1 << 31) - 1, -(1 << 31)):
+        table = b.operands(dev)["table"].clone()
+        table[1, 0] = bad
+        got = blockedAttention.pagedTreeAttention(b.q.to(dev), **{**b.operands(dev), "table": table}, scale=0.125).double().cpu()
+        assert got[:, 40:80].isnan().all()
+        for rows in (slice(0, 40), slice(80, 120)):
+            assert ((got[:, rows] - ref[:, rows]).abs() <= bound[:, rows]).all()
