@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeFew<DC, SETS>::kResident)) 
             for (int k = 0; k < KL; ++k) {
                 const int b = 64 * k + 16 * g;
                 if (SHORT) load_part<4>(kx[i][k], p + b, from.row_bytes - b);
-                else load_stream<4>(kx[i][k], p + (DC * EB > 64 * k + 64 && !ANY ? b : min(b, from.row_bytes - 16)));
+                else load_stream<4>(kx[i][k], p + (!ANY && DC > 64 && 64 * (k + 1) <= DC / 2 * EB ? b : min(b, from.row_bytes - 16)));      // (dim > DC / 2)
             }
         }
     };
