@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
         const Draft &d = cur.d;
         u32x4 q[KS];
         // scores are scaled within the exponent, by a factor above 0: the sign goes to the queries, and 0 becomes next to nothing
-        const float scale = a.scale * kLog2e * (F8 ? a.k.scale[cur.h] : 1.f), to_log2 = fmaxf(fabsf(scale), 1e-37f), lag = kTreeLag / to_log2;
+        const float scale = a.scale * kLog2e * (F8 ? a.k.scale[cur.h] : 1.f), to_log2 = fabsf(scale) < 1e-37f ? 1e-37f : fabsf(scale), lag = kTreeLag / to_log2;
         const uint32_t turn = scale < 0.f ? 0x80008000u : 0u;
         const int me = opaque((int)threadIdx.x);
 #pragma unroll

@@ -563,3 +563,13 @@ def test_page_numbers_outside_the_cache_for_many_rows(dev, roomy, dim, fp8):
         assert got[:, 40:80].isnan().all()
         for rows in (slice(0, 40), slice(80, 120)):
             assert ((got[:, rows] - ref[:, rows]).abs() <= bound[:, rows]).all()
+
+
+@pytest.mark.parametrize("nodes", [3, 8, 40])
+def test_scales_that_are_no_numbers(dev, roomy, nodes):
+    """A head whose keys have a scale of NaN: its rows are NaN, the other's are not."""
+    b = Drafts([100], [nodes], 2, 4, 128, 16, torch.bfloat16, True, seed=nodes)
+    b.scales[0][1] = float("nan")
+    got = b.run(dev, 0.1)
+    assert got[:4].isfinite().all() and got[4:].isnan().all()
+    assert b.run(dev, float("nan")).isnan().all()
