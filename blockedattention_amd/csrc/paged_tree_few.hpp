@@ -34,7 +34,8 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeFew<DC, SETS>::kResident)) 
     __shared__ TreeLds<T> sh;
     int unfinished = 0;
     TreeUnit cur, next;
-    const int64_t end = tree_deal<T>(sh, next);
+    int group;
+    const int64_t end = tree_deal<T>(sh, next, group);
     if (end < 0) return;
 
     const int mine_at = lane & 31;
@@ -146,10 +147,10 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeFew<DC, SETS>::kResident)) 
                         }
                 }
                 lds_barrier();
-                tree_store<DT, T>(sh, lds, cur, me, c, v_scale);
+                tree_store<DT, T>(sh, group, lds, cur, me, c, v_scale);
                 lds_barrier();
             }
-            tree_end<DT, F8, T>(sh, cur, me, unfinished);
+            tree_end<DT, F8, T>(sh, group, cur, me, unfinished);
             if (!more) break;
         }
         cur = next;

@@ -74,7 +74,8 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
     __shared__ TreeLds<T> sh;
     int unfinished = 0;
     TreeUnit cur, next;
-    const int64_t end = tree_deal<T>(sh, next);
+    int group;
+    const int64_t end = tree_deal<T>(sh, next, group);
     if (end < 0) return;
 
     const int piece = (int)threadIdx.x % kPieces, line = (int)threadIdx.x / kPieces, mine_at = lane & (T::kTokens - 1);
@@ -143,12 +144,12 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
                     }
                 if (T::kGroups > 1) lds_barrier();
                 else __builtin_amdgcn_wave_barrier();
-                tree_store<DT, T>(sh, lds, cur, me, c, v_scale);
+                tree_store<DT, T>(sh, group, lds, cur, me, c, v_scale);
                 if (T::kGroups > 1 && c + T::kDims < DC) lds_barrier();
                 else __builtin_amdgcn_wave_barrier();
             }
             lds_barrier();
-            tree_end<DT, F8, T>(sh, cur, me, unfinished);
+            tree_end<DT, F8, T>(sh, group, cur, me, unfinished);
             if (!more) break;
         }
         // ---- queries by way of LDS: column l32 of the scores
