@@ -11,7 +11,7 @@
 //   change  the rows' pages, as far as their holders change, and how many become free in each chunk of pages
 //   finish  every workgroup adds up those numbers, then rows, stack and verdict
 // A small table takes one launch, all of it in the LDS of one workgroup.  What bounds either are the launches and the round trips to memory in
-// each: 32 rows of up to 2000 tokens 9.1 us (three launches 14), 1024 rows of up to 16000 (8 MB) 28.
+// each: 32 rows of up to 2000 tokens 7.9 us (three launches 14), 1024 rows of up to 16000 (8 MB) 27.
 #include <algorithm>
 
 #include "ba_device.hpp"
@@ -260,8 +260,7 @@ __global__ void __launch_bounds__(kForkBegin) paged_fork_begin_kernel(PagedForkA
 
 // A workgroup has kForkRows rows and a column a thread.  Rows next to each other that hold the same page there, which those that went on from one
 // row do, add their changes up first, and a workgroup counts the freed pages of a chunk in LDS first: atomics on the same few addresses
-// wait for each other (1024 rows in sets of 16: 188 us
-// with neither, 41 with the second, 28 with both).  Many chunks need no such care.
+// wait for each other (1024 rows in sets of 16: 188 us with neither, 41 with the second, 28 with both).  Many chunks need no such care.
 __global__ void __launch_bounds__(kForkThreads) paged_fork_change_kernel(PagedForkArgs a, ForkWork w) {
     __shared__ int32_t count[kForkLocal];
     if (w.totals[1]) return;
