@@ -11,7 +11,7 @@
 //   change  the rows' pages, as far as their holders change, and how many become free in each chunk of pages
 //   finish  every workgroup adds up those numbers, then rows, stack and verdict
 // A small table takes one launch, all of it in the LDS of one workgroup.  What bounds either are the launches and the round trips to memory in
-// each: 32 rows of up to 2000 tokens 7.9 us (three launches 14), 1024 rows of up to 16000 (8 MB) 27.
+// each: 32 rows of up to 2000 tokens 7.9 us (three launches 14), 1024 rows of up to 16000 (8 MB) 24.
 #include <algorithm>
 
 #include "ba_device.hpp"
@@ -22,7 +22,10 @@ namespace ba {
 
 constexpr int kForkThreads = 256;
 constexpr int kForkBegin = 1024;             // threads of the first kernel
-constexpr int kForkChunk = 8 * kForkThreads;           // pages that a workgroup of the last kernel looks through
+// Pages that a workgroup of the last kernel looks through, a thread's share of them: few, so that many workgroups look (70 000 pages: 5.3 us, with
+// eight a thread 8.8, with sixteen 14), but every workgroup adds up all chunks' numbers, so more where there are many pages.
+constexpr int kForkFew = 2, kForkMany = 16;
+constexpr int64_t kForkManyPages = 1 << 20;
 constexpr int kForkRows = 8;                 // rows whose pages a workgroup changes
 constexpr int kForkLocal = 2048;             // chunks whose freed pages a workgroup counts in LDS
 constexpr int kForkSmall = 8192;            // pages, and entries of the table, that one workgroup deals with
@@ -32,11 +35,13 @@ struct ForkWork {
     int32_t *totals;                         // fresh pages, verdict of the first kernel, of the second
     int32_t *owners;                         // [requests]: the row of a fresh page
     int32_t *chunks;                         // freed pages of a chunk
-    int32_t n_chunks;
+    int32_t n_chunks, chunk_log;             // chunks have 2^chunk_log pages
 };
 static ForkWork fork_work(int64_t requests, int64_t pages, void *workspace, size_t *bytes) {
     ForkWork w{};
-    w.n_chunks = (int32_t)((pages + kForkChunk - 1) / kForkChunk);
+    const int64_t chunk = kForkThreads * (pages <= kForkManyPages ? kForkFew : kForkMany);
+    w.chunk_log = __builtin_ctzll(chunk);
+    w.n_chunks = (int32_t)((pages + chunk - 1) / chunk);
     char *p = (char *)workspace;
     auto take = [&](int64_t n) {
         char *const at = p;
@@ -299,8 +304,8 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_change_kernel(PagedFo
             if (was[i] < 0 || now < -1) {
                 bad = BA_PAGED_BAD_SHARES;
             } else if (now == -1) {
-                if (local) atomicAdd(&count[page[i] / kForkChunk], 1);
-                else atomicAdd(&w.chunks[page[i] / kForkChunk], 1);
+                if (local) atomicAdd(&count[page[i] >> w.chunk_log], 1);
+                else atomicAdd(&w.chunks[page[i] >> w.chunk_log], 1);
             }
         }
     }
@@ -313,14 +318,14 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_change_kernel(PagedFo
 }
 
 // Workgroups 0 .. requests - 1: their row; behind them a chunk each, with the pages that became free.
-__global__ void __launch_bounds__(kForkThreads) paged_fork_finish_kernel(PagedForkArgs a, ForkWork w) {
-    constexpr int kWaves = kForkThreads / 64, kRounds = kForkChunk / kForkThreads;
+template <int kRounds> __global__ void __launch_bounds__(kForkThreads) paged_fork_finish_kernel(PagedForkArgs a, ForkWork w) {
+    constexpr int kWaves = kForkThreads / 64;
     __shared__ int32_t sums[2][kWaves];
     const int tid = (int)threadIdx.x, wave = tid >> 6, lane = (int)lane_id();
     const bool row_group = (int)blockIdx.x < a.requests;
     const int r = (int)blockIdx.x, chunk = (int)blockIdx.x - a.requests;
     // a wavefront of a chunk has kRounds times 64 pages in order
-    const int64_t first = (int64_t)chunk * kForkChunk + wave * 64 * kRounds + lane;
+    const int64_t first = ((int64_t)chunk << w.chunk_log) + wave * 64 * kRounds + lane;
     const int64_t o = row_group ? a.origin[r] : -1;
     const int number = row_group ? w.rows[2 * r + 1] : -1;
     const int64_t len = row_group && o >= 0 && o < a.requests ? a.lens[o] : 0;
@@ -421,7 +426,9 @@ int launch_paged_fork(const PagedForkArgs &a, void *workspace, hipStream_t strea
     paged_fork_begin_kernel<<<(unsigned)(1 + groups), kForkBegin, 0, stream>>>(a, w);
     const dim3 rows((unsigned)(a.requests + kForkRows - 1) / kForkRows, (unsigned)std::min((a.width + kForkThreads - 1) / kForkThreads, 1024));
     if (a.requests > 0 && a.width > 0) paged_fork_change_kernel<<<rows, kForkThreads, 0, stream>>>(a, w);
-    paged_fork_finish_kernel<<<(unsigned)std::max(1, a.requests + w.n_chunks), kForkThreads, 0, stream>>>(a, w);
+    const unsigned last = (unsigned)std::max(1, a.requests + w.n_chunks);
+    if (a.pages <= kForkManyPages) paged_fork_finish_kernel<kForkFew><<<last, kForkThreads, 0, stream>>>(a, w);
+    else paged_fork_finish_kernel<kForkMany><<<last, kForkThreads, 0, stream>>>(a, w);
     return hipGetLastError() == hipSuccess ? BA_OK : BA_ERR_LAUNCH;
 }
 

@@ -251,3 +251,15 @@ def test_most_rows(dev):
     i64, i32 = dict(dtype=torch.int64, device=dev), dict(dtype=torch.int32, device=dev)
     with pytest.raises(RuntimeError, match="up to 8192 rows"):
         blockedAttention.pagedFork(torch.zeros((8193, 2), **i32), free, state, shares, torch.zeros(8193, **i64), torch.zeros(8193, **i64), 4)
+
+
+def test_more_than_a_million_pages(dev):
+    """Pages at both ends of a large cache, with chunks of the other size."""
+    w = Rows(50, 40, (1 << 20) + 70, 4, seed=11)
+    w.grow(torch.randint(0, 160, (50,), generator=w.g).tolist())
+    for kind in ("any", "one", "end"):
+        table, free, state, shares, lens = w.tensors(dev)
+        stack, o = len(w.free), origins(kind, 50, w.g)
+        fine, source, target = w.fork(o)
+        assert fine
+        w.check(blockedAttention.pagedFork(table, free, state, shares, lens, torch.tensor(o, device=dev), 4), free, stack, source, target)
