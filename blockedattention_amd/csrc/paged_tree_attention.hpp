@@ -8,8 +8,8 @@
 // Split.  A unit is a block of rows (nodes and the query heads that share a key head, heads fastest) of a request and key head.  Its tokens are
 // cut into tiles, and the tiles of all units, in the order of requests, key heads and blocks, are dealt out to the workgroups in equal
 // shares, with a constant for what a unit costs besides; sums and lengths are on the GPU only, so every workgroup adds them up itself.
-// (Where there are about as many units as workgroups, each gets a unit.)  A unit that lies in one share is done then; for others each workgroup leaves maxima, sums and fp32 accumulators in memory.
-// Where units have few parts, each counts itself in and the last one joins them all, in the order of the tokens whoever it is; else a
+// (Where there are about as many units as workgroups, each gets a unit.)  A unit that lies in one share is done then; for others each workgroup leaves
+// maxima, sums and fp32 accumulators in memory.  Where units have few parts, each counts itself in and the last one joins them all, in the order of the tokens whoever it is; else a
 // second kernel does.
 //
 // Tiles that not all rows see all of -- the draft's own, and where windows begin -- hide scores by the rows' bits.  Values there that are not
