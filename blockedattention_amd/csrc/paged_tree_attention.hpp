@@ -608,12 +608,13 @@ template <int DT, int DC, class T, typename K> int tree_launch(K kernel, const P
 // Small units also where requests are brief and their small units no more than there are compute units, which then share the rows (4 requests of 100
 // tokens, 128 rows: 15.9 us, with units of 128 23; 8 of 1000 35 and 39; but 24 of 200 35 and 28, 2 of 20000 104 and 68); a few of the smallest for 32
 // rows (500 tokens 14.8 us, with units of 32 17.7; 4 requests of 1000 21.0 and 22.4).
-// More than 128 dimensions have units of 16 or 128 rows, for want of registers (32 rows, 60 tokens: 43 us and 50; 4000 tokens 324 and 265).
+// More than 128 dimensions have units of 16 or 128 rows, for want of registers (64 requests, 32 rows, 60 tokens: 43 us and 50; 4000 tokens 324 and 265;
+// 2 requests, 128 rows, 60 / 400 / 1200 tokens: 14.5 / 22 / 28 and 29 / 29 / 32).
 constexpr int64_t kTreeBrief = 2048;
 static inline int tree_rows(int64_t heads, int64_t tokens, int64_t requests, int64_t group, int64_t dim, int64_t longest) {
     const int64_t rows = tokens * group, many = std::max<int64_t>(1, requests);
     const bool brief = longest <= kTreeBrief;
-    if (dim > 128) return rows <= (brief ? 32 : 24) * many ? 16 : 128;
+    if (dim > 128) return rows <= (brief ? 32 : 24) * many || (brief && heads * rows <= 16 * (int64_t)device_cu_count()) ? 16 : 128;
     if (rows <= 16 * many || (brief && rows <= 32 * many && heads * rows <= 16 * 64)) return 16;
     if (rows <= 32 * many || (brief && heads * rows <= 32 * (int64_t)device_cu_count())) return 32;
     return rows <= 64 * many && dim <= 64 ? 64 : 128;

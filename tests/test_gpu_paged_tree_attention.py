@@ -573,3 +573,14 @@ def test_scales_that_are_no_numbers(dev, roomy, nodes):
     got = b.run(dev, 0.1)
     assert got[:4].isfinite().all() and got[4:].isnan().all()
     assert b.run(dev, float("nan")).isnan().all()
+
+
+@pytest.mark.parametrize("dim,fp8", [(256, False), (160, True), (131, False)])
+def test_many_rows_of_many_dimensions_in_small_units(dev, dim, fp8):
+    """Few requests over few tokens, more rows than a unit has; the same in long tables."""
+    for room in (0, 4096):
+        Drafts.room = room
+        try:
+            Drafts([60, 0, 300], [40, 70, 1], 2, 4, dim, 16, torch.bfloat16, fp8, mask="tree", seed=dim, pad=2).check(dev, window=0 if dim == 256 else 90)
+        finally:
+            Drafts.room = 0
