@@ -472,21 +472,22 @@ __device__ __forceinline__ void tree_store(const TreeLds<T> &sh, int group, cons
     const PagedTreeAttentionArgs &a = tree_args().a;
     const TreeWork &w = tree_args().w;
     const bool begun = u.tile == 0, whole = begun && u.last == u.d.tiles;
-    const int slot = 2 * group + (begun ? 1 : 0), wave = uniform(me >> 6);
+    const int slot = 2 * group + (begun ? 1 : 0);
     const Shared shared = tree_shared<T>(w);
-    // kGroups > 1: all threads have the rows of all; else each wavefront has its own 32
-    constexpr int kThreads = T::kGroups > 1 ? kTreeThreads : 64, kLanes = T::kDims / 4, kMany = (T::kGroups > 1 ? T::kRows : 32) * kLanes;
+    // all threads have the rows of all that are there; kGroups == 1: part x / 32 has rows 32 (x / 32) ..
+    constexpr int kLanes = T::kDims / 4;
     const int dim1 = 4 * (me % kLanes), dim0 = c + dim1;
+    const int many = uniform((int)min((int64_t)T::kRows, (int64_t)u.d.rows * a.group - (int64_t)u.block * T::kRows) * kLanes);
 #pragma unroll 4
-    for (int e = T::kGroups > 1 ? me : me & 63; e < kMany; e += kThreads) {
-        const int y = e / kLanes, x = T::kGroups > 1 ? y : 32 * wave + y;
+    for (int e = me; e < many; e += kTreeThreads) {
+        const int x = e / kLanes;
         const TreeRow t = tree_row(a, w, u.d, u.h, (int64_t)u.block * T::kRows + x);
         float top = -INFINITY, sum = 0.f;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
         if (T::kGroups == 1) {
-            top = sh.m[wave][y];
-            sum = sh.l[wave][y];
-            acc = *(const f32x4 *)((const float *)(lds + wave * T::kPart) + y * T::kPitch + dim1);
+            top = sh.m[x / 32][x % 32];
+            sum = sh.l[x / 32][x % 32];
+            acc = *(const f32x4 *)((const float *)(lds + x / 32 * T::kPart) + x % 32 * T::kPitch + dim1);
         } else {
 #pragma unroll
             for (int i = 0; i < T::kGroups; ++i) top = fmaxf(top, sh.m[i][x]);
@@ -498,7 +499,7 @@ __device__ __forceinline__ void tree_store(const TreeLds<T> &sh, int group, cons
                 acc += f * *(const f32x4 *)((const float *)(lds + i * T::kPart) + x * T::kPitch + dim1);
             }
         }
-        if (t.there && dim0 < a.dim) {
+        if (dim0 < a.dim) {
             if (whole) {
                 if (sum == 0.f) acc = f32x4{0.f, 0.f, 0.f, 0.f};
                 store_result<DT>(tree_out(a, u.d, t), dim0, a.dim, acc * tree_factor(sum, v_scale));

@@ -146,11 +146,9 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
                         const f32x16 &x = o[c / 32 + j];
                         *(f32x4 *)(mineo + 32 * j + 8 * g) = f32x4{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
                     }
-                if (T::kGroups > 1) lds_barrier();
-                else __builtin_amdgcn_wave_barrier();
+                lds_barrier();
                 tree_store<DT, T>(sh, group, lds, cur, me, c, v_scale);
-                if (T::kGroups > 1 && c + T::kDims < DC) lds_barrier();
-                else __builtin_amdgcn_wave_barrier();
+                if (c + T::kDims < DC) lds_barrier();
             }
             lds_barrier();
             tree_end<DT, F8, T>(sh, group, cur, me, unfinished);
