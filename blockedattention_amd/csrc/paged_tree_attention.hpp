@@ -511,14 +511,15 @@ __device__ __forceinline__ void tree_store(const TreeLds<T> &sh, int group, cons
     }
 }
 // Values that are not finite, for the rows that see them (an infinity or a NaN of whatever weight is the result's), and what is said of a part.
-// A barrier comes before.
-template <int DT, bool F8, class T> __device__ __forceinline__ void tree_end(TreeLds<T> &sh, int group, const TreeUnit &u, int me, int &unfinished) {
+// `odd`: sh.odd, read by every wavefront before the barrier that comes before this.  Behind that barrier a wavefront may be at the next unit's tiles, where
+// it sets sh.odd, while another is still here.
+template <int DT, bool F8, class T> __device__ __forceinline__ void tree_end(TreeLds<T> &sh, int group, const TreeUnit &u, int me, bool odd, int &unfinished) {
     const PagedTreeAttentionArgs &a = tree_args().a;
     const TreeWork &w = tree_args().w;
     const Draft &d = u.d;
     const bool begun = u.tile == 0, whole = begun && u.last == d.tiles;
     const int slot = 2 * group + (begun ? 1 : 0);
-    if (sh.odd) {
+    if (odd) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         const TableRow row = table_row(u);

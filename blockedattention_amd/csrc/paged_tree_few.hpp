@@ -129,6 +129,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeFew<DC, SETS>::kResident)) 
         if (any) {
             const int me = opaque((int)threadIdx.x), my16 = me & 15, my_g = me >> 4 & 3;
             const float v_scale = F8 ? tree_args().a.v.scale[cur.h] : 1.f;
+            bool odd = false;
 #pragma unroll
             for (int z = 0; z < SETS; ++z) {
                 l[z] = quad_column_sum(l[z]);
@@ -150,10 +151,11 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeFew<DC, SETS>::kResident)) 
                         }
                 }
                 lds_barrier();
+                odd = uniform(sh.odd) != 0;
                 tree_store<DT, T>(sh, group, lds, cur, me, c, v_scale);
                 lds_barrier();
             }
-            tree_end<DT, F8, T>(sh, group, cur, me, unfinished);
+            tree_end<DT, F8, T>(sh, group, cur, me, odd, unfinished);
             if (!more) break;
         }
         cur = next;

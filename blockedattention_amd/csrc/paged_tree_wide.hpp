@@ -150,8 +150,9 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
                 tree_store<DT, T>(sh, group, lds, cur, me, c, v_scale);
                 if (c + T::kDims < DC) lds_barrier();
             }
+            const bool odd = uniform(sh.odd) != 0;
             lds_barrier();
-            tree_end<DT, F8, T>(sh, group, cur, me, unfinished);
+            tree_end<DT, F8, T>(sh, group, cur, me, odd, unfinished);
             if (!more) break;
         }
         // ---- queries by way of LDS: column l32 of the scores
