@@ -6,10 +6,11 @@
 //   exchange between the halves, and the probabilities are, packed to 16 bits, the second product's operand as they are, if that runs over the
 //   tokens in the order in which the lanes have them.
 //   Values, O[d][row] = V^T P: the transposing LDS read gives four tokens of a dimension.
-// A row's maximum is only moved when a larger one comes by more than 2^7, so accumulators are scaled seldom.  A probability is rounded to 16 bits once,
-// to the nearest: an error of half a step in each, independent of the others, so that the result's own rounding is the larger half of
-// the whole error (1.3 times that of fp32 probabilities); two terms as in the kernel for few rows would cost half as much again of the second
-// product.  The sum that it is divided by is of the rounded ones.
+// A row's maximum is only moved when a larger one comes by more than 2^7, so accumulators are scaled seldom.  Probabilities are as exact as in the kernel for
+// few rows, since which of the two answers a request depends on the other requests: two 16-bit terms (paged_attention_kernel.hpp), or, for bf16 queries
+// over an 8-bit cache, one of fp16, whose error is an eighth of the result's own rounding; e4m3 values are exact in fp16.  One term of the result's type
+// would add its own rounding's error once more (1.3 times the whole error); two cost the second product again (64 requests of 4000 tokens, 128 rows of 128
+// dimensions 240 -> 286 us, 512 rows 215 -> 265; a batch of 32 drafts 94.6 -> 97.5).
 // What bounds it: a wavefront's chain of LDS, products, exponentials, LDS, products, of which two to a SIMD hide half (two requests of 32768 to 65536
 // tokens in 8 bits, 512 rows a key head, 240 GFLOP: 335 to 355 us, 680 to 720 TFLOP/s with the matrix unit busy 33 % of the time, vector instructions
 // 38 %, LDS 36 %).  32 requests of up to 4096 tokens and 32 nodes (281 MB) take 97 us.
@@ -41,8 +42,8 @@ template <int DT> __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32
 }
 
 // Probabilities are lifted by a power of two, so that small ones stay apart from zero in fp16.  A maximum that is kept though a
-// larger one has come (by up to 2^7) leaves them below 2^13.
-template <int DT> constexpr float kTreeLift = DT == 0 ? 6.f : 0.f;
+// larger one has come (by up to 2^7) leaves them at 2^15 at most.
+template <int PT> constexpr float kTreeLift = PT == 0 ? 8.f : 0.f;
 constexpr float kTreeLag = 7.f;
 constexpr int kMatrix = 0x8, kDsRead = 0x100;                // kinds of instructions, for the scheduler
 
@@ -56,12 +57,10 @@ __device__ __forceinline__ float pair_sum(float v) {
     return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
 }
 
-// A sum and both halves of a dword: of probabilities as they are after rounding, which the values are weighed with.
-template <int DT> __device__ __forceinline__ float add_both(uint32_t x, float sum) {
+// A sum and both fp16 halves of a dword: of probabilities of one term as they are after rounding, which the values are weighed with.
+__device__ __forceinline__ float add_both(uint32_t x, float sum) {
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-    if constexpr (DT == 0) return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, x), __builtin_bit_cast(f16x2, 0x3c003c00u), sum, false);
-    else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x), __builtin_bit_cast(bf16x2, 0x3f803f80u), sum, false);
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, x), __builtin_bit_cast(f16x2, 0x3c003c00u), sum, false);
 }
 
 // DC: dimensions that the registers hold (64, 128, 256).
@@ -72,6 +71,8 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
     constexpr int EB = F8 ? 1 : 2, kPieces = DC * EB / 16;   // bytes of an element, 16-byte pieces of a row
     constexpr int kAtOnce = kTreeThreads / kPieces, kPasses = T::kTokens / kAtOnce;      // rows of a load, loads of a tile
     constexpr int KS = DC / 16, DB = DC / 32, SUBS = T::kMine / 32;
+    constexpr int PT = F8 ? 0 : DT;          // type of probabilities and values in the second product (8 bits: exact in fp16)
+    constexpr bool TWO = !(F8 && DT == 1);   // probabilities have two terms
     static_assert(kTreeThreads % kPieces == 0 && T::kTokens % kAtOnce == 0);
     const int lane = lane_id(), l32 = lane & 31, half = lane >> 5, wave = uniform((int)threadIdx.x >> 6), wr = wave % WR, wt = wave / WR;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -103,7 +104,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
     bool any = false, more = true;
     int32_t number = look_up(next, table_row(next), tree_args().a.page, true, first_of(next, next.tile) + mine_at);
     f32x16 o[DB];
-    float m = -INFINITY, l = 0.f, base = kTreeLift<DT>;      // base: what is added to scores in the exponent
+    float m = -INFINITY, l = 0.f, base = kTreeLift<PT>;      // base: what is added to scores in the exponent
     for (;;) {
         // ---- the next unit's first tile and queries are on their way while this one is finished
         constexpr int kEach = T::kRows * (DC / 8) / kTreeThreads;
@@ -190,7 +191,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
         for (int j = 0; j < DB; ++j)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[j][i] = 0.f;
-        m = -INFINITY; l = 0.f; base = kTreeLift<DT>;
+        m = -INFINITY; l = 0.f; base = kTreeLift<PT>;
         more = tree_next(cur) < end;
 
         number = look_up(cur, row, by.page, cur.tile + 1 < cur.last, first_of(cur, cur.tile + 1) + mine_at);
@@ -243,18 +244,19 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
             }
             {
                 char *const kt = buf + line * T::kPitchK + (F8 ? 32 : 16) * piece, *const vt = buf + T::kTokens * T::kPitchK + line * T::kPitchV + (F8 ? 32 : 16) * piece;
-                auto put = [&](char *to, const uint32_t (&x)[4]) {
+                auto put = [&](auto type, char *to, const uint32_t (&x)[4]) {
+                    constexpr int To = decltype(type)::value;
                     if (F8) {
-                        *(u32x4 *)to = u32x4{widen<DT, false>(x[0]), widen<DT, true>(x[0]), widen<DT, false>(x[1]), widen<DT, true>(x[1])};
-                        *(u32x4 *)(to + 16) = u32x4{widen<DT, false>(x[2]), widen<DT, true>(x[2]), widen<DT, false>(x[3]), widen<DT, true>(x[3])};
+                        *(u32x4 *)to = u32x4{widen<To, false>(x[0]), widen<To, true>(x[0]), widen<To, false>(x[1]), widen<To, true>(x[1])};
+                        *(u32x4 *)(to + 16) = u32x4{widen<To, false>(x[2]), widen<To, true>(x[2]), widen<To, false>(x[3]), widen<To, true>(x[3])};
                     } else {
                         *(u32x4 *)to = u32x4{x[0], x[1], x[2], x[3]};
                     }
                 };
 #pragma unroll
                 for (int p = 0; p < kPasses; ++p) {
-                    put(kt + p * kAtOnce * T::kPitchK, kx[p]);
-                    put(vt + p * kAtOnce * T::kPitchV, vx[p]);
+                    put(std::integral_constant<int, DT>(), kt + p * kAtOnce * T::kPitchK, kx[p]);
+                    put(std::integral_constant<int, PT>(), vt + p * kAtOnce * T::kPitchV, vx[p]);
                 }
             }
             if (i + 1 < cur.last) {
@@ -308,7 +310,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
                 for (int x = 0; x < 16; ++x) top = fmaxf(top, s[u][x]);
             top = pair_max(top);
             if (__any(top - m > lag)) {                      // (also the first that is seen: m is -inf)
-                const float to = kTreeLift<DT> - (top == -INFINITY ? 0.f : top * to_log2);
+                const float to = kTreeLift<PT> - (top == -INFINITY ? 0.f : top * to_log2);
                 const float shrink = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(to - base);
                 l *= shrink;
 #pragma unroll
@@ -321,16 +323,25 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
             if (__any(fabsf(base) > 0x1p16f)) {
 #pragma unroll
                 for (int u = 0; u < SUBS; ++u) s[u] -= m == -INFINITY ? 0.f : m;
-                add = kTreeLift<DT>;
+                add = kTreeLift<PT>;
             }
-            u32x4 p[2 * SUBS];
+            u32x4 p[2 * SUBS], rest[TWO ? 2 * SUBS : 1];
 #pragma unroll
             for (int u = 0; u < SUBS; ++u)
 #pragma unroll
                 for (int x = 0; x < 16; x += 2) {
                     const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][x], to_log2, add)), p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][x + 1], to_log2, add));
-                    p[2 * u + x / 8][x % 8 / 2] = Elem<DT>::pack2(p0, p1);
-                    l = add_both<DT>(p[2 * u + x / 8][x % 8 / 2], l);
+                    if constexpr (TWO) {
+                        const uint32_t first = first_term<PT>(p0, p1);
+                        p[2 * u + x / 8][x % 8 / 2] = first;
+                        rest[2 * u + x / 8][x % 8 / 2] = Elem<PT>::pack2(second_term<PT, F8>(p0, Elem<PT>::to_float((uint16_t)first)),
+                                                                         second_term<PT, F8>(p1, Elem<PT>::to_float((uint16_t)(first >> 16))));
+                        l += p0;
+                        l += p1;
+                    } else {
+                        p[2 * u + x / 8][x % 8 / 2] = Elem<PT>::pack2(p0, p1);
+                        l = add_both(p[2 * u + x / 8][x % 8 / 2], l);
+                    }
                 }
             // -- values: lane (dimension 32 j + l32, half) has tokens 16 k + 4 half + 0 .. 3 and 8 behind those
             const LdsBytes vt = (LdsBytes)(buf + T::kTokens * T::kPitchK) + (wt * T::kMine + 4 * half + (lane & 15) / 4) * T::kPitchV + 32 * (lane >> 4 & 1) + 8 * (lane & 3);
@@ -340,14 +351,16 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
                 for (int j = 0; j < DB; ++j) {
                     const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPiece)(vt + 16 * k * T::kPitchV + 64 * j)));
                     const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPiece)(vt + (16 * k + 8) * T::kPitchV + 64 * j)));
-                    o[j] = mfma32<DT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, p[k], o[j]);
+                    const u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
+                    o[j] = mfma32<PT>(v, p[k], o[j]);
+                    if constexpr (TWO) o[j] = mfma32<PT>(v, rest[k], o[j]);
                     constexpr int kEvery = 2 * SUBS * DB / kPasses;
                     if (!SHORT && (k * DB + j + 1) % kEvery == 0) fetch(vx[(k * DB + j) / kEvery], from, 1, (k * DB + j) / kEvery);
                 }
             __builtin_amdgcn_sched_group_barrier(kDsRead, 8, 1);
 #pragma unroll
             for (int n = 0; n < 2 * SUBS * DB; ++n) {
-                __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 1);
+                __builtin_amdgcn_sched_group_barrier(kMatrix, TWO ? 2 : 1, 1);
                 __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 1);
             }
         }

@@ -33,3 +33,26 @@ def test_workgroups_of_several_units(dev, roomy, dim, fp8, nodes):  # noqa: F811
         sees[b.accum[r]:b.accum[r + 1]] = b.sees[r][:, node]
     assert sees.any() and got[:, sees].isnan().all()
     assert ((got - ref).abs() <= bound)[:, ~sees].all()
+
+
+@pytest.mark.parametrize("dtype,fp8", [(torch.bfloat16, False), (torch.bfloat16, True), (torch.float16, False), (torch.float16, True)])
+@pytest.mark.parametrize("dim,nodes", [(64, 12), (64, 40), (128, 40), (256, 40), (100, 40), (128, 3)])
+def test_probabilities_have_more_than_16_bits(dev, roomy, monkeypatch, dtype, fp8, dim, nodes):  # noqa: F811
+    """The result's own rounding is the only one to 16 bits, whichever kernel a batch takes.
+
+    Bound: as in test_gpu_paged_tree_attention.py, but a probability p is off by 2^-16 p at most (two terms, the first cut off: bf16 2^-7 x 2^-9, fp16 less), in
+    fp16 by half a step of 2^-24 besides, or a whole one where the second term is made that, lifted by 2^8 against the largest: 2^-31 of it a token.  bf16 over e4m3: one fp16 term, 2^-11 p
+    (the kernel for few rows: two).
+    """
+    b = Drafts([300, 77, 0], [nodes, nodes, nodes], 2, 4, dim, 16, dtype, fp8, mask="tree", seed=dim)
+    import test_gpu_paged_tree_attention as base
+    u = base.U[dtype]
+    monkeypatch.setitem(base.U, dtype, 0.0)
+    ref, rest = b.expect(dim ** -0.5)
+    monkeypatch.setitem(base.U, dtype, 1.0)
+    size = b.expect(dim ** -0.5)[1] - rest - ref.abs()
+    most = torch.nan_to_num(b.v.float()).abs().max().item() * (max(b.scales[1]).item() if fp8 else 1.0)
+    term = 2.0 ** -11 if fp8 and dtype == torch.bfloat16 else 2.0 ** -16
+    bound = u * ref.abs() + rest + term * size + 400 * 2.0 ** -31 * most
+    got = b.run(dev, dim ** -0.5).double().cpu()
+    assert ((got - ref).abs() <= bound).all(), (((got - ref).abs() - bound).max().item(), ((got - ref).abs() > bound).double().mean().item())
