@@ -7,7 +7,7 @@
 // Freed pages go on the stack in ascending order, fresh pages are numbered by row and come from its end: the place of either is known
 // from counts alone, so whoever finds a freed page puts it where it belongs, on the stack or into the row that has its number.
 // Three launches, since counts have to be there before they are changed and whole before they are used:
-//   begin   shares are copied; one workgroup counts who goes on from whom and numbers the fresh pages
+//   begin   shares are copied, counts below 0 found (one of -1 would pass for a page that became free); one workgroup counts who goes on from whom and numbers the fresh pages
 //   change  the rows' pages, as far as their holders change, and how many become free in each chunk of pages
 //   finish  every workgroup adds up those numbers, then rows, stack and verdict
 // A small table takes one launch, all of it in the LDS of one workgroup.  What bounds either are the launches and the round trips to memory in
@@ -26,6 +26,7 @@ constexpr int kForkBegin = 1024;             // threads of the first kernel
 // eight a thread 8.8, with sixteen 14), but every workgroup adds up all chunks' numbers, so more where there are many pages.
 constexpr int kForkFew = 2, kForkMany = 16;
 constexpr int64_t kForkManyPages = 1 << 20;
+constexpr int kForkCopies = 1024;            // workgroups that copy the counts, at most
 constexpr int kForkRows = 8;                 // rows whose pages a workgroup changes
 constexpr int kForkLocal = 2048;             // chunks whose freed pages a workgroup counts in LDS
 constexpr int kForkSmall = 8192;            // pages, and entries of the table, that one workgroup deals with
@@ -35,13 +36,15 @@ struct ForkWork {
     int32_t *totals;                         // fresh pages, verdict of the first kernel, of the second
     int32_t *owners;                         // [requests]: the row of a fresh page
     int32_t *chunks;                         // freed pages of a chunk
-    int32_t n_chunks, chunk_log;             // chunks have 2^chunk_log pages
+    int32_t *negative;                       // [copies]: whether a workgroup that copies counts has seen one below 0
+    int32_t n_chunks, chunk_log, copies;     // chunks have 2^chunk_log pages
 };
 static ForkWork fork_work(int64_t requests, int64_t pages, void *workspace, size_t *bytes) {
     ForkWork w{};
     const int64_t chunk = kForkThreads * (pages <= kForkManyPages ? kForkFew : kForkMany);
     w.chunk_log = __builtin_ctzll(chunk);
     w.n_chunks = (int32_t)((pages + chunk - 1) / chunk);
+    w.copies = (int32_t)std::min<int64_t>(kForkCopies, (pages + kForkBegin - 1) / kForkBegin);
     char *p = (char *)workspace;
     auto take = [&](int64_t n) {
         char *const at = p;
@@ -52,6 +55,7 @@ static ForkWork fork_work(int64_t requests, int64_t pages, void *workspace, size
     w.totals = (int32_t *)take(3);
     w.owners = (int32_t *)take(requests);
     w.chunks = (int32_t *)take(w.n_chunks);
+    w.negative = (int32_t *)take(w.copies);
     if (bytes) *bytes = (size_t)(p - (char *)workspace);
     return w;
 }
@@ -153,8 +157,13 @@ __global__ void __launch_bounds__(kForkBegin) paged_fork_small_kernel(PagedForkA
     __shared__ ForkRows<kForkSmallRows> rows;
     const int tid = (int)threadIdx.x, wave = tid >> 6, lane = (int)lane_id();
     const int entries = a.requests * a.width;
+    int negative = 0;
 #pragma unroll 4
-    for (int i = tid; i < a.pages; i += kForkBegin) shares[i] = a.shares[i];
+    for (int i = tid; i < a.pages; i += kForkBegin) {
+        const int32_t n = a.shares[i];
+        shares[i] = n;
+        negative |= n < 0;
+    }
 #pragma unroll 4
     for (int i = tid; i < entries; i += kForkBegin) {
         const int r = (int)a.columns.div((uint32_t)i);
@@ -170,6 +179,7 @@ __global__ void __launch_bounds__(kForkBegin) paged_fork_small_kernel(PagedForkA
         number[r] = n;
         if (n >= 0) owner[n] = r;
     });
+    if (negative) bad_shares = BA_PAGED_BAD_SHARES;
     __syncthreads();
     if (rows.verdict == 0) {
         int bad = 0;
@@ -250,8 +260,15 @@ __global__ void __launch_bounds__(kForkBegin) paged_fork_small_kernel(PagedForkA
 __global__ void __launch_bounds__(kForkBegin) paged_fork_begin_kernel(PagedForkArgs a, ForkWork w) {
     if (blockIdx.x > 0) {
         const int64_t at = (int64_t)(blockIdx.x - 1) * kForkBegin + threadIdx.x, step = (int64_t)(gridDim.x - 1) * kForkBegin;
-        for (int64_t i = at; i < a.pages; i += step) a.shares_out[i] = a.shares[i];
+        int negative = 0;
+        for (int64_t i = at; i < a.pages; i += step) {
+            const int32_t n = a.shares[i];
+            a.shares_out[i] = n;
+            negative |= n < 0;
+        }
         for (int64_t i = at; i < w.n_chunks; i += step) w.chunks[i] = 0;
+        negative = __syncthreads_or(negative);
+        if (threadIdx.x == 0) w.negative[blockIdx.x - 1] = negative;
         return;
     }
     __shared__ ForkRows<BA_PAGED_FORK_ROWS> sh;
@@ -346,12 +363,14 @@ template <int kRounds> __global__ void __launch_bounds__(kForkThreads) paged_for
     all = wave_inclusive_scan(all);
     before = wave_inclusive_scan(before);
     if (lane == 63) { sums[0][wave] = all; sums[1][wave] = before; }
-    __syncthreads();
+    int negative = 0;
+    for (int i = tid; i < w.copies; i += kForkThreads) negative |= w.negative[i];
+    negative = __syncthreads_or(negative);
     int back = 0, ahead = 0;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) { back += sums[0][i]; ahead += sums[1][i]; }
     const int taken = w.totals[0];
-    const Outcome t = outcome(a, w.totals[1] | w.totals[2], back, taken);
+    const Outcome t = outcome(a, w.totals[1] | w.totals[2] | (negative ? BA_PAGED_BAD_SHARES : 0), back, taken);
     const bool fine = t.verdict == 0;
     const int64_t count = t.count, left = t.left;
     if (blockIdx.x == 0 && tid == 0) {
@@ -422,8 +441,7 @@ int launch_paged_fork(const PagedForkArgs &a, void *workspace, hipStream_t strea
         return hipGetLastError() == hipSuccess ? BA_OK : BA_ERR_LAUNCH;
     }
     const ForkWork w = fork_work(a.requests, a.pages, workspace, nullptr);
-    const int64_t groups = std::min<int64_t>(1024, (a.pages + kForkBegin - 1) / kForkBegin);
-    paged_fork_begin_kernel<<<(unsigned)(1 + groups), kForkBegin, 0, stream>>>(a, w);
+    paged_fork_begin_kernel<<<(unsigned)(1 + w.copies), kForkBegin, 0, stream>>>(a, w);
     const dim3 rows((unsigned)(a.requests + kForkRows - 1) / kForkRows, (unsigned)std::min((a.width + kForkThreads - 1) / kForkThreads, 1024));
     if (a.requests > 0 && a.width > 0) paged_fork_change_kernel<<<rows, kForkThreads, 0, stream>>>(a, w);
     const unsigned last = (unsigned)std::max(1, a.requests + w.n_chunks);

@@ -455,7 +455,7 @@ int ba_paged_keep(const ba_paged_cache *cache, const int32_t *table, int64_t tab
 
 /* More verdicts, of ba_paged_fork. */
 #define BA_PAGED_BAD_ORIGIN 32 /* an origin is below -1 or no row */
-#define BA_PAGED_BAD_SHARES 64 /* a page number is outside the cache, or more rows hold a page than `shares` says */
+#define BA_PAGED_BAD_SHARES 64 /* a count is below 0, a page number is outside the cache, or more rows hold a page than `shares` says */
 
 /*
  * Row r of the table goes on from row origin[r] (int64; r itself: it stays; -1: it ends): table_out, lens_out (int64) get its
