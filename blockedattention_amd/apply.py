@@ -201,8 +201,9 @@ def pagedFork(
 
     Returns ``(table, lens, state, shares, source, target)``: the new table, lengths, state and counts, and for every row the page to be
     copied and the fresh one it is copied to, or -1 (int32, for ``pagedCopy`` in every layer's cache).  A refused step changes
-    nothing and returns what came in; its verdict adds 32 (an origin that is no row) and 64 (pages and ``shares`` that do
-    not fit) to those of ``pagedResize``.  A row that shares pages may grow by ``pagedResize`` and shrink by it as far as
+    nothing and returns what came in; its verdict adds 32 (an origin that is no row) and 64 (a count below 0, a row's page that
+    is not in the cache, a page that loses more holders than ``shares`` says it has) to those of ``pagedResize``; counts that are too
+    low and are not found so are the caller's mistake.  A row that shares pages may grow by ``pagedResize`` and shrink by it as far as
     pages that it holds alone; it ends here, with origin -1.  Up to 8192 rows.
     """
     return tuple(blockAttention.pagedFork(table, free, state, shares, lens, origin, int(pageSize)))

@@ -3,7 +3,8 @@
 //
 // With k the number of rows that go on from a row, each of its full pages has k - 1 holders more, its last page, if not full,
 // min(k, 1) - 1.  `shares` counts the holders of a page beyond the first; whole-number atomics add the changes up, whose
-// order does not matter, and a page is free when that makes it -1: every holder takes 1 away, so only the last one sees it.
+// order does not matter, and a page is free when that makes it -1.  Counts below that are refused.  Both go by the counts when all changes are in: on
+// the way there, with counts that are not right, others may come up, in whatever order the atomics run.
 // Freed pages go on the stack in ascending order, fresh pages are numbered by row and come from its end: the place of either is known
 // from counts alone, so whoever finds a freed page puts it where it belongs, on the stack or into the row that has its number.
 // Three launches, since counts have to be there before they are changed and whole before they are used:
@@ -33,7 +34,7 @@ constexpr int kForkSmall = 8192;            // pages, and entries of the table, 
 
 struct ForkWork {
     int32_t *rows;                           // [requests][2]: how many go on from the row; number of its fresh page or -1
-    int32_t *totals;                         // fresh pages, verdict of the first kernel, of the second
+    int32_t *totals;                         // fresh pages, verdict of the first kernel, of the second, pages that it leaves below -1
     int32_t *owners;                         // [requests]: the row of a fresh page
     int32_t *chunks;                         // freed pages of a chunk
     int32_t *negative;                       // [copies]: whether a workgroup that copies counts has seen one below 0
@@ -52,7 +53,7 @@ static ForkWork fork_work(int64_t requests, int64_t pages, void *workspace, size
         return at;
     };
     w.rows = (int32_t *)take(2 * requests);
-    w.totals = (int32_t *)take(3);
+    w.totals = (int32_t *)take(4);
     w.owners = (int32_t *)take(requests);
     w.chunks = (int32_t *)take(w.n_chunks);
     w.negative = (int32_t *)take(w.copies);
@@ -185,14 +186,10 @@ __global__ void __launch_bounds__(kForkBegin) paged_fork_small_kernel(PagedForkA
         int bad = 0;
         for (int i = tid; i < entries; i += kForkBegin) {
             const int r = (int)a.columns.div((uint32_t)i), c = i - r * a.width;
-            const int children = rows.children[r], change = c < full[r] ? children - 1 : c < pages_of[r] ? min(children, 1) - 1 : 0;
-            if (change == 0) continue;
-            if ((uint32_t)table[i] >= (uint32_t)a.pages) {
-                bad = BA_PAGED_BAD_SHARES;
-            } else {
-                const int was = atomicAdd(&shares[table[i]], change);
-                if (was < 0 || was + change < -1) bad = BA_PAGED_BAD_SHARES;
-            }
+            const int children = rows.children[r], change = c < full[r] ? children - 1 : min(children, 1) - 1;
+            if (c >= pages_of[r]) continue;
+            if ((uint32_t)table[i] >= (uint32_t)a.pages) bad = BA_PAGED_BAD_SHARES;
+            else if (change != 0) atomicAdd(&shares[table[i]], change);
         }
         if (bad) bad_shares = bad;
     }
@@ -202,7 +199,9 @@ __global__ void __launch_bounds__(kForkBegin) paged_fork_small_kernel(PagedForkA
 #pragma unroll
     for (int i = 0; i < kRounds; ++i) {
         const int p = (wave * kRounds + i) * 64 + lane;
-        freed[i] = __ballot(p < a.pages && shares[p] == -1);
+        const int n = p < a.pages ? shares[p] : 0;
+        if (n < -1) bad_shares = BA_PAGED_BAD_SHARES;
+        freed[i] = __ballot(n == -1);
         mine += __popcll(freed[i]);
     }
     if (lane == 0) freed_by[wave] = mine;
@@ -277,7 +276,7 @@ __global__ void __launch_bounds__(kForkBegin) paged_fork_begin_kernel(PagedForkA
         w.rows[2 * r + 1] = number;
         if (number >= 0) w.owners[number] = r;
     });
-    if (threadIdx.x == 0) { w.totals[0] = total; w.totals[1] = sh.verdict; w.totals[2] = 0; }
+    if (threadIdx.x == 0) { w.totals[0] = total; w.totals[1] = sh.verdict; w.totals[2] = w.totals[3] = 0; }
 }
 
 // A workgroup has kForkRows rows and a column a thread.  Rows next to each other that hold the same page there, which those that went on from one
@@ -292,9 +291,10 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_change_kernel(PagedFo
         __syncthreads();
     }
     const int r0 = (int)blockIdx.x * kForkRows;
-    int bad = 0;
+    int bad = 0, below = 0;
     for (int64_t c = (int64_t)blockIdx.y * kForkThreads + threadIdx.x; c < a.width; c += (int64_t)gridDim.y * kForkThreads) {
         int32_t page[kForkRows], change[kForkRows], was[kForkRows];
+        bool there[kForkRows];
 #pragma unroll
         for (int i = 0; i < kForkRows; ++i) {
             const int r = min(r0 + i, a.requests - 1);
@@ -302,11 +302,12 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_change_kernel(PagedFo
             const Held h = held(a, r0 + i < a.requests ? a.lens[r] : 0);
             change[i] = c < h.full ? children - 1 : c < h.all ? min(children, 1) - 1 : 0;
             page[i] = c < h.all ? a.table[r * a.table_stride + c] : -1;
+            there[i] = c < h.all;
         }
 #pragma unroll
         for (int i = 0; i < kForkRows; ++i) {
             if ((uint32_t)page[i] >= (uint32_t)a.pages) {
-                if (change[i]) bad = BA_PAGED_BAD_SHARES;
+                if (there[i]) bad = BA_PAGED_BAD_SHARES;
                 change[i] = 0;
             } else if (i > 0 && page[i] == page[i - 1]) {
                 change[i] += change[i - 1];
@@ -317,12 +318,12 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_change_kernel(PagedFo
         for (int i = 0; i < kForkRows; ++i) was[i] = change[i] ? atomicAdd(&a.shares_out[page[i]], change[i]) : 0;
 #pragma unroll
         for (int i = 0; i < kForkRows; ++i) {
-            const int now = was[i] + change[i];
-            if (was[i] < 0 || now < -1) {
-                bad = BA_PAGED_BAD_SHARES;
-            } else if (now == -1) {
-                if (local) atomicAdd(&count[page[i] >> w.chunk_log], 1);
-                else atomicAdd(&w.chunks[page[i] >> w.chunk_log], 1);
+            // (the steps that a count takes add up to what it is in the end)
+            const int now = (int)((uint32_t)was[i] + (uint32_t)change[i]), freed = (now == -1 ? 1 : 0) - (was[i] == -1 ? 1 : 0);
+            below += (now < -1 ? 1 : 0) - (was[i] < -1 ? 1 : 0);
+            if (freed) {
+                if (local) atomicAdd(&count[page[i] >> w.chunk_log], freed);
+                else atomicAdd(&w.chunks[page[i] >> w.chunk_log], freed);
             }
         }
     }
@@ -332,6 +333,7 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_change_kernel(PagedFo
             if (count[i]) atomicAdd(&w.chunks[i], count[i]);
     }
     if (bad) atomicOr(&w.totals[2], bad);
+    if (below) atomicAdd(&w.totals[3], below);
 }
 
 // Workgroups 0 .. requests - 1: their row; behind them a chunk each, with the pages that became free.
@@ -370,7 +372,7 @@ template <int kRounds> __global__ void __launch_bounds__(kForkThreads) paged_for
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) { back += sums[0][i]; ahead += sums[1][i]; }
     const int taken = w.totals[0];
-    const Outcome t = outcome(a, w.totals[1] | w.totals[2] | (negative ? BA_PAGED_BAD_SHARES : 0), back, taken);
+    const Outcome t = outcome(a, w.totals[1] | w.totals[2] | (negative || w.totals[3] ? BA_PAGED_BAD_SHARES : 0), back, taken);
     const bool fine = t.verdict == 0;
     const int64_t count = t.count, left = t.left;
     if (blockIdx.x == 0 && tid == 0) {

@@ -455,7 +455,7 @@ int ba_paged_keep(const ba_paged_cache *cache, const int32_t *table, int64_t tab
 
 /* More verdicts, of ba_paged_fork. */
 #define BA_PAGED_BAD_ORIGIN 32 /* an origin is below -1 or no row */
-#define BA_PAGED_BAD_SHARES 64 /* a count is below 0, a page number is outside the cache, or more rows hold a page than `shares` says */
+#define BA_PAGED_BAD_SHARES 64 /* a count is below 0, a row's page number is outside the cache, or a page loses more holders than `shares` says it has */
 
 /*
  * Row r of the table goes on from row origin[r] (int64; r itself: it stays; -1: it ends): table_out, lens_out (int64) get its
@@ -467,7 +467,8 @@ int ba_paged_keep(const ba_paged_cache *cache, const int32_t *table, int64_t tab
  * its pages may always grow by ba_paged_resize, and shrink by it as far as pages that it holds alone; it ends with origin -1.
  * Entries of table_out behind a row's pages are -1.  Stack, state and verdict as for ba_paged_resize: where the verdict is not 0 the
  * stack is untouched, table_out, lens_out and shares_out are what came in, source and target -1.  BA_PAGED_NO_PAGES only where all
- * else is valid.  Outputs must not overlap inputs; inputs are not changed (the stack beyond state_in[0] is), so the same call
+ * else is valid.  Counts are looked at when all changes are in, so a verdict does not depend on the order of rows.  Too low a count of a page that does not
+ * lose more holders than that is not found: such a page may become free while a row still holds it.  Outputs must not overlap inputs; inputs are not changed (the stack beyond state_in[0] is), so the same call
  * again writes the same.  At most BA_PAGED_FORK_ROWS rows.  `workspace`: ba_paged_fork_workspace bytes, 256-byte aligned.
  */
 #define BA_PAGED_FORK_ROWS 8192
