@@ -129,6 +129,16 @@ __device__ __forceinline__ char *tree_out(const PagedTreeAttentionArgs &a, const
 // What accumulators are multiplied with: 0 for rows that see nothing.  (The reciprocal is off by 2^-23 at most, of results of 16 bits.)
 __device__ __forceinline__ float tree_factor(float l, float v_scale) { return l == 0.f ? 0.f : v_scale * __builtin_amdgcn_rcpf(l); }
 
+// A part's accumulators by its weight.  CAREFUL: the weight may be 0, where another part's scores are far larger; an infinity among them, of a value that the
+// row sees, stays one.
+template <bool CAREFUL> __device__ __forceinline__ f32x4 weighed(float f, f32x4 x) {
+    f32x4 y = f * x;
+    if (CAREFUL)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = f == 0.f && y[i] != y[i] ? x[i] : y[i];
+    return y;
+}
+
 // Joins the parts of a unit for its rows [row0, row1), by a whole workgroup: DC / 4 threads a row, kDeep rows of a thread and kAhead parts of
 // each on their way together (a load from where all dies meet takes some 2 us, however many there are).
 template <int DT, int DC, class T, int kDeep, int kAhead>
@@ -142,47 +152,58 @@ __device__ __forceinline__ void tree_join(const PagedTreeAttentionArgs &a, const
     for (int x0 = row0 + (int)threadIdx.x / kLanes; x0 < rows; x0 += kDeep * kAtOnce) {
         float m[kDeep], l[kDeep];
         f32x4 acc[kDeep];
+        auto add_up = [&](auto careful) {
+            constexpr bool CAREFUL = decltype(careful)::value;
 #pragma unroll
-        for (int z = 0; z < kDeep; ++z) {
-            m[z] = -INFINITY;
-            l[z] = 0.f;
-            acc[z] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+            for (int z = 0; z < kDeep; ++z) {
+                m[z] = -INFINITY;
+                l[z] = 0.f;
+                acc[z] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
 #pragma nounroll
-        for (int p0 = 0; p0 < u.parts; p0 += kAhead) {
-            PagedPart part[kDeep][kAhead];
-            f32x4 sum[kDeep][kAhead];
+            for (int p0 = 0; p0 < u.parts; p0 += kAhead) {
+                PagedPart part[kDeep][kAhead];
+                f32x4 sum[kDeep][kAhead];
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                const int p = p0 + i, slot = 2 * (u.begins + p) + (p == 0 ? 1 : 0);
+                for (int i = 0; i < kAhead; ++i) {
+                    const int p = p0 + i, slot = 2 * (u.begins + p) + (p == 0 ? 1 : 0);
+#pragma unroll
+                    for (int z = 0; z < kDeep; ++z) {
+                        part[z][i] = {-INFINITY, 0.f};
+                        sum[z][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                        if (p < u.parts) {
+                            const int x = min(x0 + z * kAtOnce, rows - 1);   // (what is there already once more, and not used)
+                            part[z][i] = shared.part(slot, x);
+                            sum[z][i] = shared.sum(slot, x, min(dim0, w.pitch - 4));
+                        }
+                    }
+                }
 #pragma unroll
                 for (int z = 0; z < kDeep; ++z) {
-                    part[z][i] = {-INFINITY, 0.f};
-                    sum[z][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-                    if (p < u.parts) {
-                        const int x = min(x0 + z * kAtOnce, rows - 1);   // (what is there already once more, and not used)
-                        part[z][i] = shared.part(slot, x);
-                        sum[z][i] = shared.sum(slot, x, min(dim0, w.pitch - 4));
+                    float top = m[z];
+#pragma unroll
+                    for (int i = 0; i < kAhead; ++i) top = fmaxf(top, part[z][i].m);
+                    const float base = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f(m[z] - base);
+                    l[z] *= old;
+                    acc[z] = weighed<CAREFUL>(old, acc[z]);
+                    m[z] = top;
+#pragma unroll
+                    for (int i = 0; i < kAhead; ++i) {
+                        const float f = __builtin_amdgcn_exp2f(part[z][i].m - base);
+                        l[z] += f * part[z][i].l;
+                        acc[z] += weighed<CAREFUL>(f, sum[z][i]);
                     }
                 }
             }
+        };
+        add_up(std::false_type());
+        // (once more where something is NaN: with the care for all of them the batch of drafts takes 99.7 us, 97.4 so)
+        bool again = false;
 #pragma unroll
-            for (int z = 0; z < kDeep; ++z) {
-                float top = m[z];
+        for (int z = 0; z < kDeep; ++z)
 #pragma unroll
-                for (int i = 0; i < kAhead; ++i) top = fmaxf(top, part[z][i].m);
-                const float base = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f(m[z] - base);
-                l[z] *= old;
-                acc[z] *= old;
-                m[z] = top;
-#pragma unroll
-                for (int i = 0; i < kAhead; ++i) {
-                    const float f = __builtin_amdgcn_exp2f(part[z][i].m - base);
-                    l[z] += f * part[z][i].l;
-                    acc[z] += f * sum[z][i];
-                }
-            }
-        }
+            for (int i = 0; i < 4; ++i) again |= acc[z][i] != acc[z][i];
+        if (again) add_up(std::true_type());
 #pragma unroll
         for (int z = 0; z < kDeep; ++z)
             if (const int x = x0 + z * kAtOnce; x < rows && dim0 < a.dim) {

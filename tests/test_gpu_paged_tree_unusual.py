@@ -56,3 +56,40 @@ def test_probabilities_have_more_than_16_bits(dev, roomy, monkeypatch, dtype, fp
     bound = u * ref.abs() + rest + term * size + 400 * 2.0 ** -31 * most
     got = b.run(dev, dim ** -0.5).double().cpu()
     assert ((got - ref).abs() <= bound).all(), (((got - ref).abs() - bound).max().item(), ((got - ref).abs() > bound).double().mean().item())
+
+
+@pytest.mark.parametrize("lens,nodes,heads,group,dim,fp8", [
+    (12000, 3, 1, 4, 128, False), (12000, 7, 2, 4, 64, True), (1500, 4, 8, 4, 128, False), (1500, 7, 8, 4, 64, False),      # few rows: joined by a second kernel, within the kernel
+    (12000, 40, 1, 4, 128, False), (12000, 40, 1, 4, 128, True), (9000, 12, 1, 4, 64, False), (9000, 40, 1, 4, 256, False)])
+@pytest.mark.parametrize("far", [False, True])
+def test_units_of_several_workgroups(dev, lens, nodes, heads, group, dim, fp8, far):
+    """Infinities and NaN among the drafted values of a long request; far: its first token outweighs the part that they are in by more than fp32 holds."""
+    b = Drafts([lens], [nodes], heads, group, dim, 16, torch.float16, fp8, mask="any", seed=nodes)
+    if far:
+        b.q.zero_()
+        b.q[..., 0] = 16.0
+        k = torch.zeros((heads, 1, dim), dtype=torch.float16)
+        k[..., 0] = 40.0
+        if fp8:
+            b.scales[0].fill_(1.0)
+            b.k = (b.k.float() / 128).to(FP8)
+        b.put(b.k, 0, 0, k.to(FP8) if fp8 else k)
+    scale = 1.0 if far else 0.125
+    ref, bound = b.expect(scale)
+    put_value(b, 0, 1, torch.nan, 3)
+    if not fp8:
+        put_value(b, 0, 2, torch.inf, 5)
+    got = b.run(dev, scale).double().cpu()
+    usual = torch.ones(dim, dtype=torch.bool)
+    usual[[3, 5]] = False
+    for i in range(nodes):
+        x, y = bool(b.sees[0][i, 1]), bool(b.sees[0][i, 2]) and not fp8
+        near = (got[:, i] - ref[:, i]).abs() <= bound[:, i]
+        if not x and not y:
+            assert near.all(), i
+            continue
+        if far:                                               # (else the zeros that were put there change the other dimensions)
+            assert near[:, usual].all(), i
+        assert (got[:, i, 3].isnan() if x else got[:, i, 3].isfinite()).all(), (i, got[:, i, 3])
+        assert (got[:, i, 5] == torch.inf if y else got[:, i, 5].isfinite()).all(), (i, got[:, i, 5])
+    assert b.sees[0][:, 1].any() and b.sees[0][:, 2].any()
