@@ -269,9 +269,11 @@ __device__ __forceinline__ int window_from(const PagedTreeAttentionArgs &a, cons
     }
 }
 // Staged tokens from t on that not all rows see: those of the draft, and where the rows' windows begin.
+__device__ __forceinline__ uint32_t all_see_from(const Draft &d, int window) {
+    return window ? (uint32_t)max(d.before - window + min(d.end - d.before, window), 0) : 0u;
+}
 template <class T> __device__ __forceinline__ bool hidden(const Draft &d, int window, uint32_t t) {
-    const int all_from = window ? max(d.before - window + min(d.end - d.before, window), 0) : 0;
-    return t + T::kStaged > (uint32_t)d.before || t < (uint32_t)all_from;
+    return t + T::kStaged > (uint32_t)d.before || t < all_see_from(d, window);
 }
 
 // A workgroup's LDS besides its tiles.
@@ -545,15 +547,20 @@ template <int DT, bool F8, class T> __device__ __forceinline__ void tree_end(Tre
         __syncthreads();
         const TableRow row = table_row(u);
         const Shared shared = tree_shared<T>(w);
-        const uint32_t t_end = (uint32_t)min((int64_t)d.end, (int64_t)d.start + (int64_t)u.last * T::kTokens);
+        // the part's tokens [t_first, t_end) that are hidden from some: those before `head` and from `tail` on (32 requests of 4000 tokens and 10 nodes, 40 rows a key
+        // head, one NaN in a draft: 660 us, 9200 by way of all tokens, 144 without the NaN; eight at a time 490, but drafts without any then take 104 us for 97)
+        const uint32_t t_first = (uint32_t)d.start + (uint32_t)u.tile * T::kTokens, t_end = (uint32_t)min((int64_t)d.end, (int64_t)d.start + (int64_t)u.last * T::kTokens);
+        const uint32_t head = (all_see_from(d, a.window) + T::kStaged - 1) & ~(uint32_t)(T::kStaged - 1), tail = (uint32_t)d.before & ~(uint32_t)(T::kStaged - 1);
         for (int e = me; e < T::kRows * a.dim; e += kTreeThreads) {
             const int x = e / a.dim, dim = e - x * a.dim;
             const TreeRow t = tree_row(a, w, d, u.h, (int64_t)u.block * T::kRows + x);
             const Sight s = sight_of(a, d, t, sh.row_from[x]);
             float add = 0.f;
 #pragma nounroll
-            for (uint32_t tok = (uint32_t)d.start + (uint32_t)u.tile * T::kTokens; tok < t_end; ++tok) {
-                if (!hidden<T>(d, a.window, tok & ~(uint32_t)(T::kStaged - 1)) || !(s(d, a.words, tok) & 1)) continue;
+            for (uint32_t tok = t_first; tok < t_end; ++tok) {
+                if (tok >= head && tok < tail) tok = tail;
+                if (tok >= t_end) break;
+                if (!(s(d, a.words, tok) & 1)) continue;
                 const uint32_t at_page = a.page.div(tok);
                 const int32_t in_page = row[at_page];
                 if ((uint32_t)in_page >= (uint32_t)a.pages) continue;

@@ -93,3 +93,23 @@ def test_units_of_several_workgroups(dev, lens, nodes, heads, group, dim, fp8, f
         assert (got[:, i, 3].isnan() if x else got[:, i, 3].isfinite()).all(), (i, got[:, i, 3])
         assert (got[:, i, 5] == torch.inf if y else got[:, i, 5].isfinite()).all(), (i, got[:, i, 5])
     assert b.sees[0][:, 1].any() and b.sees[0][:, 2].any()
+
+
+@pytest.mark.parametrize("nodes,room", [(6, 0), (30, 4096)])
+@pytest.mark.parametrize("base,window", [(1000, 0), (1000, 40), (1000, 64), (1024, 33), (1000, 300), (1000, 1010), (3, 1)])
+def test_places_of_values_that_are_not_finite(dev, monkeypatch, nodes, room, base, window):
+    """A NaN at each place in turn that not all rows see, and its neighbours: where windows begin, in the draft, both, or where they meet."""
+    monkeypatch.setattr(Drafts, "room", room)
+    b = Drafts([base], [nodes], 1, 4, 64, 16, torch.float16, mask="tree", seed=base + window)
+    ref, bound = b.expect(0.125, window)
+    sees = b.seen(0, window)                                  # [nodes, tokens]
+    some = (sees.any(0) != sees.all(0)).nonzero()[:, 0].tolist()
+    for t in sorted({x for t in some for x in (t - 1, t, t + 1) if 0 <= x < base + nodes})[::3]:
+        at = (int(b.table[0, t // 16]), slice(None), t % 16)
+        old = b.v[at].clone()
+        b.v[at] = torch.nan
+        b.__dict__.pop("there", None)
+        got = b.run(dev, 0.125, window).double().cpu()
+        b.v[at] = old
+        assert got[:, sees[:, t]].isnan().all(), t
+        assert ((got - ref).abs() <= bound)[:, ~sees[:, t]].all(), t
