@@ -162,9 +162,12 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
         const PagedTreeAttentionArgs &a = tree_args().a;
         const Draft &d = cur.d;
         u32x4 q[KS];
-        // scores are scaled within the exponent, by a factor above 0: the sign goes to the queries, and 0 becomes next to nothing
-        const float scale = a.scale * kLog2e * (F8 ? a.k.scale[cur.h] : 1.f), to_log2 = fabsf(scale) < 1e-37f ? 1e-37f : fabsf(scale), lag = kTreeLag / to_log2;
-        const uint32_t turn = scale < 0.f ? 0x80008000u : 0u;
+        // Scores are scaled within the exponent, by a factor above 0: the sign goes to the queries, 0 becomes the smallest number, and a scale that is no number
+        // makes the queries such, so that a row is NaN if it sees a token.
+        const float scale = a.scale * kLog2e * (F8 ? a.k.scale[cur.h] : 1.f);
+        const bool is_number = scale == scale;
+        const float to_log2 = is_number ? fmaxf(fabsf(scale), 0x1p-149f) : 1.f, lag = fminf(kTreeLag / to_log2, 0x1.fffffep127f);
+        const uint32_t turn = scale < 0.f ? 0x80008000u : 0u, nan = is_number ? 0u : 0x7fff7fffu;
         const int me = opaque((int)threadIdx.x);
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
@@ -172,7 +175,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeWide<DC, WR>::kResident)) p
             uint32_t z[4] = {y[e][0], y[e][1], y[e][2], y[e][3]};
             if (ANY && 2 * a.dim >= 16) shift_down<4>(z, max(b - (2 * a.dim - 16), 0));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) z[i] ^= turn;
+            for (int i = 0; i < 4; ++i) z[i] = (z[i] ^ turn) | nan;
             *(u32x4 *)(lds + x / (DC / 8) * T::kPitchK + b) = u32x4{z[0], z[1], z[2], z[3]};
         }
         lds_barrier();

@@ -113,3 +113,30 @@ def test_places_of_values_that_are_not_finite(dev, monkeypatch, nodes, room, bas
         b.v[at] = old
         assert got[:, sees[:, t]].isnan().all(), t
         assert ((got - ref).abs() <= bound)[:, ~sees[:, t]].all(), t
+
+
+@pytest.mark.parametrize("nodes", [3, 8, 40])
+@pytest.mark.parametrize("dim,fp8", [(64, False), (128, True), (100, False), (7, False)])
+def test_rows_that_see_nothing_whatever_the_scale(dev, roomy, nodes, dim, fp8):  # noqa: F811
+    """Zeros, beside rows of the same unit that see tokens and are NaN where the scale is."""
+    b = Drafts([0], [nodes], 2, 4, dim, 16, torch.bfloat16, fp8, mask="any", seed=3, pad=2)
+    b.sees[0][1] = False
+    b.mask[1] = 0
+    b.sees[0][2, 0] = True
+    b.mask[2, 0] |= 1
+    none = ~b.sees[0].any(1)
+    for scale in (float("nan"), float("inf"), -float("inf")):
+        got = b.run(dev, scale)
+        assert (got[:, :nodes][:, none] == 0).all() and (got[:, nodes:] == 0).all()
+        if scale != scale:
+            assert got[:, :nodes][:, ~none].isnan().all()
+
+
+@pytest.mark.parametrize("nodes", [3, 8, 40])
+@pytest.mark.parametrize("scale", [2.0 ** -125, -2.0 ** -127, 2.0 ** -131, 2.0 ** -149, 0.0])
+def test_large_scores_of_a_tiny_scale(dev, roomy, nodes, scale):  # noqa: F811
+    """Scores of up to 2^124 before they are scaled.  Where the scale is a number of few bits, times log2(e) it is off by 2^-150, half the smallest one: 2^-26 of a score's exponent."""
+    b = Drafts([70, 0], [nodes, nodes], 2, 4, 64, 16, torch.bfloat16, mask="tree", seed=nodes)
+    b.q *= 2.0 ** 58
+    b.k *= 2.0 ** 58
+    b.check(dev, scale)
