@@ -170,7 +170,7 @@ def pagedTreeAttention(
     whose keys and values are the last of its ``lens[r]`` tokens in the cache (``tokenAccum`` and ``lens`` as ``pagedResize``
     returns them).  A row sees all tokens before those and, of those, the ones whose bits its row of ``mask`` has (int64
     ``[tokens, words]``, of ``pagedTree`` or any other); without a mask those before it and itself.  ``window`` > 0 looks at the
-    last ``window`` tokens that a row sees.  Rows that see nothing give zeros, and so do rows of no request; what a
+    last ``window`` tokens that a row sees.  Rows that see nothing, or whose scores are all -infinity, give zeros, and so do rows of no request; what a
     row does not see has no influence on it.  All else is as for ``pagedAttention``.
     """
     return blockAttention.pagedTreeAttention(q, kCache, vCache, table, lens, accum, mask, float(scale), int(window), kScale, vScale)

@@ -429,7 +429,8 @@ int ba_paged_tree(const int64_t *parents, const int64_t *accum, int64_t requests
  * accum[r] of the request's tokens.  A row sees all tokens before the draft and, of the draft, the nodes whose bits are set in
  * its row of `mask` (int64, rows of mask_stride words, of which the first `words` count: nodes beyond are not seen); without a mask those
  * before it and itself, so that a draft without branches, or a piece of a prompt, needs none.  With window > 0 it sees of these
- * the last `window`.  Rows that see nothing, and rows of no request, give zeros; what a row does not see has no influence on it, whatever is there.
+ * the last `window`.  Rows that see nothing or whose scores are all -infinity, and rows of no request, give zeros; what a row does
+ * not see has no influence on it, whatever is there.
  * q and out are [heads][tokens][dim] by the strides given (in elements).  The sums do not decrease; rows beyond `tokens` do not
  * exist, and neither do tokens beyond the table's row.  A page number outside the cache makes the rows of its request NaN
  * that look at it.  Types, table, counters and workspace (ba_paged_tree_attention_workspace bytes) are those of ba_paged_attention.

@@ -140,3 +140,19 @@ def test_large_scores_of_a_tiny_scale(dev, roomy, nodes, scale):  # noqa: F811
     b.q *= 2.0 ** 58
     b.k *= 2.0 ** 58
     b.check(dev, scale)
+
+
+@pytest.mark.parametrize("base,nodes", [(0, 3), (0, 9), (0, 40), (70, 3), (70, 40), (6000, 3), (6000, 40)])
+@pytest.mark.parametrize("mask", ["any", "chain"])
+def test_scores_that_are_all_minus_infinity(dev, roomy, base, nodes, mask):  # noqa: F811
+    """No probability is above 0: zeros, as for a row that sees nothing; also where a request is split between workgroups."""
+    b = Drafts([base, 50], [nodes, nodes], 2, 4, 64, 16, torch.float16, mask=mask, seed=nodes)
+    ref, bound = b.expect(1.0)
+    b.q[:, :nodes] = 0.0
+    b.q[:, :nodes, 0] = 1.0
+    x = torch.zeros((2, base + nodes, 64), dtype=torch.float16)
+    x[..., 0] = -torch.inf
+    b.put(b.k, 0, 0, x)
+    got = b.run(dev, 1.0).double().cpu()
+    assert (got[:, :nodes] == 0).all()
+    assert ((got - ref).abs() <= bound)[:, nodes:].all()
