@@ -183,7 +183,8 @@ def pagedKeep(kCache: torch.Tensor, vCache: torch.Tensor, table: torch.Tensor, l
     their order, then -1: the token at ``lens[r] + path[r, i]`` comes to ``lens[r] + i``.  A path increases; it ends at the first entry
     that does not, is below its own index, or lies outside the row.  Returns the lengths with the accepted nodes; ``pagedResize``
     to those gives the other pages back.  Call it for every layer's cache.  Pages that are written must not be another row's
-    too (``pagedFork`` sees to that).
+    too (``pagedFork`` sees to that), so a draft whose step ``pagedResize`` refused keeps nothing: ``torch.where(state[1] == 0,
+    path, -1)`` as the path.
     """
     return blockAttention.pagedKeep(kCache, vCache, table, lens, path)
 

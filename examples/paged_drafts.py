@@ -113,6 +113,7 @@ def main(cache="bf16", steps=40, seed=0):
             paths.append(path)
         deepest = max(map(len, paths))
         path = torch.tensor([p + [-1] * (deepest - len(p)) for p in paths], dtype=torch.int64, device=dev).reshape(ROWS, deepest)
+        path = torch.where(state[1] == 0, path, -1)                       # (a step that was refused gave its tokens no places)
         kept = blockedAttention.pagedKeep(layer.k, layer.v, table, lens, path)
         _, _, lens, state = blockedAttention.pagedResize(table, free, state, grown, kept, PAGE, 0)
 

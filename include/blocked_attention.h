@@ -449,7 +449,9 @@ int ba_paged_tree_attention(const ba_paged_cache *cache, int dtype, const void *
  * all were read before any is written; lens_out[r] becomes lens[r] plus the number of accepted nodes (ba_paged_resize to that gives the
  * rest of the pages back).  A path increases, so path[r][i] >= i; it ends at the first entry that is not above the
  * one before it or is below i (as -1 is), or whose place is not in the row.  Tokens on page numbers outside the cache are not
- * moved.  lens_out must not overlap lens.  No page of a place that is written may be another row's too.
+ * moved.  lens_out must not overlap lens.  No page of a place that is written may be another row's too.  Nothing here tells whether the draft
+ * got its places: where ba_paged_resize refused the step, entries of the table behind a row's pages may name pages that other rows hold by
+ * now, so the path has to be empty then (-1 wherever state_out[1] is not 0, which needs no synchronisation).
  */
 int ba_paged_keep(const ba_paged_cache *cache, const int32_t *table, int64_t table_stride, int64_t width, const int64_t *lens,
                   const int64_t *path, int64_t path_stride, int64_t requests, int64_t depth, int64_t *lens_out, ba_stream_t stream);
