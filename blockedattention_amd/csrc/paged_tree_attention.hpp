@@ -23,7 +23,7 @@ constexpr int kTreeThreads = kPagedThreads, kTreeWaves = kPagedWaves;
 constexpr int kTreeUnit = 3;                 // what a unit costs besides its tiles, in tiles: queries, first loads, joining, results
 constexpr int kTreeShare = kTreeUnit + 1;    // of both, what a workgroup has at least: a unit of one tile
 // Where each unit can have a workgroup, it gets one, unless the longest has more than so many tiles above an equal share.  (60 requests of 1000 tokens,
-// 8 key heads, 480 units of 15 tiles for 512 workgroups: 82 us, 102 when split evenly.  28 requests of up to 1000, 12 key heads: 38.7 split, 43.4 whole;
+// 8 key heads, 480 units of 15 tiles for 512 workgroups: 95 us, 112 when split evenly.  28 requests of up to 1000, 12 key heads: 38.7 split, 43.4 whole;
 // there it is 4 tiles above a share of 7.)
 constexpr int kTreeSplit = 4;
 constexpr int kTreeWhole = 4;                // units of up to so many tiles are not split between workgroups
@@ -365,10 +365,10 @@ template <class T> __device__ __forceinline__ int64_t tree_deal(TreeLds<T> &sh, 
             *(u16_any *)(out + head_of * a.out_head_bytes + 2 * (x - head_of * a.dim)) = 0;
         }
     }
-    // Dies take workgroups in turn.  Where most units are blocks of rows of the same keys and values, a die's workgroups get shares next to each other,
-    // so that those blocks meet in its cache (16 requests of 4000 tokens, 512 rows: 228 us, 195 so).  Else such neighbours only make dies unequal
-    // (batch of drafts 98 us, 102).
-    if (group < groups && uniform(all_units) >= 2 * (int64_t)a.heads * a.requests) {
+    // Dies take workgroups in turn.  A die's workgroups get shares next to each other, so that blocks of rows of the same keys and values meet in its cache (16
+    // requests of 4000 tokens, 512 rows: 331 us, 293 so; batch of drafts 100, 97).  Small units only where most of them are such blocks: else it makes dies unequal
+    // (64 requests of 4000 tokens, 16 rows: 168 us, 170 so).
+    if (group < groups && (T::kRows >= 64 || uniform(all_units) >= 2 * (int64_t)a.heads * a.requests)) {
         const int each = (int)groups / 8, rest = (int)groups % 8, die = group % 8;
         group = die * each + min(die, rest) + group / 8;
     }
@@ -633,13 +633,13 @@ template <int DT, int DC, class T, typename K> int tree_launch(K kernel, const P
 }
 
 // Rows of a unit, and with them the kernel, by the rows that a request and key head have on the average: a unit's time hardly depends on how many of its
-// rows are there (64 requests of 4000 tokens, 8 key heads of 128: 16 rows 164 us, with units of 128 211; 32 rows 177 and 213; 64 rows of 128
-// dimensions 228 with units of 64 and 215 with 128, of 64 dimensions 137 and 161).
+// rows are there (64 requests of 4000 tokens, 8 key heads of 128: 16 rows 167 us, with units of 128 273; 32 rows 175 and 243; 64 rows of 128
+// dimensions 271 with units of 64 and 294 with 128, but over 1000 tokens, 60 requests, 86 and 80, and 261 and 232 of 80 dimensions; of 64 dimensions 140 and 170).
 // Small units also where requests are brief and their small units no more than there are compute units, which then share the rows (4 requests of 100
-// tokens, 128 rows: 15.9 us, with units of 128 23; 8 of 1000 35 and 39; but 24 of 200 35 and 28, 2 of 20000 104 and 68); a few of the smallest for 32
-// rows (500 tokens 14.8 us, with units of 32 17.7; 4 requests of 1000 21.0 and 22.4).
-// More than 128 dimensions have units of 16 or 128 rows, for want of registers (64 requests, 32 rows, 60 tokens: 43 us and 50; 4000 tokens 324 and 265;
-// 2 requests, 128 rows, 60 / 400 / 1200 tokens: 14.5 / 22 / 28 and 29 / 29 / 32).
+// tokens, 128 rows: 14.7 us, with units of 128 25; 8 of 1000 30 and 42; but 24 of 200 35 and 30, 2 of 20000 93 and 73); a few of the smallest for 32
+// rows (500 tokens 14.8 us, with units of 32 19.1; 4 requests of 1000 17.6 and 21.4).
+// More than 128 dimensions have units of 16 or 128 rows, for want of registers (8 key heads, 64 requests, 32 rows, 60 tokens: 43 us and 43; 4000 tokens 652 and
+// 594; 2 requests, 128 rows, 60 / 400 / 1200 tokens: 15 / 22 / 34 and 30 / 32 / 38).
 constexpr int64_t kTreeBrief = 2048;
 static inline int tree_rows(int64_t heads, int64_t tokens, int64_t requests, int64_t group, int64_t dim, int64_t longest) {
     const int64_t rows = tokens * group, many = std::max<int64_t>(1, requests);
