@@ -12,7 +12,7 @@
 //   change  the rows' pages, as far as their holders change, and how many become free in each chunk of pages
 //   finish  every workgroup adds up those numbers, then rows, stack and verdict
 // A small table takes one launch, all of it in the LDS of one workgroup.  What bounds either are the launches and the round trips to memory in
-// each: 32 rows of up to 2000 tokens 7.9 us (three launches 14), 1024 rows of up to 16000 (8 MB) 24.
+// each: 32 rows of up to 2000 tokens 8.0 us (three launches 14), 1024 rows of up to 16000 (8 MB) 24.8.
 #include <algorithm>
 
 #include "ba_device.hpp"

@@ -5,8 +5,8 @@
 // 16 x 16 x 32 matrix instruction with tokens as rows and one or two sets of 16 columns, which are rows of the queries here; a lane turns
 // the small matrix of its eight tokens' values in registers; probabilities enter the second product as two 16-bit terms.  A token's place is
 // worked out by one lane and handed to those that load it through LDS, whatever the pages are.
-// What bounds it: memory where requests are long (64 requests of 4000 tokens, 8 key heads of 128, 1.05 GB: 16 rows a key head 164 us, 6.4 TB/s; 32 rows
-// 176); where they are short a unit's beginning and end, some 6 us, and the sums over all requests before (492 units of 1000 tokens, 80 dimensions
+// What bounds it: memory where requests are long (64 requests of 4000 tokens, 8 key heads of 128, 1.05 GB: 16 rows a key head 168 us, 6.3 TB/s; 32 rows
+// 176; in 8 bits, 0.52 GB, 96 and 158); where they are short a unit's beginning and end, some 6 us, and the sums over all requests before (492 units of 1000 tokens, 80 dimensions
 // 43.5 us, 3.0 TB/s; one request of 500 tokens 14.5).
 #pragma once
 #include "paged_tree_attention.hpp"

@@ -12,8 +12,8 @@
 // would add its own rounding's error once more (1.3 times the whole error); two cost the second product again (64 requests of 4000 tokens, 128 rows of 128
 // dimensions 240 -> 286 us, 512 rows 215 -> 265; a batch of 32 drafts 94.6 -> 97.5).
 // What bounds it: a wavefront's chain of LDS, products, exponentials, LDS, products, of which two to a SIMD hide half (two requests of 32768 to 65536
-// tokens in 8 bits, 512 rows a key head, 240 GFLOP: 335 to 355 us, 680 to 720 TFLOP/s with the matrix unit busy 33 % of the time, vector instructions
-// 38 %, LDS 36 %).  32 requests of up to 4096 tokens and 32 nodes (281 MB) take 97 us.
+// tokens in 8 bits, 512 rows a key head, 240 GFLOP: 340 to 352 us, 680 to 705 TFLOP/s with the matrix unit busy 33 % of the time, vector instructions
+// 37 %, LDS 37 %).  32 requests of up to 4096 tokens and 32 nodes (281 MB) take 92 to 97 us by the card.
 #pragma once
 #include "paged_tree_attention.hpp"
 
